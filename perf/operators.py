@@ -281,7 +281,7 @@ def _plain_build(s):
     take = torch.where(need <= width, need - held, 0)
     first = s["cursor"].long() + torch.cumsum(take, 0) - take
     ends = torch.cumsum(new, 0)
-    fits = (need <= width) & (first + take <= s["free"].shape[0]) & (ends <= places)
+    fits = (need <= width) & ((take == 0) | (first + take <= s["free"].shape[0])) & ((new == 0) | (ends <= places))
     cols = torch.arange(width, device=held.device)[None, :]
     mine = fits[:, None] & (cols >= held[:, None]) & (cols < need[:, None])
     from_list = (first[:, None] + cols - held[:, None]).clamp(0, s["free"].shape[0] - 1)
@@ -372,7 +372,8 @@ def _exact_build(case, seed):
     for r in range(seqs):
         held, need = -(-cached[r] // ps), -(-(cached[r] + new[r]) // ps)
         take = need - held if need <= width else 0
-        fits = need <= width and asked + take <= len(free) and offsets[-1] + new[r] <= places
+        fits = need <= width and (not take or asked + take <= len(free)) and (
+            not new[r] or offsets[-1] + new[r] <= places)
         if fits:
             table[r][held:need] = free[asked:asked + take]
             used += take
