@@ -26,6 +26,8 @@ struct nc_function_st {
 
 struct nc_module_st {
     hipModule_t mod = nullptr;
+    // The embedded module's second code object (the paged cache's kernels); null in a loaded one.
+    hipModule_t paged = nullptr;
     // Guards `functions`: several host threads may launch through one module (hipModuleGetFunction,
     // the lookup the cache saves, is itself thread-safe). Entries are never removed before unload,
     // so a returned nc_function stays valid without the lock.
@@ -43,6 +45,7 @@ struct nc_module_st {
 
 extern "C" const unsigned char nc_embedded_code_object[];
 extern "C" const unsigned char nc_embedded_code_object_end[];
+extern "C" const unsigned char nc_embedded_paged_object[];
 
 namespace {
 
@@ -215,7 +218,14 @@ int nc_module_load_file(nc_module *out, const char *path) {
 int nc_module_load_embedded(nc_module *out) {
     if (nc_embedded_code_object_end <= nc_embedded_code_object)
         return fail(NC_ERROR_INVALID_IMAGE, "nc_module_load_embedded: library built without a code object");
-    return nc_module_load_data(out, nc_embedded_code_object);
+    int st = nc_module_load_data(out, nc_embedded_code_object);
+    if (st) return st;
+    st = check(hipModuleLoadData(&(*out)->paged, nc_embedded_paged_object), "hipModuleLoadData");
+    if (st) {
+        (void)nc_module_unload(*out);
+        *out = nullptr;
+    }
+    return st;
 }
 
 int nc_module_unload(nc_module module) {
@@ -224,6 +234,10 @@ int nc_module_unload(nc_module module) {
     if (module->workspace) st = check(hipFree(module->workspace), "hipFree(workspace)");
     for (void *p : module->retired) {
         const int s2 = check(hipFree(p), "hipFree(retired workspace)");
+        if (!st) st = s2;
+    }
+    if (module->paged) {
+        const int s2 = check(hipModuleUnload(module->paged), "hipModuleUnload");
         if (!st) st = s2;
     }
     int st2 = check(hipModuleUnload(module->mod), "hipModuleUnload");
@@ -284,7 +298,8 @@ int nc_module_get_function(nc_function *out, nc_module module, const char *name)
         return NC_SUCCESS;
     }
     hipFunction_t f = nullptr;
-    int st = check(hipModuleGetFunction(&f, module->mod, name), "hipModuleGetFunction");
+    const hipModule_t in = module->paged && std::strncmp(name, "nc_paged_", 9) == 0 ? module->paged : module->mod;
+    int st = check(hipModuleGetFunction(&f, in, name), "hipModuleGetFunction");
     if (st) return st;
     auto fn = std::make_unique<nc_function_st>();
     fn->fn = f;

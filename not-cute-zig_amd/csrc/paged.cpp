@@ -1,0 +1,333 @@
+// paged.cpp — host side of the paged key-value cache (include/notcute_paged.h): validation, the choice of
+// kernel and grid, launches. Nothing here allocates or synchronises.
+
+#include <algorithm>
+#include <cstdint>
+#include <cstring>
+
+#include "notcute_paged.h"
+#include "paged_args.h"
+
+extern "C" int nc_internal_fail(int status, const char *what);
+
+namespace {
+
+constexpr uint64_t kMost31 = 0x7fffffffull;
+constexpr uint64_t kMostElements = 1ull << 60;
+
+// The options with every stride resolved.
+struct Shape {
+    nc_paged_options o;
+    uint64_t group, cache_len, table_len, q_len, o_len;
+};
+
+uint64_t or_packed(uint64_t stride, uint64_t count, uint64_t inner) { return stride ? stride : count * inner; }
+
+struct Axis {
+    uint64_t n, stride;
+};
+
+// Elements from a tensor's first to behind its last, for rows of d elements at every combination of the
+// axes; fails where two rows share an element (a stride below the extent of the axes of smaller strides).
+int extent(Axis *ax, int count, uint64_t d, uint64_t *out) {
+    std::sort(ax, ax + count, [](const Axis &x, const Axis &y) { return x.stride < y.stride; });
+    uint64_t span = d;
+    for (int i = 0; i < count; ++i) {
+        if (ax[i].n <= 1) continue;
+        if (ax[i].stride < span) return NC_ERROR_INVALID_VALUE;
+        if (ax[i].stride > kMostElements / ax[i].n) return NC_ERROR_OVERFLOW;
+        span += (ax[i].n - 1) * ax[i].stride;
+        if (span > kMostElements) return NC_ERROR_OVERFLOW;
+    }
+    *out = span;
+    return NC_SUCCESS;
+}
+
+int resolve(const nc_paged_options *opts, Shape *s) {
+    if (!opts) return NC_ERROR_INVALID_VALUE;
+    s->o = *opts;
+    nc_paged_options &o = s->o;
+    if (!o.num_seqs || !o.num_q_heads || !o.num_kv_heads || !o.page_size || !o.num_pages || !o.max_pages)
+        return NC_ERROR_INVALID_VALUE;
+    if (o.head_dim != 16 && o.head_dim != 32 && o.head_dim != 64 && o.head_dim != 128) return NC_ERROR_INVALID_VALUE;
+    if (o.element_type != NC_ELEMENT_F16 && o.element_type != NC_ELEMENT_BF16) return NC_ERROR_INVALID_VALUE;
+    if (o.num_q_heads % o.num_kv_heads) return NC_ERROR_INVALID_VALUE;
+    const uint64_t counts[] = {o.num_seqs, o.num_q_heads, o.page_size, o.num_pages, o.max_pages};
+    for (uint64_t n : counts)
+        if (n > kMost31) return NC_ERROR_OVERFLOW;
+    if (o.page_size * o.num_pages > kMost31 || o.page_size * o.max_pages > kMost31) return NC_ERROR_OVERFLOW;
+    s->group = o.num_q_heads / o.num_kv_heads;
+    const uint64_t given[] = {o.table_stride, o.page_stride, o.head_stride, o.token_stride, o.row_stride, o.row_head_stride,
+                              o.q_stride, o.q_head_stride, o.o_stride, o.o_head_stride};
+    for (uint64_t x : given)
+        if (x > kMostElements) return NC_ERROR_OVERFLOW;
+    // Workgroups' shares are counted in blocks of at least 128 keys of one request and key head (or 16 of
+    // its query heads), in 32 bits.
+    const uint64_t blocks = (o.page_size * o.max_pages + 127) / 128, heads = o.num_kv_heads * ((s->group + 15) / 16);
+    if (o.num_seqs * heads > kMost31 || blocks > kMost31 / (o.num_seqs * heads)) return NC_ERROR_OVERFLOW;
+
+    const uint64_t d = o.head_dim;
+    o.table_stride = or_packed(o.table_stride, o.max_pages, 1);
+    o.token_stride = or_packed(o.token_stride, 1, d);
+    // packed values of given inner strides, each at most 2^60: checked before they are multiplied
+    if (o.token_stride > kMostElements / o.page_size) return NC_ERROR_OVERFLOW;
+    o.head_stride = or_packed(o.head_stride, o.page_size, o.token_stride);
+    if (o.head_stride > kMostElements / o.num_kv_heads) return NC_ERROR_OVERFLOW;
+    if (!o.page_stride) o.page_stride = std::max(o.num_kv_heads * o.head_stride, o.page_size * o.token_stride);
+    o.row_head_stride = or_packed(o.row_head_stride, 1, d);
+    if (o.row_head_stride > kMostElements / o.num_kv_heads) return NC_ERROR_OVERFLOW;
+    o.row_stride = or_packed(o.row_stride, o.num_kv_heads, o.row_head_stride);
+    o.q_head_stride = or_packed(o.q_head_stride, 1, d);
+    o.o_head_stride = or_packed(o.o_head_stride, 1, d);
+    if (std::max(o.q_head_stride, o.o_head_stride) > kMostElements / o.num_q_heads) return NC_ERROR_OVERFLOW;
+    o.q_stride = or_packed(o.q_stride, o.num_q_heads, o.q_head_stride);
+    o.o_stride = or_packed(o.o_stride, o.num_q_heads, o.o_head_stride);
+    if ((o.page_stride | o.head_stride | o.token_stride) % 8) return NC_ERROR_INVALID_VALUE;
+
+    Axis cache[] = {{o.num_pages, o.page_stride}, {o.num_kv_heads, o.head_stride}, {o.page_size, o.token_stride}};
+    Axis table[] = {{o.num_seqs, o.table_stride}};
+    Axis q[] = {{o.num_seqs, o.q_stride}, {o.num_q_heads, o.q_head_stride}};
+    Axis out[] = {{o.num_seqs, o.o_stride}, {o.num_q_heads, o.o_head_stride}};
+    int st = extent(cache, 3, d, &s->cache_len);
+    if (!st) st = extent(table, 1, o.max_pages, &s->table_len);
+    if (!st) st = extent(q, 2, d, &s->q_len);
+    if (!st) st = extent(out, 2, d, &s->o_len);
+    if (st) return st;
+    // one row's heads; how many rows there are is an argument of the append
+    Axis row[] = {{2, o.row_stride}, {o.num_kv_heads, o.row_head_stride}};
+    uint64_t unused;
+    return extent(row, 2, d, &unused);
+}
+
+struct Range {
+    uintptr_t lo, hi;
+};
+
+Range range_of(const void *p, uint64_t elements, uint64_t size) {
+    return {reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + elements * size};
+}
+
+bool overlap(const Range &x, const Range &y) { return x.lo < x.hi && y.lo < y.hi && x.lo < y.hi && y.lo < x.hi; }
+
+uintptr_t address(const void *p) { return reinterpret_cast<uintptr_t>(p); }
+
+int launch(nc_module module, const char *name, uint32_t grid, uint32_t threads, void *args, nc_stream stream) {
+    nc_function fn = nullptr;
+    int st = nc_module_get_function(&fn, module, name);
+    if (st) return st;
+    nc_launch_config cfg;
+    std::memset(&cfg, 0, sizeof cfg);
+    cfg.grid[0] = grid;
+    cfg.grid[1] = cfg.grid[2] = 1;
+    cfg.block[0] = threads;
+    cfg.block[1] = cfg.block[2] = 1;
+    cfg.stream = stream;
+    void *params[] = {args};
+    return nc_function_launch(fn, &cfg, params);
+}
+
+const char *decode_kernel(const nc_paged_options &o) {
+    const bool bf = o.element_type == NC_ELEMENT_BF16;
+    switch (o.head_dim) {
+    case 16: return bf ? "nc_paged_decode_d16_bf16" : "nc_paged_decode_d16";
+    case 32: return bf ? "nc_paged_decode_d32_bf16" : "nc_paged_decode_d32";
+    case 64: return bf ? "nc_paged_decode_d64_bf16" : "nc_paged_decode_d64";
+    default: return bf ? "nc_paged_decode_d128_bf16" : "nc_paged_decode_d128";
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+void nc_paged_options_init(nc_paged_options *opts) {
+    if (!opts) return;
+    std::memset(opts, 0, sizeof *opts);
+    opts->num_seqs = opts->num_q_heads = opts->num_kv_heads = opts->max_pages = 1;
+}
+
+int nc_paged_validate(const nc_paged_options *opts) {
+    Shape s;
+    return resolve(opts, &s);
+}
+
+uint64_t nc_paged_workspace_bytes(const nc_paged_options *opts) {
+    Shape s;
+    return resolve(opts, &s) ? 0 : 16;
+}
+
+int nc_paged_build(nc_module module, const int32_t *cached_lens, size_t cached_len, const int32_t *new_lens,
+                   size_t new_len, const int32_t *free_pages, size_t free_len, const int32_t *cursor,
+                   size_t cursor_len, int32_t *block_table, size_t table_len, int32_t *seq_lens, size_t seq_len,
+                   int32_t *row_offsets, size_t offsets_len, int32_t *slots, size_t slots_len, int32_t *counts,
+                   size_t counts_len, const nc_paged_options *opts, nc_stream stream) {
+    Shape s;
+    int st = resolve(opts, &s);
+    if (st) return st;
+    const nc_paged_options &o = s.o;
+    if (!module || !cached_lens || !new_lens || !cursor || !block_table || !seq_lens || !row_offsets || !counts ||
+        (!free_pages && free_len) || (!slots && slots_len))
+        return NC_ERROR_INVALID_VALUE;
+    if (cached_len < o.num_seqs || new_len < o.num_seqs || seq_len < o.num_seqs || offsets_len < o.num_seqs + 1 ||
+        table_len < s.table_len || cursor_len < 1 || counts_len < 4)
+        return NC_ERROR_INVALID_VALUE;
+    if (slots_len > kMost31 || free_len > kMost31) return NC_ERROR_OVERFLOW;
+    if ((address(cached_lens) | address(new_lens) | address(free_pages) | address(cursor) | address(block_table) |
+         address(seq_lens) | address(row_offsets) | address(slots) | address(counts)) % 4)
+        return NC_ERROR_INVALID_VALUE;
+
+    // Outputs first; a pair may be one and the same buffer only where the header says so.
+    const Range rg[] = {range_of(seq_lens, o.num_seqs, 4),    range_of(counts, 4, 4),
+                        range_of(block_table, s.table_len, 4), range_of(row_offsets, o.num_seqs + 1, 4),
+                        range_of(slots, slots_len, 4),         range_of(cached_lens, o.num_seqs, 4),
+                        range_of(cursor, 1, 4),                range_of(new_lens, o.num_seqs, 4),
+                        range_of(free_pages, free_len, 4)};
+    const bool same_lens = seq_lens == cached_lens, same_cursor = counts == cursor;
+    for (int i = 0; i < 5; ++i)
+        for (int j = i + 1; j < 9; ++j) {
+            if ((i == 0 && j == 5 && same_lens) || (i == 1 && j == 6 && same_cursor)) continue;
+            if (overlap(rg[i], rg[j]))
+                return nc_internal_fail(NC_ERROR_INVALID_VALUE, "nc_paged_build: an output overlaps another buffer");
+        }
+
+    nc_paged_build_args a;
+    std::memset(&a, 0, sizeof a);
+    a.cached = cached_lens;
+    a.fresh = new_lens;
+    a.free_pages = free_pages;
+    a.cursor = cursor;
+    a.table = block_table;
+    a.seq_lens = seq_lens;
+    a.offsets = row_offsets;
+    a.slots = slots;
+    a.counts = counts;
+    a.table_stride = o.table_stride;
+    a.num_seqs = (uint32_t)o.num_seqs;
+    a.width = (uint32_t)o.max_pages;
+    a.num_pages = (uint32_t)o.num_pages;
+    a.free_len = (uint32_t)free_len;
+    a.places = (uint32_t)slots_len;
+    a.ps = nc_paged_make_div((uint32_t)o.page_size);
+    const uint32_t threads = o.num_seqs <= 256 ? 256 : 1024;
+    // One workgroup up to 4096 slots; beyond, 2048 each.
+    const uint64_t wgs = slots_len <= 4096 ? 1 : std::min<uint64_t>((slots_len + 2047) / 2048, 1024);
+    a.chunk_rows = (uint32_t)((slots_len + wgs - 1) / wgs);
+    // no more pages than this are taken
+    const uint64_t pages = std::min<uint64_t>(free_len, slots_len / o.page_size + o.num_seqs);
+    a.chunk_pages = (uint32_t)((pages + wgs - 1) / wgs);
+    a.parts = NC_PAGED_PART_PAGES | NC_PAGED_PART_LENS;
+    // In place, several workgroups read what one of them would write: the lengths wait for a second launch.
+    const bool later = wgs > 1 && (same_lens || same_cursor);
+    if (later) a.parts = NC_PAGED_PART_PAGES;
+    st = launch(module, "nc_paged_build", (uint32_t)wgs, threads, &a, stream);
+    if (st || !later) return st;
+    a.parts = NC_PAGED_PART_LENS;
+    return launch(module, "nc_paged_build", 1, threads, &a, stream);
+}
+
+int nc_paged_append(nc_module module, const uint16_t *k_rows, size_t k_rows_len, const uint16_t *v_rows,
+                    size_t v_rows_len, const int32_t *slots, size_t slots_len, uint16_t *k_cache, size_t k_len,
+                    uint16_t *v_cache, size_t v_len, uint64_t num_rows, const nc_paged_options *opts,
+                    nc_stream stream) {
+    Shape s;
+    int st = resolve(opts, &s);
+    if (st) return st;
+    const nc_paged_options &o = s.o;
+    if (!module || !k_cache || !v_cache || k_len < s.cache_len || v_len < s.cache_len) return NC_ERROR_INVALID_VALUE;
+    if ((address(k_cache) | address(v_cache)) % 16 || k_cache == v_cache) return NC_ERROR_INVALID_VALUE;
+    if (num_rows == 0) return NC_SUCCESS;
+    if (num_rows > kMost31) return NC_ERROR_OVERFLOW;
+    Axis row[] = {{num_rows, o.row_stride}, {o.num_kv_heads, o.row_head_stride}};
+    uint64_t rows_len = 0;
+    st = extent(row, 2, o.head_dim, &rows_len);
+    if (st) return st;
+    if (!k_rows || !v_rows || !slots || k_rows_len < rows_len || v_rows_len < rows_len || slots_len < num_rows)
+        return NC_ERROR_INVALID_VALUE;
+    if ((address(k_rows) | address(v_rows)) % 2 || address(slots) % 4) return NC_ERROR_INVALID_VALUE;
+    const Range caches[] = {range_of(k_cache, s.cache_len, 2), range_of(v_cache, s.cache_len, 2)};
+    const Range ins[] = {range_of(k_rows, rows_len, 2), range_of(v_rows, rows_len, 2), range_of(slots, num_rows, 4)};
+    for (const Range &x : caches)
+        for (const Range &y : ins)
+            if (overlap(x, y)) return nc_internal_fail(NC_ERROR_INVALID_VALUE, "nc_paged_append: the rows overlap the cache");
+
+    nc_paged_append_args a;
+    std::memset(&a, 0, sizeof a);
+    a.k_rows = k_rows;
+    a.v_rows = v_rows;
+    a.slots = slots;
+    a.k = k_cache;
+    a.v = v_cache;
+    a.row_stride = o.row_stride;
+    a.row_head_stride = o.row_head_stride;
+    a.page_stride = o.page_stride;
+    a.head_stride = o.head_stride;
+    a.token_stride = o.token_stride;
+    a.num_rows = num_rows;
+    a.num_slots = (uint32_t)(o.num_pages * o.page_size);
+    a.ps = nc_paged_make_div((uint32_t)o.page_size);
+    const uint64_t chunks = o.num_kv_heads * (o.head_dim / 8);
+    if (chunks > kMost31 / 2) return NC_ERROR_OVERFLOW;
+    a.chunks = nc_paged_make_div((uint32_t)chunks);
+    a.chunk_shift = o.head_dim == 16 ? 1 : o.head_dim == 32 ? 2 : o.head_dim == 64 ? 3 : 4;
+    // about 1024 chunks a workgroup, and no more than 2^23 workgroups
+    a.wg_rows = (uint32_t)std::max<uint64_t>(std::max<uint64_t>(1, 1024 / chunks), (num_rows + (1u << 23) - 1) >> 23);
+    if (a.wg_rows * chunks > kMost31) return NC_ERROR_OVERFLOW;
+    const bool vec = (address(k_rows) | address(v_rows)) % 16 == 0 && (o.row_stride | o.row_head_stride) % 8 == 0;
+    return launch(module, vec ? "nc_paged_append_rows" : "nc_paged_append_rows_unaligned",
+                  (uint32_t)((num_rows + a.wg_rows - 1) / a.wg_rows), 256, &a, stream);
+}
+
+int nc_paged_decode(nc_module module, const uint16_t *q, size_t q_len, const uint16_t *k_cache, size_t k_len,
+                    const uint16_t *v_cache, size_t v_len, const int32_t *block_table, size_t table_len,
+                    const int32_t *seq_lens, size_t lens_len, float *o, size_t o_len, void *workspace,
+                    uint64_t workspace_bytes, const nc_paged_options *opts, nc_stream stream) {
+    Shape s;
+    int st = resolve(opts, &s);
+    if (st) return st;
+    const nc_paged_options &op = s.o;
+    const uint64_t need = nc_paged_workspace_bytes(opts);
+    if (!module || !q || !k_cache || !v_cache || !block_table || !seq_lens || !o || (!workspace && need))
+        return NC_ERROR_INVALID_VALUE;
+    if (q_len < s.q_len || k_len < s.cache_len || v_len < s.cache_len || table_len < s.table_len ||
+        lens_len < op.num_seqs || o_len < s.o_len || workspace_bytes < need)
+        return NC_ERROR_INVALID_VALUE;
+    if ((address(k_cache) | address(v_cache) | address(workspace)) % 16 || address(q) % 2 ||
+        (address(block_table) | address(seq_lens) | address(o)) % 4)
+        return NC_ERROR_INVALID_VALUE;
+    const Range outs[] = {range_of(o, s.o_len, 4), range_of(workspace, need, 1)};
+    const Range ins[] = {range_of(q, s.q_len, 2), range_of(k_cache, s.cache_len, 2), range_of(v_cache, s.cache_len, 2),
+                         range_of(block_table, s.table_len, 4), range_of(seq_lens, op.num_seqs, 4)};
+    bool bad = overlap(outs[0], outs[1]);
+    for (const Range &x : outs)
+        for (const Range &y : ins) bad = bad || overlap(x, y);
+    if (bad) return nc_internal_fail(NC_ERROR_INVALID_VALUE, "nc_paged_decode: O or the workspace overlaps another buffer");
+
+    nc_paged_decode_args a;
+    std::memset(&a, 0, sizeof a);
+    a.q = q;
+    a.k = k_cache;
+    a.v = v_cache;
+    a.table = block_table;
+    a.seq_lens = seq_lens;
+    a.o = o;
+    a.workspace = workspace;
+    a.table_stride = op.table_stride;
+    a.page_stride = op.page_stride;
+    a.head_stride = op.head_stride;
+    a.token_stride = op.token_stride;
+    a.q_stride = op.q_stride;
+    a.q_head_stride = op.q_head_stride;
+    a.o_stride = op.o_stride;
+    a.o_head_stride = op.o_head_stride;
+    a.num_seqs = (uint32_t)op.num_seqs;
+    a.num_q_heads = (uint32_t)op.num_q_heads;
+    a.num_kv_heads = (uint32_t)op.num_kv_heads;
+    a.group = (uint32_t)s.group;
+    a.num_pages = (uint32_t)op.num_pages;
+    a.max_tokens = (uint32_t)(op.max_pages * op.page_size);
+    a.scale = op.scale;
+    a.ps = nc_paged_make_div((uint32_t)op.page_size);
+    return launch(module, decode_kernel(op), (uint32_t)(op.num_seqs * op.num_q_heads), 256, &a, stream);
+}
+
+}  // extern "C"

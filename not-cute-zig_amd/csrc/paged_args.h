@@ -1,0 +1,71 @@
+// paged_args.h — what paged.cpp and paged.hip share: the kernels' argument blocks and the index
+// arithmetic that both sides (and the CPU tests) have to agree on.
+#ifndef NOTCUTE_PAGED_ARGS_H
+#define NOTCUTE_PAGED_ARGS_H
+
+#include <stdint.h>
+
+#ifdef __HIPCC__
+#define NC_HD __host__ __device__ __forceinline__
+#else
+#define NC_HD inline
+#endif
+
+// n / d for 0 <= n < 2^31 by one 32x32 high multiply: with 2^s >= d and magic = ceil(2^(31+s) / d),
+// n * magic / 2^(31+s) exceeds n/d by less than n / 2^31 / d < 1/d, so its floor is the quotient.
+struct nc_paged_div {
+    uint32_t d, magic, shift;
+};
+inline nc_paged_div nc_paged_make_div(uint32_t d) {
+    nc_paged_div r = {d, 0, 0};
+    while ((1ull << r.shift) < d) ++r.shift;
+    r.magic = (uint32_t)(((1ull << (31 + r.shift)) + d - 1) / d);
+    return r;
+}
+NC_HD uint32_t nc_paged_quot(uint32_t n, nc_paged_div v) {
+    return (uint32_t)(((uint64_t)(2u * n) * v.magic) >> 32) >> v.shift;
+}
+
+struct nc_paged_build_args {
+    const int32_t *cached, *fresh, *free_pages, *cursor;
+    int32_t *table, *seq_lens, *offsets, *slots, *counts;
+    uint64_t table_stride;
+    uint32_t num_seqs, width, num_pages, free_len, places;
+    uint32_t chunk_rows, chunk_pages; // slots and list places of one workgroup
+    uint32_t parts;                   // NC_PAGED_PART_*
+    nc_paged_div ps;
+};
+#define NC_PAGED_PART_PAGES 1u // table entries and slots
+#define NC_PAGED_PART_LENS 2u  // lengths, offsets and counts
+
+struct nc_paged_append_args {
+    const uint16_t *k_rows, *v_rows;
+    const int32_t *slots;
+    uint16_t *k, *v;
+    uint64_t row_stride, row_head_stride, page_stride, head_stride, token_stride;
+    uint64_t num_rows;
+    uint32_t num_slots;    // num_pages * page_size
+    uint32_t wg_rows;      // rows of one workgroup
+    uint32_t chunk_shift;  // log2(head_dim / 8)
+    nc_paged_div ps, chunks; // page_size, and num_kv_heads * head_dim / 8
+};
+
+struct nc_paged_decode_args {
+    const uint16_t *q, *k, *v;
+    const int32_t *table, *seq_lens;
+    float *o;
+    void *workspace;
+    uint64_t table_stride, page_stride, head_stride, token_stride, q_stride, q_head_stride, o_stride, o_head_stride;
+    uint32_t num_seqs, num_q_heads, num_kv_heads, group; // group = num_q_heads / num_kv_heads
+    uint32_t num_pages, max_tokens;                      // max_tokens = max_pages * page_size
+    float scale;
+    nc_paged_div ps;
+};
+
+// A length from device memory, cut to what the table's row can hold.
+NC_HD uint32_t nc_paged_cut(int32_t len, uint32_t most) {
+    const uint32_t n = len < 0 ? 0u : (uint32_t)len;
+    return n < most ? n : most;
+}
+
+#endif

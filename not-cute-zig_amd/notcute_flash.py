@@ -1,4 +1,5 @@
-"""Python binding of the MI355X flash-attention C ABI (``include/notcute_flash.h``).
+"""Python binding of the MI355X flash-attention C ABI (``include/notcute_flash.h``, and the paged
+key-value cache of ``include/notcute_paged.h``).
 
 This is a ctypes mirror of the reference's public ``flash`` / ``cuda`` / ``benchmark`` modules
 (src/flash.zig, src/cuda.zig, src/benchmark.zig) over ``libnotcute_flash.so``. It holds no compute:
@@ -185,6 +186,15 @@ class BenchmarkResult(ctypes.Structure):
     ]
 
 
+class PagedOptions(ctypes.Structure):
+    """nc_paged_options (include/notcute_paged.h)."""
+
+    _fields_ = [(name, ctypes.c_uint64) for name in (
+        "num_seqs", "num_q_heads", "num_kv_heads", "head_dim", "page_size", "num_pages", "max_pages", "table_stride",
+        "page_stride", "head_stride", "token_stride", "row_stride", "row_head_stride", "q_stride", "q_head_stride",
+        "o_stride", "o_head_stride")] + [("scale", ctypes.c_float), ("element_type", ctypes.c_uint32)]
+
+
 _P = ctypes.c_void_p
 _U64 = ctypes.c_uint64
 _SIGS = {
@@ -251,6 +261,15 @@ _SIGS = {
     "nc_flash_reset_scratch": (ctypes.c_int, [_P]),
     "nc_flash_kernel_scratch_bytes": (
         ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(FlashOptions), ctypes.POINTER(_U64)]),
+    "nc_paged_options_init": (None, [ctypes.POINTER(PagedOptions)]),
+    "nc_paged_validate": (ctypes.c_int, [ctypes.POINTER(PagedOptions)]),
+    "nc_paged_workspace_bytes": (_U64, [ctypes.POINTER(PagedOptions)]),
+    "nc_paged_build": (
+        ctypes.c_int, [_P] + [_P, ctypes.c_size_t] * 9 + [ctypes.POINTER(PagedOptions), _P]),
+    "nc_paged_append": (
+        ctypes.c_int, [_P] + [_P, ctypes.c_size_t] * 5 + [_U64, ctypes.POINTER(PagedOptions), _P]),
+    "nc_paged_decode": (
+        ctypes.c_int, [_P] + [_P, ctypes.c_size_t] * 6 + [_P, _U64, ctypes.POINTER(PagedOptions), _P]),
     "nc_benchmark_options_init": (None, [ctypes.POINTER(BenchmarkOptions)]),
     "nc_benchmark_run_kernel": (
         ctypes.c_int,
@@ -661,6 +680,85 @@ def flash_launch(module: Module, q: DeviceBuffer, k: DeviceBuffer, v: DeviceBuff
     check(lib().nc_flash_launch_async(module.handle, q.ptr + 2 * q_offset, ql, k.ptr + 2 * k_offset, kl,
                                       v.ptr + 2 * v_offset, vl, o.ptr + 4 * o_offset, ol, ctypes.byref(opts),
                                       stream), "flash.launch")
+
+
+# ---------------------------------------------------------------------------------------------
+# paged key-value cache (include/notcute_paged.h)
+# ---------------------------------------------------------------------------------------------
+
+def paged_options(*, head_dim: int, page_size: int, num_pages: int, num_seqs: int = 1, num_q_heads: int = 1,
+                  num_kv_heads: Optional[int] = None, max_pages: int = 1, table_stride: int = 0, page_stride: int = 0,
+                  head_stride: int = 0, token_stride: int = 0, row_stride: int = 0, row_head_stride: int = 0,
+                  q_stride: int = 0, q_head_stride: int = 0, o_stride: int = 0, o_head_stride: int = 0,
+                  scale: Optional[float] = None, dtype: str = "f16") -> PagedOptions:
+    """The options of a paged cache and of the tensors that its calls take (nc_paged_options). Strides of 0
+    stand for packed ones, num_kv_heads defaults to num_q_heads and scale to 1/sqrt(head_dim)."""
+    o = PagedOptions()
+    lib().nc_paged_options_init(ctypes.byref(o))
+    o.num_seqs, o.num_q_heads, o.head_dim = num_seqs, num_q_heads, head_dim
+    o.num_kv_heads = num_q_heads if num_kv_heads is None else num_kv_heads
+    o.page_size, o.num_pages, o.max_pages, o.table_stride = page_size, num_pages, max_pages, table_stride
+    o.page_stride, o.head_stride, o.token_stride = page_stride, head_stride, token_stride
+    o.row_stride, o.row_head_stride = row_stride, row_head_stride
+    o.q_stride, o.q_head_stride, o.o_stride, o.o_head_stride = q_stride, q_head_stride, o_stride, o_head_stride
+    o.scale = (1.0 / float(np.sqrt(head_dim)) if head_dim > 0 else 0.0) if scale is None else scale
+    o.element_type = ELEMENT_TYPES[dtype]
+    return o
+
+
+def paged_validate(opts: PagedOptions) -> None:
+    check(lib().nc_paged_validate(ctypes.byref(opts)), "paged.validate")
+
+
+def paged_workspace_bytes(opts: PagedOptions) -> int:
+    """Bytes of device memory that paged_decode needs for these options, to be zeroed once; 0 for invalid ones."""
+    return int(lib().nc_paged_workspace_bytes(ctypes.byref(opts)))
+
+
+def paged_workspace(opts: PagedOptions) -> DeviceBuffer:
+    """A workspace for paged_decode with these options, zeroed."""
+    paged_validate(opts)
+    buf = DeviceBuffer(paged_workspace_bytes(opts))
+    buf.memset(0)
+    return buf
+
+
+def paged_build(module: Module, cached_lens: DeviceBuffer, new_lens: DeviceBuffer, free_pages: DeviceBuffer,
+                cursor: DeviceBuffer, block_table: DeviceBuffer, seq_lens: DeviceBuffer, row_offsets: DeviceBuffer,
+                slots: DeviceBuffer, counts: DeviceBuffer, opts: PagedOptions, stream: Optional[int] = None) -> None:
+    """Block tables, slot map and row offsets of a step from the requests' lengths (nc_paged_build). Every
+    buffer holds int32; the whole of `slots` is written and the whole of `free_pages` is the list. seq_lens may
+    be cached_lens, and counts may be cursor."""
+    check(lib().nc_paged_build(
+        module.handle, cached_lens.ptr, cached_lens.nbytes >> 2, new_lens.ptr, new_lens.nbytes >> 2, free_pages.ptr,
+        free_pages.nbytes >> 2, cursor.ptr, cursor.nbytes >> 2, block_table.ptr, block_table.nbytes >> 2, seq_lens.ptr,
+        seq_lens.nbytes >> 2, row_offsets.ptr, row_offsets.nbytes >> 2, slots.ptr, slots.nbytes >> 2, counts.ptr,
+        counts.nbytes >> 2, ctypes.byref(opts), stream), "paged.build")
+
+
+def paged_append(module: Module, k_rows: DeviceBuffer, v_rows: DeviceBuffer, slots: DeviceBuffer,
+                 k_cache: DeviceBuffer, v_cache: DeviceBuffer, opts: PagedOptions, stream: Optional[int] = None, *,
+                 num_rows: Optional[int] = None) -> None:
+    """New K and V rows into the cache's pages (nc_paged_append): row i to slots[i], for the first num_rows rows
+    (by default as many as there are slots)."""
+    places = slots.nbytes >> 2
+    n = places if num_rows is None else num_rows
+    if n < 0:
+        raise ValueError(f"paged_append: num_rows {n}")
+    check(lib().nc_paged_append(
+        module.handle, k_rows.ptr, k_rows.nbytes >> 1, v_rows.ptr, v_rows.nbytes >> 1, slots.ptr, places, k_cache.ptr,
+        k_cache.nbytes >> 1, v_cache.ptr, v_cache.nbytes >> 1, n, ctypes.byref(opts), stream), "paged.append")
+
+
+def paged_decode(module: Module, q: DeviceBuffer, k_cache: DeviceBuffer, v_cache: DeviceBuffer,
+                 block_table: DeviceBuffer, seq_lens: DeviceBuffer, o: DeviceBuffer, workspace: DeviceBuffer,
+                 opts: PagedOptions, stream: Optional[int] = None) -> None:
+    """Attention of one new token per request over its pages (nc_paged_decode); `workspace` is
+    paged_workspace(opts) or a zeroed buffer of paged_workspace_bytes(opts) and more."""
+    check(lib().nc_paged_decode(
+        module.handle, q.ptr, q.nbytes >> 1, k_cache.ptr, k_cache.nbytes >> 1, v_cache.ptr, v_cache.nbytes >> 1,
+        block_table.ptr, block_table.nbytes >> 2, seq_lens.ptr, seq_lens.nbytes >> 2, o.ptr, o.nbytes >> 2,
+        workspace.ptr, workspace.nbytes, ctypes.byref(opts), stream), "paged.decode")
 
 
 # ---------------------------------------------------------------------------------------------
