@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <cstdio>
 #include <cstring>
 
 #include "notcute_paged.h"
@@ -126,14 +127,30 @@ int launch(nc_module module, const char *name, uint32_t grid, uint32_t threads, 
     return nc_function_launch(fn, &cfg, params);
 }
 
-const char *decode_kernel(const nc_paged_options &o) {
-    const bool bf = o.element_type == NC_ELEMENT_BF16;
-    switch (o.head_dim) {
-    case 16: return bf ? "nc_paged_decode_d16_bf16" : "nc_paged_decode_d16";
-    case 32: return bf ? "nc_paged_decode_d32_bf16" : "nc_paged_decode_d32";
-    case 64: return bf ? "nc_paged_decode_d64_bf16" : "nc_paged_decode_d64";
-    default: return bf ? "nc_paged_decode_d128_bf16" : "nc_paged_decode_d128";
-    }
+// The attention's kernel, grid and workspace for a set of options.
+struct DecodePlan {
+    char name[40];
+    uint32_t grid, rows;
+    uint64_t piece_ml, piece_o, bytes;  // offsets of the partials, and all of the workspace
+};
+
+constexpr uint32_t kCus = 256;  // MI355X
+
+DecodePlan decode_plan(const Shape &s) {
+    const nc_paged_options &o = s.o;
+    DecodePlan p;
+    // A 16-key tile lies in one page, and its rows' offsets fit 32 bits.
+    const bool uniform = o.page_size % 16 == 0 && o.token_stride < (1ull << 26);
+    std::snprintf(p.name, sizeof p.name, "nc_paged_decode_d%u%s%s", (unsigned)o.head_dim, uniform ? "" : "_odd",
+                  o.element_type == NC_ELEMENT_BF16 ? "_bf16" : "");
+    const uint64_t keys = nc_paged_block_keys((uint32_t)o.head_dim);
+    const uint64_t blocks = o.num_seqs * o.num_kv_heads * ((s.group + 15) / 16) * ((o.page_size * o.max_pages + keys - 1) / keys);
+    p.grid = (uint32_t)std::min<uint64_t>(blocks, 3 * kCus);
+    p.rows = (uint32_t)std::min<uint64_t>(s.group, 16);
+    p.piece_ml = NC_PAGED_MAX_WGS * 4;
+    p.piece_o = p.piece_ml + (uint64_t)p.grid * 2 * p.rows * 2 * 4;
+    p.bytes = p.piece_o + (uint64_t)p.grid * 2 * p.rows * o.head_dim * 4;
+    return p;
 }
 
 }  // namespace
@@ -153,7 +170,7 @@ int nc_paged_validate(const nc_paged_options *opts) {
 
 uint64_t nc_paged_workspace_bytes(const nc_paged_options *opts) {
     Shape s;
-    return resolve(opts, &s) ? 0 : 16;
+    return resolve(opts, &s) ? 0 : decode_plan(s).bytes;
 }
 
 int nc_paged_build(nc_module module, const int32_t *cached_lens, size_t cached_len, const int32_t *new_lens,
@@ -285,8 +302,9 @@ int nc_paged_decode(nc_module module, const uint16_t *q, size_t q_len, const uin
     int st = resolve(opts, &s);
     if (st) return st;
     const nc_paged_options &op = s.o;
-    const uint64_t need = nc_paged_workspace_bytes(opts);
-    if (!module || !q || !k_cache || !v_cache || !block_table || !seq_lens || !o || (!workspace && need))
+    const DecodePlan plan = decode_plan(s);
+    const uint64_t need = plan.bytes;
+    if (!module || !q || !k_cache || !v_cache || !block_table || !seq_lens || !o || !workspace)
         return NC_ERROR_INVALID_VALUE;
     if (q_len < s.q_len || k_len < s.cache_len || v_len < s.cache_len || table_len < s.table_len ||
         lens_len < op.num_seqs || o_len < s.o_len || workspace_bytes < need)
@@ -310,7 +328,12 @@ int nc_paged_decode(nc_module module, const uint16_t *q, size_t q_len, const uin
     a.table = block_table;
     a.seq_lens = seq_lens;
     a.o = o;
-    a.workspace = workspace;
+    a.counters = static_cast<uint32_t *>(workspace);
+    a.part_ml = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.piece_ml);
+    a.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.piece_o);
+    a.rows = plan.rows;
+    a.q_vec = address(q) % 16 == 0 && (op.q_stride | op.q_head_stride) % 8 == 0;
+    a.o_vec = address(o) % 16 == 0 && (op.o_stride | op.o_head_stride) % 4 == 0;
     a.table_stride = op.table_stride;
     a.page_stride = op.page_stride;
     a.head_stride = op.head_stride;
@@ -327,7 +350,7 @@ int nc_paged_decode(nc_module module, const uint16_t *q, size_t q_len, const uin
     a.max_tokens = (uint32_t)(op.max_pages * op.page_size);
     a.scale = op.scale;
     a.ps = nc_paged_make_div((uint32_t)op.page_size);
-    return launch(module, decode_kernel(op), (uint32_t)(op.num_seqs * op.num_q_heads), 256, &a, stream);
+    return launch(module, plan.name, plan.grid, 256, &a, stream);
 }
 
 }  // extern "C"

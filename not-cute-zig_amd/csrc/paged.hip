@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "paged_args.h"
 
 namespace {
@@ -15,14 +17,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
-
-template <bool BF>
-__device__ __forceinline__ float to_f32(uint16_t h) {
-    if constexpr (BF)
-        return __uint_as_float((uint32_t)h << 16);
-    else
-        return (float)__builtin_bit_cast(_Float16, h);
-}
 
 __device__ __forceinline__ uint64_t wave_scan(uint64_t x, uint32_t lane) {
 #pragma unroll
@@ -198,72 +192,510 @@ extern "C" __global__ __launch_bounds__(256) void nc_paged_append_rows_unaligned
 }
 
 // -------------------------------------------------------------------------------------------------
-// Single-token attention: one workgroup per request and query head, its waves taking every fourth key.
+// Single-token attention. Up to 16 query heads of one key head are the 16 columns of the matrix products, so
+// K and V are read once for all of them. The work is cut into blocks of nc_paged_block_keys() keys, counted
+// over all requests and heads, and every workgroup takes an equal run of them, whatever the lengths: it finds
+// its first by a prefix sum over the requests' lengths. A run that begins or ends inside a request's keys
+// leaves a partial (max, sum, O); the last of a request's workgroups to arrive joins them in order.
+//
+// One wave takes KT x 32 keys of a block at a time. Scores: S = K Q^T with K rows straight from memory as the
+// A operand (lane l: key l%16, dims 8(l/16)..+7 of 32), so lane l holds the scores of query l%16 and keys
+// 4(l/16)+r of each 16. These registers are the B operand of O^T += V^T P^T as they stand, if V's k index runs
+// the same way: the lane loads D/16 dims of the eight keys 16t + 4(l/16) + r and turns them in registers.
+// Nothing but the final join of the four waves goes through LDS. K and V are read once and the rest is small, so
+// the read rate bounds it; the matrix cores have time for weights in two (f16) or three (bf16) parts, whose
+// sum is the f32 weight to 2^-21 or better: rounding them to one 16-bit number would cost 2^-12 or 2^-9.
 // -------------------------------------------------------------------------------------------------
 namespace {
 
-template <int D, bool BF>
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+// Memory that no kernel in flight writes, read by scalar loads.
+typedef const __attribute__((address_space(4))) int32_t *const_ints;
+
+__device__ __forceinline__ const_ints as_const(const int32_t *p) { return (const_ints)(uintptr_t)p; }
+
+template <bool BF>
+__device__ __forceinline__ floatx4 mfma_k32(u32x4 x, u32x4 y, floatx4 c) {
+    if constexpr (BF)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, x), __builtin_bit_cast(half8, y), c, 0, 0, 0);
+}
+template <bool BF>
+__device__ __forceinline__ floatx4 mfma_k16(u32x2 x, u32x2 y, floatx4 c) {
+    if constexpr (BF)
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4v, x), __builtin_bit_cast(short4v, y), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(half4, x), __builtin_bit_cast(half4, y), c, 0, 0, 0);
+}
+
+// Two f32 rounded to nearest as a pair of 16-bit numbers; x and y become what that leaves.
+template <bool BF>
+__device__ __forceinline__ uint32_t take_pair(float &x, float &y) {
+    if constexpr (BF) {
+        const bf16x2 h = {(__bf16)x, (__bf16)y};
+        x -= (float)h[0];
+        y -= (float)h[1];
+        return __builtin_bit_cast(uint32_t, h);
+    } else {
+        const half2v h = {(_Float16)x, (_Float16)y};
+        x -= (float)h[0];
+        y -= (float)h[1];
+        return __builtin_bit_cast(uint32_t, h);
+    }
+}
+
+// Over the four lanes l, l^16, l^32, l^48; all get the result.
+__device__ __forceinline__ float quad_max(float x) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+__device__ __forceinline__ uint32_t wave_scan32(uint32_t x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1, 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2, 3
+    return x;
+}
+
+// Partials go between workgroups of different XCDs, whose L2 caches are not coherent for ordinary accesses:
+// relaxed atomics at agent scope are. Their order against the counter is made by waits (see join()).
+__device__ __forceinline__ void put2(float *p, float x, float y) {
+    const uint64_t v = (uint64_t)__float_as_uint(x) | (uint64_t)__float_as_uint(y) << 32;
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void get2(const float *p, float &x, float &y) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    x = __uint_as_float((uint32_t)v);
+    y = __uint_as_float((uint32_t)(v >> 32));
+}
+
+__device__ __forceinline__ float finite_or_0(float m) { return m == neg_inf() ? 0.f : m; }
+
+// Which keys a workgroup is at: request r of length len, whose blocks begin behind `pre` blocks of the
+// requests before it.
+struct Place {
+    uint32_t r, len, pre;
+};
+
+template <int D, bool BF, bool UNI>
+struct Decode {
+    static constexpr int KT = D == 16 ? 4 : D == 32 ? 2 : 1;  // 32-key tiles of a wave's step
+    static constexpr int NT = 2 * KT;                        // 16-key tiles
+    static constexpr uint32_t WK = 32 * KT, BK = 4 * WK;      // keys of a wave's step, and of a block
+    static constexpr int E = D / 16;                         // dims of a lane in V and O
+    static constexpr int KK = D < 32 ? 1 : D / 32;           // products of a score
+    static constexpr int OP = D + 4;                         // pitch of a row of partial O in LDS
+    // Weights are 2^(SHIFT + score - max): in f16 the low part of a small weight stays a normal number, in bf16
+    // a sum of a million V at the type's largest value stays finite.
+    static constexpr float SHIFT = BF ? -16.f : 12.f;
+    using KReg = typename std::conditional<D == 16, u32x2, u32x4>::type;
+
+    const nc_paged_decode_args &a;
+    const uint32_t lane, w, c, g;
+    float (*s_o)[16][OP];   // [4]
+    float (*s_ml)[16][2];   // [4]
+    uint32_t *s_word;
+
+    u32x4 qv[KK];
+    floatx4 acc[E];
+    float m, l;
+
+    static __device__ __forceinline__ uint32_t blocks_of(uint32_t len) { return (len + BK - 1) / BK; }
+
+    // Q of the block's query heads as the B operand: lane (c, g) holds query c, dims 8g.. (4g.. for D = 16).
+    __device__ __forceinline__ void load_q(uint32_t r, uint32_t head0, uint32_t rows) {
+        const uint16_t *p = a.q + r * a.q_stride + (head0 + min(c, rows - 1u)) * a.q_head_stride;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            constexpr int N = D == 16 ? 4 : 8;
+            const uint16_t *x = p + 32 * kk + N * g;
+            u32x4 t = {0u, 0u, 0u, 0u};
+            if (a.q_vec) {
+                if constexpr (D == 16) {
+                    const u32x2 y = *reinterpret_cast<const u32x2 *>(x);
+                    t[0] = y[0];
+                    t[1] = y[1];
+                } else {
+                    t = *reinterpret_cast<const u32x4 *>(x);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i) t[i] = uint32_t(x[2 * i]) | uint32_t(x[2 * i + 1]) << 16;
+            }
+            qv[kk] = t;
+        }
+    }
+
+    // Table entries of a step's 16-key tiles: uniform where a tile lies in one page, else one per lane (key c
+    // of the tile). Past the request's end the last key's entry.
+    __device__ __forceinline__ void load_pages(uint32_t (&e)[NT], uint64_t row, uint32_t k0, uint32_t len) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if constexpr (UNI)
+                e[t] = (uint32_t)as_const(a.table)[row + nc_paged_quot(min(k0 + 16 * t, len - 1u), a.ps)];
+            else
+                e[t] = (uint32_t)a.table[row + nc_paged_quot(min(k0 + 16 * t + c, len - 1u), a.ps)];
+        }
+    }
+
+    // One step: the keys k0..k0+WK-1 of a request of length len, k0 < len, on the pages e.
+    __device__ __forceinline__ void step(const uint32_t (&e)[NT], uint32_t k0, uint32_t len, uint32_t kvh) {
+        KReg kr[NT][KK];
+        u32x4 vr[NT][4];  // E dims in the first E/2 dwords (D = 16: half of one)
+        uint32_t seen[NT];  // bit i: key i of the tile counts
+        const uint16_t *kh = a.k + kvh * a.head_stride, *vh = a.v + kvh * a.head_stride;
+        const uint16_t *vb[NT][4];
+        auto load_k = [&](int t, const uint16_t *p) {
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) kr[t][kk] = *reinterpret_cast<const KReg *>(p + 32 * kk);
+        };
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const uint32_t k1 = k0 + 16 * t;
+            if constexpr (UNI) {
+                // A tile without keys, or on a page outside the pool, reads the pool's page 0 and counts for nothing.
+                const bool in = k1 < len && e[t] < a.num_pages;
+                seen[t] = in ? (k1 + 16 <= len ? 0xffffu : (1u << (len - k1)) - 1u) : 0u;
+                const uint32_t ka = min(k1, (len - 1u) & ~15u);  // below 2^31
+                const uint64_t at = (in ? e[t] : 0u) * a.page_stride + (ka - nc_paged_quot(ka, a.ps) * a.ps.d) * a.token_stride;
+                const uint32_t ts = (uint32_t)a.token_stride;
+                load_k(t, kh + at + (c * ts + (D == 16 ? 4 : 8) * g));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vb[t][i] = vh + at + ((4 * g + i) * ts + E * c);
+            } else {
+                const uint32_t key = min(k1 + c, len - 1u);
+                const bool in = k1 + c < len && e[t] < a.num_pages;
+                seen[t] = (uint32_t)__ballot(in) & 0xffffu;
+                const uint64_t at = (in ? e[t] : 0u) * a.page_stride + (key - nc_paged_quot(key, a.ps) * a.ps.d) * a.token_stride;
+                load_k(t, kh + at + (D == 16 ? 4 : 8) * g);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int from = 4 * (int)g + i;
+                    const uint32_t lo = __shfl((uint32_t)at, from, 64), hi = __shfl((uint32_t)(at >> 32), from, 64);
+                    vb[t][i] = vh + ((uint64_t)hi << 32 | lo) + E * c;
+                }
+            }
+        }
+        bool full = true;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            full = full && seen[t] == 0xffffu;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (E == 8) {
+                    vr[t][i] = *reinterpret_cast<const u32x4 *>(vb[t][i]);
+                } else if constexpr (E == 4) {
+                    const u32x2 x = *reinterpret_cast<const u32x2 *>(vb[t][i]);
+                    vr[t][i][0] = x[0];
+                    vr[t][i][1] = x[1];
+                } else if constexpr (E == 2) {
+                    vr[t][i][0] = *reinterpret_cast<const uint32_t *>(vb[t][i]);
+                } else {
+                    vr[t][i][0] = *vb[t][i];
+                }
+            }
+        }
+
+        float s[NT][4];
+        const float sc = a.scale * kLog2e;
+        float top = neg_inf();
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            floatx4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+                if constexpr (D == 16)
+                    x = mfma_k16<BF>(kr[t][kk], u32x2{qv[kk][0], qv[kk][1]}, x);
+                else
+                    x = mfma_k32<BF>(kr[t][kk], qv[kk], x);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[t][i] = x[i] * sc;
+        }
+        if (!full) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool in = seen[t] >> (4 * g + i) & 1u;
+                    s[t][i] = in ? s[t][i] : neg_inf();
+#pragma unroll
+                    for (int j = 0; j < (E + 1) / 2; ++j) vr[t][i][j] = in ? vr[t][i][j] : 0u;  // 0 * NaN would be NaN
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][i]);
+        top = fmaxf(m, quad_max(top));
+        const float ref = finite_or_0(top) - SHIFT;
+        if (!__all(top == m)) {
+            const float f = __builtin_amdgcn_exp2f(m - finite_or_0(top));
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < E; ++i) acc[i] *= f;
+            m = top;
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - ref);
+                l += s[t][i];
+            }
+        constexpr int PARTS = BF ? 3 : 2;
+#pragma unroll
+        for (int u = 0; u < KT; ++u) {
+            u32x4 p[PARTS];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int n = 0; n < PARTS; ++n) p[n][j] = take_pair<BF>(s[2 * u + j / 2][2 * (j % 2)], s[2 * u + j / 2][2 * (j % 2) + 1]);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                u32x4 x;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t lo = vr[2 * u + j / 2][2 * (j % 2)][i / 2], hi = vr[2 * u + j / 2][2 * (j % 2) + 1][i / 2];
+                    x[j] = __builtin_amdgcn_perm(hi, lo, i % 2 ? 0x07060302u : 0x05040100u);
+                }
+#pragma unroll
+                for (int n = 0; n < PARTS; ++n) acc[i] = mfma_k32<BF>(x, p[n], acc[i]);
+            }
+        }
+    }
+
+    // The pieces of workgroups first..last of one request and head: added in order, so that it does not matter
+    // who came last, and written to O.
+    __device__ __forceinline__ void join_pieces(uint32_t first, uint32_t last, uint32_t rows, float *o) {
+        const uint32_t items = rows * (D / 4);
+        for (uint32_t it = threadIdx.x; it < items; it += 256) {
+            const uint32_t q = it / (D / 4), x = 4 * (it % (D / 4));
+            float top = neg_inf(), sum = 0.f;
+            floatx4 out = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+            for (uint32_t i = first; i <= last; ++i) {
+                const uint64_t piece = (uint64_t)i * 2 + (i == first) , at = piece * a.rows + q;
+                float pm, pl;
+                floatx4 po;
+                get2(a.part_ml + 2 * at, pm, pl);
+                float p0, p1, p2, p3;
+                get2(a.part_o + at * D + x, p0, p1);
+                get2(a.part_o + at * D + x + 2, p2, p3);
+                po = {p0, p1, p2, p3};
+                const float t = fmaxf(top, pm), f = __builtin_amdgcn_exp2f(top - finite_or_0(t)),
+                            h = __builtin_amdgcn_exp2f(pm - finite_or_0(t));
+                sum = sum * f + pl * h;
+                out = out * f + po * h;
+                top = t;
+            }
+            store_o(o, q, x, out, sum);
+        }
+    }
+
+    __device__ __forceinline__ void store_o(float *o, uint32_t q, uint32_t x, floatx4 v, float sum) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = sum == 0.f ? 0.f : v[i] / sum;
+        float *p = o + q * a.o_head_stride + x;
+        if (a.o_vec) {
+            *reinterpret_cast<floatx4 *>(p) = v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = v[i];
+        }
+    }
+
+    // The four waves' (m, l, O) of one run of blocks: to O if the run is all of the request's, else to this
+    // workgroup's piece, and the last workgroup joins. n workgroups share `blocks` blocks.
+    __device__ __forceinline__ void finish(uint32_t rows, float *o, bool whole, uint32_t i, uint32_t first, uint32_t last) {
+        const float sum = quad_sum(l);
+        if (g == 0) {
+            s_ml[w][c][0] = m;
+            s_ml[w][c][1] = sum;
+        }
+        if (c < rows) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < E; ++j) s_o[w][c][(4 * g + r) * E + j] = acc[j][r];
+        }
+        __syncthreads();
+        const uint32_t items = rows * (D / 4);
+        for (uint32_t it = threadIdx.x; it < items; it += 256) {
+            const uint32_t q = it / (D / 4), x = 4 * (it % (D / 4));
+            float top = neg_inf(), lsum = 0.f;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) top = fmaxf(top, s_ml[n][q][0]);
+            floatx4 out = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const float f = __builtin_amdgcn_exp2f(s_ml[n][q][0] - finite_or_0(top));
+                lsum += f * s_ml[n][q][1];
+                out += f * *reinterpret_cast<const floatx4 *>(&s_o[n][q][x]);
+            }
+            if (whole) {
+                store_o(o, q, x, out, lsum);
+            } else {
+                const uint64_t at = ((uint64_t)i * 2 + (i == first)) * a.rows + q;
+                put2(a.part_o + at * D + x, out[0], out[1]);
+                put2(a.part_o + at * D + x + 2, out[2], out[3]);
+                if (x == 0) put2(a.part_ml + 2 * at, top, lsum);
+            }
+        }
+        if (!whole) {
+            // Every thread's stores have arrived before the count says so, and the partials are read only after the
+            // count showed the last of them.
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (threadIdx.x == 0)
+                *s_word = __hip_atomic_fetch_add(a.counters + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (*s_word == last - first) {
+                join_pieces(first, last, rows, o);
+                if (threadIdx.x == 0) __hip_atomic_store(a.counters + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+        __syncthreads();  // LDS is free again
+    }
+
+    __device__ __forceinline__ void run() {
+        const uint32_t R = a.num_seqs, per = (R + 63u) / 64u;  // requests of a lane
+        const uint32_t qgroups = (a.group + 15u) / 16u, heads = a.num_kv_heads * qgroups;
+        const uint32_t zero_r = blockIdx.x;
+        const int32_t zero_len = zero_r < R ? as_const(a.seq_lens)[zero_r] : 1;
+        uint32_t mine = 0, len0 = 0;
+        for (uint32_t j = 0; j < per; ++j) {
+            const uint32_t r = lane * per + j;
+            if (r < R) {
+                len0 = nc_paged_cut(a.seq_lens[r], a.max_tokens);
+                mine += blocks_of(len0);
+            }
+        }
+        const uint32_t incl = wave_scan32(mine);
+        const uint32_t blocks = __builtin_amdgcn_readlane(incl, 63) * heads, n = min(gridDim.x, blocks), i = blockIdx.x;
+        if (i < n) {
+            const nc_paged_share share = nc_paged_share_of(i, blocks, n);
+            uint32_t b = share.first;
+            const uint32_t end = share.first + share.count;
+            Place at;
+            {
+                const uint32_t t = b / heads;  // the same request's block if it had one head
+                const uint32_t from = __builtin_ctzll(__ballot(incl - mine <= t && t < incl));
+                at.pre = __builtin_amdgcn_readlane(incl - mine, from);
+                at.r = from * per;
+                at.len = __builtin_amdgcn_readlane(len0, from);
+                if (per > 1) {
+                    const uint32_t r0 = at.r, most = min(per, R - r0);
+                    for (uint32_t x = 0; x < most; x += 64) {
+                        const uint32_t len = x + lane < most ? nc_paged_cut(a.seq_lens[r0 + x + lane], a.max_tokens) : 0u;
+                        const uint32_t nb = blocks_of(len), sc = wave_scan32(nb);
+                        const uint64_t hit = __ballot(t < at.pre + sc);
+                        if (hit) {
+                            const uint32_t y = __builtin_ctzll(hit);
+                            at.r = r0 + x + y;
+                            at.len = __builtin_amdgcn_readlane(len, y);
+                            at.pre += __builtin_amdgcn_readlane(sc - nb, y);
+                            break;
+                        }
+                        at.pre += __builtin_amdgcn_readlane(sc, 63);
+                    }
+                }
+            }
+            uint32_t nb = blocks_of(at.len);
+            uint32_t head = (b - at.pre * heads) / nb, b0 = b - at.pre * heads - head * nb;
+            while (true) {
+                const uint32_t b1 = min(nb, b0 + (end - b));
+                const uint32_t kvh = head / qgroups, qg = head - kvh * qgroups;
+                const uint32_t rows = min(16u, a.group - 16u * qg), head0 = kvh * a.group + 16u * qg;
+                load_q(at.r, head0, rows);
+                m = neg_inf();
+                l = 0.f;
+#pragma unroll
+                for (int x = 0; x < E; ++x) acc[x] = floatx4{0.f, 0.f, 0.f, 0.f};
+                uint32_t k0 = b0 * BK + w * WK;
+                const uint32_t k1 = min(b1 * BK, at.len);
+                const uint64_t row = at.r * a.table_stride;
+                if (k0 < k1) {
+                    uint32_t e[NT];
+                    load_pages(e, row, k0, at.len);
+                    while (true) {
+                        uint32_t next[NT];
+                        load_pages(next, row, k0 + BK, at.len);
+                        step(e, k0, at.len, kvh);
+                        k0 += BK;
+                        if (k0 >= k1) break;
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) e[t] = next[t];
+                    }
+                }
+                const uint32_t seg = at.pre * heads + head * nb;  // the request's and head's first block
+                const bool whole = b0 == 0 && b1 == nb;
+                finish(rows, a.o + at.r * a.o_stride + head0 * a.o_head_stride, whole, i,
+                       whole ? i : nc_paged_owner_of(seg, blocks, n), whole ? i : nc_paged_owner_of(seg + nb - 1, blocks, n));
+                b += b1 - b0;
+                if (b >= end) break;
+                b0 = 0;
+                if (++head == heads) {
+                    head = 0;
+                    at.pre += nb;
+                    do at.len = ++at.r < R ? nc_paged_cut(as_const(a.seq_lens)[at.r], a.max_tokens) : 1u;
+                    while (at.len == 0);  // the share has blocks left, so there is one
+                    if (at.r >= R) break;
+                    nb = blocks_of(at.len);
+                }
+            }
+        }
+        // Requests without keys
+        int32_t zl = zero_len;
+        for (uint32_t r = zero_r; r < R;) {
+            if (nc_paged_cut(zl, a.max_tokens) == 0)
+                for (uint32_t x = threadIdx.x; x < a.num_q_heads * D; x += 256)
+                    a.o[r * a.o_stride + (x / D) * a.o_head_stride + x % D] = 0.f;
+            r += gridDim.x;
+            if (r < R) zl = as_const(a.seq_lens)[r];
+        }
+    }
+};
+
+template <int D, bool BF, bool UNI>
 __device__ __forceinline__ void decode_body(const nc_paged_decode_args &a) {
-    constexpr int E = (D + 63) / 64;  // dims of a lane
-    __shared__ float s_o[4][D], s_ml[4][2];
-    const uint32_t r = blockIdx.x / a.num_q_heads, head = blockIdx.x % a.num_q_heads, kh = head / a.group;
-    const uint32_t lane = threadIdx.x & 63u, w = threadIdx.x >> 6;
-    const uint32_t len = nc_paged_cut(a.seq_lens[r], a.max_tokens);
-    const float sc = a.scale * kLog2e;
-    float q[E], acc[E] = {}, m = neg_inf(), l = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const uint32_t c = lane + 64 * e;
-        q[e] = c < D ? to_f32<BF>(a.q[r * a.q_stride + head * a.q_head_stride + c]) : 0.f;
-    }
-    for (uint32_t j = w; j < len; j += 4) {
-        const uint32_t at = nc_paged_quot(j, a.ps);
-        const uint32_t page = (uint32_t)a.table[r * a.table_stride + at];
-        if (page >= a.num_pages) continue;
-        const uint64_t base = page * a.page_stride + kh * a.head_stride + (j - at * a.ps.d) * a.token_stride;
-        float s = 0.f, v[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const uint32_t c = lane + 64 * e;
-            v[e] = c < D ? to_f32<BF>(a.v[base + c]) : 0.f;
-            s += q[e] * (c < D ? to_f32<BF>(a.k[base + c]) : 0.f);
-        }
-#pragma unroll
-        for (int x = 32; x; x >>= 1) s += __shfl_xor(s, x, 64);
-        s *= sc;
-        const float mn = fmaxf(m, s), base_m = mn == neg_inf() ? 0.f : mn;
-        const float alpha = __builtin_amdgcn_exp2f(m - base_m), p = __builtin_amdgcn_exp2f(s - base_m);
-        l = l * alpha + p;
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = acc[e] * alpha + p * v[e];
-        m = mn;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (lane + 64 * e < D) s_o[w][lane + 64 * e] = acc[e];
-    if (lane == 0) {
-        s_ml[w][0] = m;
-        s_ml[w][1] = l;
-    }
-    __syncthreads();
-    if (threadIdx.x < D) {
-        float top = neg_inf(), sum = 0.f, o = 0.f;
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, s_ml[i][0]);
-        if (top == neg_inf()) top = 0.f;
-        for (int i = 0; i < 4; ++i) {
-            const float f = __builtin_amdgcn_exp2f(s_ml[i][0] - top);
-            sum += f * s_ml[i][1];
-            o += f * s_o[i][threadIdx.x];
-        }
-        a.o[r * a.o_stride + head * a.o_head_stride + threadIdx.x] = sum == 0.f ? 0.f : o / sum;
-    }
+    using X = Decode<D, BF, UNI>;
+    __shared__ __attribute__((aligned(16))) float s_o[4][16][X::OP];
+    __shared__ float s_ml[4][16][2];
+    __shared__ uint32_t s_word;
+    const uint32_t lane = threadIdx.x & 63u;
+    X x{a, lane, (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane & 15u, lane >> 4, s_o, s_ml, &s_word};
+    x.run();
 }
 
 }  // namespace
 
-#define NC_DECODE(D, T, BF)                                                                                     \
-    extern "C" __global__ __launch_bounds__(256) void nc_paged_decode_d##D##T(const nc_paged_decode_args a) {    \
-        decode_body<D, BF>(a);                                                                                  \
+// `_odd`: pages of any size; the others take sizes that are multiples of 16.
+#define NC_DECODE(D, T, BF)                                                                                      \
+    extern "C" __global__ __launch_bounds__(256, 3) void nc_paged_decode_d##D##T(const nc_paged_decode_args a) {  \
+        decode_body<D, BF, true>(a);                                                                             \
+    }                                                                                                            \
+    extern "C" __global__ __launch_bounds__(256, 3) void nc_paged_decode_d##D##_odd##T(const nc_paged_decode_args a) { \
+        decode_body<D, BF, false>(a);                                                                            \
     }
 NC_DECODE(16, , false)
 NC_DECODE(32, , false)

@@ -50,17 +50,40 @@ struct nc_paged_append_args {
     nc_paged_div ps, chunks; // page_size, and num_kv_heads * head_dim / 8
 };
 
+// The attention's work, in blocks of this many keys of one request and key head (of 16 of its query heads,
+// where it has more): four waves' tiles.
+NC_HD uint32_t nc_paged_block_keys(uint32_t head_dim) { return head_dim == 16 ? 512u : head_dim == 32 ? 256u : 128u; }
+
+// Workgroup i of n takes blocks [first, first + count) of all of them (n <= blocks), and the one that takes
+// block b.
+struct nc_paged_share {
+    uint32_t first, count;
+};
+NC_HD nc_paged_share nc_paged_share_of(uint32_t i, uint32_t blocks, uint32_t n) {
+    const uint32_t each = blocks / n, more = blocks - each * n;
+    return {i * each + (i < more ? i : more), each + (i < more ? 1u : 0u)};
+}
+NC_HD uint32_t nc_paged_owner_of(uint32_t b, uint32_t blocks, uint32_t n) {
+    const uint32_t each = blocks / n, more = blocks - each * n, big = more * (each + 1u);
+    return b < big ? b / (each + 1u) : more + (b - big) / each;
+}
+
 struct nc_paged_decode_args {
     const uint16_t *q, *k, *v;
     const int32_t *table, *seq_lens;
     float *o;
-    void *workspace;
+    uint32_t *counters; // NC_PAGED_MAX_WGS of them, all 0 between launches
+    float *part_ml;     // per workgroup two pieces of `rows` (max, sum) pairs
+    float *part_o;      // per workgroup two pieces of rows x head_dim sums
     uint64_t table_stride, page_stride, head_stride, token_stride, q_stride, q_head_stride, o_stride, o_head_stride;
     uint32_t num_seqs, num_q_heads, num_kv_heads, group; // group = num_q_heads / num_kv_heads
     uint32_t num_pages, max_tokens;                      // max_tokens = max_pages * page_size
+    uint32_t rows;                                       // query heads of one block: min(group, 16)
+    uint32_t q_vec, o_vec;                               // Q, O rows are 16-byte aligned
     float scale;
     nc_paged_div ps;
 };
+#define NC_PAGED_MAX_WGS 2048u
 
 // A length from device memory, cut to what the table's row can hold.
 NC_HD uint32_t nc_paged_cut(int32_t len, uint32_t most) {
