@@ -20,6 +20,7 @@ constexpr uint64_t kMostElements = 1ull << 60;
 struct Shape {
     nc_paged_options o;
     uint64_t group, cache_len, table_len, q_len, o_len;
+    uint64_t heads, seq_blocks;  // the attention's: key heads (parts of them), and most blocks of a request
 };
 
 uint64_t or_packed(uint64_t stride, uint64_t count, uint64_t inner) { return stride ? stride : count * inner; }
@@ -62,10 +63,11 @@ int resolve(const nc_paged_options *opts, Shape *s) {
                               o.q_stride, o.q_head_stride, o.o_stride, o.o_head_stride};
     for (uint64_t x : given)
         if (x > kMostElements) return NC_ERROR_OVERFLOW;
-    // Workgroups' shares are counted in blocks of at least 128 keys of one request and key head (or 16 of
-    // its query heads), in 32 bits.
-    const uint64_t blocks = (o.page_size * o.max_pages + 127) / 128, heads = o.num_kv_heads * ((s->group + 15) / 16);
-    if (o.num_seqs * heads > kMost31 || blocks > kMost31 / (o.num_seqs * heads)) return NC_ERROR_OVERFLOW;
+    // Workgroups' shares are counted in blocks, in 32 bits.
+    s->heads = o.num_kv_heads * nc_paged_head_parts((uint32_t)s->group);
+    const uint64_t keys = nc_paged_step_keys((uint32_t)o.head_dim) * (4u >> nc_paged_wave_shift((uint32_t)s->group));
+    s->seq_blocks = (o.page_size * o.max_pages + keys - 1) / keys;
+    if (o.num_seqs * s->heads > kMost31 || s->seq_blocks > kMost31 / (o.num_seqs * s->heads)) return NC_ERROR_OVERFLOW;
 
     const uint64_t d = o.head_dim;
     o.table_stride = or_packed(o.table_stride, o.max_pages, 1);
@@ -143,10 +145,8 @@ DecodePlan decode_plan(const Shape &s) {
     const bool uniform = o.page_size % 16 == 0 && o.token_stride < (1ull << 26);
     std::snprintf(p.name, sizeof p.name, "nc_paged_decode_d%u%s%s", (unsigned)o.head_dim, uniform ? "" : "_odd",
                   o.element_type == NC_ELEMENT_BF16 ? "_bf16" : "");
-    const uint64_t keys = nc_paged_block_keys((uint32_t)o.head_dim);
-    const uint64_t blocks = o.num_seqs * o.num_kv_heads * ((s.group + 15) / 16) * ((o.page_size * o.max_pages + keys - 1) / keys);
-    p.grid = (uint32_t)std::min<uint64_t>(blocks, 3 * kCus);
-    p.rows = (uint32_t)std::min<uint64_t>(s.group, 16);
+    p.grid = (uint32_t)std::min<uint64_t>(o.num_seqs * s.heads * s.seq_blocks, 3 * kCus);
+    p.rows = (uint32_t)std::min<uint64_t>(s.group, 64);
     p.piece_ml = NC_PAGED_MAX_WGS * 4;
     p.piece_o = p.piece_ml + (uint64_t)p.grid * 2 * p.rows * 2 * 4;
     p.bytes = p.piece_o + (uint64_t)p.grid * 2 * p.rows * o.head_dim * 4;
@@ -332,6 +332,8 @@ int nc_paged_decode(nc_module module, const uint16_t *q, size_t q_len, const uin
     a.part_ml = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.piece_ml);
     a.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.piece_o);
     a.rows = plan.rows;
+    a.wave_shift = nc_paged_wave_shift(a.rows);
+    a.head_parts = nc_paged_head_parts((uint32_t)s.group);
     a.q_vec = address(q) % 16 == 0 && (op.q_stride | op.q_head_stride) % 8 == 0;
     a.o_vec = address(o) % 16 == 0 && (op.o_stride | op.o_head_stride) % 4 == 0;
     a.table_stride = op.table_stride;

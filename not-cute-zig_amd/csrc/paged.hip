@@ -193,10 +193,11 @@ extern "C" __global__ __launch_bounds__(256) void nc_paged_append_rows_unaligned
 
 // -------------------------------------------------------------------------------------------------
 // Single-token attention. Up to 16 query heads of one key head are the 16 columns of the matrix products, so
-// K and V are read once for all of them. The work is cut into blocks of nc_paged_block_keys() keys, counted
-// over all requests and heads, and every workgroup takes an equal run of them, whatever the lengths: it finds
-// its first by a prefix sum over the requests' lengths. A run that begins or ends inside a request's keys
-// leaves a partial (max, sum, O); the last of a request's workgroups to arrive joins them in order.
+// K and V are read once for all of them; with up to 64, two or four waves of a workgroup take the same keys at
+// the same time, and all but one find them in the caches. The work is cut into blocks, counted over all requests
+// and heads, and every workgroup takes a run of equally many, whatever the lengths: it finds its first by a
+// prefix sum over the requests' lengths. A run that begins or ends inside a request's keys leaves a piece
+// (max, sum, O); the last of a request's workgroups to arrive joins them in order.
 //
 // One wave takes KT x 32 keys of a block at a time. Scores: S = K Q^T with K rows straight from memory as the
 // A operand (lane l: key l%16, dims 8(l/16)..+7 of 32), so lane l holds the scores of query l%16 and keys
@@ -300,7 +301,7 @@ template <int D, bool BF, bool UNI>
 struct Decode {
     static constexpr int KT = D == 16 ? 4 : D == 32 ? 2 : 1;  // 32-key tiles of a wave's step
     static constexpr int NT = 2 * KT;                        // 16-key tiles
-    static constexpr uint32_t WK = 32 * KT, BK = 4 * WK;      // keys of a wave's step, and of a block
+    static constexpr uint32_t WK = 32 * KT;                  // keys of a wave's step: nc_paged_step_keys(D)
     static constexpr int E = D / 16;                         // dims of a lane in V and O
     static constexpr int KK = D < 32 ? 1 : D / 32;           // products of a score
     static constexpr int OP = D + 4;                         // pitch of a row of partial O in LDS
@@ -311,6 +312,7 @@ struct Decode {
 
     const nc_paged_decode_args &a;
     const uint32_t lane, w, c, g;
+    const uint32_t bk;  // keys of a block
     float (*s_o)[16][OP];   // [4]
     float (*s_ml)[16][2];   // [4]
     uint32_t *s_word;
@@ -319,11 +321,14 @@ struct Decode {
     floatx4 acc[E];
     float m, l;
 
-    static __device__ __forceinline__ uint32_t blocks_of(uint32_t len) { return (len + BK - 1) / BK; }
+    // bk = WK * 2^(2 - wave_shift)
+    __device__ __forceinline__ uint32_t blocks_of(uint32_t len) const {
+        return (len + bk - 1) >> (__builtin_ctz(WK) + 2 - a.wave_shift);
+    }
 
     // Q of the block's query heads as the B operand: lane (c, g) holds query c, dims 8g.. (4g.. for D = 16).
-    __device__ __forceinline__ void load_q(uint32_t r, uint32_t head0, uint32_t rows) {
-        const uint16_t *p = a.q + r * a.q_stride + (head0 + min(c, rows - 1u)) * a.q_head_stride;
+    __device__ __forceinline__ void load_q(uint32_t r, uint32_t head0, uint32_t row, uint32_t rows) {
+        const uint16_t *p = a.q + r * a.q_stride + (head0 + min(row + c, rows - 1u)) * a.q_head_stride;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
             constexpr int N = D == 16 ? 4 : 8;
@@ -484,31 +489,74 @@ struct Decode {
         }
     }
 
-    // The pieces of workgroups first..last of one request and head: added in order, so that it does not matter
-    // who came last, and written to O.
+    // The pieces of workgroups first..last of one request and head: added in an order that does not depend on who
+    // came last, and written to O. Four columns of a row are a thread's; where that leaves threads over, groups of
+    // them take every so many-th piece and are added up through LDS. PF pieces are on their way at a time.
+    template <int PF>
     __device__ __forceinline__ void join_pieces(uint32_t first, uint32_t last, uint32_t rows, float *o) {
-        const uint32_t items = rows * (D / 4);
-        for (uint32_t it = threadIdx.x; it < items; it += 256) {
+        const uint32_t items = rows * (D / 4), groups = items > 128 ? 1u : 256u / items;
+        floatx4 *s_sum = reinterpret_cast<floatx4 *>(&s_o[0][0][0]);  // one per thread, and behind them (max, sum)
+        float *s_stat = reinterpret_cast<float *>(s_sum + 256);
+        for (uint32_t i0 = 0; i0 < items; i0 += 256) {
+            const uint32_t grp = groups == 1 ? 0u : threadIdx.x / items, it = groups == 1 ? i0 + threadIdx.x : threadIdx.x - grp * items;
+            const bool mine = it < items && grp < groups;
             const uint32_t q = it / (D / 4), x = 4 * (it % (D / 4));
             float top = neg_inf(), sum = 0.f;
             floatx4 out = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-            for (uint32_t i = first; i <= last; ++i) {
-                const uint64_t piece = (uint64_t)i * 2 + (i == first) , at = piece * a.rows + q;
-                float pm, pl;
-                floatx4 po;
-                get2(a.part_ml + 2 * at, pm, pl);
-                float p0, p1, p2, p3;
-                get2(a.part_o + at * D + x, p0, p1);
-                get2(a.part_o + at * D + x + 2, p2, p3);
-                po = {p0, p1, p2, p3};
-                const float t = fmaxf(top, pm), f = __builtin_amdgcn_exp2f(top - finite_or_0(t)),
-                            h = __builtin_amdgcn_exp2f(pm - finite_or_0(t));
-                sum = sum * f + pl * h;
-                out = out * f + po * h;
-                top = t;
+            if (mine) {
+                for (uint32_t i = first + grp; i <= last; i += PF * groups) {
+                    float pm[PF], pl[PF];
+                    floatx4 po[PF];
+#pragma unroll
+                    for (int n = 0; n < PF; ++n) {
+                        const uint32_t j = min(i + n * groups, last);
+                        const uint64_t at = ((uint64_t)j * 2 + (j == first)) * a.rows + q;
+                        float p0, p1, p2, p3;
+                        get2(a.part_ml + 2 * at, pm[n], pl[n]);
+                        get2(a.part_o + at * D + x, p0, p1);
+                        get2(a.part_o + at * D + x + 2, p2, p3);
+                        po[n] = floatx4{p0, p1, p2, p3};
+                    }
+                    float t = top;
+#pragma unroll
+                    for (int n = 0; n < PF; ++n) {
+                        if (i + n * groups > last) pm[n] = neg_inf();
+                        t = fmaxf(t, pm[n]);
+                    }
+                    const float ref = finite_or_0(t), f = __builtin_amdgcn_exp2f(top - ref);
+                    sum *= f;
+                    out *= f;
+#pragma unroll
+                    for (int n = 0; n < PF; ++n) {
+                        if (i + n * groups <= last) {
+                            const float h = __builtin_amdgcn_exp2f(pm[n] - ref);
+                            sum += pl[n] * h;
+                            out += po[n] * h;
+                        }
+                    }
+                    top = t;
+                }
             }
-            store_o(o, q, x, out, sum);
+            if (groups > 1) {
+                s_sum[threadIdx.x] = out;
+                s_stat[2 * threadIdx.x] = top;
+                s_stat[2 * threadIdx.x + 1] = sum;
+                __syncthreads();
+                if (mine && grp == 0) {
+                    float t = top;
+                    for (uint32_t n = 1; n < groups; ++n) t = fmaxf(t, s_stat[2 * (threadIdx.x + n * items)]);
+                    const float ref = finite_or_0(t), f = __builtin_amdgcn_exp2f(top - ref);
+                    sum *= f;
+                    out *= f;
+                    for (uint32_t n = 1; n < groups; ++n) {
+                        const uint32_t y = threadIdx.x + n * items;
+                        const float h = __builtin_amdgcn_exp2f(s_stat[2 * y] - ref);
+                        sum += s_stat[2 * y + 1] * h;
+                        out += s_sum[y] * h;
+                    }
+                }
+            }
+            if (mine && grp == 0) store_o(o, q, x, out, sum);
         }
     }
 
@@ -525,14 +573,14 @@ struct Decode {
     }
 
     // The four waves' (m, l, O) of one run of blocks: to O if the run is all of the request's, else to this
-    // workgroup's piece, and the last workgroup joins. n workgroups share `blocks` blocks.
+    // workgroup's (i's) piece, and the last of workgroups first..last to arrive joins them.
     __device__ __forceinline__ void finish(uint32_t rows, float *o, bool whole, uint32_t i, uint32_t first, uint32_t last) {
         const float sum = quad_sum(l);
         if (g == 0) {
             s_ml[w][c][0] = m;
             s_ml[w][c][1] = sum;
         }
-        if (c < rows) {
+        if (16 * (w & ((1u << a.wave_shift) - 1u)) + c < rows) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -542,15 +590,14 @@ struct Decode {
         const uint32_t items = rows * (D / 4);
         for (uint32_t it = threadIdx.x; it < items; it += 256) {
             const uint32_t q = it / (D / 4), x = 4 * (it % (D / 4));
+            const uint32_t q16 = q & 15u, by = 1u << a.wave_shift;  // waves q / 16, + by, ... hold query q
             float top = neg_inf(), lsum = 0.f;
-#pragma unroll
-            for (int n = 0; n < 4; ++n) top = fmaxf(top, s_ml[n][q][0]);
+            for (uint32_t n = q >> 4; n < 4; n += by) top = fmaxf(top, s_ml[n][q16][0]);
             floatx4 out = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const float f = __builtin_amdgcn_exp2f(s_ml[n][q][0] - finite_or_0(top));
-                lsum += f * s_ml[n][q][1];
-                out += f * *reinterpret_cast<const floatx4 *>(&s_o[n][q][x]);
+            for (uint32_t n = q >> 4; n < 4; n += by) {
+                const float f = __builtin_amdgcn_exp2f(s_ml[n][q16][0] - finite_or_0(top));
+                lsum += f * s_ml[n][q16][1];
+                out += f * *reinterpret_cast<const floatx4 *>(&s_o[n][q16][x]);
             }
             if (whole) {
                 store_o(o, q, x, out, lsum);
@@ -570,7 +617,13 @@ struct Decode {
                 *s_word = __hip_atomic_fetch_add(a.counters + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __syncthreads();
             if (*s_word == last - first) {
-                join_pieces(first, last, rows, o);
+                const uint32_t pieces = (last - first + 1) * min(rows * (D / 4), 256u);  // a thread's, times 256
+                if (pieces <= 2 * 256)
+                    join_pieces<2>(first, last, rows, o);
+                else if (pieces <= 4 * 256)
+                    join_pieces<4>(first, last, rows, o);
+                else
+                    join_pieces<8>(first, last, rows, o);
                 if (threadIdx.x == 0) __hip_atomic_store(a.counters + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
         }
@@ -579,7 +632,8 @@ struct Decode {
 
     __device__ __forceinline__ void run() {
         const uint32_t R = a.num_seqs, per = (R + 63u) / 64u;  // requests of a lane
-        const uint32_t qgroups = (a.group + 15u) / 16u, heads = a.num_kv_heads * qgroups;
+        const uint32_t heads = a.num_kv_heads * a.head_parts;
+        const uint32_t qt = w & ((1u << a.wave_shift) - 1u), kw = w >> a.wave_shift;  // query heads' and keys' part
         const uint32_t zero_r = blockIdx.x;
         const int32_t zero_len = zero_r < R ? as_const(a.seq_lens)[zero_r] : 1;
         uint32_t mine = 0, len0 = 0;
@@ -591,11 +645,11 @@ struct Decode {
             }
         }
         const uint32_t incl = wave_scan32(mine);
-        const uint32_t blocks = __builtin_amdgcn_readlane(incl, 63) * heads, n = min(gridDim.x, blocks), i = blockIdx.x;
-        if (i < n) {
-            const nc_paged_share share = nc_paged_share_of(i, blocks, n);
-            uint32_t b = share.first;
-            const uint32_t end = share.first + share.count;
+        const uint32_t blocks = __builtin_amdgcn_readlane(incl, 63) * heads, i = blockIdx.x;
+        const uint32_t each = nc_paged_each(blocks, gridDim.x);
+        uint32_t b = i * each;
+        if (b < blocks) {
+            const uint32_t end = min(b + each, blocks);
             Place at;
             {
                 const uint32_t t = b / heads;  // the same request's block if it had one head
@@ -624,24 +678,24 @@ struct Decode {
             uint32_t head = (b - at.pre * heads) / nb, b0 = b - at.pre * heads - head * nb;
             while (true) {
                 const uint32_t b1 = min(nb, b0 + (end - b));
-                const uint32_t kvh = head / qgroups, qg = head - kvh * qgroups;
-                const uint32_t rows = min(16u, a.group - 16u * qg), head0 = kvh * a.group + 16u * qg;
-                load_q(at.r, head0, rows);
+                const uint32_t kvh = head / a.head_parts, part = head - kvh * a.head_parts;
+                const uint32_t rows = min(64u, a.group - 64u * part), head0 = kvh * a.group + 64u * part;
+                load_q(at.r, head0, 16u * qt, rows);
                 m = neg_inf();
                 l = 0.f;
 #pragma unroll
                 for (int x = 0; x < E; ++x) acc[x] = floatx4{0.f, 0.f, 0.f, 0.f};
-                uint32_t k0 = b0 * BK + w * WK;
-                const uint32_t k1 = min(b1 * BK, at.len);
+                uint32_t k0 = b0 * bk + kw * WK;
+                const uint32_t k1 = min(b1 * bk, at.len);
                 const uint64_t row = at.r * a.table_stride;
                 if (k0 < k1) {
                     uint32_t e[NT];
                     load_pages(e, row, k0, at.len);
                     while (true) {
                         uint32_t next[NT];
-                        load_pages(next, row, k0 + BK, at.len);
+                        load_pages(next, row, k0 + bk, at.len);
                         step(e, k0, at.len, kvh);
-                        k0 += BK;
+                        k0 += bk;
                         if (k0 >= k1) break;
 #pragma unroll
                         for (int t = 0; t < NT; ++t) e[t] = next[t];
@@ -649,8 +703,7 @@ struct Decode {
                 }
                 const uint32_t seg = at.pre * heads + head * nb;  // the request's and head's first block
                 const bool whole = b0 == 0 && b1 == nb;
-                finish(rows, a.o + at.r * a.o_stride + head0 * a.o_head_stride, whole, i,
-                       whole ? i : nc_paged_owner_of(seg, blocks, n), whole ? i : nc_paged_owner_of(seg + nb - 1, blocks, n));
+                finish(rows, a.o + at.r * a.o_stride + head0 * a.o_head_stride, whole, i, seg / each, (seg + nb - 1) / each);
                 b += b1 - b0;
                 if (b >= end) break;
                 b0 = 0;
@@ -679,11 +732,13 @@ struct Decode {
 template <int D, bool BF, bool UNI>
 __device__ __forceinline__ void decode_body(const nc_paged_decode_args &a) {
     using X = Decode<D, BF, UNI>;
-    __shared__ __attribute__((aligned(16))) float s_o[4][16][X::OP];
+    // the waves' O, or the join's 256 x (4 columns, max, sum)
+    __shared__ __attribute__((aligned(16))) float s_mem[4 * 16 * X::OP > 256 * 6 ? 4 * 16 * X::OP : 256 * 6];
     __shared__ float s_ml[4][16][2];
     __shared__ uint32_t s_word;
     const uint32_t lane = threadIdx.x & 63u;
-    X x{a, lane, (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane & 15u, lane >> 4, s_o, s_ml, &s_word};
+    X x{a, lane, (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane & 15u, lane >> 4, X::WK * (4u >> a.wave_shift),
+        reinterpret_cast<float (*)[16][X::OP]>(s_mem), s_ml, &s_word};
     x.run();
 }
 

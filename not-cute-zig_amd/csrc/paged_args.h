@@ -50,23 +50,16 @@ struct nc_paged_append_args {
     nc_paged_div ps, chunks; // page_size, and num_kv_heads * head_dim / 8
 };
 
-// The attention's work, in blocks of this many keys of one request and key head (of 16 of its query heads,
-// where it has more): four waves' tiles.
-NC_HD uint32_t nc_paged_block_keys(uint32_t head_dim) { return head_dim == 16 ? 512u : head_dim == 32 ? 256u : 128u; }
+// The attention's work is counted in blocks: the keys of one request and key head that a workgroup's four waves
+// take in a step. A wave takes step_keys of them for 16 query heads; where a key head has more than 16, two or
+// four waves take the same keys for 16 heads each (wave_shift 1 or 2), and past 64 the workgroup's heads count
+// as another head.
+NC_HD uint32_t nc_paged_step_keys(uint32_t head_dim) { return head_dim == 16 ? 128u : head_dim == 32 ? 64u : 32u; }
+NC_HD uint32_t nc_paged_wave_shift(uint32_t group) { return group <= 16 ? 0u : group <= 32 ? 1u : 2u; }
+NC_HD uint32_t nc_paged_head_parts(uint32_t group) { return (group + 63u) / 64u; }
 
-// Workgroup i of n takes blocks [first, first + count) of all of them (n <= blocks), and the one that takes
-// block b.
-struct nc_paged_share {
-    uint32_t first, count;
-};
-NC_HD nc_paged_share nc_paged_share_of(uint32_t i, uint32_t blocks, uint32_t n) {
-    const uint32_t each = blocks / n, more = blocks - each * n;
-    return {i * each + (i < more ? i : more), each + (i < more ? 1u : 0u)};
-}
-NC_HD uint32_t nc_paged_owner_of(uint32_t b, uint32_t blocks, uint32_t n) {
-    const uint32_t each = blocks / n, more = blocks - each * n, big = more * (each + 1u);
-    return b < big ? b / (each + 1u) : more + (b - big) / each;
-}
+// Workgroup i takes blocks [i * each, (i + 1) * each) of all; `each` is the least that `most` workgroups can do with.
+NC_HD uint32_t nc_paged_each(uint32_t blocks, uint32_t most) { return (blocks + most - 1u) / most; }
 
 struct nc_paged_decode_args {
     const uint16_t *q, *k, *v;
@@ -78,7 +71,8 @@ struct nc_paged_decode_args {
     uint64_t table_stride, page_stride, head_stride, token_stride, q_stride, q_head_stride, o_stride, o_head_stride;
     uint32_t num_seqs, num_q_heads, num_kv_heads, group; // group = num_q_heads / num_kv_heads
     uint32_t num_pages, max_tokens;                      // max_tokens = max_pages * page_size
-    uint32_t rows;                                       // query heads of one block: min(group, 16)
+    uint32_t rows;                                       // query heads of a piece: min(group, 64)
+    uint32_t wave_shift, head_parts;
     uint32_t q_vec, o_vec;                               // Q, O rows are 16-byte aligned
     float scale;
     nc_paged_div ps;

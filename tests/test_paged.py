@@ -282,19 +282,16 @@ int main() {
             if (nc_paged_quot(n, v) != n / d) { std::printf("%u / %u\n", n, d); return 1; }
         }
     }
-    // every block has one owner, the owners' shares are runs in order and differ by at most one block
+    // shares of nc_paged_each() cover all blocks with no more workgroups than there are, none of them idle
     for (int k = 0; k < 20000; ++k) {
         x ^= x << 13; x ^= x >> 7; x ^= x << 17;
         const uint32_t blocks = k % 2 ? (uint32_t)(x % 5000) + 1 : (uint32_t)(x % most) + 1;
-        const uint32_t n = (uint32_t)((x >> 32) % (blocks < 2048 ? blocks : 2048)) + 1;
-        uint32_t at = 0;
-        for (uint32_t i = 0; i < n; ++i) {
-            const nc_paged_share s = nc_paged_share_of(i, blocks, n);
-            if (s.first != at || s.count < blocks / n || s.count > blocks / n + 1) return 3;
-            if (nc_paged_owner_of(s.first, blocks, n) != i || nc_paged_owner_of(s.first + s.count - 1, blocks, n) != i) return 4;
-            at += s.count;
-        }
-        if (at != blocks) return 5;
+        const uint32_t n = (uint32_t)((x >> 32) % 2048) + 1, each = nc_paged_each(blocks, n);
+        if (each == 0 || (uint64_t)each * n < blocks || (each > 1 && (uint64_t)(each - 1) * n >= blocks)) return 3;
+    }
+    for (uint32_t g = 1; g < 300; ++g) {  // the waves' and parts' query heads cover the group, 16 a wave
+        const uint32_t rows = g < 64 ? g : 64, sh = nc_paged_wave_shift(rows);
+        if ((16u << sh) < rows || (sh && (8u << sh) >= rows) || nc_paged_head_parts(g) * 64 < g || (nc_paged_head_parts(g) - 1) * 64 >= g) return 4;
     }
     if (nc_paged_cut(-1, 5) != 0 || nc_paged_cut(INT32_MIN, 5) != 0 || nc_paged_cut(4, 5) != 4 ||
         nc_paged_cut(INT32_MAX, 5) != 5) return 2;
