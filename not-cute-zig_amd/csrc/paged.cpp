@@ -14,13 +14,14 @@ extern "C" int nc_internal_fail(int status, const char *what);
 namespace {
 
 constexpr uint64_t kMost31 = 0x7fffffffull;
+constexpr uint64_t kMostUnits = 1ull << 30;
 constexpr uint64_t kMostElements = 1ull << 60;
 
 // The options with every stride resolved.
 struct Shape {
     nc_paged_options o;
     uint64_t group, cache_len, table_len, q_len, o_len;
-    uint64_t heads, seq_blocks;  // the attention's: key heads (parts of them), and most blocks of a request
+    uint64_t heads, seq_units;  // the attention's: key heads (parts of them), and most units of a head
 };
 
 uint64_t or_packed(uint64_t stride, uint64_t count, uint64_t inner) { return stride ? stride : count * inner; }
@@ -63,11 +64,11 @@ int resolve(const nc_paged_options *opts, Shape *s) {
                               o.q_stride, o.q_head_stride, o.o_stride, o.o_head_stride};
     for (uint64_t x : given)
         if (x > kMostElements) return NC_ERROR_OVERFLOW;
-    // Workgroups' shares are counted in blocks, in 32 bits.
+    // Workgroups' shares are counted in units, in 32 bits.
     s->heads = o.num_kv_heads * nc_paged_head_parts((uint32_t)s->group);
-    const uint64_t keys = nc_paged_step_keys((uint32_t)o.head_dim) * (4u >> nc_paged_wave_shift((uint32_t)s->group));
-    s->seq_blocks = (o.page_size * o.max_pages + keys - 1) / keys;
-    if (o.num_seqs * s->heads > kMost31 || s->seq_blocks > kMost31 / (o.num_seqs * s->heads)) return NC_ERROR_OVERFLOW;
+    const uint64_t keys = nc_paged_step_keys((uint32_t)o.head_dim) * (NC_PAGED_WAVES >> nc_paged_wave_shift((uint32_t)s->group));
+    s->seq_units = (o.page_size * o.max_pages + keys - 1) / keys + NC_PAGED_HEAD_UNITS;
+    if (o.num_seqs * s->heads > kMostUnits || s->seq_units > kMostUnits / (o.num_seqs * s->heads)) return NC_ERROR_OVERFLOW;
 
     const uint64_t d = o.head_dim;
     o.table_stride = or_packed(o.table_stride, o.max_pages, 1);
@@ -132,20 +133,22 @@ int launch(nc_module module, const char *name, uint32_t grid, uint32_t threads, 
 // The attention's kernel, grid and workspace for a set of options.
 struct DecodePlan {
     char name[40];
-    uint32_t grid, rows;
+    uint32_t grid, rows, long_log2, short_log2;
     uint64_t piece_ml, piece_o, bytes;  // offsets of the partials, and all of the workspace
 };
 
-constexpr uint32_t kCus = 256;  // MI355X
+constexpr uint32_t kCusLog2 = 8;  // MI355X: 256 CUs
 
 DecodePlan decode_plan(const Shape &s) {
     const nc_paged_options &o = s.o;
     DecodePlan p;
-    // A 16-key tile lies in one page, and its rows' offsets fit 32 bits.
-    const bool uniform = o.page_size % 16 == 0 && o.token_stride < (1ull << 26);
+    // A 16-key tile lies in one page, and a page's byte offsets fit 32 bits.
+    const bool uniform = o.page_size % 16 == 0 && o.page_stride < (1ull << 31) && o.page_size * o.token_stride < (1ull << 30);
     std::snprintf(p.name, sizeof p.name, "nc_paged_decode_d%u%s%s", (unsigned)o.head_dim, uniform ? "" : "_odd",
                   o.element_type == NC_ELEMENT_BF16 ? "_bf16" : "");
-    p.grid = (uint32_t)std::min<uint64_t>(o.num_seqs * s.heads * s.seq_blocks, 3 * kCus);
+    p.long_log2 = kCusLog2;
+    p.short_log2 = kCusLog2 + 1;
+    p.grid = (uint32_t)std::min<uint64_t>(o.num_seqs * s.heads * s.seq_units, 1u << p.short_log2);
     p.rows = (uint32_t)std::min<uint64_t>(s.group, 64);
     p.piece_ml = NC_PAGED_MAX_WGS * 4;
     p.piece_o = p.piece_ml + (uint64_t)p.grid * 2 * p.rows * 2 * 4;
@@ -332,8 +335,14 @@ int nc_paged_decode(nc_module module, const uint16_t *q, size_t q_len, const uin
     a.part_ml = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.piece_ml);
     a.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.piece_o);
     a.rows = plan.rows;
+    a.long_log2 = plan.long_log2;
+    a.short_log2 = plan.short_log2;
+    a.heads = nc_paged_make_div((uint32_t)s.heads);
     a.wave_shift = nc_paged_wave_shift(a.rows);
     a.head_parts = nc_paged_head_parts((uint32_t)s.group);
+    // A piece is written and read once more: at most a quarter of what its run reads of the cache.
+    const uint32_t block_keys = nc_paged_step_keys((uint32_t)op.head_dim) * (NC_PAGED_WAVES >> a.wave_shift);
+    a.each_least = std::max(1u, 8 * a.rows / block_keys);
     a.q_vec = address(q) % 16 == 0 && (op.q_stride | op.q_head_stride) % 8 == 0;
     a.o_vec = address(o) % 16 == 0 && (op.o_stride | op.o_head_stride) % 4 == 0;
     a.table_stride = op.table_stride;
@@ -352,7 +361,7 @@ int nc_paged_decode(nc_module module, const uint16_t *q, size_t q_len, const uin
     a.max_tokens = (uint32_t)(op.max_pages * op.page_size);
     a.scale = op.scale;
     a.ps = nc_paged_make_div((uint32_t)op.page_size);
-    return launch(module, plan.name, plan.grid, 256, &a, stream);
+    return launch(module, plan.name, plan.grid, 64 * NC_PAGED_WAVES, &a, stream);
 }
 
 }  // extern "C"

@@ -242,9 +242,10 @@ template <bool BF>
 __device__ __forceinline__ uint32_t take_pair(float &x, float &y) {
     if constexpr (BF) {
         const bf16x2 h = {(__bf16)x, (__bf16)y};
-        x -= (float)h[0];
-        y -= (float)h[1];
-        return __builtin_bit_cast(uint32_t, h);
+        const uint32_t u = __builtin_bit_cast(uint32_t, h);
+        x -= __uint_as_float(u << 16);
+        y -= __uint_as_float(u & 0xffff0000u);
+        return u;
     } else {
         const half2v h = {(_Float16)x, (_Float16)y};
         x -= (float)h[0];
@@ -289,52 +290,83 @@ __device__ __forceinline__ void get2(const float *p, float &x, float &y) {
     y = __uint_as_float((uint32_t)(v >> 32));
 }
 
-__device__ __forceinline__ float finite_or_0(float m) { return m == neg_inf() ? 0.f : m; }
+// The argument block where the launch put it. again() hides that it is the same one, so that what only a head's
+// beginning or end needs is read there once more and does not stay in scalar registers: a few dozen too many of
+// them were written to and read back from a vector register in every step.
+typedef const __attribute__((address_space(4))) nc_paged_decode_args *Args;
+__device__ __forceinline__ Args again(Args p) {
+    asm volatile("" : "+s"(p));
+    return p;
+}
 
-// Which keys a workgroup is at: request r of length len, whose blocks begin behind `pre` blocks of the
-// requests before it.
-struct Place {
-    uint32_t r, len, pre;
-};
+__device__ __forceinline__ float finite_or_0(float m) { return m == neg_inf() ? 0.f : m; }
 
 template <int D, bool BF, bool UNI>
 struct Decode {
-    static constexpr int KT = D == 16 ? 4 : D == 32 ? 2 : 1;  // 32-key tiles of a wave's step
-    static constexpr int NT = 2 * KT;                        // 16-key tiles
-    static constexpr uint32_t WK = 32 * KT;                  // keys of a wave's step: nc_paged_step_keys(D)
-    static constexpr int E = D / 16;                         // dims of a lane in V and O
-    static constexpr int KK = D < 32 ? 1 : D / 32;           // products of a score
-    static constexpr int OP = D + 4;                         // pitch of a row of partial O in LDS
+    static constexpr int KT = D <= 32 ? 2 : 1;  // 32-key tiles of a wave's step
+    static constexpr int NT = 2 * KT;           // 16-key tiles
+    static constexpr uint32_t WK = 32 * KT;     // keys of a wave's step: nc_paged_step_keys(D)
+    static constexpr int E = D / 16;            // dims of a lane in V and O
+    static constexpr int KK = D < 32 ? 1 : D / 32;  // products of a score
+    static constexpr int KE = D == 16 ? 4 : 8;  // dims of a lane in one product
+    static constexpr int OP = D + 4;            // pitch of a row of partial O in LDS
+    static constexpr uint32_t NW = NC_PAGED_WAVES, THREADS = 64 * NW;
     // Weights are 2^(SHIFT + score - max): in f16 the low part of a small weight stays a normal number, in bf16
     // a sum of a million V at the type's largest value stays finite.
     static constexpr float SHIFT = BF ? -16.f : 12.f;
     using KReg = typename std::conditional<D == 16, u32x2, u32x4>::type;
+    using VReg = typename std::conditional<E == 8, u32x4, typename std::conditional<E == 4, u32x2, uint32_t>::type>::type;
 
-    const nc_paged_decode_args &a;
+    // K and V of a wave's step, on their way or there, and which keys count: the first seen[t] of a tile, or
+    // (pages of any size) those whose bits are set in it.
+    struct Step {
+        KReg k[NT][KK];
+        VReg v[NT][4];
+        uint32_t seen[NT];
+    };
+    struct Pages {
+        uint32_t e[NT];
+    };
+    // One request's table row and one key head of the pools. Off: a page fits 32 bits where a tile lies in one.
+    using Off = typename std::conditional<UNI, uint32_t, uint64_t>::type;
+    struct Cache {
+        const int32_t *table;
+        const uint16_t *k, *v;
+        Off page_stride, token_stride;
+        uint32_t num_pages;
+        nc_paged_div ps;
+    };
+
+    const Args args;
     const uint32_t lane, w, c, g;
-    const uint32_t bk;  // keys of a block
-    float (*s_o)[16][OP];   // [4]
-    float (*s_ml)[16][2];   // [4]
+    const uint32_t wave_shift;
+    const uint32_t bk;       // keys of a block
+    const uint32_t qt, kw;   // this wave's part of the query heads, and of a block's keys
+    float (*s_o)[16][OP];    // [NW]
+    float (*s_ml)[16][2];    // [NW]
     uint32_t *s_word;
 
+    uint32_t kat, vat[4];    // byte offsets of the lane's K and V in a tile
+    float sc;                // scale * log2(e)
     u32x4 qv[KK];
     floatx4 acc[E];
     float m, l;
 
-    // bk = WK * 2^(2 - wave_shift)
+    // bk = WK * (NW >> wave_shift)
     __device__ __forceinline__ uint32_t blocks_of(uint32_t len) const {
-        return (len + bk - 1) >> (__builtin_ctz(WK) + 2 - a.wave_shift);
+        return (len + bk - 1) >> (__builtin_ctz(WK * NW) - wave_shift);
     }
+    static __device__ __forceinline__ uint32_t units_of(uint32_t nb) { return nb ? nb + NC_PAGED_HEAD_UNITS : 0u; }
 
-    // Q of the block's query heads as the B operand: lane (c, g) holds query c, dims 8g.. (4g.. for D = 16).
-    __device__ __forceinline__ void load_q(uint32_t r, uint32_t head0, uint32_t row, uint32_t rows) {
-        const uint16_t *p = a.q + r * a.q_stride + (head0 + min(row + c, rows - 1u)) * a.q_head_stride;
+    // Q of a block's query heads as the B operand: lane (c, g) holds query c of the wave's 16, dims KE*g.. of 32.
+    __device__ __forceinline__ void load_q(uint32_t r, uint32_t head0, uint32_t rows) {
+        const Args a = again(args);
+        const uint16_t *p = a->q + r * a->q_stride + (head0 + min(16u * qt + c, rows - 1u)) * a->q_head_stride;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
-            constexpr int N = D == 16 ? 4 : 8;
-            const uint16_t *x = p + 32 * kk + N * g;
+            const uint16_t *x = p + 32 * kk + KE * g;
             u32x4 t = {0u, 0u, 0u, 0u};
-            if (a.q_vec) {
+            if (a->q_vec) {
                 if constexpr (D == 16) {
                     const u32x2 y = *reinterpret_cast<const u32x2 *>(x);
                     t[0] = y[0];
@@ -344,7 +376,7 @@ struct Decode {
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < N / 2; ++i) t[i] = uint32_t(x[2 * i]) | uint32_t(x[2 * i + 1]) << 16;
+                for (int i = 0; i < KE / 2; ++i) t[i] = uint32_t(x[2 * i]) | uint32_t(x[2 * i + 1]) << 16;
             }
             qv[kk] = t;
         }
@@ -352,99 +384,134 @@ struct Decode {
 
     // Table entries of a step's 16-key tiles: uniform where a tile lies in one page, else one per lane (key c
     // of the tile). Past the request's end the last key's entry.
-    __device__ __forceinline__ void load_pages(uint32_t (&e)[NT], uint64_t row, uint32_t k0, uint32_t len) {
+    __device__ __forceinline__ Pages load_pages(const Cache &a, uint32_t k0, uint32_t len) const {
+        Pages p;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             if constexpr (UNI)
-                e[t] = (uint32_t)as_const(a.table)[row + nc_paged_quot(min(k0 + 16 * t, len - 1u), a.ps)];
+                p.e[t] = (uint32_t)as_const(a.table)[nc_paged_quot(min(k0 + 16 * t, len - 1u), a.ps)];
             else
-                e[t] = (uint32_t)a.table[row + nc_paged_quot(min(k0 + 16 * t + c, len - 1u), a.ps)];
+                p.e[t] = (uint32_t)a.table[nc_paged_quot(min(k0 + 16 * t + c, len - 1u), a.ps)];
         }
+        return p;
     }
 
-    // One step: the keys k0..k0+WK-1 of a request of length len, k0 < len, on the pages e.
-    __device__ __forceinline__ void step(const uint32_t (&e)[NT], uint32_t k0, uint32_t len, uint32_t kvh) {
-        KReg kr[NT][KK];
-        u32x4 vr[NT][4];  // E dims in the first E/2 dwords (D = 16: half of one)
-        uint32_t seen[NT];  // bit i: key i of the tile counts
-        const uint16_t *kh = a.k + kvh * a.head_stride, *vh = a.v + kvh * a.head_stride;
-        const uint16_t *vb[NT][4];
-        auto load_k = [&](int t, const uint16_t *p) {
+    // Sets the loads of the keys k0..k0+WK-1 of one key head under way, those below `end`.
+    // UNI: a tile is a buffer of its own whose length ends with its last key that counts, so that what lies
+    // behind is neither read nor waited for, and is 0. Else rows that do not count read the pool's first row.
+    __device__ __forceinline__ void issue(Step &st, const Cache &a, const Pages &pages, uint32_t k0, uint32_t end) const {
+        if constexpr (UNI) {
+            const uint32_t ts = 2u * a.token_stride;
+            __amdgpu_buffer_rsrc_t vb[NT];
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) kr[t][kk] = *reinterpret_cast<const KReg *>(p + 32 * kk);
-        };
+            for (int t = 0; t < NT; ++t) {
+                const uint32_t k1 = k0 + 16 * t;
+                const bool in = k1 < end && pages.e[t] < a.num_pages;
+                const uint32_t n = in ? min(end - k1, 16u) : 0u;
+                st.seen[t] = n;
+                const uint32_t tok = k1 - nc_paged_quot(k1, a.ps) * a.ps.d;
+                const uint64_t at = in ? (uint64_t)pages.e[t] * a.page_stride + tok * a.token_stride : 0u;
+                const __amdgpu_buffer_rsrc_t kb = tile(a.k + at, n * ts);
+                vb[t] = tile(a.v + at, n * ts);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const uint32_t k1 = k0 + 16 * t;
-            if constexpr (UNI) {
-                // A tile without keys, or on a page outside the pool, reads the pool's page 0 and counts for nothing.
-                const bool in = k1 < len && e[t] < a.num_pages;
-                seen[t] = in ? (k1 + 16 <= len ? 0xffffu : (1u << (len - k1)) - 1u) : 0u;
-                const uint32_t ka = min(k1, (len - 1u) & ~15u);  // below 2^31
-                const uint64_t at = (in ? e[t] : 0u) * a.page_stride + (ka - nc_paged_quot(ka, a.ps) * a.ps.d) * a.token_stride;
-                const uint32_t ts = (uint32_t)a.token_stride;
-                load_k(t, kh + at + (c * ts + (D == 16 ? 4 : 8) * g));
+                for (int kk = 0; kk < KK; ++kk) {
+                    if constexpr (D == 16)
+                        st.k[t][kk] = __builtin_amdgcn_raw_buffer_load_b64(kb, kat, 0, 0);
+                    else
+                        st.k[t][kk] = __builtin_amdgcn_raw_buffer_load_b128(kb, kat + 64 * kk, 0, 0);
+                }
+            }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) vb[t][i] = vh + at + ((4 * g + i) * ts + E * c);
-            } else {
-                const uint32_t key = min(k1 + c, len - 1u);
-                const bool in = k1 + c < len && e[t] < a.num_pages;
-                seen[t] = (uint32_t)__ballot(in) & 0xffffu;
-                const uint64_t at = (in ? e[t] : 0u) * a.page_stride + (key - nc_paged_quot(key, a.ps) * a.ps.d) * a.token_stride;
-                load_k(t, kh + at + (D == 16 ? 4 : 8) * g);
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (E == 8)
+                        st.v[t][i] = __builtin_amdgcn_raw_buffer_load_b128(vb[t], vat[i], 0, 0);
+                    else if constexpr (E == 4)
+                        st.v[t][i] = __builtin_amdgcn_raw_buffer_load_b64(vb[t], vat[i], 0, 0);
+                    else if constexpr (E == 2)
+                        st.v[t][i] = __builtin_amdgcn_raw_buffer_load_b32(vb[t], vat[i], 0, 0);
+                    else
+                        st.v[t][i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vb[t], vat[i], 0, 0);
+                }
+        } else {
+            const uint16_t *vb[NT][4];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const uint32_t key = k0 + 16 * t + c;
+                const bool in = key < end && pages.e[t] < a.num_pages;
+                st.seen[t] = (uint32_t)__ballot(in) & 0xffffu;
+                const uint64_t at = in ? pages.e[t] * a.page_stride + (key - nc_paged_quot(key, a.ps) * a.ps.d) * a.token_stride : 0u;
+                const uint16_t *kp = a.k + at + KE * g;
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) st.k[t][kk] = *reinterpret_cast<const KReg *>(kp + 32 * kk);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int from = 4 * (int)g + i;
                     const uint32_t lo = __shfl((uint32_t)at, from, 64), hi = __shfl((uint32_t)(at >> 32), from, 64);
-                    vb[t][i] = vh + ((uint64_t)hi << 32 | lo) + E * c;
+                    vb[t][i] = a.v + ((uint64_t)hi << 32 | lo) + E * c;
                 }
             }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (E > 1)
+                        st.v[t][i] = *reinterpret_cast<const VReg *>(vb[t][i]);
+                    else
+                        st.v[t][i] = *vb[t][i];
+                }
         }
+    }
+
+    // A raw buffer of `bytes` bytes.
+    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile(const uint16_t *p, uint32_t bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p), 0, (int)bytes, 0x00020000);
+    }
+
+    static __device__ __forceinline__ uint32_t word(const VReg &v, int i) {
+        if constexpr (E > 2)
+            return v[i];
+        else
+            return v;
+    }
+
+    __device__ __forceinline__ void compute(Step &st) {
         bool full = true;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            full = full && seen[t] == 0xffffu;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (E == 8) {
-                    vr[t][i] = *reinterpret_cast<const u32x4 *>(vb[t][i]);
-                } else if constexpr (E == 4) {
-                    const u32x2 x = *reinterpret_cast<const u32x2 *>(vb[t][i]);
-                    vr[t][i][0] = x[0];
-                    vr[t][i][1] = x[1];
-                } else if constexpr (E == 2) {
-                    vr[t][i][0] = *reinterpret_cast<const uint32_t *>(vb[t][i]);
-                } else {
-                    vr[t][i][0] = *vb[t][i];
-                }
-            }
-        }
-
+        for (int t = 0; t < NT; ++t) full = full && st.seen[t] == (UNI ? 16u : 0xffffu);
         float s[NT][4];
-        const float sc = a.scale * kLog2e;
         float top = neg_inf();
+        floatx4 dot[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            floatx4 x = {0.f, 0.f, 0.f, 0.f};
+        for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) {
+            for (int t = 0; t < NT; ++t) {
+                const floatx4 x = kk ? dot[t] : floatx4{0.f, 0.f, 0.f, 0.f};
                 if constexpr (D == 16)
-                    x = mfma_k16<BF>(kr[t][kk], u32x2{qv[kk][0], qv[kk][1]}, x);
+                    dot[t] = mfma_k16<BF>(st.k[t][kk], u32x2{qv[kk][0], qv[kk][1]}, x);
                 else
-                    x = mfma_k32<BF>(kr[t][kk], qv[kk], x);
+                    dot[t] = mfma_k32<BF>(st.k[t][kk], qv[kk], x);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[t][i] = x[i] * sc;
-        }
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[t][i] = dot[t][i] * sc;
         if (!full) {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const bool in = seen[t] >> (4 * g + i) & 1u;
+                    const bool in = UNI ? 4 * g + i < st.seen[t] : st.seen[t] >> (4 * g + i) & 1u;
                     s[t][i] = in ? s[t][i] : neg_inf();
+                    if constexpr (!UNI) {  // 0 * NaN would be NaN
+                        if constexpr (E > 2) {
 #pragma unroll
-                    for (int j = 0; j < (E + 1) / 2; ++j) vr[t][i][j] = in ? vr[t][i][j] : 0u;  // 0 * NaN would be NaN
+                            for (int j = 0; j < E / 2; ++j) st.v[t][i][j] = in ? st.v[t][i][j] : 0u;
+                        } else {
+                            st.v[t][i] = in ? st.v[t][i] : 0u;
+                        }
+                    }
                 }
         }
 #pragma unroll
@@ -475,17 +542,56 @@ struct Decode {
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int n = 0; n < PARTS; ++n) p[n][j] = take_pair<BF>(s[2 * u + j / 2][2 * (j % 2)], s[2 * u + j / 2][2 * (j % 2) + 1]);
+            constexpr int G = E < 4 ? E : 4;  // products of so many dims in turn: each waits for its last one
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                u32x4 x;
+            for (int i0 = 0; i0 < E; i0 += G) {
+                u32x4 x[G];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t lo = vr[2 * u + j / 2][2 * (j % 2)][i / 2], hi = vr[2 * u + j / 2][2 * (j % 2) + 1][i / 2];
-                    x[j] = __builtin_amdgcn_perm(hi, lo, i % 2 ? 0x07060302u : 0x05040100u);
-                }
+                for (int i = 0; i < G; ++i)
 #pragma unroll
-                for (int n = 0; n < PARTS; ++n) acc[i] = mfma_k32<BF>(x, p[n], acc[i]);
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t lo = word(st.v[2 * u + j / 2][2 * (j % 2)], (i0 + i) / 2);
+                        const uint32_t hi = word(st.v[2 * u + j / 2][2 * (j % 2) + 1], (i0 + i) / 2);
+                        x[i][j] = __builtin_amdgcn_perm(hi, lo, i % 2 ? 0x07060302u : 0x05040100u);
+                    }
+#pragma unroll
+                for (int n = 0; n < PARTS; ++n)
+#pragma unroll
+                    for (int i = 0; i < G; ++i) acc[i0 + i] = mfma_k32<BF>(x[i], p[n], acc[i0 + i]);
             }
+        }
+    }
+
+    // The keys k0, k0 + bk, ... below `end` of one key head: a step's loads are under way before the step before
+    // it is computed, and the table entries a step earlier. Every step's loads are the same ones whatever there
+    // is to load, so that waiting for one step's does not mean waiting for the next step's too.
+    __device__ __forceinline__ void sweep(uint32_t r, uint32_t kvh, uint32_t k0, uint32_t end, uint32_t len) {
+        if (k0 >= end) return;
+        const Args a = again(args);
+        Cache cache;
+        cache.table = a->table + r * a->table_stride;
+        cache.k = a->k + kvh * a->head_stride;
+        cache.v = a->v + kvh * a->head_stride;
+        cache.page_stride = a->page_stride;
+        cache.token_stride = a->token_stride;
+        cache.num_pages = a->num_pages;
+        cache.ps.d = a->ps.d;
+        cache.ps.magic = a->ps.magic;
+        cache.ps.shift = a->ps.shift;
+        Step x, y;
+        Pages pages = load_pages(cache, k0, len);
+        issue(x, cache, pages, k0, end);
+        pages = load_pages(cache, k0 + bk, len);
+        while (true) {
+            issue(y, cache, pages, k0 + bk, end);
+            pages = load_pages(cache, k0 + 2 * bk, len);
+            compute(x);
+            if (k0 + bk >= end) break;
+            issue(x, cache, pages, k0 + 2 * bk, end);
+            pages = load_pages(cache, k0 + 3 * bk, len);
+            compute(y);
+            k0 += 2 * bk;
+            if (k0 >= end) break;
         }
     }
 
@@ -494,10 +600,12 @@ struct Decode {
     // them take every so many-th piece and are added up through LDS. PF pieces are on their way at a time.
     template <int PF>
     __device__ __forceinline__ void join_pieces(uint32_t first, uint32_t last, uint32_t rows, float *o) {
-        const uint32_t items = rows * (D / 4), groups = items > 128 ? 1u : 256u / items;
+        const Args a = again(args);
+        const uint32_t items = rows * (D / 4), groups = items > THREADS / 2 ? 1u : THREADS / items, piece_rows = a->rows;
+        const float *part_ml = a->part_ml, *part_o = a->part_o;
         floatx4 *s_sum = reinterpret_cast<floatx4 *>(&s_o[0][0][0]);  // one per thread, and behind them (max, sum)
-        float *s_stat = reinterpret_cast<float *>(s_sum + 256);
-        for (uint32_t i0 = 0; i0 < items; i0 += 256) {
+        float *s_stat = reinterpret_cast<float *>(s_sum + THREADS);
+        for (uint32_t i0 = 0; i0 < items; i0 += THREADS) {
             const uint32_t grp = groups == 1 ? 0u : threadIdx.x / items, it = groups == 1 ? i0 + threadIdx.x : threadIdx.x - grp * items;
             const bool mine = it < items && grp < groups;
             const uint32_t q = it / (D / 4), x = 4 * (it % (D / 4));
@@ -510,19 +618,16 @@ struct Decode {
 #pragma unroll
                     for (int n = 0; n < PF; ++n) {
                         const uint32_t j = min(i + n * groups, last);
-                        const uint64_t at = ((uint64_t)j * 2 + (j == first)) * a.rows + q;
+                        const uint64_t at = ((uint64_t)j * 2 + (j == first)) * piece_rows + q;
                         float p0, p1, p2, p3;
-                        get2(a.part_ml + 2 * at, pm[n], pl[n]);
-                        get2(a.part_o + at * D + x, p0, p1);
-                        get2(a.part_o + at * D + x + 2, p2, p3);
+                        get2(part_ml + 2 * at, pm[n], pl[n]);
+                        get2(part_o + at * D + x, p0, p1);
+                        get2(part_o + at * D + x + 2, p2, p3);
                         po[n] = floatx4{p0, p1, p2, p3};
                     }
                     float t = top;
 #pragma unroll
-                    for (int n = 0; n < PF; ++n) {
-                        if (i + n * groups > last) pm[n] = neg_inf();
-                        t = fmaxf(t, pm[n]);
-                    }
+                    for (int n = 0; n < PF; ++n) t = fmaxf(t, pm[n]);
                     const float ref = finite_or_0(t), f = __builtin_amdgcn_exp2f(top - ref);
                     sum *= f;
                     out *= f;
@@ -561,10 +666,12 @@ struct Decode {
     }
 
     __device__ __forceinline__ void store_o(float *o, uint32_t q, uint32_t x, floatx4 v, float sum) {
+        const float inv = 1.f / sum;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = sum == 0.f ? 0.f : v[i] / sum;
-        float *p = o + q * a.o_head_stride + x;
-        if (a.o_vec) {
+        for (int i = 0; i < 4; ++i) v[i] = sum == 0.f ? 0.f : v[i] * inv;
+        const Args a = args;
+        float *p = o + q * a->o_head_stride + x;
+        if (a->o_vec) {
             *reinterpret_cast<floatx4 *>(p) = v;
         } else {
 #pragma unroll
@@ -573,14 +680,22 @@ struct Decode {
     }
 
     // The four waves' (m, l, O) of one run of blocks: to O if the run is all of the request's, else to this
-    // workgroup's (i's) piece, and the last of workgroups first..last to arrive joins them.
-    __device__ __forceinline__ void finish(uint32_t rows, float *o, bool whole, uint32_t i, uint32_t first, uint32_t last) {
+    // workgroup's (i's) piece, and the last to arrive of the workgroups that share the units b_lo..b_lo+nb-1, `each`
+    // apiece, joins them.
+    __device__ __forceinline__ void finish(uint32_t rows, uint32_t r, uint32_t head0, bool whole, uint32_t i, uint32_t b_lo, uint32_t nb, uint32_t each) {
+        const Args a = again(args);
+        uint32_t first = i, last = i;
+        if (!whole) {
+            first = b_lo / each;
+            last = (b_lo + nb - 1u) / each;
+        }
+        float *o = a->o + r * a->o_stride + head0 * a->o_head_stride;
         const float sum = quad_sum(l);
         if (g == 0) {
             s_ml[w][c][0] = m;
             s_ml[w][c][1] = sum;
         }
-        if (16 * (w & ((1u << a.wave_shift) - 1u)) + c < rows) {
+        if (16 * qt + c < rows) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -588,24 +703,34 @@ struct Decode {
         }
         __syncthreads();
         const uint32_t items = rows * (D / 4);
-        for (uint32_t it = threadIdx.x; it < items; it += 256) {
+        for (uint32_t it = threadIdx.x; it < items; it += THREADS) {
             const uint32_t q = it / (D / 4), x = 4 * (it % (D / 4));
-            const uint32_t q16 = q & 15u, by = 1u << a.wave_shift;  // waves q / 16, + by, ... hold query q
-            float top = neg_inf(), lsum = 0.f;
-            for (uint32_t n = q >> 4; n < 4; n += by) top = fmaxf(top, s_ml[n][q16][0]);
-            floatx4 out = {0.f, 0.f, 0.f, 0.f};
-            for (uint32_t n = q >> 4; n < 4; n += by) {
-                const float f = __builtin_amdgcn_exp2f(s_ml[n][q16][0] - finite_or_0(top));
-                lsum += f * s_ml[n][q16][1];
-                out += f * *reinterpret_cast<const floatx4 *>(&s_o[n][q16][x]);
+            // waves q/16, q/16 + 2^wave_shift, ... hold query q
+            float wm[NW], wl[NW], top = neg_inf(), lsum = 0.f;
+            floatx4 wo[NW], out = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (uint32_t n = 0; n < NW; ++n) {
+                const uint32_t j = ((q >> 4) + (n << wave_shift)) & (NW - 1u);
+                wm[n] = n < NW >> wave_shift ? s_ml[j][q & 15u][0] : neg_inf();
+                wl[n] = s_ml[j][q & 15u][1];
+                wo[n] = *reinterpret_cast<const floatx4 *>(&s_o[j][q & 15u][x]);
+                top = fmaxf(top, wm[n]);
+            }
+#pragma unroll
+            for (uint32_t n = 0; n < NW; ++n) {
+                const float f = __builtin_amdgcn_exp2f(wm[n] - finite_or_0(top));
+                if (n < NW >> wave_shift) {
+                    lsum += f * wl[n];
+                    out += f * wo[n];
+                }
             }
             if (whole) {
                 store_o(o, q, x, out, lsum);
             } else {
-                const uint64_t at = ((uint64_t)i * 2 + (i == first)) * a.rows + q;
-                put2(a.part_o + at * D + x, out[0], out[1]);
-                put2(a.part_o + at * D + x + 2, out[2], out[3]);
-                if (x == 0) put2(a.part_ml + 2 * at, top, lsum);
+                const uint64_t at = ((uint64_t)i * 2 + (i == first)) * a->rows + q;
+                put2(a->part_o + at * D + x, out[0], out[1]);
+                put2(a->part_o + at * D + x + 2, out[2], out[3]);
+                if (x == 0) put2(a->part_ml + 2 * at, top, lsum);
             }
         }
         if (!whole) {
@@ -614,130 +739,133 @@ struct Decode {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
             if (threadIdx.x == 0)
-                *s_word = __hip_atomic_fetch_add(a.counters + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                *s_word = __hip_atomic_fetch_add(a->counters + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __syncthreads();
             if (*s_word == last - first) {
-                const uint32_t pieces = (last - first + 1) * min(rows * (D / 4), 256u);  // a thread's, times 256
-                if (pieces <= 2 * 256)
-                    join_pieces<2>(first, last, rows, o);
-                else if (pieces <= 4 * 256)
+                if (last - first < 4)
                     join_pieces<4>(first, last, rows, o);
                 else
                     join_pieces<8>(first, last, rows, o);
-                if (threadIdx.x == 0) __hip_atomic_store(a.counters + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (threadIdx.x == 0) __hip_atomic_store(a->counters + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
         }
         __syncthreads();  // LDS is free again
     }
 
     __device__ __forceinline__ void run() {
-        const uint32_t R = a.num_seqs, per = (R + 63u) / 64u;  // requests of a lane
-        const uint32_t heads = a.num_kv_heads * a.head_parts;
-        const uint32_t qt = w & ((1u << a.wave_shift) - 1u), kw = w >> a.wave_shift;  // query heads' and keys' part
+        const Args a = args;
+        const int32_t *lens = a->seq_lens;
+        const uint32_t max_tokens = a->max_tokens;
+        sc = a->scale * kLog2e;
+        const uint32_t R = a->num_seqs, per = (R + 63u) / 64u;  // requests of a lane
         const uint32_t zero_r = blockIdx.x;
-        const int32_t zero_len = zero_r < R ? as_const(a.seq_lens)[zero_r] : 1;
-        uint32_t mine = 0, len0 = 0;
+        const int32_t zero_len = zero_r < R ? as_const(lens)[zero_r] : 1;
+        uint32_t mine = 0, some = 0, len0 = 0;  // units, and requests with keys
         for (uint32_t j = 0; j < per; ++j) {
             const uint32_t r = lane * per + j;
             if (r < R) {
-                len0 = nc_paged_cut(a.seq_lens[r], a.max_tokens);
-                mine += blocks_of(len0);
+                len0 = nc_paged_cut(lens[r], max_tokens);
+                mine += units_of(blocks_of(len0));
+                some += len0 != 0;
             }
         }
-        const uint32_t incl = wave_scan32(mine);
-        const uint32_t blocks = __builtin_amdgcn_readlane(incl, 63) * heads, i = blockIdx.x;
-        const uint32_t each = nc_paged_each(blocks, gridDim.x);
-        uint32_t b = i * each;
-        if (b < blocks) {
-            const uint32_t end = min(b + each, blocks);
-            Place at;
+        kat = 2u * (c * (uint32_t)a->token_stride + KE * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vat[i] = 2u * ((4 * g + i) * (uint32_t)a->token_stride + E * c);
+        const uint32_t incl = wave_scan32(mine), heads = a->heads.d;
+        const uint32_t total = __builtin_amdgcn_readlane(incl, 63), with_keys = __builtin_amdgcn_readlane(wave_scan32(some), 63);
+        const uint32_t units = total * heads, i = blockIdx.x;
+        // Heads of many blocks: half the workgroups, which leaves half the pieces to join; one with its loads under way
+        // a step ahead keeps a CU's share of the memory busy. Heads of few: the others hide each head's beginning and end.
+        const uint32_t most_log2 = total >= NC_PAGED_LONG_UNITS * with_keys ? a->long_log2 : a->short_log2;
+        const uint32_t each = nc_paged_each(units, most_log2, a->each_least), u0 = i * each, u1 = min(u0 + each, units);
+        if (u0 < units) {
+            // Request r, of length len, whose units begin behind `pre` of the requests before it (times the heads).
+            uint32_t r, len, pre;
             {
-                const uint32_t t = b / heads;  // the same request's block if it had one head
+                const uint32_t t = nc_paged_quot(u0, {heads, a->heads.magic, a->heads.shift});  // the same request's unit if it had one head
                 const uint32_t from = __builtin_ctzll(__ballot(incl - mine <= t && t < incl));
-                at.pre = __builtin_amdgcn_readlane(incl - mine, from);
-                at.r = from * per;
-                at.len = __builtin_amdgcn_readlane(len0, from);
+                pre = __builtin_amdgcn_readlane(incl - mine, from);
+                r = from * per;
+                len = __builtin_amdgcn_readlane(len0, from);
                 if (per > 1) {
-                    const uint32_t r0 = at.r, most = min(per, R - r0);
+                    const uint32_t r0 = r, most = min(per, R - r0);
                     for (uint32_t x = 0; x < most; x += 64) {
-                        const uint32_t len = x + lane < most ? nc_paged_cut(a.seq_lens[r0 + x + lane], a.max_tokens) : 0u;
-                        const uint32_t nb = blocks_of(len), sc = wave_scan32(nb);
-                        const uint64_t hit = __ballot(t < at.pre + sc);
+                        const uint32_t n = x + lane < most ? nc_paged_cut(lens[r0 + x + lane], max_tokens) : 0u;
+                        const uint32_t un = units_of(blocks_of(n)), sc = wave_scan32(un);
+                        const uint64_t hit = __ballot(t < pre + sc);
                         if (hit) {
                             const uint32_t y = __builtin_ctzll(hit);
-                            at.r = r0 + x + y;
-                            at.len = __builtin_amdgcn_readlane(len, y);
-                            at.pre += __builtin_amdgcn_readlane(sc - nb, y);
+                            r = r0 + x + y;
+                            len = __builtin_amdgcn_readlane(n, y);
+                            pre += __builtin_amdgcn_readlane(sc - un, y);
                             break;
                         }
-                        at.pre += __builtin_amdgcn_readlane(sc, 63);
+                        pre += __builtin_amdgcn_readlane(sc, 63);
                     }
                 }
+                pre *= heads;
             }
-            uint32_t nb = blocks_of(at.len);
-            uint32_t head = (b - at.pre * heads) / nb, b0 = b - at.pre * heads - head * nb;
-            while (true) {
-                const uint32_t b1 = min(nb, b0 + (end - b));
-                const uint32_t kvh = head / a.head_parts, part = head - kvh * a.head_parts;
-                const uint32_t rows = min(64u, a.group - 64u * part), head0 = kvh * a.group + 64u * part;
-                load_q(at.r, head0, 16u * qt, rows);
-                m = neg_inf();
-                l = 0.f;
-#pragma unroll
-                for (int x = 0; x < E; ++x) acc[x] = floatx4{0.f, 0.f, 0.f, 0.f};
-                uint32_t k0 = b0 * bk + kw * WK;
-                const uint32_t k1 = min(b1 * bk, at.len);
-                const uint64_t row = at.r * a.table_stride;
-                if (k0 < k1) {
-                    uint32_t e[NT];
-                    load_pages(e, row, k0, at.len);
-                    while (true) {
-                        uint32_t next[NT];
-                        load_pages(next, row, k0 + bk, at.len);
-                        step(e, k0, at.len, kvh);
-                        k0 += bk;
-                        if (k0 >= k1) break;
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) e[t] = next[t];
-                    }
+            uint32_t nb = blocks_of(len), head = heads > 1 ? (u0 - pre) / units_of(nb) : 0u, seg = pre + head * units_of(nb);
+            while (seg < u1) {  // the head's units: its own cost, then one per block
+                const bool short_head = nb <= NC_PAGED_WHOLE_BLOCKS;
+                const uint32_t b_lo = seg + NC_PAGED_HEAD_UNITS;  // unit of block 0
+                uint32_t b0 = u0 > b_lo ? u0 - b_lo : 0u, b1 = u1 > b_lo ? min(nb, u1 - b_lo) : 0u;
+                if (short_head) {  // all of it is the workgroup's that has its first unit
+                    b0 = 0;
+                    b1 = seg >= u0 ? nb : 0u;
                 }
-                const uint32_t seg = at.pre * heads + head * nb;  // the request's and head's first block
-                const bool whole = b0 == 0 && b1 == nb;
-                finish(rows, a.o + at.r * a.o_stride + head0 * a.o_head_stride, whole, i, seg / each, (seg + nb - 1) / each);
-                b += b1 - b0;
-                if (b >= end) break;
-                b0 = 0;
+                if (b0 < b1) {
+                    uint32_t kvh = head, part = 0;
+                    if (a->head_parts > 1) {
+                        kvh = head / a->head_parts;
+                        part = head - kvh * a->head_parts;
+                    }
+                    const uint32_t rows = min(64u, a->group - 64u * part), head0 = kvh * a->group + 64u * part;
+                    load_q(r, head0, rows);
+                    m = neg_inf();
+                    l = 0.f;
+#pragma unroll
+                    for (int x = 0; x < E; ++x) acc[x] = floatx4{0.f, 0.f, 0.f, 0.f};
+                    sweep(r, kvh, b0 * bk + kw * WK, min(b1 * bk, len), len);
+                    finish(rows, r, head0, b0 == 0 && b1 == nb, i, b_lo, nb, each);
+                }
+                seg += units_of(nb);
                 if (++head == heads) {
                     head = 0;
-                    at.pre += nb;
-                    do at.len = ++at.r < R ? nc_paged_cut(as_const(a.seq_lens)[at.r], a.max_tokens) : 1u;
-                    while (at.len == 0);  // the share has blocks left, so there is one
-                    if (at.r >= R) break;
-                    nb = blocks_of(at.len);
+                    do len = ++r < R ? nc_paged_cut(as_const(lens)[r], max_tokens) : 1u;
+                    while (len == 0);
+                    if (r >= R) break;
+                    nb = blocks_of(len);
                 }
             }
         }
         // Requests without keys
         int32_t zl = zero_len;
         for (uint32_t r = zero_r; r < R;) {
-            if (nc_paged_cut(zl, a.max_tokens) == 0)
-                for (uint32_t x = threadIdx.x; x < a.num_q_heads * D; x += 256)
-                    a.o[r * a.o_stride + (x / D) * a.o_head_stride + x % D] = 0.f;
+            if (nc_paged_cut(zl, max_tokens) == 0) {
+                const Args z = again(args);
+                for (uint32_t x = threadIdx.x; x < z->num_q_heads * D; x += THREADS)
+                    z->o[r * z->o_stride + (x / D) * z->o_head_stride + x % D] = 0.f;
+            }
             r += gridDim.x;
-            if (r < R) zl = as_const(a.seq_lens)[r];
+            if (r < R) zl = as_const(lens)[r];
         }
     }
 };
 
 template <int D, bool BF, bool UNI>
-__device__ __forceinline__ void decode_body(const nc_paged_decode_args &a) {
+__device__ __forceinline__ void decode_body() {
+    const Args a = (Args)__builtin_amdgcn_kernarg_segment_ptr();
     using X = Decode<D, BF, UNI>;
-    // the waves' O, or the join's 256 x (4 columns, max, sum)
-    __shared__ __attribute__((aligned(16))) float s_mem[4 * 16 * X::OP > 256 * 6 ? 4 * 16 * X::OP : 256 * 6];
-    __shared__ float s_ml[4][16][2];
+    // the waves' O, or the join's (4 columns, max, sum) of every thread
+    __shared__ __attribute__((aligned(16))) float s_mem[X::NW * 16 * X::OP > X::THREADS * 6 ? X::NW * 16 * X::OP : X::THREADS * 6];
+    __shared__ float s_ml[X::NW][16][2];
     __shared__ uint32_t s_word;
     const uint32_t lane = threadIdx.x & 63u;
-    X x{a, lane, (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane & 15u, lane >> 4, X::WK * (4u >> a.wave_shift),
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t shift = a->wave_shift;
+    X x{a, lane, w, lane & 15u, lane >> 4, shift, X::WK * (X::NW >> shift), w & ((1u << shift) - 1u), w >> shift,
         reinterpret_cast<float (*)[16][X::OP]>(s_mem), s_ml, &s_word};
     x.run();
 }
@@ -746,11 +874,11 @@ __device__ __forceinline__ void decode_body(const nc_paged_decode_args &a) {
 
 // `_odd`: pages of any size; the others take sizes that are multiples of 16.
 #define NC_DECODE(D, T, BF)                                                                                      \
-    extern "C" __global__ __launch_bounds__(256, 3) void nc_paged_decode_d##D##T(const nc_paged_decode_args a) {  \
-        decode_body<D, BF, true>(a);                                                                             \
+    extern "C" __global__ __launch_bounds__(64 * NC_PAGED_WAVES, 2) void nc_paged_decode_d##D##T(const nc_paged_decode_args) {  \
+        decode_body<D, BF, true>();                                                                             \
     }                                                                                                            \
-    extern "C" __global__ __launch_bounds__(256, 3) void nc_paged_decode_d##D##_odd##T(const nc_paged_decode_args a) { \
-        decode_body<D, BF, false>(a);                                                                            \
+    extern "C" __global__ __launch_bounds__(64 * NC_PAGED_WAVES, 2) void nc_paged_decode_d##D##_odd##T(const nc_paged_decode_args) { \
+        decode_body<D, BF, false>();                                                                            \
     }
 NC_DECODE(16, , false)
 NC_DECODE(32, , false)

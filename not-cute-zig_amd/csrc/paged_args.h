@@ -54,12 +54,23 @@ struct nc_paged_append_args {
 // take in a step. A wave takes step_keys of them for 16 query heads; where a key head has more than 16, two or
 // four waves take the same keys for 16 heads each (wave_shift 1 or 2), and past 64 the workgroup's heads count
 // as another head.
-NC_HD uint32_t nc_paged_step_keys(uint32_t head_dim) { return head_dim == 16 ? 128u : head_dim == 32 ? 64u : 32u; }
+#define NC_PAGED_WAVES 4u
+NC_HD uint32_t nc_paged_step_keys(uint32_t head_dim) { return head_dim <= 32 ? 64u : 32u; }
 NC_HD uint32_t nc_paged_wave_shift(uint32_t group) { return group <= 16 ? 0u : group <= 32 ? 1u : 2u; }
 NC_HD uint32_t nc_paged_head_parts(uint32_t group) { return (group + 63u) / 64u; }
 
-// Workgroup i takes blocks [i * each, (i + 1) * each) of all; `each` is the least that `most` workgroups can do with.
-NC_HD uint32_t nc_paged_each(uint32_t blocks, uint32_t most) { return (blocks + most - 1u) / most; }
+// Shares are counted in units: one per block, and NC_PAGED_HEAD_UNITS before a head's first block for what a head costs
+// however short it is. Workgroup i takes units [i * each, (i + 1) * each), where `each` is the least that
+// 2^most_log2 workgroups can do with, and no less than `least`.
+#define NC_PAGED_HEAD_UNITS 2u
+// A head of no more blocks than this is not split: the workgroup that has its first unit takes all of it.
+#define NC_PAGED_WHOLE_BLOCKS 4u
+// Heads of this many units on the average are long ones.
+#define NC_PAGED_LONG_UNITS 8u
+NC_HD uint32_t nc_paged_each(uint32_t units, uint32_t most_log2, uint32_t least) {
+    const uint32_t each = (units + (1u << most_log2) - 1u) >> most_log2;
+    return each < least ? least : each;
+}
 
 struct nc_paged_decode_args {
     const uint16_t *q, *k, *v;
@@ -73,6 +84,8 @@ struct nc_paged_decode_args {
     uint32_t num_pages, max_tokens;                      // max_tokens = max_pages * page_size
     uint32_t rows;                                       // query heads of a piece: min(group, 64)
     uint32_t wave_shift, head_parts;
+    uint32_t long_log2, short_log2, each_least; // workgroups for long heads and for short ones, units of a share
+    nc_paged_div heads;                         // num_kv_heads * head_parts
     uint32_t q_vec, o_vec;                               // Q, O rows are 16-byte aligned
     float scale;
     nc_paged_div ps;

@@ -282,12 +282,13 @@ int main() {
             if (nc_paged_quot(n, v) != n / d) { std::printf("%u / %u\n", n, d); return 1; }
         }
     }
-    // shares of nc_paged_each() cover all blocks with no more workgroups than there are, none of them idle
+    // shares of nc_paged_each() cover all units with no more workgroups than there are, and no smaller one does
     for (int k = 0; k < 20000; ++k) {
         x ^= x << 13; x ^= x >> 7; x ^= x << 17;
-        const uint32_t blocks = k % 2 ? (uint32_t)(x % 5000) + 1 : (uint32_t)(x % most) + 1;
-        const uint32_t n = (uint32_t)((x >> 32) % 2048) + 1, each = nc_paged_each(blocks, n);
-        if (each == 0 || (uint64_t)each * n < blocks || (each > 1 && (uint64_t)(each - 1) * n >= blocks)) return 3;
+        const uint32_t units = k % 2 ? (uint32_t)(x % 5000) + 1 : (uint32_t)(x % (1u << 30)) + 1;
+        const uint32_t lg = (uint32_t)((x >> 32) % 12), n = 1u << lg, least = k % 3 ? 1 : (uint32_t)(x % 17) + 1;
+        const uint32_t each = nc_paged_each(units, lg, least);
+        if (each < least || (uint64_t)each * n < units || (each > least && (uint64_t)(each - 1) * n >= units)) return 3;
     }
     for (uint32_t g = 1; g < 300; ++g) {  // the waves' and parts' query heads cover the group, 16 a wave
         const uint32_t rows = g < 64 ? g : 64, sh = nc_paged_wave_shift(rows);
