@@ -146,8 +146,8 @@ DecodePlan decode_plan(const Shape &s) {
     const bool uniform = o.page_size % 16 == 0 && o.page_stride < (1ull << 31) && o.page_size * o.token_stride < (1ull << 30);
     std::snprintf(p.name, sizeof p.name, "nc_paged_decode_d%u%s%s", (unsigned)o.head_dim, uniform ? "" : "_odd",
                   o.element_type == NC_ELEMENT_BF16 ? "_bf16" : "");
-    p.long_log2 = kCusLog2;
-    p.short_log2 = kCusLog2 + 1;
+    p.long_log2 = kCusLog2 + (uniform && o.head_dim > 16 ? 0 : 1);
+    p.short_log2 = p.long_log2 + 1;
     p.grid = (uint32_t)std::min<uint64_t>(o.num_seqs * s.heads * s.seq_units, 1u << p.short_log2);
     p.rows = (uint32_t)std::min<uint64_t>(s.group, 64);
     p.piece_ml = NC_PAGED_MAX_WGS * 4;

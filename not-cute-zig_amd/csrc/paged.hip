@@ -581,6 +581,18 @@ struct Decode {
         Step x, y;
         Pages pages = load_pages(cache, k0, len);
         issue(x, cache, pages, k0, end);
+        if constexpr (!UNI) {
+            while (true) {
+                pages = load_pages(cache, k0 + bk, len);
+                compute(x);
+                if ((k0 += bk) >= end) return;
+                issue(x, cache, pages, k0, end);
+            }
+        }
+        if (k0 + bk >= end) {
+            compute(x);
+            return;
+        }
         pages = load_pages(cache, k0 + bk, len);
         while (true) {
             issue(y, cache, pages, k0 + bk, end);

@@ -64,7 +64,7 @@ NC_HD uint32_t nc_paged_head_parts(uint32_t group) { return (group + 63u) / 64u;
 // 2^most_log2 workgroups can do with, and no less than `least`.
 #define NC_PAGED_HEAD_UNITS 2u
 // A head of no more blocks than this is not split: the workgroup that has its first unit takes all of it.
-#define NC_PAGED_WHOLE_BLOCKS 4u
+#define NC_PAGED_WHOLE_BLOCKS 2u
 // Heads of this many units on the average are long ones.
 #define NC_PAGED_LONG_UNITS 8u
 NC_HD uint32_t nc_paged_each(uint32_t units, uint32_t most_log2, uint32_t least) {
