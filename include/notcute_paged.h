@@ -8,7 +8,8 @@
  *
  * An extension: the reference has no cache. Conventions as in notcute_flash.h: nc_status return codes,
  * plain device pointers with element counts, f16 (or bf16) bit patterns as uint16_t, O in f32,
- * asynchronous on the given stream. No call allocates, synchronises or copies; every one may be captured
+ * asynchronous on the given stream. A call's tensors come as one block of pointers and lengths in elements,
+ * which it reads before it returns. No call allocates, synchronises or copies; every one may be captured
  * into a HIP graph (nc_paged_build may be two launches, the others are one). The kernels are in the
  * embedded code object: `module` is one from nc_module_load_embedded.
  *
@@ -92,20 +93,48 @@ int nc_paged_validate(const nc_paged_options *opts);
  * Lengths in elements: cached_len, new_len, seq_len >= num_seqs; offsets_len >= num_seqs + 1; table_len >=
  * (num_seqs - 1)*table_stride + max_pages; counts_len >= 4, cursor_len >= 1; slots_len places are written
  * (0 to 2^31 - 1 of them, slots may be NULL for 0), free_len may be 0. */
-int nc_paged_build(nc_module module, const int32_t *cached_lens, size_t cached_len, const int32_t *new_lens,
-                   size_t new_len, const int32_t *free_pages, size_t free_len, const int32_t *cursor,
-                   size_t cursor_len, int32_t *block_table, size_t table_len, int32_t *seq_lens, size_t seq_len,
-                   int32_t *row_offsets, size_t offsets_len, int32_t *slots, size_t slots_len, int32_t *counts,
-                   size_t counts_len, const nc_paged_options *opts, nc_stream stream);
+typedef struct nc_paged_build_buffers {
+    const int32_t *cached_lens;
+    uint64_t cached_len;
+    const int32_t *new_lens;
+    uint64_t new_len;
+    const int32_t *free_pages;
+    uint64_t free_len;
+    const int32_t *cursor;
+    uint64_t cursor_len;
+    int32_t *block_table;
+    uint64_t table_len;
+    int32_t *seq_lens;
+    uint64_t seq_len;
+    int32_t *row_offsets;
+    uint64_t offsets_len;
+    int32_t *slots;
+    uint64_t slots_len;
+    int32_t *counts;
+    uint64_t counts_len;
+} nc_paged_build_buffers;
+int nc_paged_build(nc_module module, const nc_paged_build_buffers *buffers, const nc_paged_options *opts,
+                   nc_stream stream);
 
 /* K and V rows into the cache: row i (element i*row_stride + h*row_head_stride of k_rows and v_rows, at any
  * element alignment) goes to slot slots[i], for the num_rows first rows; a slot outside the pool (-1) is
  * skipped. Slots of one call are distinct: of two rows with the same slot, either may be kept, element by
  * element. The caches are 16-byte aligned, are not one and the same, and do not overlap the rows
  * (NC_ERROR_INVALID_VALUE). num_rows = 0 does nothing. */
-int nc_paged_append(nc_module module, const uint16_t *k_rows, size_t k_rows_len, const uint16_t *v_rows,
-                    size_t v_rows_len, const int32_t *slots, size_t slots_len, uint16_t *k_cache, size_t k_len,
-                    uint16_t *v_cache, size_t v_len, uint64_t num_rows, const nc_paged_options *opts,
+typedef struct nc_paged_append_buffers {
+    const uint16_t *k_rows;
+    uint64_t k_rows_len;
+    const uint16_t *v_rows;
+    uint64_t v_rows_len;
+    const int32_t *slots;
+    uint64_t slots_len;
+    uint16_t *k_cache;
+    uint64_t k_len;
+    uint16_t *v_cache;
+    uint64_t v_len;
+    uint64_t num_rows;
+} nc_paged_append_buffers;
+int nc_paged_append(nc_module module, const nc_paged_append_buffers *buffers, const nc_paged_options *opts,
                     nc_stream stream);
 
 /* Device memory that nc_paged_decode needs for these options (0 when they are invalid). The caller zeroes
@@ -120,10 +149,24 @@ uint64_t nc_paged_workspace_bytes(const nc_paged_options *opts);
  * (NC_ERROR_INVALID_VALUE). Rows of O behind the last request are not touched. How the keys are split over
  * workgroups follows the lengths of all requests, so a request's rounding may differ with its neighbours;
  * equal calls give equal bits. */
-int nc_paged_decode(nc_module module, const uint16_t *q, size_t q_len, const uint16_t *k_cache, size_t k_len,
-                    const uint16_t *v_cache, size_t v_len, const int32_t *block_table, size_t table_len,
-                    const int32_t *seq_lens, size_t lens_len, float *o, size_t o_len, void *workspace,
-                    uint64_t workspace_bytes, const nc_paged_options *opts, nc_stream stream);
+typedef struct nc_paged_decode_buffers {
+    const uint16_t *q;
+    uint64_t q_len;
+    const uint16_t *k_cache;
+    uint64_t k_len;
+    const uint16_t *v_cache;
+    uint64_t v_len;
+    const int32_t *block_table;
+    uint64_t table_len;
+    const int32_t *seq_lens;
+    uint64_t lens_len;
+    float *o;
+    uint64_t o_len;
+    void *workspace;
+    uint64_t workspace_bytes;
+} nc_paged_decode_buffers;
+int nc_paged_decode(nc_module module, const nc_paged_decode_buffers *buffers, const nc_paged_options *opts,
+                    nc_stream stream);
 
 #ifdef __cplusplus
 }

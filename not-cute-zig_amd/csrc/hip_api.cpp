@@ -9,6 +9,7 @@
 
 #include <hip/hip_runtime_api.h>
 
+#include <atomic>
 #include <cstdio>
 #include <cstring>
 #include <memory>
@@ -18,6 +19,7 @@
 #include <vector>
 
 #include "notcute_flash.h"
+#include "paged_args.h"
 
 struct nc_function_st {
     hipFunction_t fn = nullptr;
@@ -28,6 +30,7 @@ struct nc_module_st {
     hipModule_t mod = nullptr;
     // The embedded module's second code object (the paged cache's kernels); null in a loaded one.
     hipModule_t paged = nullptr;
+    std::atomic<nc_function> paged_functions[NC_PAGED_KERNELS] = {};  // its functions, once looked up
     // Guards `functions`: several host threads may launch through one module (hipModuleGetFunction,
     // the lookup the cache saves, is itself thread-safe). Entries are never removed before unload,
     // so a returned nc_function stays valid without the lock.
@@ -307,6 +310,21 @@ int nc_module_get_function(nc_function *out, nc_module module, const char *name)
     *out = fn.get();
     module->functions.emplace(name, std::move(fn));
     return NC_SUCCESS;
+}
+
+// A function kept under `slot`, so that a launch neither takes the lock nor hashes the name. For paged.cpp.
+extern "C" int nc_internal_module_kept_function(nc_module module, uint32_t slot, const char *name, nc_function *out) {
+    if (!module || slot >= NC_PAGED_KERNELS) return fail(NC_ERROR_INVALID_VALUE, "function: invalid argument");
+    *out = module->paged_functions[slot].load(std::memory_order_acquire);
+    if (*out) return NC_SUCCESS;
+    int st;
+    try {
+        st = nc_module_get_function(out, module, name);
+    } catch (...) {
+        return fail(NC_ERROR_OUT_OF_MEMORY, "function: host allocation failed");
+    }
+    if (!st) module->paged_functions[slot].store(*out, std::memory_order_release);
+    return st;
 }
 
 int nc_function_launch(nc_function fn, const nc_launch_config *cfg, void **kernel_params) {

@@ -3,13 +3,14 @@
 
 #include <algorithm>
 #include <cstdint>
-#include <cstdio>
 #include <cstring>
 
 #include "notcute_paged.h"
 #include "paged_args.h"
 
 extern "C" int nc_internal_fail(int status, const char *what);
+// hip_api.cpp: a function of the module, looked up once and kept under `slot` (below NC_PAGED_KERNELS).
+extern "C" int nc_internal_module_kept_function(nc_module module, uint32_t slot, const char *name, nc_function *out);
 
 namespace {
 
@@ -115,9 +116,19 @@ bool overlap(const Range &x, const Range &y) { return x.lo < x.hi && y.lo < y.hi
 
 uintptr_t address(const void *p) { return reinterpret_cast<uintptr_t>(p); }
 
-int launch(nc_module module, const char *name, uint32_t grid, uint32_t threads, void *args, nc_stream stream) {
+// Every kernel of paged.hip by its place here, under which the module keeps its function.
+const char *const kKernels[] = {
+    "nc_paged_build",          "nc_paged_append_rows",       "nc_paged_append_rows_unaligned",
+    "nc_paged_decode_d16",     "nc_paged_decode_d16_bf16",   "nc_paged_decode_d16_odd",  "nc_paged_decode_d16_odd_bf16",
+    "nc_paged_decode_d32",     "nc_paged_decode_d32_bf16",   "nc_paged_decode_d32_odd",  "nc_paged_decode_d32_odd_bf16",
+    "nc_paged_decode_d64",     "nc_paged_decode_d64_bf16",   "nc_paged_decode_d64_odd",  "nc_paged_decode_d64_odd_bf16",
+    "nc_paged_decode_d128",    "nc_paged_decode_d128_bf16",  "nc_paged_decode_d128_odd", "nc_paged_decode_d128_odd_bf16",
+};
+enum : uint32_t { kBuild, kAppend, kAppendUnaligned, kDecode };
+
+int launch(nc_module module, uint32_t kernel, uint32_t grid, uint32_t threads, void *args, nc_stream stream) {
     nc_function fn = nullptr;
-    int st = nc_module_get_function(&fn, module, name);
+    int st = nc_internal_module_kept_function(module, kernel, kKernels[kernel], &fn);
     if (st) return st;
     nc_launch_config cfg;
     std::memset(&cfg, 0, sizeof cfg);
@@ -132,8 +143,7 @@ int launch(nc_module module, const char *name, uint32_t grid, uint32_t threads, 
 
 // The attention's kernel, grid and workspace for a set of options.
 struct DecodePlan {
-    char name[40];
-    uint32_t grid, rows, long_log2, short_log2;
+    uint32_t kernel, grid, rows, long_log2, short_log2;
     uint64_t piece_ml, piece_o, bytes;  // offsets of the partials, and all of the workspace
 };
 
@@ -144,9 +154,10 @@ DecodePlan decode_plan(const Shape &s) {
     DecodePlan p;
     // A 16-key tile lies in one page, and a page's byte offsets fit 32 bits.
     const bool uniform = o.page_size % 16 == 0 && o.page_stride < (1ull << 31) && o.page_size * o.token_stride < (1ull << 30);
-    std::snprintf(p.name, sizeof p.name, "nc_paged_decode_d%u%s%s", (unsigned)o.head_dim, uniform ? "" : "_odd",
-                  o.element_type == NC_ELEMENT_BF16 ? "_bf16" : "");
-    p.long_log2 = kCusLog2 + (uniform && o.head_dim > 16 ? 0 : 1);
+    const uint32_t d = o.head_dim == 16 ? 0 : o.head_dim == 32 ? 1 : o.head_dim == 64 ? 2 : 3;
+    p.kernel = kDecode + 4 * d + (uniform ? 0 : 2) + (o.element_type == NC_ELEMENT_BF16 ? 1 : 0);
+    // Workgroups for long heads: one per CU, where a step's loads are wide and a step ahead.
+    p.long_log2 = kCusLog2 + (o.head_dim <= (uniform ? 16u : 32u) ? 1 : 0);
     p.short_log2 = p.long_log2 + 1;
     p.grid = (uint32_t)std::min<uint64_t>(o.num_seqs * s.heads * s.seq_units, 1u << p.short_log2);
     p.rows = (uint32_t)std::min<uint64_t>(s.group, 64);
@@ -155,6 +166,8 @@ DecodePlan decode_plan(const Shape &s) {
     p.bytes = p.piece_o + (uint64_t)p.grid * 2 * p.rows * o.head_dim * 4;
     return p;
 }
+
+static_assert(sizeof kKernels / sizeof kKernels[0] == NC_PAGED_KERNELS, "one place per kernel");
 
 }  // namespace
 
@@ -176,33 +189,32 @@ uint64_t nc_paged_workspace_bytes(const nc_paged_options *opts) {
     return resolve(opts, &s) ? 0 : decode_plan(s).bytes;
 }
 
-int nc_paged_build(nc_module module, const int32_t *cached_lens, size_t cached_len, const int32_t *new_lens,
-                   size_t new_len, const int32_t *free_pages, size_t free_len, const int32_t *cursor,
-                   size_t cursor_len, int32_t *block_table, size_t table_len, int32_t *seq_lens, size_t seq_len,
-                   int32_t *row_offsets, size_t offsets_len, int32_t *slots, size_t slots_len, int32_t *counts,
-                   size_t counts_len, const nc_paged_options *opts, nc_stream stream) {
+int nc_paged_build(nc_module module, const nc_paged_build_buffers *buffers, const nc_paged_options *opts,
+                   nc_stream stream) {
+    if (!buffers) return NC_ERROR_INVALID_VALUE;
+    const nc_paged_build_buffers &t = *buffers;
     Shape s;
     int st = resolve(opts, &s);
     if (st) return st;
     const nc_paged_options &o = s.o;
-    if (!module || !cached_lens || !new_lens || !cursor || !block_table || !seq_lens || !row_offsets || !counts ||
-        (!free_pages && free_len) || (!slots && slots_len))
+    if (!module || !t.cached_lens || !t.new_lens || !t.cursor || !t.block_table || !t.seq_lens || !t.row_offsets || !t.counts ||
+        (!t.free_pages && t.free_len) || (!t.slots && t.slots_len))
         return NC_ERROR_INVALID_VALUE;
-    if (cached_len < o.num_seqs || new_len < o.num_seqs || seq_len < o.num_seqs || offsets_len < o.num_seqs + 1 ||
-        table_len < s.table_len || cursor_len < 1 || counts_len < 4)
+    if (t.cached_len < o.num_seqs || t.new_len < o.num_seqs || t.seq_len < o.num_seqs || t.offsets_len < o.num_seqs + 1 ||
+        t.table_len < s.table_len || t.cursor_len < 1 || t.counts_len < 4)
         return NC_ERROR_INVALID_VALUE;
-    if (slots_len > kMost31 || free_len > kMost31) return NC_ERROR_OVERFLOW;
-    if ((address(cached_lens) | address(new_lens) | address(free_pages) | address(cursor) | address(block_table) |
-         address(seq_lens) | address(row_offsets) | address(slots) | address(counts)) % 4)
+    if (t.slots_len > kMost31 || t.free_len > kMost31) return NC_ERROR_OVERFLOW;
+    if ((address(t.cached_lens) | address(t.new_lens) | address(t.free_pages) | address(t.cursor) | address(t.block_table) |
+         address(t.seq_lens) | address(t.row_offsets) | address(t.slots) | address(t.counts)) % 4)
         return NC_ERROR_INVALID_VALUE;
 
     // Outputs first; a pair may be one and the same buffer only where the header says so.
-    const Range rg[] = {range_of(seq_lens, o.num_seqs, 4),    range_of(counts, 4, 4),
-                        range_of(block_table, s.table_len, 4), range_of(row_offsets, o.num_seqs + 1, 4),
-                        range_of(slots, slots_len, 4),         range_of(cached_lens, o.num_seqs, 4),
-                        range_of(cursor, 1, 4),                range_of(new_lens, o.num_seqs, 4),
-                        range_of(free_pages, free_len, 4)};
-    const bool same_lens = seq_lens == cached_lens, same_cursor = counts == cursor;
+    const Range rg[] = {range_of(t.seq_lens, o.num_seqs, 4),    range_of(t.counts, 4, 4),
+                        range_of(t.block_table, s.table_len, 4), range_of(t.row_offsets, o.num_seqs + 1, 4),
+                        range_of(t.slots, t.slots_len, 4),         range_of(t.cached_lens, o.num_seqs, 4),
+                        range_of(t.cursor, 1, 4),                range_of(t.new_lens, o.num_seqs, 4),
+                        range_of(t.free_pages, t.free_len, 4)};
+    const bool same_lens = t.seq_lens == t.cached_lens, same_cursor = t.counts == t.cursor;
     for (int i = 0; i < 5; ++i)
         for (int j = i + 1; j < 9; ++j) {
             if ((i == 0 && j == 5 && same_lens) || (i == 1 && j == 6 && same_cursor)) continue;
@@ -212,77 +224,77 @@ int nc_paged_build(nc_module module, const int32_t *cached_lens, size_t cached_l
 
     nc_paged_build_args a;
     std::memset(&a, 0, sizeof a);
-    a.cached = cached_lens;
-    a.fresh = new_lens;
-    a.free_pages = free_pages;
-    a.cursor = cursor;
-    a.table = block_table;
-    a.seq_lens = seq_lens;
-    a.offsets = row_offsets;
-    a.slots = slots;
-    a.counts = counts;
+    a.cached = t.cached_lens;
+    a.fresh = t.new_lens;
+    a.free_pages = t.free_pages;
+    a.cursor = t.cursor;
+    a.table = t.block_table;
+    a.seq_lens = t.seq_lens;
+    a.offsets = t.row_offsets;
+    a.slots = t.slots;
+    a.counts = t.counts;
     a.table_stride = o.table_stride;
     a.num_seqs = (uint32_t)o.num_seqs;
     a.width = (uint32_t)o.max_pages;
     a.num_pages = (uint32_t)o.num_pages;
-    a.free_len = (uint32_t)free_len;
-    a.places = (uint32_t)slots_len;
+    a.free_len = (uint32_t)t.free_len;
+    a.places = (uint32_t)t.slots_len;
     a.ps = nc_paged_make_div((uint32_t)o.page_size);
     const uint32_t threads = o.num_seqs <= 256 ? 256 : 1024;
     // One workgroup up to 4096 slots; beyond, 2048 each.
-    const uint64_t wgs = slots_len <= 4096 ? 1 : std::min<uint64_t>((slots_len + 2047) / 2048, 1024);
-    a.chunk_rows = (uint32_t)((slots_len + wgs - 1) / wgs);
+    const uint64_t wgs = t.slots_len <= 4096 ? 1 : std::min<uint64_t>((t.slots_len + 2047) / 2048, 1024);
+    a.chunk_rows = (uint32_t)((t.slots_len + wgs - 1) / wgs);
     // no more pages than this are taken
-    const uint64_t pages = std::min<uint64_t>(free_len, slots_len / o.page_size + o.num_seqs);
+    const uint64_t pages = std::min<uint64_t>(t.free_len, t.slots_len / o.page_size + o.num_seqs);
     a.chunk_pages = (uint32_t)((pages + wgs - 1) / wgs);
     a.parts = NC_PAGED_PART_PAGES | NC_PAGED_PART_LENS;
     // In place, several workgroups read what one of them would write: the lengths wait for a second launch.
     const bool later = wgs > 1 && (same_lens || same_cursor);
     if (later) a.parts = NC_PAGED_PART_PAGES;
-    st = launch(module, "nc_paged_build", (uint32_t)wgs, threads, &a, stream);
+    st = launch(module, kBuild, (uint32_t)wgs, threads, &a, stream);
     if (st || !later) return st;
     a.parts = NC_PAGED_PART_LENS;
-    return launch(module, "nc_paged_build", 1, threads, &a, stream);
+    return launch(module, kBuild, 1, threads, &a, stream);
 }
 
-int nc_paged_append(nc_module module, const uint16_t *k_rows, size_t k_rows_len, const uint16_t *v_rows,
-                    size_t v_rows_len, const int32_t *slots, size_t slots_len, uint16_t *k_cache, size_t k_len,
-                    uint16_t *v_cache, size_t v_len, uint64_t num_rows, const nc_paged_options *opts,
+int nc_paged_append(nc_module module, const nc_paged_append_buffers *buffers, const nc_paged_options *opts,
                     nc_stream stream) {
+    if (!buffers) return NC_ERROR_INVALID_VALUE;
+    const nc_paged_append_buffers &t = *buffers;
     Shape s;
     int st = resolve(opts, &s);
     if (st) return st;
     const nc_paged_options &o = s.o;
-    if (!module || !k_cache || !v_cache || k_len < s.cache_len || v_len < s.cache_len) return NC_ERROR_INVALID_VALUE;
-    if ((address(k_cache) | address(v_cache)) % 16 || k_cache == v_cache) return NC_ERROR_INVALID_VALUE;
-    if (num_rows == 0) return NC_SUCCESS;
-    if (num_rows > kMost31) return NC_ERROR_OVERFLOW;
-    Axis row[] = {{num_rows, o.row_stride}, {o.num_kv_heads, o.row_head_stride}};
+    if (!module || !t.k_cache || !t.v_cache || t.k_len < s.cache_len || t.v_len < s.cache_len) return NC_ERROR_INVALID_VALUE;
+    if ((address(t.k_cache) | address(t.v_cache)) % 16 || t.k_cache == t.v_cache) return NC_ERROR_INVALID_VALUE;
+    if (t.num_rows == 0) return NC_SUCCESS;
+    if (t.num_rows > kMost31) return NC_ERROR_OVERFLOW;
+    Axis row[] = {{t.num_rows, o.row_stride}, {o.num_kv_heads, o.row_head_stride}};
     uint64_t rows_len = 0;
     st = extent(row, 2, o.head_dim, &rows_len);
     if (st) return st;
-    if (!k_rows || !v_rows || !slots || k_rows_len < rows_len || v_rows_len < rows_len || slots_len < num_rows)
+    if (!t.k_rows || !t.v_rows || !t.slots || t.k_rows_len < rows_len || t.v_rows_len < rows_len || t.slots_len < t.num_rows)
         return NC_ERROR_INVALID_VALUE;
-    if ((address(k_rows) | address(v_rows)) % 2 || address(slots) % 4) return NC_ERROR_INVALID_VALUE;
-    const Range caches[] = {range_of(k_cache, s.cache_len, 2), range_of(v_cache, s.cache_len, 2)};
-    const Range ins[] = {range_of(k_rows, rows_len, 2), range_of(v_rows, rows_len, 2), range_of(slots, num_rows, 4)};
+    if ((address(t.k_rows) | address(t.v_rows)) % 2 || address(t.slots) % 4) return NC_ERROR_INVALID_VALUE;
+    const Range caches[] = {range_of(t.k_cache, s.cache_len, 2), range_of(t.v_cache, s.cache_len, 2)};
+    const Range ins[] = {range_of(t.k_rows, rows_len, 2), range_of(t.v_rows, rows_len, 2), range_of(t.slots, t.num_rows, 4)};
     for (const Range &x : caches)
         for (const Range &y : ins)
             if (overlap(x, y)) return nc_internal_fail(NC_ERROR_INVALID_VALUE, "nc_paged_append: the rows overlap the cache");
 
     nc_paged_append_args a;
     std::memset(&a, 0, sizeof a);
-    a.k_rows = k_rows;
-    a.v_rows = v_rows;
-    a.slots = slots;
-    a.k = k_cache;
-    a.v = v_cache;
+    a.k_rows = t.k_rows;
+    a.v_rows = t.v_rows;
+    a.slots = t.slots;
+    a.k = t.k_cache;
+    a.v = t.v_cache;
     a.row_stride = o.row_stride;
     a.row_head_stride = o.row_head_stride;
     a.page_stride = o.page_stride;
     a.head_stride = o.head_stride;
     a.token_stride = o.token_stride;
-    a.num_rows = num_rows;
+    a.num_rows = t.num_rows;
     a.num_slots = (uint32_t)(o.num_pages * o.page_size);
     a.ps = nc_paged_make_div((uint32_t)o.page_size);
     const uint64_t chunks = o.num_kv_heads * (o.head_dim / 8);
@@ -290,34 +302,34 @@ int nc_paged_append(nc_module module, const uint16_t *k_rows, size_t k_rows_len,
     a.chunks = nc_paged_make_div((uint32_t)chunks);
     a.chunk_shift = o.head_dim == 16 ? 1 : o.head_dim == 32 ? 2 : o.head_dim == 64 ? 3 : 4;
     // about 1024 chunks a workgroup, and no more than 2^23 workgroups
-    a.wg_rows = (uint32_t)std::max<uint64_t>(std::max<uint64_t>(1, 1024 / chunks), (num_rows + (1u << 23) - 1) >> 23);
+    a.wg_rows = (uint32_t)std::max<uint64_t>(std::max<uint64_t>(1, 1024 / chunks), (t.num_rows + (1u << 23) - 1) >> 23);
     if (a.wg_rows * chunks > kMost31) return NC_ERROR_OVERFLOW;
-    const bool vec = (address(k_rows) | address(v_rows)) % 16 == 0 && (o.row_stride | o.row_head_stride) % 8 == 0;
-    return launch(module, vec ? "nc_paged_append_rows" : "nc_paged_append_rows_unaligned",
-                  (uint32_t)((num_rows + a.wg_rows - 1) / a.wg_rows), 256, &a, stream);
+    const bool vec = (address(t.k_rows) | address(t.v_rows)) % 16 == 0 && (o.row_stride | o.row_head_stride) % 8 == 0;
+    return launch(module, vec ? kAppend : kAppendUnaligned,
+                  (uint32_t)((t.num_rows + a.wg_rows - 1) / a.wg_rows), 256, &a, stream);
 }
 
-int nc_paged_decode(nc_module module, const uint16_t *q, size_t q_len, const uint16_t *k_cache, size_t k_len,
-                    const uint16_t *v_cache, size_t v_len, const int32_t *block_table, size_t table_len,
-                    const int32_t *seq_lens, size_t lens_len, float *o, size_t o_len, void *workspace,
-                    uint64_t workspace_bytes, const nc_paged_options *opts, nc_stream stream) {
+int nc_paged_decode(nc_module module, const nc_paged_decode_buffers *buffers, const nc_paged_options *opts,
+                    nc_stream stream) {
+    if (!buffers) return NC_ERROR_INVALID_VALUE;
+    const nc_paged_decode_buffers &t = *buffers;
     Shape s;
     int st = resolve(opts, &s);
     if (st) return st;
     const nc_paged_options &op = s.o;
     const DecodePlan plan = decode_plan(s);
     const uint64_t need = plan.bytes;
-    if (!module || !q || !k_cache || !v_cache || !block_table || !seq_lens || !o || !workspace)
+    if (!module || !t.q || !t.k_cache || !t.v_cache || !t.block_table || !t.seq_lens || !t.o || !t.workspace)
         return NC_ERROR_INVALID_VALUE;
-    if (q_len < s.q_len || k_len < s.cache_len || v_len < s.cache_len || table_len < s.table_len ||
-        lens_len < op.num_seqs || o_len < s.o_len || workspace_bytes < need)
+    if (t.q_len < s.q_len || t.k_len < s.cache_len || t.v_len < s.cache_len || t.table_len < s.table_len ||
+        t.lens_len < op.num_seqs || t.o_len < s.o_len || t.workspace_bytes < need)
         return NC_ERROR_INVALID_VALUE;
-    if ((address(k_cache) | address(v_cache) | address(workspace)) % 16 || address(q) % 2 ||
-        (address(block_table) | address(seq_lens) | address(o)) % 4)
+    if ((address(t.k_cache) | address(t.v_cache) | address(t.workspace)) % 16 || address(t.q) % 2 ||
+        (address(t.block_table) | address(t.seq_lens) | address(t.o)) % 4)
         return NC_ERROR_INVALID_VALUE;
-    const Range outs[] = {range_of(o, s.o_len, 4), range_of(workspace, need, 1)};
-    const Range ins[] = {range_of(q, s.q_len, 2), range_of(k_cache, s.cache_len, 2), range_of(v_cache, s.cache_len, 2),
-                         range_of(block_table, s.table_len, 4), range_of(seq_lens, op.num_seqs, 4)};
+    const Range outs[] = {range_of(t.o, s.o_len, 4), range_of(t.workspace, need, 1)};
+    const Range ins[] = {range_of(t.q, s.q_len, 2), range_of(t.k_cache, s.cache_len, 2), range_of(t.v_cache, s.cache_len, 2),
+                         range_of(t.block_table, s.table_len, 4), range_of(t.seq_lens, op.num_seqs, 4)};
     bool bad = overlap(outs[0], outs[1]);
     for (const Range &x : outs)
         for (const Range &y : ins) bad = bad || overlap(x, y);
@@ -325,15 +337,15 @@ int nc_paged_decode(nc_module module, const uint16_t *q, size_t q_len, const uin
 
     nc_paged_decode_args a;
     std::memset(&a, 0, sizeof a);
-    a.q = q;
-    a.k = k_cache;
-    a.v = v_cache;
-    a.table = block_table;
-    a.seq_lens = seq_lens;
-    a.o = o;
-    a.counters = static_cast<uint32_t *>(workspace);
-    a.part_ml = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.piece_ml);
-    a.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.piece_o);
+    a.q = t.q;
+    a.k = t.k_cache;
+    a.v = t.v_cache;
+    a.table = t.block_table;
+    a.seq_lens = t.seq_lens;
+    a.o = t.o;
+    a.counters = static_cast<uint32_t *>(t.workspace);
+    a.part_ml = reinterpret_cast<float *>(static_cast<char *>(t.workspace) + plan.piece_ml);
+    a.part_o = reinterpret_cast<float *>(static_cast<char *>(t.workspace) + plan.piece_o);
     a.rows = plan.rows;
     a.long_log2 = plan.long_log2;
     a.short_log2 = plan.short_log2;
@@ -343,8 +355,8 @@ int nc_paged_decode(nc_module module, const uint16_t *q, size_t q_len, const uin
     // A piece is written and read once more: at most a quarter of what its run reads of the cache.
     const uint32_t block_keys = nc_paged_step_keys((uint32_t)op.head_dim) * (NC_PAGED_WAVES >> a.wave_shift);
     a.each_least = std::max(1u, 8 * a.rows / block_keys);
-    a.q_vec = address(q) % 16 == 0 && (op.q_stride | op.q_head_stride) % 8 == 0;
-    a.o_vec = address(o) % 16 == 0 && (op.o_stride | op.o_head_stride) % 4 == 0;
+    a.q_vec = address(t.q) % 16 == 0 && (op.q_stride | op.q_head_stride) % 8 == 0;
+    a.o_vec = address(t.o) % 16 == 0 && (op.o_stride | op.o_head_stride) % 4 == 0;
     a.table_stride = op.table_stride;
     a.page_stride = op.page_stride;
     a.head_stride = op.head_stride;
@@ -361,7 +373,7 @@ int nc_paged_decode(nc_module module, const uint16_t *q, size_t q_len, const uin
     a.max_tokens = (uint32_t)(op.max_pages * op.page_size);
     a.scale = op.scale;
     a.ps = nc_paged_make_div((uint32_t)op.page_size);
-    return launch(module, plan.name, plan.grid, 64 * NC_PAGED_WAVES, &a, stream);
+    return launch(module, plan.kernel, plan.grid, 64 * NC_PAGED_WAVES, &a, stream);
 }
 
 }  // extern "C"

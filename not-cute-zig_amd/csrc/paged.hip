@@ -608,12 +608,13 @@ struct Decode {
     }
 
     // The pieces of workgroups first..last of one request and head: added in an order that does not depend on who
-    // came last, and written to O. Four columns of a row are a thread's; where that leaves threads over, groups of
-    // them take every so many-th piece and are added up through LDS. PF pieces are on their way at a time.
+    // came last, and written to O. Four columns of a row are a thread's, and PF pieces are on their way at a time; where
+    // there are more, and threads over, groups of them take every so many-th piece and are added up through LDS.
     template <int PF>
     __device__ __forceinline__ void join_pieces(uint32_t first, uint32_t last, uint32_t rows, float *o) {
         const Args a = again(args);
-        const uint32_t items = rows * (D / 4), groups = items > THREADS / 2 ? 1u : THREADS / items, piece_rows = a->rows;
+        const uint32_t items = rows * (D / 4), piece_rows = a->rows;
+        const uint32_t groups = items > THREADS / 2 ? 1u : min(THREADS / items, (last - first) / PF + 1u);
         const float *part_ml = a->part_ml, *part_o = a->part_o;
         floatx4 *s_sum = reinterpret_cast<floatx4 *>(&s_o[0][0][0]);  // one per thread, and behind them (max, sum)
         float *s_stat = reinterpret_cast<float *>(s_sum + THREADS);

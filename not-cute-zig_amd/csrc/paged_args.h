@@ -26,6 +26,8 @@ NC_HD uint32_t nc_paged_quot(uint32_t n, nc_paged_div v) {
     return (uint32_t)(((uint64_t)(2u * n) * v.magic) >> 32) >> v.shift;
 }
 
+#define NC_PAGED_KERNELS 19u // kernels of paged.hip
+
 struct nc_paged_build_args {
     const int32_t *cached, *fresh, *free_pages, *cursor;
     int32_t *table, *seq_lens, *offsets, *slots, *counts;

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import Optional, Sequence
 
 import numpy as np
@@ -264,12 +265,9 @@ _SIGS = {
     "nc_paged_options_init": (None, [ctypes.POINTER(PagedOptions)]),
     "nc_paged_validate": (ctypes.c_int, [ctypes.POINTER(PagedOptions)]),
     "nc_paged_workspace_bytes": (_U64, [ctypes.POINTER(PagedOptions)]),
-    "nc_paged_build": (
-        ctypes.c_int, [_P] + [_P, ctypes.c_size_t] * 9 + [ctypes.POINTER(PagedOptions), _P]),
-    "nc_paged_append": (
-        ctypes.c_int, [_P] + [_P, ctypes.c_size_t] * 5 + [_U64, ctypes.POINTER(PagedOptions), _P]),
-    "nc_paged_decode": (
-        ctypes.c_int, [_P] + [_P, ctypes.c_size_t] * 6 + [_P, _U64, ctypes.POINTER(PagedOptions), _P]),
+    "nc_paged_build": (ctypes.c_int, [_P, _P, _P, _P]),
+    "nc_paged_append": (ctypes.c_int, [_P, _P, _P, _P]),
+    "nc_paged_decode": (ctypes.c_int, [_P, _P, _P, _P]),
     "nc_benchmark_options_init": (None, [ctypes.POINTER(BenchmarkOptions)]),
     "nc_benchmark_run_kernel": (
         ctypes.c_int,
@@ -686,6 +684,13 @@ def flash_launch(module: Module, q: DeviceBuffer, k: DeviceBuffer, v: DeviceBuff
 # paged key-value cache (include/notcute_paged.h)
 # ---------------------------------------------------------------------------------------------
 
+# nc_paged_{build,append,decode}_buffers, packed in one go: pointers and lengths one by one as ctypes arguments take
+# twice the time of the rest of such a call.
+_BUILD_BUFFERS = struct.Struct("=18Q")
+_APPEND_BUFFERS = struct.Struct("=11Q")
+_DECODE_BUFFERS = struct.Struct("=14Q")
+
+
 def paged_options(*, head_dim: int, page_size: int, num_pages: int, num_seqs: int = 1, num_q_heads: int = 1,
                   num_kv_heads: Optional[int] = None, max_pages: int = 1, table_stride: int = 0, page_stride: int = 0,
                   head_stride: int = 0, token_stride: int = 0, row_stride: int = 0, row_head_stride: int = 0,
@@ -729,11 +734,13 @@ def paged_build(module: Module, cached_lens: DeviceBuffer, new_lens: DeviceBuffe
     """Block tables, slot map and row offsets of a step from the requests' lengths (nc_paged_build). Every
     buffer holds int32; the whole of `slots` is written and the whole of `free_pages` is the list. seq_lens may
     be cached_lens, and counts may be cursor."""
-    check(lib().nc_paged_build(
-        module.handle, cached_lens.ptr, cached_lens.nbytes >> 2, new_lens.ptr, new_lens.nbytes >> 2, free_pages.ptr,
+    st = (_lib or lib()).nc_paged_build(module.handle, _BUILD_BUFFERS.pack(
+        cached_lens.ptr, cached_lens.nbytes >> 2, new_lens.ptr, new_lens.nbytes >> 2, free_pages.ptr,
         free_pages.nbytes >> 2, cursor.ptr, cursor.nbytes >> 2, block_table.ptr, block_table.nbytes >> 2, seq_lens.ptr,
         seq_lens.nbytes >> 2, row_offsets.ptr, row_offsets.nbytes >> 2, slots.ptr, slots.nbytes >> 2, counts.ptr,
-        counts.nbytes >> 2, ctypes.byref(opts), stream), "paged.build")
+        counts.nbytes >> 2), ctypes.byref(opts), stream)
+    if st:
+        check(st, "paged.build")
 
 
 def paged_append(module: Module, k_rows: DeviceBuffer, v_rows: DeviceBuffer, slots: DeviceBuffer,
@@ -745,9 +752,11 @@ def paged_append(module: Module, k_rows: DeviceBuffer, v_rows: DeviceBuffer, slo
     n = places if num_rows is None else num_rows
     if n < 0:
         raise ValueError(f"paged_append: num_rows {n}")
-    check(lib().nc_paged_append(
-        module.handle, k_rows.ptr, k_rows.nbytes >> 1, v_rows.ptr, v_rows.nbytes >> 1, slots.ptr, places, k_cache.ptr,
-        k_cache.nbytes >> 1, v_cache.ptr, v_cache.nbytes >> 1, n, ctypes.byref(opts), stream), "paged.append")
+    st = (_lib or lib()).nc_paged_append(module.handle, _APPEND_BUFFERS.pack(
+        k_rows.ptr, k_rows.nbytes >> 1, v_rows.ptr, v_rows.nbytes >> 1, slots.ptr, places, k_cache.ptr,
+        k_cache.nbytes >> 1, v_cache.ptr, v_cache.nbytes >> 1, n), ctypes.byref(opts), stream)
+    if st:
+        check(st, "paged.append")
 
 
 def paged_decode(module: Module, q: DeviceBuffer, k_cache: DeviceBuffer, v_cache: DeviceBuffer,
@@ -755,10 +764,12 @@ def paged_decode(module: Module, q: DeviceBuffer, k_cache: DeviceBuffer, v_cache
                  opts: PagedOptions, stream: Optional[int] = None) -> None:
     """Attention of one new token per request over its pages (nc_paged_decode); `workspace` is
     paged_workspace(opts) or a zeroed buffer of paged_workspace_bytes(opts) and more."""
-    check(lib().nc_paged_decode(
-        module.handle, q.ptr, q.nbytes >> 1, k_cache.ptr, k_cache.nbytes >> 1, v_cache.ptr, v_cache.nbytes >> 1,
-        block_table.ptr, block_table.nbytes >> 2, seq_lens.ptr, seq_lens.nbytes >> 2, o.ptr, o.nbytes >> 2,
-        workspace.ptr, workspace.nbytes, ctypes.byref(opts), stream), "paged.decode")
+    st = (_lib or lib()).nc_paged_decode(module.handle, _DECODE_BUFFERS.pack(
+        q.ptr, q.nbytes >> 1, k_cache.ptr, k_cache.nbytes >> 1, v_cache.ptr, v_cache.nbytes >> 1, block_table.ptr,
+        block_table.nbytes >> 2, seq_lens.ptr, seq_lens.nbytes >> 2, o.ptr, o.nbytes >> 2, workspace.ptr,
+        workspace.nbytes), ctypes.byref(opts), stream)
+    if st:
+        check(st, "paged.decode")
 
 
 # ---------------------------------------------------------------------------------------------
