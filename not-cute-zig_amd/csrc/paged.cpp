@@ -240,9 +240,9 @@ int nc_paged_build(nc_module module, const nc_paged_build_buffers *buffers, cons
     a.free_len = (uint32_t)t.free_len;
     a.places = (uint32_t)t.slots_len;
     a.ps = nc_paged_make_div((uint32_t)o.page_size);
-    const uint32_t threads = o.num_seqs <= 256 ? 256 : 1024;
-    // One workgroup up to 4096 slots; beyond, 2048 each.
-    const uint64_t wgs = t.slots_len <= 4096 ? 1 : std::min<uint64_t>((t.slots_len + 2047) / 2048, 1024);
+    const uint32_t threads = o.num_seqs <= 64 ? 64 : o.num_seqs <= 256 ? 256 : 1024;
+    // One workgroup up to 4096 slots (and as many threads as the requests need); beyond, a few slots a thread.
+    const uint64_t wgs = t.slots_len <= 4096 ? 1 : std::min<uint64_t>((t.slots_len + 4 * threads - 1) / (4 * threads), 1024);
     a.chunk_rows = (uint32_t)((t.slots_len + wgs - 1) / wgs);
     // no more pages than this are taken
     const uint64_t pages = std::min<uint64_t>(t.free_len, t.slots_len / o.page_size + o.num_seqs);
@@ -301,8 +301,8 @@ int nc_paged_append(nc_module module, const nc_paged_append_buffers *buffers, co
     if (chunks > kMost31 / 2) return NC_ERROR_OVERFLOW;
     a.chunks = nc_paged_make_div((uint32_t)chunks);
     a.chunk_shift = o.head_dim == 16 ? 1 : o.head_dim == 32 ? 2 : o.head_dim == 64 ? 3 : 4;
-    // about 1024 chunks a workgroup, and no more than 2^23 workgroups
-    a.wg_rows = (uint32_t)std::max<uint64_t>(std::max<uint64_t>(1, 1024 / chunks), (t.num_rows + (1u << 23) - 1) >> 23);
+    // a chunk a thread, and no more than 2^23 workgroups
+    a.wg_rows = (uint32_t)std::max<uint64_t>(std::max<uint64_t>(1, 256 / chunks), (t.num_rows + (1u << 23) - 1) >> 23);
     if (a.wg_rows * chunks > kMost31) return NC_ERROR_OVERFLOW;
     const bool vec = (address(t.k_rows) | address(t.v_rows)) % 16 == 0 && (o.row_stride | o.row_head_stride) % 8 == 0;
     return launch(module, vec ? kAppend : kAppendUnaligned,

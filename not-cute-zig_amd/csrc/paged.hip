@@ -18,13 +18,19 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
-__device__ __forceinline__ uint64_t wave_scan(uint64_t x, uint32_t lane) {
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-        const uint64_t y = __shfl_up(x, d, 64);
-        if (lane >= d) x += y;
-    }
+// Inclusive sums over the wave's lanes.
+__device__ __forceinline__ uint32_t wave_scan32(uint32_t x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1, 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2, 3
     return x;
+}
+// Of numbers below 2^32, whose sums may pass that: their halves' sums do not.
+__device__ __forceinline__ uint64_t wave_scan64(uint32_t x) {
+    return wave_scan32(x & 0xffffu) + ((uint64_t)wave_scan32(x >> 16) << 16);
 }
 
 // Largest j in [0, n) with s[j] <= x, for s ascending and s[0] <= x; n is a power of two.
@@ -38,14 +44,17 @@ __device__ __forceinline__ uint32_t last_not_above(const uint32_t *s, uint32_t n
 }  // namespace
 
 // -------------------------------------------------------------------------------------------------
-// Block tables, slot map and offsets. Two prefix sums over the requests (new rows, pages taken), then
-// every slot and every new table entry finds its request by a binary search of them. Each workgroup
-// scans all requests, a workgroup's threads at a time, and does its own share of the slots and of the list:
-// for a step of one token a request the scan is all there is, and one workgroup does everything.
+// Block tables, slot map and offsets: two prefix sums over the requests (new rows, pages taken). For a step of
+// few tokens a request one workgroup does it all, and a request's thread writes its own slots and table entries.
+// Else every slot and every new table entry finds its request by a binary search of the sums; each workgroup
+// scans all requests, a workgroup's threads at a time, and does its own share of the slots and of the list.
+// Latency is all there is: the lengths, the list's pages behind the sums, the stores.
 // -------------------------------------------------------------------------------------------------
 extern "C" __global__ __launch_bounds__(1024) void nc_paged_build(const nc_paged_build_args a) {
+    enum : uint8_t { kRefused, kGranted, kDone };
+    constexpr uint32_t kFew = 8;  // rows that a request's thread writes itself
     __shared__ uint32_t s_row[1024], s_first[1024], s_held[1024], s_cached[1024];
-    __shared__ uint8_t s_ok[1024];
+    __shared__ uint8_t s_state[1024];
     __shared__ uint64_t s_rows[16], s_pages[16];
     __shared__ uint32_t s_taken, s_refused;
 
@@ -71,41 +80,64 @@ extern "C" __global__ __launch_bounds__(1024) void nc_paged_build(const nc_paged
         }
         uint32_t held = nc_paged_quot(c, a.ps);
         held += held * a.ps.d != c;
-        const bool fits = (uint64_t)c + n <= most;
+        const bool fits = (uint64_t)c + n <= most, few = gridDim.x == 1 && n <= kFew;
+        int32_t *row = a.table + r * a.table_stride;
+        int32_t open = -1;  // the page that the cached tokens end in, if it has places left
+        if (pages_part && few && n && fits && held * a.ps.d != c) open = row[held - 1];
         uint32_t take = 0;
         if (fits) {
             const uint32_t need = nc_paged_quot(c + n, a.ps);
             take = need + (need * a.ps.d != c + n) - held;
         }
-        const uint64_t rs = wave_scan(n, lane), ps = wave_scan(take, lane);
-        if (lane == 63) {
-            s_rows[w] = rs;
-            s_pages[w] = ps;
-        }
-        __syncthreads();
+        const uint64_t rs = wave_scan64(n), ps = wave_scan64(take);
         uint64_t row0 = rows + rs - n, first = pages + ps - take, row_end = rows, page_end = pages;
-        for (uint32_t i = 0; i < nw; ++i) {
-            const uint64_t x = s_rows[i], y = s_pages[i];
-            if (i < w) {
-                row0 += x;
-                first += y;
+        if (nw > 1) {
+            if (lane == 63) {
+                s_rows[w] = rs;
+                s_pages[w] = ps;
             }
-            row_end += x;
-            page_end += y;
+            __syncthreads();
+            for (uint32_t i = 0; i < nw; ++i) {
+                const uint64_t x = s_rows[i], y = s_pages[i];
+                if (i < w) {
+                    row0 += x;
+                    first += y;
+                }
+                row_end += x;
+                page_end += y;
+            }
+        } else {
+            row_end += __shfl(rs, 63, 64);
+            page_end += __shfl(ps, 63, 64);
         }
         const bool ok = fits && (n == 0 || row0 + n <= a.places) && (take == 0 || first + take <= a.free_len);
-        if (pages_part) {
+        if (pages_part && few) {
+            int32_t page = open;
+            uint32_t in = c - (held - 1u) * a.ps.d;  // the next token's place in it; past its end without one
+            uint64_t from = first;
+            for (uint32_t t = 0; t < n && row0 + t < a.places; ++t) {
+                if (ok && in == a.ps.d) {
+                    row[held + (from - first)] = page = a.free_pages[from];
+                    ++from;
+                    in = 0;
+                }
+                a.slots[row0 + t] = ok && (uint32_t)page < a.num_pages ? (int32_t)((uint32_t)page * a.ps.d + in) : -1;
+                ++in;
+            }
+        }
+        if (pages_part && __syncthreads_or(!few)) {
             s_row[tid] = (uint32_t)min(row0, (uint64_t)a.places);
             s_first[tid] = (uint32_t)min(first, (uint64_t)a.free_len);
             s_held[tid] = held;
             s_cached[tid] = c;
-            s_ok[tid] = ok;
+            s_state[tid] = few ? kDone : ok ? kGranted : kRefused;
             __syncthreads();
             const uint64_t lo = max(min(rows, (uint64_t)a.places), row_lo), hi = min(row_end, row_hi);
             for (uint64_t i = lo + tid; i < hi; i += nt) {
                 const uint32_t j = last_not_above(s_row, nt, (uint32_t)i);
                 int32_t slot = -1;
-                if (s_ok[j]) {
+                if (s_state[j] == kDone) continue;
+                if (s_state[j] == kGranted) {
                     const uint32_t pos = s_cached[j] + ((uint32_t)i - s_row[j]);
                     const uint32_t at = nc_paged_quot(pos, a.ps), h = s_held[j];
                     const int32_t page = at < h ? a.table[(t0 + j) * a.table_stride + at] : a.free_pages[s_first[j] + at - h];
@@ -116,7 +148,7 @@ extern "C" __global__ __launch_bounds__(1024) void nc_paged_build(const nc_paged
             const uint64_t plo = max(pages, list_lo), phi = min(page_end, list_hi);
             for (uint64_t e = plo + tid; e < phi; e += nt) {
                 const uint32_t j = last_not_above(s_first, nt, (uint32_t)e);
-                if (s_ok[j]) a.table[(t0 + j) * a.table_stride + s_held[j] + ((uint32_t)e - s_first[j])] = a.free_pages[e];
+                if (s_state[j] == kGranted) a.table[(t0 + j) * a.table_stride + s_held[j] + ((uint32_t)e - s_first[j])] = a.free_pages[e];
             }
         }
         if (lens && r < a.num_seqs) {
@@ -132,7 +164,7 @@ extern "C" __global__ __launch_bounds__(1024) void nc_paged_build(const nc_paged
     if (pages_part)  // padding behind the last row
         for (uint64_t i = max(min(rows, (uint64_t)a.places), row_lo) + tid; i < row_hi; i += nt) a.slots[i] = -1;
     if (lens) {
-        const uint32_t tk = (uint32_t)wave_scan(taken, lane), rf = (uint32_t)wave_scan(refused, lane);
+        const uint32_t tk = wave_scan32(taken), rf = wave_scan32(refused);
         if (lane == 63) {
             atomicAdd(&s_taken, tk);
             atomicAdd(&s_refused, rf);
@@ -150,20 +182,22 @@ extern "C" __global__ __launch_bounds__(1024) void nc_paged_build(const nc_paged
 }
 
 // -------------------------------------------------------------------------------------------------
-// Row append: a copy, 16 bytes of K and of V per thread and step. VEC: the rows are 16-byte aligned.
+// Row append: a copy, 16 bytes of K and of V per thread (more in flight per thread, or four times the rows per
+// workgroup, took 2-25 % longer). What bounds it is the copy's rate. Streaming stores: 30000 rows x 8 heads x 64, off
+// alignment, 26.1 -> 20.5 us (6.0 TB/s of rows read and written), 2048 x 8 x 128 4.1 -> 3.6 us; but where a head's
+// row is 32 bytes and stands alone (page size 1) 8.7 -> 10.7 us, so not for head_dim 16. VEC: the rows are
+// 16-byte aligned.
 // -------------------------------------------------------------------------------------------------
 namespace {
 
 template <bool VEC>
 __device__ __forceinline__ u32x4 load8(const uint16_t *p) {
-    if constexpr (VEC) {
-        return *reinterpret_cast<const u32x4 *>(p);
-    } else {
-        u32x4 r;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = uint32_t(p[2 * i]) | (uint32_t(p[2 * i + 1]) << 16);
-        return r;
-    }
+    u32x4 r;
+    if constexpr (VEC)
+        r = *reinterpret_cast<const u32x4 *>(p);
+    else
+        __builtin_memcpy(&r, p, 16);  // one load: global memory takes them at any alignment
+    return r;
 }
 
 template <bool VEC>
@@ -179,8 +213,14 @@ __device__ __forceinline__ void append_body(const nc_paged_append_args &a) {
         const uint64_t src = (row0 + i) * a.row_stride + h * a.row_head_stride + 8 * x;
         const uint64_t dst = page * a.page_stride + h * a.head_stride + t * a.token_stride + 8 * x;
         const u32x4 kv = load8<VEC>(a.k_rows + src), vv = load8<VEC>(a.v_rows + src);
-        *reinterpret_cast<u32x4 *>(a.k + dst) = kv;
-        *reinterpret_cast<u32x4 *>(a.v + dst) = vv;
+        u32x4 *kd = reinterpret_cast<u32x4 *>(a.k + dst), *vd = reinterpret_cast<u32x4 *>(a.v + dst);
+        if (a.chunk_shift > 1) {
+            __builtin_nontemporal_store(kv, kd);
+            __builtin_nontemporal_store(vv, vd);
+        } else {
+            *kd = kv;
+            *vd = vv;
+        }
     }
 }
 
@@ -266,16 +306,6 @@ __device__ __forceinline__ float quad_sum(float x) {
     x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
     auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
-__device__ __forceinline__ uint32_t wave_scan32(uint32_t x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1, 3
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2, 3
-    return x;
 }
 
 // Partials go between workgroups of different XCDs, whose L2 caches are not coherent for ordinary accesses:
