@@ -118,13 +118,14 @@ uintptr_t address(const void *p) { return reinterpret_cast<uintptr_t>(p); }
 
 // Every kernel of paged.hip by its place here, under which the module keeps its function.
 const char *const kKernels[] = {
-    "nc_paged_build",          "nc_paged_append_rows",       "nc_paged_append_rows_unaligned",
+    "nc_paged_build",          "nc_paged_append_rows",      "nc_paged_append_rows_unaligned",
+    "nc_paged_append_rows_d16", "nc_paged_append_rows_d16_unaligned",
     "nc_paged_decode_d16",     "nc_paged_decode_d16_bf16",   "nc_paged_decode_d16_odd",  "nc_paged_decode_d16_odd_bf16",
     "nc_paged_decode_d32",     "nc_paged_decode_d32_bf16",   "nc_paged_decode_d32_odd",  "nc_paged_decode_d32_odd_bf16",
     "nc_paged_decode_d64",     "nc_paged_decode_d64_bf16",   "nc_paged_decode_d64_odd",  "nc_paged_decode_d64_odd_bf16",
     "nc_paged_decode_d128",    "nc_paged_decode_d128_bf16",  "nc_paged_decode_d128_odd", "nc_paged_decode_d128_odd_bf16",
 };
-enum : uint32_t { kBuild, kAppend, kAppendUnaligned, kDecode };
+enum : uint32_t { kBuild, kAppend, kAppendD16 = kAppend + 2, kDecode = kAppend + 4 };
 
 int launch(nc_module module, uint32_t kernel, uint32_t grid, uint32_t threads, void *args, nc_stream stream) {
     nc_function fn = nullptr;
@@ -305,7 +306,7 @@ int nc_paged_append(nc_module module, const nc_paged_append_buffers *buffers, co
     a.wg_rows = (uint32_t)std::max<uint64_t>(std::max<uint64_t>(1, 256 / chunks), (t.num_rows + (1u << 23) - 1) >> 23);
     if (a.wg_rows * chunks > kMost31) return NC_ERROR_OVERFLOW;
     const bool vec = (address(t.k_rows) | address(t.v_rows)) % 16 == 0 && (o.row_stride | o.row_head_stride) % 8 == 0;
-    return launch(module, vec ? kAppend : kAppendUnaligned,
+    return launch(module, (o.head_dim == 16 ? kAppendD16 : kAppend) + (vec ? 0 : 1),
                   (uint32_t)((t.num_rows + a.wg_rows - 1) / a.wg_rows), 256, &a, stream);
 }
 

@@ -200,7 +200,7 @@ __device__ __forceinline__ u32x4 load8(const uint16_t *p) {
     return r;
 }
 
-template <bool VEC>
+template <bool VEC, bool STREAM>
 __device__ __forceinline__ void append_body(const nc_paged_append_args &a) {
     const uint64_t row0 = (uint64_t)blockIdx.x * a.wg_rows;
     const uint32_t rows = (uint32_t)min((uint64_t)a.wg_rows, a.num_rows - row0), total = rows * a.chunks.d;
@@ -214,7 +214,7 @@ __device__ __forceinline__ void append_body(const nc_paged_append_args &a) {
         const uint64_t dst = page * a.page_stride + h * a.head_stride + t * a.token_stride + 8 * x;
         const u32x4 kv = load8<VEC>(a.k_rows + src), vv = load8<VEC>(a.v_rows + src);
         u32x4 *kd = reinterpret_cast<u32x4 *>(a.k + dst), *vd = reinterpret_cast<u32x4 *>(a.v + dst);
-        if (a.chunk_shift > 1) {
+        if constexpr (STREAM) {
             __builtin_nontemporal_store(kv, kd);
             __builtin_nontemporal_store(vv, vd);
         } else {
@@ -226,10 +226,14 @@ __device__ __forceinline__ void append_body(const nc_paged_append_args &a) {
 
 }  // namespace
 
-extern "C" __global__ __launch_bounds__(256) void nc_paged_append_rows(const nc_paged_append_args a) { append_body<true>(a); }
-extern "C" __global__ __launch_bounds__(256) void nc_paged_append_rows_unaligned(const nc_paged_append_args a) {
-    append_body<false>(a);
-}
+#define NC_APPEND(T, VEC, STREAM)                                                                                     \
+    extern "C" __global__ __launch_bounds__(256) void nc_paged_append_rows##T(const nc_paged_append_args a) {          \
+        append_body<VEC, STREAM>(a);                                                                                  \
+    }
+NC_APPEND(, true, true)
+NC_APPEND(_unaligned, false, true)
+NC_APPEND(_d16, true, false)
+NC_APPEND(_d16_unaligned, false, false)
 
 // -------------------------------------------------------------------------------------------------
 // Single-token attention. Up to 16 query heads of one key head are the 16 columns of the matrix products, so
