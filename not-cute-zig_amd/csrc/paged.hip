@@ -97,15 +97,20 @@ extern "C" __global__ __launch_bounds__(1024) void nc_paged_build(const nc_paged
                 s_pages[w] = ps;
             }
             __syncthreads();
-            for (uint32_t i = 0; i < nw; ++i) {
-                const uint64_t x = s_rows[i], y = s_pages[i];
-                if (i < w) {
-                    row0 += x;
-                    first += y;
+            // the waves' sums, summed by every wave: lane i has those of waves 0..i
+            uint64_t x = lane < nw ? s_rows[lane] : 0, y = lane < nw ? s_pages[lane] : 0;
+#pragma unroll
+            for (uint32_t d = 1; d < 16; d <<= 1) {
+                const uint64_t u = __shfl_up(x, d, 16), v = __shfl_up(y, d, 16);
+                if ((lane & 15u) >= d) {
+                    x += u;
+                    y += v;
                 }
-                row_end += x;
-                page_end += y;
             }
+            row0 += w ? __shfl(x, w - 1u, 64) : 0;
+            first += w ? __shfl(y, w - 1u, 64) : 0;
+            row_end += __shfl(x, nw - 1u, 64);
+            page_end += __shfl(y, nw - 1u, 64);
         } else {
             row_end += __shfl(rs, 63, 64);
             page_end += __shfl(ps, 63, 64);
