@@ -718,7 +718,7 @@ struct Decode {
     }
 
     __device__ __forceinline__ void store_o(float *o, uint32_t q, uint32_t x, floatx4 v, float sum) {
-        const float inv = 1.f / sum;
+        const float inv = __builtin_amdgcn_rcpf(sum);  // to an ulp
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = sum == 0.f ? 0.f : v[i] * inv;
         const Args a = args;
