@@ -11,6 +11,7 @@ runner (modal_run.py:34-69), on one MI355X through the C ABI.
     python flash_harness.py profile-flash --counters DIR   # the same under rocprofv3 counter passes
                                                   # (the Nsight Compute run of modal_run.py:108-146)
     python flash_harness.py benchmark-flash       # runFlashBenchmark (src/main.zig:760-766)
+    python flash_harness.py paged                 # decoding steps over a paged cache (an extension), JSONL
     python flash_harness.py timeline --workload c3    # per-wave timeline of the selected kernel
     python flash_harness.py compare-table FILE... # the baseline-vs-not-cute table (modal_run.py:34-69)
 
@@ -729,6 +730,121 @@ def cmd_timeline(args) -> int:
     return 0
 
 
+# ---------------------------------------------------------------------------------------------
+# paged: a batch of requests through prompt and decoding steps over a paged cache
+# ---------------------------------------------------------------------------------------------
+
+# (requests, query heads, key heads, head_dim, page_size, longest prompt, element type)
+PAGED_CASES = [(1, 8, 8, 64, 16, 100, "f16"), (8, 32, 8, 64, 16, 1000, "f16"), (33, 16, 16, 32, 7, 500, "f16"),
+               (16, 32, 4, 128, 64, 777, "bf16")]
+# Weights keep f32's accuracy, so all that is left is the sums' order and the scores' rounding.
+PAGED_TOL = 1e-4
+
+
+class PagedBatch:
+    """A batch's cache, tables and workspace, and what went into them (for the check)."""
+
+    def __init__(self, seqs, q_heads, kv_heads, head_dim, page_size, longest, dtype, seed=0):
+        self.rng = np.random.default_rng(seed)
+        self.dtype, self.d, self.kv_heads = dtype, head_dim, kv_heads
+        width = -(-(longest + 64) // page_size)
+        self.opts = nc.paged_options(num_seqs=seqs, num_q_heads=q_heads, num_kv_heads=kv_heads, head_dim=head_dim,
+                                     page_size=page_size, num_pages=seqs * width, max_pages=width, dtype=dtype)
+        self.shape_q = (seqs, q_heads, head_dim)
+        cache = seqs * width * kv_heads * page_size * head_dim * 2
+        self.k, self.v = nc.DeviceBuffer(cache), nc.DeviceBuffer(cache)
+        self.free = nc.DeviceBuffer.from_array(self.rng.permutation(seqs * width).astype(np.int32))
+        self.table = nc.DeviceBuffer.from_array(np.full((seqs, width), -1, np.int32))
+        self.lens = nc.DeviceBuffer.from_array(np.zeros(seqs, np.int32))
+        self.counts = nc.DeviceBuffer.from_array(np.zeros(4, np.int32))
+        self.offsets, self.work = nc.DeviceBuffer(4 * (seqs + 1)), nc.paged_workspace(self.opts)
+        self.rows = [[] for _ in range(seqs)]  # (k, v) of every token
+
+    def _random(self, *shape):
+        x = self.rng.standard_normal(shape).astype(np.float32)
+        if self.dtype == "bf16":  # the upper half of a binary32, truncated: as good as any other values
+            return (x.view(np.uint32) >> 16).astype(np.uint16)
+        return x.astype(np.float16).view(np.uint16)
+
+    def step(self, module, new, stream=None):
+        """One step's launches: tables and slots, rows into the cache, attention. Returns O's buffer and Q."""
+        total = int(sum(new))
+        k, v = (self._random(total, self.kv_heads, self.d) for _ in range(2))
+        at = np.concatenate([[0], np.cumsum(new)])
+        for r, rows in enumerate(self.rows):
+            rows += [(k[i], v[i]) for i in range(at[r], at[r + 1])]
+        q = self._random(*self.shape_q)
+        bufs = [nc.DeviceBuffer.from_array(x) for x in (np.asarray(new, np.int32), k, v, q)]
+        slots, o = nc.DeviceBuffer(4 * total), nc.DeviceBuffer(4 * q.size)
+        self.last = (bufs, slots, o)
+
+        nc.paged_build(module, self.lens, bufs[0], self.free, _Part(self.counts, 4), self.table, self.lens, self.offsets,
+                       slots, self.counts, self.opts, stream)
+        nc.paged_append(module, bufs[1], bufs[2], slots, self.k, self.v, self.opts, stream)
+        nc.paged_decode(module, bufs[3], self.k, self.v, self.table, self.lens, o, self.work, self.opts, stream)
+        return o, q
+
+    def reference(self, q):
+        """softmax(scale q K^T) V of every request's tokens in float64."""
+        out = np.zeros(self.shape_q)
+        group = self.shape_q[1] // self.kv_heads
+        qf = decode(q, self.dtype)
+        for r, rows in enumerate(self.rows):
+            if not rows:
+                continue
+            k = decode(np.array([x for x, _ in rows]), self.dtype)
+            v = decode(np.array([x for _, x in rows]), self.dtype)
+            for h in range(self.shape_q[1]):
+                s = float(np.float32(self.opts.scale)) * (k[:, h // group] @ qf[r, h])
+                p = np.exp(s - s.max())
+                out[r, h] = (p / p.sum()) @ v[:, h // group]
+        return out
+
+
+class _Part:
+    """The first bytes of a buffer."""
+
+    def __init__(self, buf, nbytes):
+        self.ptr, self.nbytes = buf.ptr, nbytes
+
+
+def cmd_paged(module: nc.Module, args) -> int:
+    """Prompts of ragged lengths, then single tokens, for each case; every step's attention against float64, and
+    the last step's attention timed by an event pair per launch."""
+    status = 0
+    for seqs, q_heads, kv_heads, d, page_size, longest, dtype in PAGED_CASES:
+        batch = PagedBatch(seqs, q_heads, kv_heads, d, page_size, longest, dtype)
+        shape = f"seqs={seqs},q_heads={q_heads},kv_heads={kv_heads},head={d},page={page_size},longest={longest},{dtype}"
+        prompts = batch.rng.integers(0, longest + 1, seqs)
+        prompts[0] = longest
+        err, refused = 0.0, 0
+        for new in (prompts, np.ones(seqs, int), batch.rng.integers(0, 2, seqs)):
+            if new.sum() == 0:
+                continue
+            o, q = batch.step(module, new)
+            nc.synchronize()
+            refused += int(batch.counts.download(np.int32, 4)[3])
+            err = max(err, float(np.max(np.abs(o.download(np.float32, q.size).reshape(q.shape) - batch.reference(q)))))
+        (_, _, _, qb), _, ob = batch.last
+        start, stop, samples = nc.Event(), nc.Event(), []
+        for i in range(args.warmup + args.iters):
+            start.record()
+            nc.paged_decode(module, qb, batch.k, batch.v, batch.table, batch.lens, ob, batch.work, batch.opts)
+            stop.record()
+            stop.synchronize()
+            if i >= args.warmup:
+                samples.append(nc.Event.elapsed(start, stop))
+        start.destroy()
+        stop.destroy()
+        tokens = sum(len(r) for r in batch.rows)
+        flops, bytes_ = 4 * tokens * q_heads * d, tokens * kv_heads * d * 4 + seqs * q_heads * d * 6
+        ok = err <= PAGED_TOL and refused == 0
+        status |= 0 if ok else 1
+        rec = make_record("not_cute", shape, ok, sum(samples) / len(samples), min(samples), max(samples), bytes_, flops, err)
+        emit({**rec, "kernel": "paged_attention"})
+    return status
+
+
 def cmd_table(args) -> int:
     recs = []
     for path in args.files:
@@ -751,7 +867,8 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
     m.add_argument("--shapes", choices=("reference", "configs"), default="reference")
     m.add_argument("--limit", type=int, default=0, help="only the first N shapes")
     for q in (p, b, m, sub.add_parser("profile-flash", help="attributes and occupancy of the c3 kernel"),
-              sub.add_parser("benchmark-flash", help="runFlashBenchmark's five cases")):
+              sub.add_parser("benchmark-flash", help="runFlashBenchmark's five cases"),
+              sub.add_parser("paged", help="decoding steps over a paged cache, checked and timed (JSONL on stdout)")):
         q.add_argument("--warmup", type=int, default=5)
         q.add_argument("--iters", type=int, default=20)
     pf = sub.choices["profile-flash"]
@@ -780,7 +897,7 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
     nc.init()
     module = nc.Module.load_embedded()
     return {"flash": cmd_flash, "compare": cmd_compare, "profile-flash": cmd_profile,
-            "benchmark-flash": cmd_benchmark, "materialized": cmd_materialized}[args.cmd](module, args)
+            "benchmark-flash": cmd_benchmark, "materialized": cmd_materialized, "paged": cmd_paged}[args.cmd](module, args)
 
 
 if __name__ == "__main__":

@@ -50,6 +50,37 @@ def test_options_layout_matches_binding(tmp_path):
         assert seen[f] == (getattr(nc.PagedOptions, f).offset, ctypes.sizeof(t)), f
 
 
+def test_buffer_blocks_match_binding(tmp_path):
+    """The binding packs a call's pointers and lengths as 8-byte words in the structs' order."""
+    fields = {"build": "cached_lens cached_len new_lens new_len free_pages free_len cursor cursor_len block_table "
+                       "table_len seq_lens seq_len row_offsets offsets_len slots slots_len counts counts_len",
+              "append": "k_rows k_rows_len v_rows v_rows_len slots slots_len k_cache k_len v_cache v_len num_rows",
+              "decode": "q q_len k_cache k_len v_cache v_len block_table table_len seq_lens lens_len o o_len workspace "
+                        "workspace_bytes"}
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "notcute_paged.h"', "int main(void) {"]
+    for name, fs in fields.items():
+        lines.append(f'printf("%zu", sizeof(nc_paged_{name}_buffers));')
+        lines += [f'printf(" %zu", offsetof(nc_paged_{name}_buffers, {f}));' for f in fs.split()]
+        lines.append('printf("\\n");')
+    src = tmp_path / "blocks.c"
+    src.write_text("\n".join(lines + ["return 0; }"]) + "\n")
+    exe = tmp_path / "blocks"
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-Werror", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines()
+    packs = (nc._BUILD_BUFFERS, nc._APPEND_BUFFERS, nc._DECODE_BUFFERS)
+    for line, fs, pack in zip(out, fields.values(), packs):
+        n = len(fs.split())
+        assert [int(x) for x in line.split()] == [8 * n] + [8 * i for i in range(n)]
+        assert pack.size == 8 * n
+
+
+def test_null_blocks_are_refused():
+    for name in ("build", "append", "decode"):
+        f = getattr(nc.lib(), f"nc_paged_{name}")
+        assert nc.STATUS_NAMES[f(0x10, None, ctypes.byref(good()), None)] == INVALID
+        assert nc.STATUS_NAMES[f(0x10, bytes(144), None, None)] == INVALID
+
+
 def test_defaults():
     o = nc.PagedOptions()
     nc.lib().nc_paged_options_init(ctypes.byref(o))

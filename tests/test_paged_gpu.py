@@ -99,7 +99,7 @@ def test_decode_page_sizes(gpu, ps):
     decode_case(gpu, ps + 1, [130, 45], 3, 1, 32, ps, "bf16", layout="nhd")
 
 
-@pytest.mark.parametrize("group", [1, 2, 3, 5, 7, 8, 15, 16, 17, 20, 32, 33, 48, 64])
+@pytest.mark.parametrize("group", [1, 2, 3, 5, 7, 8, 15, 16, 17, 20, 32, 33, 48, 64, 65, 100, 130])
 def test_decode_groups(gpu, group):
     decode_case(gpu, group, [200, 3, 0, 64], 2, group, 64, 16)
     decode_case(gpu, group + 500, [77], 1, group, 128, 24, "bf16")
@@ -130,6 +130,56 @@ def test_decode_many_requests(gpu, count):
     lens[rng.random(count) < 0.2] = 0
     lens[-1] = 0
     decode_case(gpu, count, lens.tolist(), 1, 2, 32, 16)
+
+
+def test_decode_more_requests_than_lanes_twice(gpu):
+    """Over 64 requests a lane of the wave that finds a workgroup's first."""
+    rng = np.random.default_rng(5)
+    lens = rng.integers(0, 3, 4500)
+    lens[[700, 4499]] = [900, 40]
+    decode_case(gpu, 6, lens.tolist(), 1, 1, 16, 16)
+
+
+def test_decode_wide_groups_over_long_requests(gpu):
+    """Several waves on the same keys, heads in parts, and pieces to join."""
+    decode_case(gpu, 14, [5000, 130], 1, 40, 64, 16)
+    decode_case(gpu, 15, [3000, 0, 700], 2, 70, 128, 32, "bf16")
+    decode_case(gpu, 16, [4001], 1, 64, 32, 5)
+    decode_case(gpu, 17, [9000], 1, 20, 16, 16, "bf16")
+
+
+def test_decode_leaves_the_counters_at_zero(gpu):
+    opts = nc.paged_options(num_seqs=2, num_q_heads=4, num_kv_heads=2, head_dim=64, page_size=16, num_pages=2000, max_pages=1000)
+    work = nc.paged_workspace(opts)
+    for seed, lens in ((1, [15000, 300]), (2, [40, 16000]), (3, [0, 5])):
+        decode_case(gpu, seed, lens, 2, 2, 64, 16, work=work)
+        assert not np.any(work.download(np.uint32, 2048)), "a counter of the workspace is not 0"
+
+
+def test_decode_and_build_table_strides(gpu):
+    """Rows of the table apart from each other: what stands between them is neither read nor written."""
+    rng = np.random.default_rng(18)
+    lens, ps, width, stride = [50, 0, 33], 16, 4, 11
+    pool = pc.Pool(rng, 12, 2, ps, 64)
+    table = pc.make_table(rng, lens, ps, 12, width)
+    wide = np.full((3, stride), 0x7FFFFFF0, dtype=np.int32)
+    wide[:, :width] = table
+    q = pc.encode(rng.standard_normal((3, 4, 64)), "f16")
+    opts = nc.paged_options(num_seqs=3, num_q_heads=4, max_pages=width, table_stride=stride, **pool.options())
+    flat = wide.ravel()[:2 * stride + width]  # no longer than has to be
+    out = run_decode(gpu, pool, flat, lens, q, opts, 2)
+    ref, bound = pc.ref_decode(q, pool, table, lens, opts.scale, 2)
+    check(out, ref, bound, opts, "table stride")
+    tab, free = dev(flat), np.arange(12, dtype=np.int32)
+    bopts = nc.paged_options(num_seqs=3, head_dim=64, page_size=ps, num_pages=12, max_pages=width, table_stride=stride)
+    cached, new = np.array(lens), np.array([10, 20, 31])
+    outs = [nc.DeviceBuffer(4 * n) for n in (3, 4, 61, 4)]
+    nc.paged_build(gpu, dev(cached.astype(np.int32)), dev(new.astype(np.int32)), dev(free), dev(np.zeros(1, np.int32)), tab, *outs, bopts)
+    nc.synchronize()
+    want = pc.ref_build(cached, new, free, 0, table, 61, ps, 12)
+    wide[:, :width] = want[0]
+    assert np.array_equal(tab.download(np.int32, flat.size), wide.ravel()[:flat.size])
+    assert np.array_equal(outs[2].download(np.int32, 61), want[3])
 
 
 def test_decode_all_empty(gpu):
@@ -558,3 +608,18 @@ def test_decode_continues_a_flash_prompt(gpu):
     nc.synchronize()
     last = do.download(np.float32, heads * S * d).reshape(heads, S, d)[:, -1]
     assert np.max(np.abs(out.download(np.float32, heads * d).reshape(heads, d) - last)) <= fc.MAX_ABS
+
+
+def test_harness_command(gpu, capsys):
+    """flash_harness.py paged: prompts and decoding steps over a paged cache, a record per case, each within its
+    tolerance."""
+    import json
+
+    import flash_harness as fh
+
+    assert fh.main(["paged", "--warmup", "1", "--iters", "3"]) == 0
+    recs = [json.loads(line) for line in capsys.readouterr().out.splitlines() if line.startswith("{")]
+    assert len(recs) == len(fh.PAGED_CASES)
+    for r in recs:
+        assert set(r) == set(fh.RECORD_KEYS) and r["kernel"] == "paged_attention"
+        assert r["correct"] and r["max_abs_error"] <= fh.PAGED_TOL and r["min_ms"] > 0
