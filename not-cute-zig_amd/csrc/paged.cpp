@@ -162,7 +162,7 @@ DecodePlan decode_plan(const Shape &s) {
     p.short_log2 = p.long_log2 + 1;
     p.grid = (uint32_t)std::min<uint64_t>(o.num_seqs * s.heads * s.seq_units, 1u << p.short_log2);
     p.rows = (uint32_t)std::min<uint64_t>(s.group, 64);
-    p.piece_ml = NC_PAGED_MAX_WGS * 4;
+    p.piece_ml = NC_PAGED_ROUNDS * 2 * NC_PAGED_MAX_WGS * 4;
     p.piece_o = p.piece_ml + (uint64_t)p.grid * 2 * p.rows * 2 * 4;
     p.bytes = p.piece_o + (uint64_t)p.grid * 2 * p.rows * o.head_dim * 4;
     return p;
@@ -350,6 +350,7 @@ int nc_paged_decode(nc_module module, const nc_paged_decode_buffers *buffers, co
     a.part_ml = reinterpret_cast<float *>(static_cast<char *>(t.workspace) + plan.piece_ml);
     a.part_o = reinterpret_cast<float *>(static_cast<char *>(t.workspace) + plan.piece_o);
     a.rows = plan.rows;
+    a.fan = nc_paged_fan(plan.rows, (uint32_t)op.head_dim);
     a.long_log2 = plan.long_log2;
     a.short_log2 = plan.short_log2;
     a.heads = nc_paged_make_div((uint32_t)s.heads);

@@ -246,7 +246,7 @@ NC_APPEND(_d16_unaligned, false, false)
 // the same time, and all but one find them in the caches. The work is cut into blocks, counted over all requests
 // and heads, and every workgroup takes a run of equally many, whatever the lengths: it finds its first by a
 // prefix sum over the requests' lengths. A run that begins or ends inside a request's keys leaves a piece
-// (max, sum, O); the last of a request's workgroups to arrive joins them in order.
+// (max, sum, O); the last of a request's workgroups to arrive join them in order.
 //
 // One wave takes KT x 32 keys of a block at a time. Scores: S = K Q^T with K rows straight from memory as the
 // A operand (lane l: key l%16, dims 8(l/16)..+7 of 32), so lane l holds the scores of query l%16 and keys
@@ -301,6 +301,23 @@ __device__ __forceinline__ uint32_t take_pair(float &x, float &y) {
         y -= (float)h[1];
         return __builtin_bit_cast(uint32_t, h);
     }
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, false));
+}
+// Over each 4 neighbouring lanes, or each 16; all get the result.
+template <bool MAX>
+__device__ __forceinline__ float near(float x, bool sixteen) {
+    auto add = [](float u, float v) { return MAX ? fmaxf(u, v) : u + v; };
+    x = add(x, dpp<0xb1>(x));  // quad_perm 1,0,3,2 and 2,3,0,1
+    x = add(x, dpp<0x4e>(x));
+    if (sixteen) {
+        x = add(x, dpp<0x124>(x));  // row_ror:4 and 8
+        x = add(x, dpp<0x128>(x));
+    }
+    return x;
 }
 
 // Over the four lanes l, l^16, l^32, l^48; all get the result.
@@ -581,7 +598,7 @@ struct Decode {
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int n = 0; n < PARTS; ++n) p[n][j] = take_pair<BF>(s[2 * u + j / 2][2 * (j % 2)], s[2 * u + j / 2][2 * (j % 2) + 1]);
-            constexpr int G = E < 4 ? E : 4;  // products of so many dims in turn: each waits for its last one
+            constexpr int G = E < 2 ? E : 2;  // products of so many dims in turn: each waits for its last one
 #pragma unroll
             for (int i0 = 0; i0 < E; i0 += G) {
                 u32x4 x[G];
@@ -646,74 +663,147 @@ struct Decode {
         }
     }
 
-    // The pieces of workgroups first..last of one request and head: added in an order that does not depend on who
-    // came last, and written to O. Four columns of a row are a thread's, and PF pieces are on their way at a time; where
-    // there are more, and threads over, groups of them take every so many-th piece and are added up through LDS.
-    template <int PF>
-    __device__ __forceinline__ void join_pieces(uint32_t first, uint32_t last, uint32_t rows, float *o) {
+    // Row q of the piece of workgroup j, `first` of which began the request and head.
+    static __device__ __forceinline__ uint64_t piece_row(uint32_t j, uint32_t first, uint32_t piece_rows, uint32_t q) {
+        return ((uint64_t)j * 2 + (j == first)) * piece_rows + q;
+    }
+
+    static __device__ __forceinline__ floatx4 get4(const float *p) {
+        float p0, p1, p2, p3;
+        get2(p, p0, p1);
+        get2(p + 2, p2, p3);
+        return floatx4{p0, p1, p2, p3};
+    }
+
+    // Up to N pieces, which are all: every thread has their maxima and sums with its columns, in one go.
+    template <uint32_t N>
+    __device__ __forceinline__ void merge_few(uint32_t lead, uint32_t stride, uint32_t count, uint32_t first, uint32_t rows, float *o) {
+        const Args a = again(args);
+        const float *part_ml = a->part_ml, *part_o = a->part_o;
+        for (uint32_t it = threadIdx.x; it < rows * (D / 4); it += THREADS) {
+            const uint32_t q = it / (D / 4), x = 4 * (it % (D / 4));
+            float pm[N], pl[N], top = neg_inf(), sum = 0.f;
+            floatx4 po[N], out = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (uint32_t n = 0; n < N; ++n) {
+                const uint64_t at = piece_row(lead + min(n, count - 1u) * stride, first, a->rows, q);
+                get2(part_ml + 2 * at, pm[n], pl[n]);
+                po[n] = get4(part_o + at * D + x);
+            }
+#pragma unroll
+            for (uint32_t n = 0; n < N; ++n) top = fmaxf(top, pm[n]);
+#pragma unroll
+            for (uint32_t n = 0; n < N; ++n)
+                if (n < count) {
+                    const float f = __builtin_amdgcn_exp2f(pm[n] - finite_or_0(top));
+                    sum += f * pl[n];
+                    out += f * po[n];
+                }
+            store_o(o, q, x, out, sum);
+        }
+    }
+
+    // Adds `count` pieces of one request and head, those of workgroups lead, lead + stride, ..., in their order: to O if
+    // there are no others, else in the place of the first of them. Their maxima, a piece a lane, give every piece's
+    // factor, kept in LDS; the first pieces of O are on their way meanwhile. Four columns of a row are a thread's;
+    // where that leaves threads over, groups of them take every so many-th piece.
+    __device__ __forceinline__ void merge(uint32_t lead, uint32_t stride, uint32_t count, uint32_t first, bool all, uint32_t rows, float *o) {
+        constexpr uint32_t PF = 4;
         const Args a = again(args);
         const uint32_t items = rows * (D / 4), piece_rows = a->rows;
-        const uint32_t groups = items > THREADS / 2 ? 1u : min(THREADS / items, (last - first) / PF + 1u);
-        const float *part_ml = a->part_ml, *part_o = a->part_o;
-        floatx4 *s_sum = reinterpret_cast<floatx4 *>(&s_o[0][0][0]);  // one per thread, and behind them (max, sum)
-        float *s_stat = reinterpret_cast<float *>(s_sum + THREADS);
-        for (uint32_t i0 = 0; i0 < items; i0 += THREADS) {
-            const uint32_t grp = groups == 1 ? 0u : threadIdx.x / items, it = groups == 1 ? i0 + threadIdx.x : threadIdx.x - grp * items;
-            const bool mine = it < items && grp < groups;
+        const uint32_t groups = items > THREADS / 2 ? 1u : min(THREADS / items, (count - 1u) / PF + 1u);
+        float *part_ml = a->part_ml, *part_o = a->part_o;
+        float *s_f = &s_o[0][0][0], *s_tot = s_f + NC_PAGED_MERGE_ROWS;
+        floatx4 *s_sum = reinterpret_cast<floatx4 *>(s_tot + 2 * 64);
+        const uint32_t grp = groups == 1 ? 0u : threadIdx.x / items;
+        const bool works = grp < groups;
+        uint32_t it = threadIdx.x - grp * items;
+        floatx4 po[PF];
+        auto load = [&](uint32_t n0) {
             const uint32_t q = it / (D / 4), x = 4 * (it % (D / 4));
-            float top = neg_inf(), sum = 0.f;
+#pragma unroll
+            for (uint32_t n = 0; n < PF; ++n)
+                po[n] = get4(part_o + piece_row(lead + min(n0 + n * groups, count - 1u) * stride, first, piece_rows, q) * D + x);
+        };
+        if (works && it < items) load(grp);
+        const bool sixteen = count > 4u;
+        const uint32_t per = sixteen ? 4u : 16u;  // rows of a wave at a time
+        for (uint32_t q0 = w * per; q0 < rows; q0 += NW * per) {
+            const uint32_t n = lane & (sixteen ? 15u : 3u), q = q0 + (sixteen ? lane >> 4 : lane >> 2);
+            float pm = neg_inf(), pl = 0.f;
+            if (n < count && q < rows) get2(part_ml + 2 * piece_row(lead + n * stride, first, piece_rows, q), pm, pl);
+            const float top = near<true>(pm, sixteen), f = __builtin_amdgcn_exp2f(pm - finite_or_0(top));
+            const float sum = near<false>(f * pl, sixteen);
+            if (n < count && q < rows) s_f[n * rows + q] = f;
+            if (n == 0 && q < rows) {
+                s_tot[2 * q] = top;
+                s_tot[2 * q + 1] = sum;
+            }
+        }
+        __syncthreads();
+        for (bool next = false; it < items || groups > 1; it += THREADS, next = true) {
+            const uint32_t q = it / (D / 4), x = 4 * (it % (D / 4));
             floatx4 out = {0.f, 0.f, 0.f, 0.f};
-            if (mine) {
-                for (uint32_t i = first + grp; i <= last; i += PF * groups) {
-                    float pm[PF], pl[PF];
-                    floatx4 po[PF];
+            if (works && it < items) {
+                for (uint32_t n0 = grp; n0 < count; n0 += PF * groups) {
+                    if (next || n0 != grp) load(n0);
 #pragma unroll
-                    for (int n = 0; n < PF; ++n) {
-                        const uint32_t j = min(i + n * groups, last);
-                        const uint64_t at = ((uint64_t)j * 2 + (j == first)) * piece_rows + q;
-                        float p0, p1, p2, p3;
-                        get2(part_ml + 2 * at, pm[n], pl[n]);
-                        get2(part_o + at * D + x, p0, p1);
-                        get2(part_o + at * D + x + 2, p2, p3);
-                        po[n] = floatx4{p0, p1, p2, p3};
-                    }
-                    float t = top;
-#pragma unroll
-                    for (int n = 0; n < PF; ++n) t = fmaxf(t, pm[n]);
-                    const float ref = finite_or_0(t), f = __builtin_amdgcn_exp2f(top - ref);
-                    sum *= f;
-                    out *= f;
-#pragma unroll
-                    for (int n = 0; n < PF; ++n) {
-                        if (i + n * groups <= last) {
-                            const float h = __builtin_amdgcn_exp2f(pm[n] - ref);
-                            sum += pl[n] * h;
-                            out += po[n] * h;
-                        }
-                    }
-                    top = t;
+                    for (uint32_t n = 0; n < PF; ++n)
+                        if (n0 + n * groups < count) out += s_f[(n0 + n * groups) * rows + q] * po[n];
                 }
             }
             if (groups > 1) {
                 s_sum[threadIdx.x] = out;
-                s_stat[2 * threadIdx.x] = top;
-                s_stat[2 * threadIdx.x + 1] = sum;
                 __syncthreads();
-                if (mine && grp == 0) {
-                    float t = top;
-                    for (uint32_t n = 1; n < groups; ++n) t = fmaxf(t, s_stat[2 * (threadIdx.x + n * items)]);
-                    const float ref = finite_or_0(t), f = __builtin_amdgcn_exp2f(top - ref);
-                    sum *= f;
-                    out *= f;
-                    for (uint32_t n = 1; n < groups; ++n) {
-                        const uint32_t y = threadIdx.x + n * items;
-                        const float h = __builtin_amdgcn_exp2f(s_stat[2 * y] - ref);
-                        sum += s_stat[2 * y + 1] * h;
-                        out += s_sum[y] * h;
-                    }
+                if (grp == 0)
+                    for (uint32_t n = 1; n < groups; ++n) out += s_sum[threadIdx.x + n * items];
+            }
+            if (grp == 0 && it < items) {
+                if (all) {
+                    store_o(o, q, x, out, s_tot[2 * q + 1]);
+                } else {
+                    const uint64_t at = piece_row(lead, first, piece_rows, q);
+                    put2(part_o + at * D + x, out[0], out[1]);
+                    put2(part_o + at * D + x + 2, out[2], out[3]);
+                    if (x == 0) put2(part_ml + 2 * at, s_tot[2 * q], s_tot[2 * q + 1]);
                 }
             }
-            if (mine && grp == 0) store_o(o, q, x, out, sum);
+            if (groups > 1) break;
+        }
+    }
+
+    // After workgroup i's piece of a request and head whose pieces are those of workgroups first..last: the last
+    // of every `fan` to arrive adds theirs up, and the last of those that did, until there is one. A CU reads pieces at a
+    // few ten GB/s: one that adds up all 256 of a long request took longer than its keys.
+    __device__ __forceinline__ void join(uint32_t i, uint32_t first, uint32_t last, uint32_t rows, float *o) {
+        const Args a = again(args);
+        const uint32_t pieces = last - first + 1u, fan = a->fan;
+        uint32_t *counters = a->counters;
+        uint32_t c = i - first;
+        for (uint32_t stride = 1;; stride *= fan) {
+            // Every thread's stores have arrived before the count says so, and pieces are read only after the count
+            // showed the last of them.
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            c -= c % (fan * stride);
+            const uint32_t lead = first + c, count = min(fan, (pieces - c - 1u) / stride + 1u);
+            uint32_t *counter = counters + 2 * lead + (lead == first);
+            if (threadIdx.x == 0) {
+                const uint32_t before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (before == count - 1u) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                *s_word = before;
+            }
+            __syncthreads();
+            if (*s_word != count - 1u) return;
+            const bool all = pieces <= fan * stride;
+            if (all && count <= 4u)
+                merge_few<4>(lead, stride, count, first, rows, o);
+            else if (all && count <= 8u)
+                merge_few<8>(lead, stride, count, first, rows, o);
+            else
+                merge(lead, stride, count, first, all, rows, o);
+            if (all) return;
+            counters += 2 * NC_PAGED_MAX_WGS;  // of the next round
         }
     }
 
@@ -732,8 +822,8 @@ struct Decode {
     }
 
     // The four waves' (m, l, O) of one run of blocks: to O if the run is all of the request's, else to this
-    // workgroup's (i's) piece, and the last to arrive of the workgroups that share the units b_lo..b_lo+nb-1, `each`
-    // apiece, joins them.
+    // workgroup's (i's) piece, to be joined with those of the workgroups that share the units b_lo..b_lo+nb-1, `each`
+    // apiece.
     __device__ __forceinline__ void finish(uint32_t rows, uint32_t r, uint32_t head0, bool whole, uint32_t i, uint32_t b_lo, uint32_t nb, uint32_t each) {
         const Args a = again(args);
         uint32_t first = i, last = i;
@@ -779,28 +869,13 @@ struct Decode {
             if (whole) {
                 store_o(o, q, x, out, lsum);
             } else {
-                const uint64_t at = ((uint64_t)i * 2 + (i == first)) * a->rows + q;
+                const uint64_t at = piece_row(i, first, a->rows, q);
                 put2(a->part_o + at * D + x, out[0], out[1]);
                 put2(a->part_o + at * D + x + 2, out[2], out[3]);
                 if (x == 0) put2(a->part_ml + 2 * at, top, lsum);
             }
         }
-        if (!whole) {
-            // Every thread's stores have arrived before the count says so, and the partials are read only after the
-            // count showed the last of them.
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (threadIdx.x == 0)
-                *s_word = __hip_atomic_fetch_add(a->counters + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __syncthreads();
-            if (*s_word == last - first) {
-                if (last - first < 4)
-                    join_pieces<4>(first, last, rows, o);
-                else
-                    join_pieces<8>(first, last, rows, o);
-                if (threadIdx.x == 0) __hip_atomic_store(a->counters + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-        }
+        if (!whole) join(i, first, last, rows, o);
         __syncthreads();  // LDS is free again
     }
 
@@ -910,8 +985,9 @@ template <int D, bool BF, bool UNI>
 __device__ __forceinline__ void decode_body() {
     const Args a = (Args)__builtin_amdgcn_kernarg_segment_ptr();
     using X = Decode<D, BF, UNI>;
-    // the waves' O, or the join's (4 columns, max, sum) of every thread
-    __shared__ __attribute__((aligned(16))) float s_mem[X::NW * 16 * X::OP > X::THREADS * 6 ? X::NW * 16 * X::OP : X::THREADS * 6];
+    // the waves' O, or a merge's factors, sums of rows and partial sums
+    constexpr uint32_t kWaves = X::NW * 16 * X::OP, kMerge = NC_PAGED_MERGE_ROWS + 2 * 64 + 4 * X::THREADS;
+    __shared__ __attribute__((aligned(16))) float s_mem[kWaves > kMerge ? kWaves : kMerge];
     __shared__ float s_ml[X::NW][16][2];
     __shared__ uint32_t s_word;
     const uint32_t lane = threadIdx.x & 63u;

@@ -74,11 +74,19 @@ NC_HD uint32_t nc_paged_each(uint32_t units, uint32_t most_log2, uint32_t least)
     return each < least ? least : each;
 }
 
+// Pieces that one workgroup adds up, by their size: of up to 16 KB reading 16 of them takes about as long as another
+// round, of more only 4. At most NC_PAGED_MAX_WGS pieces are one after NC_PAGED_ROUNDS rounds, and
+// NC_PAGED_MERGE_ROWS holds the rows of all that one adds up.
+#define NC_PAGED_MAX_WGS 1024u
+#define NC_PAGED_ROUNDS 5u
+#define NC_PAGED_MERGE_ROWS 1024u
+NC_HD uint32_t nc_paged_fan(uint32_t rows, uint32_t head_dim) { return rows * head_dim <= 4096u ? 16u : 4u; }
+
 struct nc_paged_decode_args {
     const uint16_t *q, *k, *v;
     const int32_t *table, *seq_lens;
     float *o;
-    uint32_t *counters; // NC_PAGED_MAX_WGS of them, all 0 between launches
+    uint32_t *counters; // NC_PAGED_ROUNDS times two per workgroup, all 0 between launches
     float *part_ml;     // per workgroup two pieces of `rows` (max, sum) pairs
     float *part_o;      // per workgroup two pieces of rows x head_dim sums
     uint64_t table_stride, page_stride, head_stride, token_stride, q_stride, q_head_stride, o_stride, o_head_stride;
@@ -86,13 +94,13 @@ struct nc_paged_decode_args {
     uint32_t num_pages, max_tokens;                      // max_tokens = max_pages * page_size
     uint32_t rows;                                       // query heads of a piece: min(group, 64)
     uint32_t wave_shift, head_parts;
+    uint32_t fan; // nc_paged_fan()
     uint32_t long_log2, short_log2, each_least; // workgroups for long heads and for short ones, units of a share
     nc_paged_div heads;                         // num_kv_heads * head_parts
     uint32_t q_vec, o_vec;                               // Q, O rows are 16-byte aligned
     float scale;
     nc_paged_div ps;
 };
-#define NC_PAGED_MAX_WGS 2048u
 
 // A length from device memory, cut to what the table's row can hold.
 NC_HD uint32_t nc_paged_cut(int32_t len, uint32_t most) {

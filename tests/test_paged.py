@@ -325,6 +325,14 @@ int main() {
         const uint32_t rows = g < 64 ? g : 64, sh = nc_paged_wave_shift(rows);
         if ((16u << sh) < rows || (sh && (8u << sh) >= rows) || nc_paged_head_parts(g) * 64 < g || (nc_paged_head_parts(g) - 1) * 64 >= g) return 4;
     }
+    // the join's rounds and LDS suffice for every size of piece
+    for (uint32_t d = 16; d <= 128; d *= 2)
+        for (uint32_t rows = 1; rows <= 64; ++rows) {
+            const uint32_t fan = nc_paged_fan(rows, d);
+            uint64_t most_pieces = 1;
+            for (uint32_t i = 0; i < NC_PAGED_ROUNDS; ++i) most_pieces *= fan;
+            if (most_pieces < NC_PAGED_MAX_WGS || fan > 16 || fan * rows > NC_PAGED_MERGE_ROWS) return 6;
+        }
     if (nc_paged_cut(-1, 5) != 0 || nc_paged_cut(INT32_MIN, 5) != 0 || nc_paged_cut(4, 5) != 4 ||
         nc_paged_cut(INT32_MAX, 5) != 5) return 2;
     return 0;
