@@ -368,8 +368,8 @@ struct Decode {
     static constexpr int OP = D + 4;            // pitch of a row of partial O in LDS
     static constexpr uint32_t NW = NC_PAGED_WAVES, THREADS = 64 * NW;
     // Weights are 2^(SHIFT + score - max): in f16 the low part of a small weight stays a normal number, in bf16
-    // a sum of a million V at the type's largest value stays finite.
-    static constexpr float SHIFT = BF ? -16.f : 12.f;
+    // the sum of 2^31 V at the type's largest value (2^128) stays finite, and V below 2^-94 may count as 0.
+    static constexpr float SHIFT = BF ? -32.f : 12.f;
     using KReg = typename std::conditional<D == 16, u32x2, u32x4>::type;
     using VReg = typename std::conditional<E == 8, u32x4, typename std::conditional<E == 4, u32x2, uint32_t>::type>::type;
 

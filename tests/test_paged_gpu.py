@@ -270,6 +270,25 @@ def test_decode_infinite_scores(gpu):
         assert np.all(np.abs(out[0] - ref[0]) <= bound[0])
 
 
+@pytest.mark.parametrize("d,dtype", [(16, "bf16"), (128, "bf16"), (64, "f16")])
+def test_decode_sums_at_the_largest_value(gpu, d, dtype):
+    """200000 keys of one score and V at the type's largest value: O is that value, and no sum on the way passes
+    f32's range. The weights are one power of two, so their sums are exact; O is added up in at most 200000/32
+    steps of a wave, 4 waves and 1024 pieces, 2^-24 each, and the quotient is within 2^-22."""
+    n, pages = 200000, 4
+    rng = np.random.default_rng(72)
+    pool = pc.Pool(rng, pages, 1, 16, d, dtype)
+    most = 3.3895313892515355e38 if dtype == "bf16" else 65504.0
+    for p in range(pages):
+        for t in range(16):
+            pool.put(1, p, 0, t, pc.encode(np.full(d, most), dtype))
+    table = (np.arange(n // 16, dtype=np.int32) % pages).reshape(1, -1)
+    q = np.zeros((1, 2, d), dtype=np.uint16)
+    opts = nc.paged_options(num_seqs=1, num_q_heads=2, max_pages=n // 16, **pool.options())
+    out = run_decode(gpu, pool, table, [n], q, opts, 2).astype(np.float64)
+    assert np.all(np.abs(out / most - 1.0) <= (n / 32 + 4 + 1024) * 2.0 ** -24 + 2.0 ** -22)
+
+
 def test_decode_shared_pages(gpu):
     """Two requests with a common prefix read the same pages."""
     rng = np.random.default_rng(80)
