@@ -60,6 +60,7 @@ int resolve(const nc_paged_options *opts, Shape *s) {
     for (uint64_t n : counts)
         if (n > kMost31) return NC_ERROR_OVERFLOW;
     if (o.page_size * o.num_pages > kMost31 || o.page_size * o.max_pages > kMost31) return NC_ERROR_OVERFLOW;
+    if (o.num_q_heads > kMost31 / o.head_dim) return NC_ERROR_OVERFLOW;  // numbers of one request's outputs
     s->group = o.num_q_heads / o.num_kv_heads;
     const uint64_t given[] = {o.table_stride, o.page_stride, o.head_stride, o.token_stride, o.row_stride, o.row_head_stride,
                               o.q_stride, o.q_head_stride, o.o_stride, o.o_head_stride};

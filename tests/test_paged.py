@@ -126,6 +126,15 @@ def test_validate_accepts(kw):
     assert nc.paged_workspace_bytes(good(**kw)) > 0
 
 
+def test_validate_counts_a_requests_outputs():
+    """num_q_heads * head_dim is an index of 32 bits in the kernels: 2^31 of them are refused, one head less is not."""
+    most = dict(num_kv_heads=1, head_dim=64, num_seqs=1, page_size=16, num_pages=4, max_pages=4)
+    nc.paged_validate(nc.paged_options(num_q_heads=2 ** 25 - 1, **most))
+    with pytest.raises(nc.NcError) as e:
+        nc.paged_validate(nc.paged_options(num_q_heads=2 ** 25, **most))
+    assert e.value.name == OVERFLOW
+
+
 def test_unknown_element_type():
     o = good()
     o.element_type = 2
