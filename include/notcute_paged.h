@@ -121,8 +121,8 @@ int nc_paged_build(nc_module module, const nc_paged_build_buffers *buffers, cons
 /* K and V rows into the cache: row i (element i*row_stride + h*row_head_stride of k_rows and v_rows, at any
  * element alignment) goes to slot slots[i], for the num_rows first rows; a slot outside the pool (-1) is
  * skipped. Slots of one call are distinct: of two rows with the same slot, either may be kept, element by
- * element. The caches are 16-byte aligned, are not one and the same, and do not overlap the rows
- * (NC_ERROR_INVALID_VALUE). num_rows = 0 does nothing. */
+ * element. The caches are 16-byte aligned, do not overlap the rows, and no row of the one shares an element
+ * with a row of the other (NC_ERROR_INVALID_VALUE). num_rows = 0 does nothing. */
 typedef struct nc_paged_append_buffers {
     const uint16_t *k_rows;
     uint64_t k_rows_len;

@@ -115,6 +115,19 @@ Range range_of(const void *p, uint64_t elements, uint64_t size) {
 
 bool overlap(const Range &x, const Range &y) { return x.lo < x.hi && y.lo < y.hi && x.lo < y.hi && y.lo < x.hi; }
 
+// Whether two sets of rows of d elements on the same axes share an element, the second `delta` elements behind the first:
+// whether delta + sum i_k stride_k, |i_k| < n_k, comes within d of 0. The axes ascend as extent() leaves them, and
+// those below a stride reach less far than it: one of the three multiples about -delta is the only one that can.
+bool rows_meet(const Axis *ax, int count, int64_t d, int64_t delta) {
+    if (count == 0) return delta > -d && delta < d;
+    const Axis &x = ax[count - 1];
+    if (x.n <= 1) return rows_meet(ax, count - 1, d, delta);
+    const int64_t stride = (int64_t)x.stride, most = (int64_t)x.n - 1, near = -(delta / stride);
+    for (int64_t i = std::max(near - 1, -most); i <= std::min(near + 1, most); ++i)
+        if (rows_meet(ax, count - 1, d, delta + i * stride)) return true;
+    return false;
+}
+
 uintptr_t address(const void *p) { return reinterpret_cast<uintptr_t>(p); }
 
 // Every kernel of paged.hip by its place here, under which the module keeps its function.
@@ -270,7 +283,16 @@ int nc_paged_append(nc_module module, const nc_paged_append_buffers *buffers, co
     if (st) return st;
     const nc_paged_options &o = s.o;
     if (!module || !t.k_cache || !t.v_cache || t.k_len < s.cache_len || t.v_len < s.cache_len) return NC_ERROR_INVALID_VALUE;
-    if ((address(t.k_cache) | address(t.v_cache)) % 16 || t.k_cache == t.v_cache) return NC_ERROR_INVALID_VALUE;
+    if ((address(t.k_cache) | address(t.v_cache)) % 16) return NC_ERROR_INVALID_VALUE;
+    const Range caches[] = {range_of(t.k_cache, s.cache_len, 2), range_of(t.v_cache, s.cache_len, 2)};
+    // K and V may be interleaved, but no row of one may be part of a row of the other.
+    Axis cache[] = {{o.num_pages, o.page_stride}, {o.num_kv_heads, o.head_stride}, {o.page_size, o.token_stride}};
+    uint64_t unused;
+    st = extent(cache, 3, o.head_dim, &unused);
+    if (st) return st;
+    const int64_t apart = (int64_t)(address(t.v_cache) - address(t.k_cache)) / 2;
+    if (overlap(caches[0], caches[1]) && rows_meet(cache, 3, (int64_t)o.head_dim, apart))
+        return nc_internal_fail(NC_ERROR_INVALID_VALUE, "nc_paged_append: rows of K and V share memory");
     if (t.num_rows == 0) return NC_SUCCESS;
     if (t.num_rows > kMost31) return NC_ERROR_OVERFLOW;
     Axis row[] = {{t.num_rows, o.row_stride}, {o.num_kv_heads, o.row_head_stride}};
@@ -280,7 +302,6 @@ int nc_paged_append(nc_module module, const nc_paged_append_buffers *buffers, co
     if (!t.k_rows || !t.v_rows || !t.slots || t.k_rows_len < rows_len || t.v_rows_len < rows_len || t.slots_len < t.num_rows)
         return NC_ERROR_INVALID_VALUE;
     if ((address(t.k_rows) | address(t.v_rows)) % 2 || address(t.slots) % 4) return NC_ERROR_INVALID_VALUE;
-    const Range caches[] = {range_of(t.k_cache, s.cache_len, 2), range_of(t.v_cache, s.cache_len, 2)};
     const Range ins[] = {range_of(t.k_rows, rows_len, 2), range_of(t.v_rows, rows_len, 2), range_of(t.slots, t.num_rows, 4)};
     for (const Range &x : caches)
         for (const Range &y : ins)

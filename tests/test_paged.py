@@ -245,6 +245,38 @@ def test_append_refuses_misaligned_overlapping_and_negative():
     nc.paged_append(FakeModule, opts=o, num_rows=0, **append_buffers(o))  # nothing to do, nothing touched
 
 
+@pytest.mark.parametrize("strides", [
+    dict(), dict(token_stride=128), dict(token_stride=2 * 2 * 64, head_stride=2 * 64, page_stride=16 * 256),
+    dict(token_stride=128, head_stride=64), dict(token_stride=72, page_stride=4096), dict(num_pages=1, page_stride=8),
+    dict(page_size=1, num_pages=9, token_stride=8, head_stride=64), dict(num_kv_heads=1, num_q_heads=1, head_stride=8)])
+def test_append_refuses_rows_of_k_and_v_that_meet(strides):
+    """V at every 16-byte distance from K: refused exactly where some row of V holds an element of a row of K.
+    With no rows to append, an accepted call launches nothing."""
+    o = good(**dict(dict(num_pages=3), **strides))
+    nc.paged_validate(o)
+    d, ps, H, P = o.head_dim, o.page_size, o.num_kv_heads, o.num_pages
+    ts = o.token_stride or d
+    hs = o.head_stride or ps * ts
+    pg = o.page_stride or max(H * hs, ps * ts)
+    at = (np.arange(P)[:, None, None] * pg + np.arange(H)[None, :, None] * hs + np.arange(ps)[None, None, :] * ts).ravel()
+    held = np.zeros(at.max() + d, dtype=bool)
+    held[(at[:, None] + np.arange(d)).ravel()] = True
+    n = held.size
+    for delta in list(range(8, min(n, 1600), 8)) + [n // 8 * 8 - 8, n // 8 * 8, (n + 7) // 8 * 8]:
+        meet = bool(np.any(held[delta:] & held[:n - delta])) if delta < n else False
+        for sign in (1, -1):
+            bufs = append_buffers(o)
+            bufs["k_cache"] = Fake(0x4000000, n, 2)
+            bufs["v_cache"] = Fake(0x4000000 + sign * 2 * delta, n, 2)
+            try:
+                nc.paged_append(FakeModule, opts=o, num_rows=0, **bufs)
+                refused = False
+            except nc.NcError as e:
+                assert e.name == INVALID
+                refused = True
+            assert refused == meet, (delta, sign)
+
+
 def decode_buffers(o):
     cache = o.num_pages * o.num_kv_heads * o.page_size * o.head_dim
     qo = o.num_seqs * o.num_q_heads * o.head_dim
