@@ -140,13 +140,17 @@ int nc_paged_append(nc_module module, const nc_paged_append_buffers *buffers, co
                     nc_stream stream);
 
 /* Device memory that nc_paged_decode needs for these options (0 when they are invalid). The caller zeroes
- * it once before its first use; every launch leaves it ready for the next, of any options that need no
- * more. Launches that overlap in time need workspaces of their own. */
+ * it once before its first use; every launch that runs to its end leaves it ready for the next, of any
+ * options that need no more. Launches that overlap in time need workspaces of their own (two streams, or two
+ * graphs that may run at once). */
 uint64_t nc_paged_workspace_bytes(const nc_paged_options *opts);
 
 /* O[r][i] = sum_j p_j V[j] over the seq_lens[r] tokens j of request r, p = softmax_j(scale * Q[r][i] . K[j]),
- * for every query head i. Sums, softmax and weights are f32 or more exact. A request of length 0, one whose
- * pages are all absent and one whose scores are all -infinity get zeros. Q at any element alignment, O at any
+ * for every query head i. Scores, maxima, exponentials and sums are f32; the weights enter the product with V
+ * as two (f16) or three (bf16) 16-bit numbers, whose sum is the f32 weight to 2^-21 or better. A request of
+ * length 0, one whose pages are all absent and one whose scores are all -infinity get zeros. A NaN among the
+ * keys that count gives NaN, and so does an infinite V among them; what lies elsewhere in the pools may be
+ * anything. Q at any element alignment, O at any
  * float; caches and workspace 16-byte aligned. O and the workspace overlap nothing else
  * (NC_ERROR_INVALID_VALUE). Rows of O behind the last request are not touched. How the keys are split over
  * workgroups follows the lengths of all requests, so a request's rounding may differ with its neighbours;
