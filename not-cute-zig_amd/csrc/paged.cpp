@@ -171,8 +171,8 @@ DecodePlan decode_plan(const Shape &s) {
     const bool uniform = o.page_size % 16 == 0 && o.page_stride < (1ull << 31) && o.page_size * o.token_stride < (1ull << 30);
     const uint32_t d = o.head_dim == 16 ? 0 : o.head_dim == 32 ? 1 : o.head_dim == 64 ? 2 : 3;
     p.kernel = kDecode + 4 * d + (uniform ? 0 : 2) + (o.element_type == NC_ELEMENT_BF16 ? 1 : 0);
-    // Workgroups for long heads: one per CU, where a step's loads are wide and a step ahead.
-    p.long_log2 = kCusLog2 + (o.head_dim <= (uniform ? 16u : 32u) ? 1 : 0);
+    // Workgroups for long heads: one per CU where a step's loads are wide and a step ahead, else two.
+    p.long_log2 = kCusLog2 + (o.head_dim <= 32 ? 1 : 0);
     p.short_log2 = p.long_log2 + 1;
     p.grid = (uint32_t)std::min<uint64_t>(o.num_seqs * s.heads * s.seq_units, 1u << p.short_log2);
     p.rows = (uint32_t)std::min<uint64_t>(s.group, 64);
@@ -256,10 +256,12 @@ int nc_paged_build(nc_module module, const nc_paged_build_buffers *buffers, cons
     a.places = (uint32_t)t.slots_len;
     a.ps = nc_paged_make_div((uint32_t)o.page_size);
     const uint32_t threads = o.num_seqs <= 64 ? 64 : o.num_seqs <= 256 ? 256 : 1024;
-    // One workgroup up to 4096 slots. Beyond, a slot a thread, or two where a workgroup needs several rounds to scan the
-    // requests: 256 requests of 140000 rows 5.3 us (two a thread 5.7, four 7.0), 2000 of 530000 11.4 us (one 17.7, four 12.9).
+    // One workgroup where its threads write a slot each, or a request's thread its few. Else a slot a thread, or two where a
+    // workgroup needs several rounds to scan the requests: 3 requests of 1400 rows 3.9 us (one workgroup 17.1, of 1024 threads
+    // 7.1), 256 of 140000 5.3 (two a thread 5.7, four 7.0), 2000 of 530000 11.4 (one 17.7, four 12.9).
     const uint64_t chunk = threads * (o.num_seqs > 1024 ? 2 : 1);
-    const uint64_t wgs = t.slots_len <= 4096 ? 1 : std::min<uint64_t>((t.slots_len + chunk - 1) / chunk, 1024);
+    const uint64_t single = std::max<uint64_t>(threads, std::min<uint64_t>(4096, 8 * o.num_seqs));
+    const uint64_t wgs = t.slots_len <= single ? 1 : std::min<uint64_t>((t.slots_len + chunk - 1) / chunk, 1024);
     a.chunk_rows = (uint32_t)((t.slots_len + wgs - 1) / wgs);
     // no more pages than this are taken
     const uint64_t pages = std::min<uint64_t>(t.free_len, t.slots_len / o.page_size + o.num_seqs);

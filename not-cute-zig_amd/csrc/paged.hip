@@ -365,6 +365,11 @@ struct Decode {
     static constexpr int E = D / 16;            // dims of a lane in V and O
     static constexpr int KK = D < 32 ? 1 : D / 32;  // products of a score
     static constexpr int KE = D == 16 ? 4 : 8;  // dims of a lane in one product
+    // Whether a step's loads are under way before the one before it is computed. It costs registers, and pays where a
+    // step's loads are wide: 2 requests of 105543 keys over 2 heads of 64 on pages of 1 56.8 -> 48.0 us. Heads of 16 or 32
+    // are better off with more workgroups instead (33 requests of up to 2047, 16 heads of 32, 13.7 -> 11.5 us on pages of
+    // 16, and 14.5 -> 11.2 of 7), and with heads of 128 on odd pages both the addresses and two steps do not fit (2 % slower).
+    static constexpr bool AHEAD = D == 64 || (D == 128 && UNI);
     static constexpr int OP = D + 4;            // pitch of a row of partial O in LDS
     static constexpr uint32_t NW = NC_PAGED_WAVES, THREADS = 64 * NW;
     // Weights are 2^(SHIFT + score - max): in f16 the low part of a small weight stays a normal number, in bf16
@@ -618,7 +623,7 @@ struct Decode {
         }
     }
 
-    // The keys k0, k0 + bk, ... below `end` of one key head: a step's loads are under way before the step before
+    // The keys k0, k0 + bk, ... below `end` of one key head: AHEAD, a step's loads are under way before the step before
     // it is computed, and the table entries a step earlier. Every step's loads are the same ones whatever there
     // is to load, so that waiting for one step's does not mean waiting for the next step's too.
     __device__ __forceinline__ void sweep(uint32_t r, uint32_t kvh, uint32_t k0, uint32_t end, uint32_t len) {
@@ -637,7 +642,7 @@ struct Decode {
         Step x, y;
         Pages pages = load_pages(cache, k0, len);
         issue(x, cache, pages, k0, end);
-        if constexpr (!UNI) {
+        if constexpr (!AHEAD) {
             while (true) {
                 pages = load_pages(cache, k0 + bk, len);
                 compute(x);
@@ -726,14 +731,17 @@ struct Decode {
                 po[n] = get4(part_o + piece_row(lead + min(n0 + n * groups, count - 1u) * stride, first, piece_rows, q) * D + x);
         };
         if (works && it < items) load(grp);
-        const bool sixteen = count > 4u;
-        const uint32_t per = sixteen ? 4u : 16u;  // rows of a wave at a time
+        const uint32_t lanes = count > 16u ? 6u : count > 4u ? 4u : 2u;  // log2 of a row's
+        const uint32_t per = 64u >> lanes;                                // rows of a wave at a time
         for (uint32_t q0 = w * per; q0 < rows; q0 += NW * per) {
-            const uint32_t n = lane & (sixteen ? 15u : 3u), q = q0 + (sixteen ? lane >> 4 : lane >> 2);
+            const uint32_t n = lane & ((1u << lanes) - 1u), q = q0 + (lane >> lanes);
             float pm = neg_inf(), pl = 0.f;
             if (n < count && q < rows) get2(part_ml + 2 * piece_row(lead + n * stride, first, piece_rows, q), pm, pl);
-            const float top = near<true>(pm, sixteen), f = __builtin_amdgcn_exp2f(pm - finite_or_0(top));
-            const float sum = near<false>(f * pl, sixteen);
+            float top = near<true>(pm, lanes > 2u);
+            if (lanes > 4u) top = quad_max(top);
+            const float f = __builtin_amdgcn_exp2f(pm - finite_or_0(top));
+            float sum = near<false>(f * pl, lanes > 2u);
+            if (lanes > 4u) sum = quad_sum(sum);
             if (n < count && q < rows) s_f[n * rows + q] = f;
             if (n == 0 && q < rows) {
                 s_tot[2 * q] = top;
@@ -777,7 +785,7 @@ struct Decode {
     // few ten GB/s: one that adds up all 256 of a long request took longer than its keys.
     __device__ __forceinline__ void join(uint32_t i, uint32_t first, uint32_t last, uint32_t rows, float *o) {
         const Args a = again(args);
-        const uint32_t pieces = last - first + 1u, fan = a->fan;
+        const uint32_t pieces = last - first + 1u, fan = nc_paged_one_round(pieces, a->rows * D) ? pieces : a->fan;
         uint32_t *counters = a->counters;
         uint32_t c = i - first;
         for (uint32_t stride = 1;; stride *= fan) {
