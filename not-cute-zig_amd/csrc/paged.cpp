@@ -131,13 +131,20 @@ bool rows_meet(const Axis *ax, int count, int64_t d, int64_t delta) {
 uintptr_t address(const void *p) { return reinterpret_cast<uintptr_t>(p); }
 
 // Every kernel of paged.hip by its place here, under which the module keeps its function.
+#define NC_DECODE_NAMES(D)                                                                \
+    "nc_paged_decode_d" #D, "nc_paged_decode_d" #D "_bf16", "nc_paged_decode_d" #D "_odd", \
+        "nc_paged_decode_d" #D "_odd_bf16", "nc_paged_decode_d" #D "_many",               \
+        "nc_paged_decode_d" #D "_many_bf16", "nc_paged_decode_d" #D "_many_odd", "nc_paged_decode_d" #D "_many_odd_bf16"
 const char *const kKernels[] = {
-    "nc_paged_build",          "nc_paged_append_rows",      "nc_paged_append_rows_unaligned",
-    "nc_paged_append_rows_d16", "nc_paged_append_rows_d16_unaligned",
-    "nc_paged_decode_d16",     "nc_paged_decode_d16_bf16",   "nc_paged_decode_d16_odd",  "nc_paged_decode_d16_odd_bf16",
-    "nc_paged_decode_d32",     "nc_paged_decode_d32_bf16",   "nc_paged_decode_d32_odd",  "nc_paged_decode_d32_odd_bf16",
-    "nc_paged_decode_d64",     "nc_paged_decode_d64_bf16",   "nc_paged_decode_d64_odd",  "nc_paged_decode_d64_odd_bf16",
-    "nc_paged_decode_d128",    "nc_paged_decode_d128_bf16",  "nc_paged_decode_d128_odd", "nc_paged_decode_d128_odd_bf16",
+    "nc_paged_build",
+    "nc_paged_append_rows",
+    "nc_paged_append_rows_unaligned",
+    "nc_paged_append_rows_d16",
+    "nc_paged_append_rows_d16_unaligned",
+    NC_DECODE_NAMES(16),
+    NC_DECODE_NAMES(32),
+    NC_DECODE_NAMES(64),
+    NC_DECODE_NAMES(128),
 };
 enum : uint32_t { kBuild, kAppend, kAppendD16 = kAppend + 2, kDecode = kAppend + 4 };
 
@@ -164,19 +171,23 @@ struct DecodePlan {
 
 constexpr uint32_t kCusLog2 = 8;  // MI355X: 256 CUs
 
-DecodePlan decode_plan(const Shape &s) {
+DecodePlan decode_plan(const Shape &s, bool o_vec) {
     const nc_paged_options &o = s.o;
     DecodePlan p;
     // A 16-key tile lies in one page, and a page's byte offsets fit 32 bits.
     const bool uniform = o.page_size % 16 == 0 && o.page_stride < (1ull << 31) && o.page_size * o.token_stride < (1ull << 30);
     const uint32_t d = o.head_dim == 16 ? 0 : o.head_dim == 32 ? 1 : o.head_dim == 64 ? 2 : 3;
-    p.kernel = kDecode + 4 * d + (uniform ? 0 : 2) + (o.element_type == NC_ELEMENT_BF16 ? 1 : 0);
     // Workgroups for long heads: one per CU where a step's loads are wide and a step ahead. Two for small heads, and for pages
     // of any size where waves share their keys and have half as much under way (4 requests of 20000 over 4 heads, 20 query
     // heads each: heads of 64 38.6 -> 30.4 us, of 128 62.1 -> 54.6; on pages of 16 heads of 64 lose 7 %, of 128 28 %).
     const bool two = o.head_dim <= 32 || (!uniform && s.group > 16);
     p.long_log2 = kCusLog2 + (two ? 1 : 0);
     p.short_log2 = kCusLog2 + (o.head_dim <= 32 ? 2 : 1);
+    // More heads than workgroups: where a workgroup has several short ones, its waves take one each (200 requests of 60
+    // tokens, 32 heads of 64, pages of 24, 41.8 -> 26.8 us; 256 of 50, 8 heads of 128, 15.9 -> 13.3; 128 of 120 over 8 heads,
+    // two a workgroup, 13.9 -> 14.3). That code makes every call 0.1 us longer, so it has kernels of its own.
+    const bool many = s.group <= 16 && o_vec && o.num_seqs * s.heads > 1u << p.short_log2;
+    p.kernel = kDecode + 8 * d + (many ? 4 : 0) + (uniform ? 0 : 2) + (o.element_type == NC_ELEMENT_BF16 ? 1 : 0);
     p.grid = (uint32_t)std::min<uint64_t>(o.num_seqs * s.heads * s.seq_units, 1u << p.short_log2);
     p.rows = (uint32_t)std::min<uint64_t>(s.group, 64);
     p.piece_ml = NC_PAGED_ROUNDS * 2 * NC_PAGED_MAX_WGS * 4;
@@ -204,7 +215,7 @@ int nc_paged_validate(const nc_paged_options *opts) {
 
 uint64_t nc_paged_workspace_bytes(const nc_paged_options *opts) {
     Shape s;
-    return resolve(opts, &s) ? 0 : decode_plan(s).bytes;
+    return resolve(opts, &s) ? 0 : decode_plan(s, true).bytes;
 }
 
 int nc_paged_build(nc_module module, const nc_paged_build_buffers *buffers, const nc_paged_options *opts,
@@ -347,7 +358,8 @@ int nc_paged_decode(nc_module module, const nc_paged_decode_buffers *buffers, co
     int st = resolve(opts, &s);
     if (st) return st;
     const nc_paged_options &op = s.o;
-    const DecodePlan plan = decode_plan(s);
+    const bool o_vec = address(t.o) % 16 == 0 && (op.o_stride | op.o_head_stride) % 4 == 0;
+    const DecodePlan plan = decode_plan(s, o_vec);
     const uint64_t need = plan.bytes;
     if (!module || !t.q || !t.k_cache || !t.v_cache || !t.block_table || !t.seq_lens || !t.o || !t.workspace)
         return NC_ERROR_INVALID_VALUE;
@@ -387,7 +399,7 @@ int nc_paged_decode(nc_module module, const nc_paged_decode_buffers *buffers, co
     const uint32_t block_keys = nc_paged_step_keys((uint32_t)op.head_dim) * (NC_PAGED_WAVES >> a.wave_shift);
     a.each_least = std::max(1u, 8 * a.rows / block_keys);
     a.q_vec = address(t.q) % 16 == 0 && (op.q_stride | op.q_head_stride) % 8 == 0;
-    a.o_vec = address(t.o) % 16 == 0 && (op.o_stride | op.o_head_stride) % 4 == 0;
+    a.o_vec = o_vec;
     a.table_stride = op.table_stride;
     a.page_stride = op.page_stride;
     a.head_stride = op.head_stride;

@@ -357,7 +357,7 @@ __device__ __forceinline__ Args again(Args p) {
 
 __device__ __forceinline__ float finite_or_0(float m) { return m == neg_inf() ? 0.f : m; }
 
-template <int D, bool BF, bool UNI>
+template <int D, bool BF, bool UNI, bool MANY>
 struct Decode {
     static constexpr int KT = D <= 32 ? 2 : 1;  // 32-key tiles of a wave's step
     static constexpr int NT = 2 * KT;           // 16-key tiles
@@ -623,10 +623,10 @@ struct Decode {
         }
     }
 
-    // The keys k0, k0 + bk, ... below `end` of one key head: AHEAD, a step's loads are under way before the step before
+    // The keys k0, k0 + by, ... below `end` of one key head: AHEAD, a step's loads are under way before the step before
     // it is computed, and the table entries a step earlier. Every step's loads are the same ones whatever there
     // is to load, so that waiting for one step's does not mean waiting for the next step's too.
-    __device__ __forceinline__ void sweep(uint32_t r, uint32_t kvh, uint32_t k0, uint32_t end, uint32_t len) {
+    __device__ __forceinline__ void sweep(uint32_t r, uint32_t kvh, uint32_t k0, uint32_t end, uint32_t len, uint32_t by) {
         if (k0 >= end) return;
         const Args a = again(args);
         Cache cache;
@@ -644,26 +644,26 @@ struct Decode {
         issue(x, cache, pages, k0, end);
         if constexpr (!AHEAD) {
             while (true) {
-                pages = load_pages(cache, k0 + bk, len);
+                pages = load_pages(cache, k0 + by, len);
                 compute(x);
-                if ((k0 += bk) >= end) return;
+                if ((k0 += by) >= end) return;
                 issue(x, cache, pages, k0, end);
             }
         }
-        if (k0 + bk >= end) {
+        if (k0 + by >= end) {
             compute(x);
             return;
         }
-        pages = load_pages(cache, k0 + bk, len);
+        pages = load_pages(cache, k0 + by, len);
         while (true) {
-            issue(y, cache, pages, k0 + bk, end);
-            pages = load_pages(cache, k0 + 2 * bk, len);
+            issue(y, cache, pages, k0 + by, end);
+            pages = load_pages(cache, k0 + 2 * by, len);
             compute(x);
-            if (k0 + bk >= end) break;
-            issue(x, cache, pages, k0 + 2 * bk, end);
-            pages = load_pages(cache, k0 + 3 * bk, len);
+            if (k0 + by >= end) break;
+            issue(x, cache, pages, k0 + 2 * by, end);
+            pages = load_pages(cache, k0 + 3 * by, len);
             compute(y);
-            k0 += 2 * bk;
+            k0 += 2 * by;
             if (k0 >= end) break;
         }
     }
@@ -829,6 +829,23 @@ struct Decode {
         }
     }
 
+    // O of a head that the wave had to itself: lane (c, g) has dims 4gE..4gE+4E-1 of query c.
+    __device__ __forceinline__ void finish_wave(uint32_t r, uint32_t head0, uint32_t rows) {
+        const Args a = again(args);
+        const float sum = quad_sum(l);
+        if (c >= rows) return;
+        float *o = a->o + r * a->o_stride + head0 * a->o_head_stride;
+        const float inv = __builtin_amdgcn_rcpf(sum);  // to an ulp
+        o += c * a->o_head_stride + 4 * E * g;
+        float v[4 * E];
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int j = 0; j < E; ++j) v[x * E + j] = sum == 0.f ? 0.f : acc[j][x] * inv;
+#pragma unroll
+        for (int x = 0; x < E; ++x) *reinterpret_cast<floatx4 *>(o + 4 * x) = floatx4{v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]};
+    }
+
     // The four waves' (m, l, O) of one run of blocks: to O if the run is all of the request's, else to this
     // workgroup's (i's) piece, to be joined with those of the workgroups that share the units b_lo..b_lo+nb-1, `each`
     // apiece.
@@ -950,8 +967,18 @@ struct Decode {
                     b0 = 0;
                     b1 = seg >= u0 ? nb : 0u;
                 }
-                if (b0 < b1) {
-                    uint32_t kvh = head, part = 0;
+                // Short heads of a request in a row, whose first units are here: a wave each if that takes no more steps than
+                // there are heads.
+                uint32_t n = 1;
+                if constexpr (MANY) {
+                    if (nb == 1 && seg >= u0) {
+                        n = min(min(heads - head, NW), (u1 - seg + units_of(1) - 1u) / units_of(1));
+                        if (len > n * WK) n = 1;
+                    }
+                }
+                const bool alone = MANY && n > 1;
+                if (alone ? w < n : b0 < b1) {
+                    uint32_t kvh = alone ? head + w : head, part = 0;
                     if (a->head_parts > 1) {
                         kvh = head / a->head_parts;
                         part = head - kvh * a->head_parts;
@@ -962,11 +989,14 @@ struct Decode {
                     l = 0.f;
 #pragma unroll
                     for (int x = 0; x < E; ++x) acc[x] = floatx4{0.f, 0.f, 0.f, 0.f};
-                    sweep(r, kvh, b0 * bk + kw * WK, min(b1 * bk, len), len);
-                    finish(rows, r, head0, b0 == 0 && b1 == nb, i, b_lo, nb, each);
+                    sweep(r, kvh, alone ? 0 : b0 * bk + kw * WK, alone ? len : min(b1 * bk, len), len, alone ? WK : bk);
+                    if (alone)
+                        finish_wave(r, head0, rows);
+                    else
+                        finish(rows, r, head0, b0 == 0 && b1 == nb, i, b_lo, nb, each);
                 }
-                seg += units_of(nb);
-                if (++head == heads) {
+                seg += n * units_of(nb);
+                if ((head += n) == heads) {
                     head = 0;
                     do len = ++r < R ? nc_paged_cut(as_const(lens)[r], max_tokens) : 1u;
                     while (len == 0);
@@ -989,10 +1019,10 @@ struct Decode {
     }
 };
 
-template <int D, bool BF, bool UNI>
+template <int D, bool BF, bool UNI, bool MANY>
 __device__ __forceinline__ void decode_body() {
     const Args a = (Args)__builtin_amdgcn_kernarg_segment_ptr();
-    using X = Decode<D, BF, UNI>;
+    using X = Decode<D, BF, UNI, MANY>;
     // the waves' O, or a merge's factors, sums of rows and partial sums
     constexpr uint32_t kWaves = X::NW * 16 * X::OP, kMerge = NC_PAGED_MERGE_ROWS + 2 * 64 + 4 * X::THREADS;
     __shared__ __attribute__((aligned(16))) float s_mem[kWaves > kMerge ? kWaves : kMerge];
@@ -1008,14 +1038,16 @@ __device__ __forceinline__ void decode_body() {
 
 }  // namespace
 
-// `_odd`: pages of any size; the others take sizes that are multiples of 16.
-#define NC_DECODE(D, T, BF)                                                                                      \
-    extern "C" __global__ __launch_bounds__(64 * NC_PAGED_WAVES, 2) void nc_paged_decode_d##D##T(const nc_paged_decode_args) {  \
-        decode_body<D, BF, true>();                                                                             \
-    }                                                                                                            \
-    extern "C" __global__ __launch_bounds__(64 * NC_PAGED_WAVES, 2) void nc_paged_decode_d##D##_odd##T(const nc_paged_decode_args) { \
-        decode_body<D, BF, false>();                                                                            \
+// `_odd`: pages of any size; the others take sizes that are multiples of 16. `_many`: a wave may take a head for itself.
+#define NC_DECODE_KERNEL(NAME, D, BF, UNI, MANY)                                                          \
+    extern "C" __global__ __launch_bounds__(64 * NC_PAGED_WAVES, 2) void NAME(const nc_paged_decode_args) { \
+        decode_body<D, BF, UNI, MANY>();                                                                  \
     }
+#define NC_DECODE(D, T, BF)                                                \
+    NC_DECODE_KERNEL(nc_paged_decode_d##D##T, D, BF, true, false)           \
+    NC_DECODE_KERNEL(nc_paged_decode_d##D##_odd##T, D, BF, false, false)    \
+    NC_DECODE_KERNEL(nc_paged_decode_d##D##_many##T, D, BF, true, true)     \
+    NC_DECODE_KERNEL(nc_paged_decode_d##D##_many_odd##T, D, BF, false, true)
 NC_DECODE(16, , false)
 NC_DECODE(32, , false)
 NC_DECODE(64, , false)

@@ -26,7 +26,7 @@ NC_HD uint32_t nc_paged_quot(uint32_t n, nc_paged_div v) {
     return (uint32_t)(((uint64_t)(2u * n) * v.magic) >> 32) >> v.shift;
 }
 
-#define NC_PAGED_KERNELS 21u // kernels of paged.hip
+#define NC_PAGED_KERNELS 37u // kernels of paged.hip
 
 struct nc_paged_build_args {
     const int32_t *cached, *fresh, *free_pages, *cursor;

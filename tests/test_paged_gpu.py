@@ -123,6 +123,17 @@ def test_decode_long(gpu):
     decode_case(gpu, 10, [12345, 1, 20000], 2, 3, 32, 5)
 
 
+@pytest.mark.parametrize("d,group,ps,dtype,pad", [(16, 1, 16, "f16", 0), (16, 3, 5, "bf16", 0), (32, 16, 16, "bf16", 1),
+                                                  (32, 2, 7, "f16", 0), (64, 5, 16, "f16", 0), (64, 1, 24, "bf16", 3),
+                                                  (128, 2, 32, "bf16", 0), (128, 16, 9, "f16", 0)])
+def test_decode_many_short_heads(gpu, d, group, ps, dtype, pad):
+    """More heads than workgroups, most of no more keys than a block: a workgroup's waves take one each, next to longer
+    requests and empty ones. Lengths around a wave's step (32, 64) and a block (128, 256)."""
+    lens = [1, 31, 32, 33, 0, 63, 64, 65, 100, 127, 128, 129, 2, 255, 256, 257, 17, 700, 0, 5, 16, 15, 90, 3, 48, 1]
+    decode_case(gpu, 140 + d + group, lens, 43, group, d, ps, dtype, o_stride=43 * group * d + pad,
+                q_stride=43 * group * d + 8 * pad)
+
+
 @pytest.mark.parametrize("count", [63, 64, 65, 200, 257, 700, 1500])
 def test_decode_many_requests(gpu, count):
     rng = np.random.default_rng(count)
