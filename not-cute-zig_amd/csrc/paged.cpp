@@ -69,7 +69,7 @@ int resolve(const nc_paged_options *opts, Shape *s) {
     // Workgroups' shares are counted in units, in 32 bits.
     s->heads = o.num_kv_heads * nc_paged_head_parts((uint32_t)s->group);
     const uint64_t keys = nc_paged_step_keys((uint32_t)o.head_dim) * (NC_PAGED_WAVES >> nc_paged_wave_shift((uint32_t)s->group));
-    s->seq_units = (o.page_size * o.max_pages + keys - 1) / keys + NC_PAGED_HEAD_UNITS;
+    s->seq_units = (o.page_size * o.max_pages + keys - 1) / keys + nc_paged_head_units((uint32_t)o.head_dim);
     if (o.num_seqs * s->heads > kMostUnits || s->seq_units > kMostUnits / (o.num_seqs * s->heads)) return NC_ERROR_OVERFLOW;
 
     const uint64_t d = o.head_dim;
@@ -182,6 +182,8 @@ DecodePlan decode_plan(const Shape &s, bool o_vec) {
     // heads each: heads of 64 38.6 -> 30.4 us, of 128 62.1 -> 54.6; on pages of 16 heads of 64 lose 7 %, of 128 28 %).
     const bool two = o.head_dim <= 32 || (!uniform && s.group > 16);
     p.long_log2 = kCusLog2 + (two ? 1 : 0);
+    // Short heads: as many as are resident (heads of 64 and 128 with twice as many: 512 requests of 100 over 8 heads of 128
+    // 48.9 -> 52.2 us).
     p.short_log2 = kCusLog2 + (o.head_dim <= 32 ? 2 : 1);
     // More heads than workgroups: where a workgroup has several short ones, its waves take one each (200 requests of 60
     // tokens, 32 heads of 64, pages of 24, 41.8 -> 26.8 us; 256 of 50, 8 heads of 128, 15.9 -> 13.3; 128 of 120 over 8 heads,

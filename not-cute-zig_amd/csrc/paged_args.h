@@ -61,21 +61,26 @@ NC_HD uint32_t nc_paged_step_keys(uint32_t head_dim) { return head_dim <= 32 ? 6
 NC_HD uint32_t nc_paged_wave_shift(uint32_t group) { return group <= 16 ? 0u : group <= 32 ? 1u : 2u; }
 NC_HD uint32_t nc_paged_head_parts(uint32_t group) { return (group + 63u) / 64u; }
 
-// Shares are counted in units: one per block, and NC_PAGED_HEAD_UNITS before a head's first block for what a head costs
-// however short it is. Workgroup i takes units [i * each, (i + 1) * each), where `each` is the least that
-// 2^most_log2 workgroups can do with, and no less than `least`.
-#define NC_PAGED_HEAD_UNITS 2u
-// A head of no more blocks than this is not split: the workgroup that has its first unit takes all of it.
+// Shares are counted in units: one per block, and before a head's first block so many for what a head costs however
+// short it is. Workgroup i takes units [i * each, (i + 1) * each), where `each` is the least that 2^most_log2
+// workgroups can do with, and no less than `least`. (One unit a head instead of two: 33 requests of up to 2047, 16 heads of
+// 32, 11.3 -> 10.7 us, but 16 of 1000 over 8 heads of 128 16.7 -> 17.1 and 64 ragged ones over 4 of 64 29.6 -> 30.1; two only
+// for heads of two blocks or fewer: the first 15.9, the last 33.)
+NC_HD uint32_t nc_paged_head_units(uint32_t head_dim) { return head_dim <= 32 ? 1u : 2u; }
+// A head of no more blocks than this is not split: the workgroup that has its first unit takes all of it. (Of 1: 118
+// requests of up to 2719, 3 heads of 32, 11.5 -> 12.0 us; of 4: 12.3, and 4 of 500 over 8 heads of 128 7.6 -> 9.5.)
 #define NC_PAGED_WHOLE_BLOCKS 2u
-// Heads of this many units on the average are long ones.
+// Heads of this many units on the average are long ones. (From 14 on: 16 requests of 1000 over 8 heads of 128 16.5 -> 17.3 us,
+// 200 ragged ones of up to 8000 141 -> 148; from 5 on: no change.)
 #define NC_PAGED_LONG_UNITS 8u
 NC_HD uint32_t nc_paged_each(uint32_t units, uint32_t most_log2, uint32_t least) {
     const uint32_t each = (units + (1u << most_log2) - 1u) >> most_log2;
     return each < least ? least : each;
 }
 
-// Pieces that one workgroup adds up, by their size: of up to 16 KB reading 16 of them takes about as long as another
-// round, of more only 4. At most NC_PAGED_MAX_WGS pieces are one after NC_PAGED_ROUNDS rounds, and
+// Pieces that one workgroup adds up in a round, by their size: of up to 16 KB reading 16 of them takes about as long as
+// another round (4: 63 pieces of 1 KB 8.7 -> 10.6 us), of more only 4. All in one round, one request of 100000 tokens, 8
+// query heads on one key head of 128, took 36 us, in rounds 20.5; with 64 query heads 194 and 58. At most NC_PAGED_MAX_WGS pieces are one after NC_PAGED_ROUNDS rounds, and
 // NC_PAGED_MERGE_ROWS holds the rows of all that one adds up.
 #define NC_PAGED_MAX_WGS 1024u
 #define NC_PAGED_ROUNDS 5u
