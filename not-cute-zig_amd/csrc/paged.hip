@@ -68,7 +68,7 @@ extern "C" __global__ __launch_bounds__(1024) void nc_paged_build(const nc_paged
     const uint64_t list_lo = cur + (uint64_t)b * a.chunk_pages;
     const uint64_t list_hi = b == last ? a.free_len : min((uint64_t)a.free_len, list_lo + a.chunk_pages);
     const uint32_t most = a.width * a.ps.d;  // tokens of a table row
-    uint64_t rows = 0, pages = cur;  // rows and list places of the requests before this round's
+    uint64_t rows = 0, pages = cur;  // rows and list places of the requests before this pass's
     uint32_t taken = 0, refused = 0;
     if (tid == 0) s_taken = s_refused = 0;
 
