@@ -169,6 +169,14 @@ def test_decode_one_long_head(gpu, d, group, ps, dtype):
         assert np.array_equal(out.view(np.uint32), again.view(np.uint32))
 
 
+@pytest.mark.parametrize("d,group,ps", [(128, 1, 16), (64, 4, 16), (64, 2, 24), (32, 3, 7), (16, 8, 16)])
+def test_decode_piece_counts(gpu, d, group, ps):
+    """Lengths of 15 to 66 blocks of one head, a piece each: at the edges of what is added up at once."""
+    block = 256 if d <= 32 else 128
+    for blocks in (15, 16, 17, 31, 32, 33, 34, 63, 64, 65, 66):
+        decode_case(gpu, blocks + d, [blocks * block - blocks % 3], 1, group, d, ps)
+
+
 def test_decode_leaves_the_counters_at_zero(gpu):
     opts = nc.paged_options(num_seqs=2, num_q_heads=4, num_kv_heads=2, head_dim=64, page_size=16, num_pages=2000, max_pages=1000)
     work = nc.paged_workspace(opts)
@@ -456,6 +464,15 @@ def build_case(gpu, seed, R, ps, width, max_cached, max_new, places=None, spare=
     for name, g, w in zip(("table", "lens", "offsets", "slots", "counts"), got, want):
         assert np.array_equal(g, w), f"{name}: differs at {np.argwhere(np.asarray(g) != np.asarray(w))[:5].ravel()}"
     return want
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("R,ps,width,max_new,places", [
+    (1, 16, 300, 4000, None), (1, 1, 70, 64, 64), (1, 1, 70, 64, 65), (3, 32, 129, 946, 1600), (8, 7, 80, 100, 4096),
+    (60, 16, 30, 200, 128), (64, 24, 9, 8, 512), (64, 24, 9, 9, 513), (65, 16, 9, 9, 521), (2, 16, 9, 1, 5000)])
+def test_build_few_requests_many_slots(gpu, R, ps, width, max_new, places, in_place):
+    """Where a step's slots go from one workgroup to several, and slot maps with much padding or too few places."""
+    build_case(gpu, 500 + R + ps, R, ps, width, 50, max_new, places=places, cursor=4, in_place=in_place)
 
 
 @pytest.mark.parametrize("in_place", [False, True])
