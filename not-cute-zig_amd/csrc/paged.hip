@@ -249,6 +249,8 @@ NC_APPEND(_d16_unaligned, false, false)
 // prefix sum over the requests' lengths. A run that begins or ends inside a request's keys leaves a piece
 // (max, sum, O), and the workgroups that arrive last add the pieces up, in rounds and in a fixed order. Heads of
 // at most two blocks are not split, and where there are more heads than workgroups a wave takes a short one for itself.
+// Where the heads of a token are next to each other (_next), two or four waves take neighbouring heads of the same keys, so
+// that what shares a line or a row of memory is read at one time; their query heads are one piece.
 //
 // One wave takes KT x 32 keys of a block at a time. Scores: S = K Q^T with K rows straight from memory as the
 // A operand (lane l: key l%16, dims 8(l/16)..+7 of 32), so lane l holds the scores of query l%16 and keys
@@ -259,7 +261,7 @@ NC_APPEND(_d16_unaligned, false, false)
 // sum is the f32 weight to 2^-21 or better: rounding them to one 16-bit number would cost 2^-12 or 2^-9.
 //
 // Measured in replayed graphs (bytes of K and V that count): 96 requests of 8192 over 8 heads of 128, 64 query heads, 532 us
-// (6.0 TB/s; a large copy moves 4.95); one of 120001 over 8 heads of 64, 59 us (4.2); 64 ragged ones of up to 16000 over
+// (6.0 TB/s; a large copy moves 4.95); one of 120001 over 8 heads of 64, 49 us (5.0), token-major 54 (4.5); 64 ragged ones of up to 16000 over
 // 4 heads of 64, 29 us (4.3); 16 of 1000 over 8 of 128, 16.5 us (4.0); one of 100 4.4 us. The short ones are a chain of waits:
 // launch, lengths, table, K and V, O, and for a piece the stores, the count and the others' pieces.
 // -------------------------------------------------------------------------------------------------
@@ -364,7 +366,7 @@ __device__ __forceinline__ Args again(Args p) {
 
 __device__ __forceinline__ float finite_or_0(float m) { return m == neg_inf() ? 0.f : m; }
 
-template <int D, bool BF, bool UNI, bool MANY>
+template <int D, bool BF, bool UNI, bool MANY, bool NEXT>
 struct Decode {
     static constexpr int KT = D <= 32 ? 2 : 1;  // 32-key tiles of a wave's step
     static constexpr int NT = 2 * KT;           // 16-key tiles
@@ -429,7 +431,8 @@ struct Decode {
     // Q of a block's query heads as the B operand: lane (c, g) holds query c of the wave's 16, dims KE*g.. of 32.
     __device__ __forceinline__ void load_q(uint32_t r, uint32_t head0, uint32_t rows) {
         const Args a = again(args);
-        const uint16_t *p = a->q + r * a->q_stride + (head0 + min(16u * qt + c, rows - 1u)) * a->q_head_stride;
+        const uint32_t row = NEXT ? qt * a->group + min(c, a->group - 1u) : min(16u * qt + c, rows - 1u);
+        const uint16_t *p = a->q + r * a->q_stride + (head0 + row) * a->q_head_stride;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
             const uint16_t *x = p + 32 * kk + KE * g;
@@ -869,7 +872,7 @@ struct Decode {
             s_ml[w][c][0] = m;
             s_ml[w][c][1] = sum;
         }
-        if (16 * qt + c < rows) {
+        if (NEXT ? c < a->group : 16 * qt + c < rows) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -879,15 +882,16 @@ struct Decode {
         const uint32_t items = rows * (D / 4);
         for (uint32_t it = threadIdx.x; it < items; it += THREADS) {
             const uint32_t q = it / (D / 4), x = 4 * (it % (D / 4));
-            // waves q/16, q/16 + 2^wave_shift, ... hold query q
+            // waves q/16 (NEXT: q/group), that + 2^wave_shift, ... hold query q
+            const uint32_t j0 = NEXT ? q * a->group_inverse >> 16 : q >> 4, qc = NEXT ? q - j0 * a->group : q & 15u;
             float wm[NW], wl[NW], top = neg_inf(), lsum = 0.f;
             floatx4 wo[NW], out = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (uint32_t n = 0; n < NW; ++n) {
-                const uint32_t j = ((q >> 4) + (n << wave_shift)) & (NW - 1u);
-                wm[n] = n < NW >> wave_shift ? s_ml[j][q & 15u][0] : neg_inf();
-                wl[n] = s_ml[j][q & 15u][1];
-                wo[n] = *reinterpret_cast<const floatx4 *>(&s_o[j][q & 15u][x]);
+                const uint32_t j = (j0 + (n << wave_shift)) & (NW - 1u);
+                wm[n] = n < NW >> wave_shift ? s_ml[j][qc][0] : neg_inf();
+                wl[n] = s_ml[j][qc][1];
+                wo[n] = *reinterpret_cast<const floatx4 *>(&s_o[j][qc][x]);
                 top = fmaxf(top, wm[n]);
             }
 #pragma unroll
@@ -986,11 +990,14 @@ struct Decode {
                 const bool alone = MANY && n > 1;
                 if (alone ? w < n : b0 < b1) {
                     uint32_t kvh = alone ? head + w : head, part = 0;
-                    if (a->head_parts > 1) {
+                    if constexpr (NEXT) {
+                        kvh = (head << wave_shift) + qt;
+                    } else if (a->head_parts > 1) {
                         kvh = head / a->head_parts;
                         part = head - kvh * a->head_parts;
                     }
-                    const uint32_t rows = min(64u, a->group - 64u * part), head0 = kvh * a->group + 64u * part;
+                    const uint32_t rows = NEXT ? a->rows : min(64u, a->group - 64u * part);
+                    const uint32_t head0 = NEXT ? head * a->rows : kvh * a->group + 64u * part;
                     load_q(r, head0, rows);
                     m = neg_inf();
                     l = 0.f;
@@ -1026,10 +1033,10 @@ struct Decode {
     }
 };
 
-template <int D, bool BF, bool UNI, bool MANY>
+template <int D, bool BF, bool UNI, bool MANY, bool NEXT>
 __device__ __forceinline__ void decode_body() {
     const Args a = (Args)__builtin_amdgcn_kernarg_segment_ptr();
-    using X = Decode<D, BF, UNI, MANY>;
+    using X = Decode<D, BF, UNI, MANY, NEXT>;
     // the waves' O, or a merge's factors, sums of rows and partial sums
     constexpr uint32_t kWaves = X::NW * 16 * X::OP, kMerge = NC_PAGED_MERGE_ROWS + 2 * 64 + 4 * X::THREADS;
     __shared__ __attribute__((aligned(16))) float s_mem[kWaves > kMerge ? kWaves : kMerge];
@@ -1046,15 +1053,18 @@ __device__ __forceinline__ void decode_body() {
 }  // namespace
 
 // `_odd`: pages of any size; the others take sizes that are multiples of 16. `_many`: a wave may take a head for itself.
-#define NC_DECODE_KERNEL(NAME, D, BF, UNI, MANY)                                                          \
+// `_next`: the waves take neighbouring heads.
+#define NC_DECODE_KERNEL(NAME, D, BF, UNI, MANY, NEXT)                                                    \
     extern "C" __global__ __launch_bounds__(64 * NC_PAGED_WAVES, 2) void NAME(const nc_paged_decode_args) { \
-        decode_body<D, BF, UNI, MANY>();                                                                  \
+        decode_body<D, BF, UNI, MANY, NEXT>();                                                            \
     }
-#define NC_DECODE(D, T, BF)                                                \
-    NC_DECODE_KERNEL(nc_paged_decode_d##D##T, D, BF, true, false)           \
-    NC_DECODE_KERNEL(nc_paged_decode_d##D##_odd##T, D, BF, false, false)    \
-    NC_DECODE_KERNEL(nc_paged_decode_d##D##_many##T, D, BF, true, true)     \
-    NC_DECODE_KERNEL(nc_paged_decode_d##D##_many_odd##T, D, BF, false, true)
+#define NC_DECODE(D, T, BF)                                                       \
+    NC_DECODE_KERNEL(nc_paged_decode_d##D##T, D, BF, true, false, false)           \
+    NC_DECODE_KERNEL(nc_paged_decode_d##D##_odd##T, D, BF, false, false, false)    \
+    NC_DECODE_KERNEL(nc_paged_decode_d##D##_many##T, D, BF, true, true, false)     \
+    NC_DECODE_KERNEL(nc_paged_decode_d##D##_many_odd##T, D, BF, false, true, false) \
+    NC_DECODE_KERNEL(nc_paged_decode_d##D##_next##T, D, BF, true, false, true)     \
+    NC_DECODE_KERNEL(nc_paged_decode_d##D##_next_odd##T, D, BF, false, false, true)
 NC_DECODE(16, , false)
 NC_DECODE(32, , false)
 NC_DECODE(64, , false)

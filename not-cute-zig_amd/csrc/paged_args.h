@@ -26,7 +26,7 @@ NC_HD uint32_t nc_paged_quot(uint32_t n, nc_paged_div v) {
     return (uint32_t)(((uint64_t)(2u * n) * v.magic) >> 32) >> v.shift;
 }
 
-#define NC_PAGED_KERNELS 37u // kernels of paged.hip
+#define NC_PAGED_KERNELS 53u // kernels of paged.hip
 
 struct nc_paged_build_args {
     const int32_t *cached, *fresh, *free_pages, *cursor;
@@ -55,7 +55,8 @@ struct nc_paged_append_args {
 // The attention's work is counted in blocks: the keys of one request and key head that a workgroup's four waves
 // take in a step. A wave takes step_keys of them for 16 query heads; where a key head has more than 16, two or
 // four waves take the same keys for 16 heads each (wave_shift 1 or 2), and past 64 the workgroup's heads count
-// as another head.
+// as another head. Neighbouring heads (the _next kernels) are shared out in the same way: 1 << wave_shift of them count
+// as one, a wave each.
 #define NC_PAGED_WAVES 4u
 NC_HD uint32_t nc_paged_step_keys(uint32_t head_dim) { return head_dim <= 32 ? 64u : 32u; }
 NC_HD uint32_t nc_paged_wave_shift(uint32_t group) { return group <= 16 ? 0u : group <= 32 ? 1u : 2u; }
@@ -104,11 +105,12 @@ struct nc_paged_decode_args {
     uint64_t table_stride, page_stride, head_stride, token_stride, q_stride, q_head_stride, o_stride, o_head_stride;
     uint32_t num_seqs, num_q_heads, num_kv_heads, group; // group = num_q_heads / num_kv_heads
     uint32_t num_pages, max_tokens;                      // max_tokens = max_pages * page_size
-    uint32_t rows;                                       // query heads of a piece: min(group, 64)
+    uint32_t rows;                                       // query heads of a piece: min(group, 64), or of its neighbouring heads
+    uint32_t group_inverse;                              // q * group_inverse >> 16 is q / group for q < 64, group <= 16
     uint32_t wave_shift, head_parts;
     uint32_t fan; // nc_paged_fan()
     uint32_t long_log2, short_log2, each_least; // workgroups for long heads and for short ones, units of a share
-    nc_paged_div heads;                         // num_kv_heads * head_parts
+    nc_paged_div heads;                         // num_kv_heads * head_parts, or of neighbouring heads so many fewer
     uint32_t q_vec, o_vec;                               // Q, O rows are 16-byte aligned
     float scale;
     nc_paged_div ps;

@@ -177,6 +177,34 @@ def test_decode_piece_counts(gpu, d, group, ps):
         decode_case(gpu, blocks + d, [blocks * block - blocks % 3], 1, group, d, ps)
 
 
+@pytest.mark.parametrize("d,heads,group,ps,layout,dtype", [
+    (16, 4, 4, 16, "nhd", "f16"), (16, 2, 8, 1, "hnd", "bf16"), (16, 8, 3, 5, "nhd", "f16"), (16, 12, 1, 32, "inter", "bf16"),
+    (32, 4, 2, 16, "nhd", "bf16"), (32, 6, 4, 7, "nhd", "f16"), (32, 4, 1, 1, "hnd", "f16"), (32, 2, 3, 16, "nhd", "f16"),
+    (64, 4, 4, 16, "nhd", "f16"), (64, 8, 1, 1, "hnd", "bf16"), (64, 4, 3, 24, "nhd", "bf16"), (64, 12, 2, 64, "inter", "f16"),
+    (128, 4, 4, 32, "nhd", "bf16"), (128, 8, 1, 10, "nhd", "f16"), (128, 4, 2, 1, "nhd", "bf16"), (128, 4, 3, 16, "inter", "f16")])
+def test_decode_heads_beside_each_other(gpu, d, heads, group, ps, layout, dtype):
+    """Token-major pages, where waves take neighbouring heads: ragged requests with empty ones, a long one whose pieces
+    are added up, strides and alignments, an absent page in the middle."""
+    lens = [1, 0, 31, 33, 64, 65, 129, 700, 2000, 5, 257, 32, 63, 0]
+    seed = 700 + d + heads + group + ps
+    decode_case(gpu, seed, lens, heads, group, d, ps, dtype, layout, width=3000 // ps)
+    decode_case(gpu, seed + 1, lens, heads, group, d, ps, dtype, layout, width=3000 // ps, pad=8, sigma=4.0,
+                q_stride=heads * group * d + 3, o_stride=heads * group * d + 1, q_elem=1, o_elem=3)
+    first, again = (decode_case(gpu, seed + 2, [20011, 3], heads, group, d, ps, dtype, layout) for _ in range(2))
+    assert np.array_equal(first.view(np.uint32), again.view(np.uint32))
+    rng = np.random.default_rng(seed)
+    n, width = 900, -(-1000 // ps)
+    held = -(-n // ps)
+    pool = pc.Pool(rng, held + 2, heads, ps, d, dtype, layout)
+    table = pc.make_table(rng, [n], ps, held + 2, width, spare=-1)
+    table[0, held // 2] = held + 2  # names no page
+    q = pc.encode(rng.standard_normal((1, heads * group, d)), dtype)
+    opts = nc.paged_options(num_seqs=1, num_q_heads=heads * group, max_pages=width, **pool.options())
+    out = run_decode(gpu, pool, table, [n], q, opts, group)
+    ref, bound = pc.ref_decode(q, pool, table, [n], opts.scale, group)
+    check(out, ref, bound, opts, "absent page")
+
+
 def test_decode_leaves_the_counters_at_zero(gpu):
     opts = nc.paged_options(num_seqs=2, num_q_heads=4, num_kv_heads=2, head_dim=64, page_size=16, num_pages=2000, max_pages=1000)
     work = nc.paged_workspace(opts)
