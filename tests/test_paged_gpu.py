@@ -645,6 +645,61 @@ def test_captured_step_replays(gpu):
         stream.destroy()
 
 
+def test_first_launches_captured(gpu):
+    """A fresh module whose first launch of each kernel is recorded into a graph, which is then replayed with eager work in
+    between."""
+    module = nc.Module.load_embedded()
+    s = Serving(13, d=32, ps=16, dtype="bf16", heads=4, width=40, pages=60)
+    s.prepare([30, 0, 100, 7, 1], 150)
+    s.upload()
+    stream = nc.Stream()
+    graph = nc.Graph.capture(stream, lambda: s.launch(module, stream.handle))
+    try:
+        for step, new in enumerate(([30, 0, 100, 7, 1], [1, 1, 1, 0, 1], [3, 1, 0, 1, 1], [1, 1, 1, 1, 1])):
+            if step:
+                s.prepare(new, 150)
+                s.upload()
+            decode_case(gpu, 1100 + step, [500, 70], 2, 2, 32, 7)
+            graph.launch(stream)
+            stream.synchronize()
+            s.verify(f"replay {step}")
+    finally:
+        graph.destroy()
+        stream.destroy()
+        module.unload()
+
+
+def test_two_threads_launch_through_one_module(gpu):
+    """Two host threads at once, each with a stream, buffers and a workspace of its own."""
+    import threading
+
+    module = nc.Module.load_embedded()
+    sides = [Serving(21 + i, d=64 if i else 128, ps=16, layers=1, width=30, pages=80) for i in range(2)]
+    streams = [nc.Stream() for _ in sides]
+    errors = []
+
+    def steps(s, stream):
+        try:
+            for new in ([40, 0, 300, 7, 1], [1, 1, 1, 0, 1], [1, 1, 1, 1, 1], [2, 0, 1, 1, 9]):
+                s.prepare(new, 360)
+                s.upload()
+                s.launch(module, stream.handle)
+                stream.synchronize()
+                s.verify("thread")
+        except BaseException as e:  # shown by the main thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=steps, args=x) for x in zip(sides, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for stream in streams:
+        stream.destroy()
+    module.unload()
+    assert not errors, errors
+
+
 def test_two_streams_with_workspaces_of_their_own(gpu):
     """Calls that overlap in time, each with its own workspace, give what they give alone."""
     rng = np.random.default_rng(12)
