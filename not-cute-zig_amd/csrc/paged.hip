@@ -381,9 +381,10 @@ struct Decode {
     static constexpr bool AHEAD = D == 64 || (D == 128 && UNI);
     static constexpr int OP = D + 4;            // pitch of a row of partial O in LDS
     static constexpr uint32_t NW = NC_PAGED_WAVES, THREADS = 64 * NW;
-    // Weights are 2^(SHIFT + score - max): in f16 the low part of a small weight stays a normal number, in bf16
-    // the sum of 2^31 V at the type's largest value (2^128) stays finite, and V below 2^-94 may count as 0.
-    static constexpr float SHIFT = BF ? -32.f : 12.f;
+    // Weights are 2^(score - max) times UNIT: in f16 the low part of a small weight stays a normal number, in bf16
+    // the sum of 2^31 V at the type's largest value (2^128) stays finite, and V below 2^-94 may count as 0. The product
+    // is exact; added to the exponent (-32 and a score of 2^-24 steps) it took 1.3e-6 of every weight.
+    static constexpr float UNIT = BF ? 0x1p-32f : 0x1p12f;
     using KReg = typename std::conditional<D == 16, u32x2, u32x4>::type;
     using VReg = typename std::conditional<E == 8, u32x4, typename std::conditional<E == 4, u32x2, uint32_t>::type>::type;
 
@@ -590,9 +591,9 @@ struct Decode {
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][i]);
         top = fmaxf(m, quad_max(top));
-        const float ref = finite_or_0(top) - SHIFT;
+        const float ref = finite_or_0(top);
         if (!__all(top == m)) {
-            const float f = __builtin_amdgcn_exp2f(m - finite_or_0(top));
+            const float f = __builtin_amdgcn_exp2f(m - ref);
             l *= f;
 #pragma unroll
             for (int i = 0; i < E; ++i) acc[i] *= f;
@@ -602,7 +603,7 @@ struct Decode {
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - ref);
+                s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - ref) * UNIT;
                 l += s[t][i];
             }
         constexpr int PARTS = BF ? 3 : 2;
