@@ -258,7 +258,9 @@ NC_APPEND(_d16_unaligned, false, false)
 // the same way: the lane loads D/16 dims of the eight keys 16t + 4(l/16) + r and turns them in registers.
 // Nothing but the final join of the four waves goes through LDS. K and V are read once and the rest is small, so
 // the read rate bounds it; the matrix cores have time for weights in two (f16) or three (bf16) parts, whose
-// sum is the f32 weight to 2^-21 or better: rounding them to one 16-bit number would cost 2^-12 or 2^-9.
+// sum is the f32 weight to 2^-21 or better (UNIT says down to which weight): rounding them to one 16-bit number would
+// cost 2^-11 or 2^-8. The f16 parts' own accumulators cost 0 to 2 % (33 requests of up to 2047 over 16 heads of 32 11.1 -> 11.4
+// us with the product with UNIT; 96 of 8192 over 8 of 128 536 on both sides).
 //
 // Measured in replayed graphs (bytes of K and V that count): 96 requests of 8192 over 8 heads of 128, 64 query heads, 532 us
 // (6.0 TB/s; a large copy moves 4.95); one of 120001 over 8 heads of 64, 49 us (5.0), token-major 54 (4.5); 64 ragged ones of up to 16000 over
@@ -295,7 +297,9 @@ __device__ __forceinline__ floatx4 mfma_k16(u32x2 x, u32x2 y, floatx4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(half4, x), __builtin_bit_cast(half4, y), c, 0, 0, 0);
 }
 
-// Two f32 rounded to nearest as a pair of 16-bit numbers; x and y become what that leaves.
+// Two f32 rounded to nearest as a pair of 16-bit numbers; x and y become what that leaves, in f16 times kLowUnit: at most
+// half a step of a number below 2^16, times 2^12 below 2^16 too, and exact.
+constexpr float kLowUnit = 0x1p12f;
 template <bool BF>
 __device__ __forceinline__ uint32_t take_pair(float &x, float &y) {
     if constexpr (BF) {
@@ -306,8 +310,8 @@ __device__ __forceinline__ uint32_t take_pair(float &x, float &y) {
         return u;
     } else {
         const half2v h = {(_Float16)x, (_Float16)y};
-        x -= (float)h[0];
-        y -= (float)h[1];
+        x = (x - (float)h[0]) * kLowUnit;
+        y = (y - (float)h[1]) * kLowUnit;
         return __builtin_bit_cast(uint32_t, h);
     }
 }
@@ -381,10 +385,14 @@ struct Decode {
     static constexpr bool AHEAD = D == 64 || (D == 128 && UNI);
     static constexpr int OP = D + 4;            // pitch of a row of partial O in LDS
     static constexpr uint32_t NW = NC_PAGED_WAVES, THREADS = 64 * NW;
-    // Weights are 2^(score - max) times UNIT: in f16 the low part of a small weight stays a normal number, in bf16
-    // the sum of 2^31 V at the type's largest value (2^128) stays finite, and V below 2^-94 may count as 0. The product
-    // is exact; added to the exponent (-32 and a score of 2^-24 steps) it took 1.3e-6 of every weight.
-    static constexpr float UNIT = BF ? 0x1p-32f : 0x1p12f;
+    // Weights are 2^(score - max) times UNIT, in 16-bit parts. f16: the largest fits, the high part is normal down to 2^-29 of
+    // it and the low part, which has a unit of its own (kLowUnit), wherever the high part is: 2^-22 of the weight, or below
+    // 2^-29 of the largest one 2^-52 of that. (Both parts in one unit of 2^12 lost all weights below 2^-37, which are what
+    // counts where the largest one's V is 0.) bf16: the sum of 2^31 V at the type's largest value (2^128) stays finite, and V
+    // below 2^-94 may count as 0; the parts are normal down to 2^-78 of the largest weight. The product with UNIT is exact;
+    // added to the exponent (-32 and a score of 2^-24 steps) it took 1.3e-6 of every weight.
+    static constexpr float UNIT = BF ? 0x1p-32f : 0x1p15f;
+    static constexpr int PARTS = BF ? 3 : 2;
     using KReg = typename std::conditional<D == 16, u32x2, u32x4>::type;
     using VReg = typename std::conditional<E == 8, u32x4, typename std::conditional<E == 4, u32x2, uint32_t>::type>::type;
 
@@ -606,17 +614,22 @@ struct Decode {
                 s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - ref) * UNIT;
                 l += s[t][i];
             }
-        constexpr int PARTS = BF ? 3 : 2;
+        u32x4 p[KT][PARTS];
 #pragma unroll
-        for (int u = 0; u < KT; ++u) {
-            u32x4 p[PARTS];
+        for (int u = 0; u < KT; ++u)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int n = 0; n < PARTS; ++n) p[n][j] = take_pair<BF>(s[2 * u + j / 2][2 * (j % 2)], s[2 * u + j / 2][2 * (j % 2) + 1]);
-            constexpr int G = E < 2 ? E : 2;  // products of so many dims in turn: each waits for its last one
+                for (int n = 0; n < PARTS; ++n)
+                    p[u][n][j] = take_pair<BF>(s[2 * u + j / 2][2 * (j % 2)], s[2 * u + j / 2][2 * (j % 2) + 1]);
+        constexpr int G = E < 2 ? E : 2;  // products of so many dims in turn: each waits for its last one
 #pragma unroll
-            for (int i0 = 0; i0 < E; i0 += G) {
+        for (int i0 = 0; i0 < E; i0 += G) {
+            floatx4 low[G];  // the f16 low parts' product, in units of its own
+#pragma unroll
+            for (int i = 0; i < G; ++i) low[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < KT; ++u) {
                 u32x4 x[G];
 #pragma unroll
                 for (int i = 0; i < G; ++i)
@@ -629,7 +642,16 @@ struct Decode {
 #pragma unroll
                 for (int n = 0; n < PARTS; ++n)
 #pragma unroll
-                    for (int i = 0; i < G; ++i) acc[i0 + i] = mfma_k32<BF>(x[i], p[n], acc[i0 + i]);
+                    for (int i = 0; i < G; ++i) {
+                        floatx4 &sum = !BF && n ? low[i] : acc[i0 + i];
+                        sum = mfma_k32<BF>(x[i], p[u][n], sum);
+                    }
+            }
+            if constexpr (!BF) {
+#pragma unroll
+                for (int i = 0; i < G; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i0 + i][j] = __builtin_fmaf(low[i][j], 1.f / kLowUnit, acc[i0 + i][j]);
             }
         }
     }

@@ -78,3 +78,29 @@ def test_one_weight_beside_the_largest(gpu, d, ps, dtype):
     out = attend(gpu, rng, keys, values, d, ps, dtype)
     off = np.abs(out / want[:, None] - 1.0).max() * 2.0 ** 24
     assert off <= {"f16": 4, "bf16": 1}[dtype] + 2 + 6 + 3 + 2 + 1 + 3 * np.log(2.0), f"off by {off:.1f} x 2^-24"
+
+
+@pytest.mark.parametrize("least,most,dtype", [(16, 24, "f16"), (24, 32, "f16"), (32, 40, "f16"), (20, 45, "bf16"), (45, 70, "bf16")])
+@pytest.mark.parametrize("d,ps", [(16, 16), (32, 7), (64, 16), (64, 5), (128, 16), (128, 3)])
+def test_small_weights_where_the_largest_counts_for_nothing(gpu, d, ps, least, most, dtype):
+    """One key of the largest score with V = 0 and 199 keys `least` to `most` bits below it: O is made of theirs alone.
+
+    In units of 2^-24, relative to sum w |v|: the exponential 2, the parts' sum 4 (2^-22), sums over n keys and up to 40
+    joins of lanes, waves and pieces 2 each (an ulp), the factors of a larger maximum and of the waves' join 3 each, the
+    quotient 3, the score's three roundings times itself (scores are multiples of 2^-8 bits, so their differences are
+    exact). Weights of less than 2^-29 (f16) or 2^-70 (bf16) are off by up to 2^-51 or 2^-93 of the largest weight."""
+    rng = np.random.default_rng(1000 * d + 100 * ps + most)
+    R, n = 40, 200
+    keys, values = np.zeros((R, n, 3)), rng.integers(-64, 65, (R, n)) / 16.0
+    for r in range(R):
+        keys[r, :, 0] = -rng.integers(least, most, n)
+        keys[r, :, 1] = -rng.integers(0, 256, n)
+        top = 0 if r % 2 else rng.integers(0, n)
+        keys[r, top] = values[r, top] = 0.0
+    w = weights(keys)
+    want = (w * values).sum(1) / w.sum(1)
+    out = attend(gpu, rng, keys, values, d, ps, dtype)
+    units = 2 + 4 + 2 * (n + 40) + 6 + 3 + 3 * LN2 * (most + 1)
+    bound = units * 2.0 ** -24 * (w * np.abs(values)).sum(1) + {"f16": 2.0 ** -51, "bf16": 2.0 ** -93}[dtype] * np.abs(values).sum(1)
+    off = (np.abs(out - want[:, None]).max(1) / bound).max()
+    assert off <= 1.0, f"off by {off:.2f} bounds"
