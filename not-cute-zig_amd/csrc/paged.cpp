@@ -167,7 +167,7 @@ int launch(nc_module module, uint32_t kernel, uint32_t grid, uint32_t threads, v
 
 // The attention's kernel, grid and workspace for a set of options.
 struct DecodePlan {
-    uint32_t kernel, grid, rows, wave_shift, heads, block_keys, long_log2, short_log2;
+    uint32_t kernel, grid, rows, wave_shift, side, many, each_least, long_log2, short_log2;
     uint64_t piece_ml, piece_o, bytes;  // offsets of the partials, and all of the workspace
 };
 
@@ -192,29 +192,39 @@ DecodePlan decode_plan(const Shape &s, bool o_vec) {
     // (100 requests of 4000 over 4 heads of 16, pages of 1, 67.4 -> 36.0 us; 200 of up to 1000 over 8 18.6 -> 13.5; with 16 query
     // heads to each of 2 10.8 -> 13.1), and wider ones for their order in memory, unless there are many (one of 120001 over 8
     // heads of 64 59.0 -> 54.4, 8 of 4000 over 8 of 128 32.7 -> 31.2; 30 of up to 6000 over 2 of 128 13.1 -> 14.5, 210 of up to 122
-    // over 32 of 128 40.1 -> 45.1). Short requests are faster over all waves (2 of 200 over 8 heads of 32 4.5 us, 6.4 beside).
+    // over 32 of 128 40.1 -> 45.1). Short requests are faster over all waves, so the kernel looks at the lengths
+    // (NC_PAGED_NEXT_TOKENS: 0.2 us where it finds them short); where the table has no room for a long one, it need not.
     uint32_t side = 0;
-    if ((o.head_stride < o.token_stride || o.page_size == 1) && o.max_pages * o.page_size > 512) {
+    if ((o.head_stride < o.token_stride || o.page_size == 1) && o.max_pages * o.page_size > NC_PAGED_NEXT_TOKENS) {
         const uint64_t numbers = s.group * o.head_dim;  // of one head's piece
         if (o.head_dim <= 32)
             side = o.num_kv_heads % 4 == 0 && numbers <= 64 ? 2 : o.num_kv_heads % 2 == 0 && numbers <= 128 ? 1 : 0;
         else
             side = o.num_kv_heads % 4 == 0 && s.group <= 4 && o.num_seqs * s.heads <= 2u << p.short_log2;
     }
-    p.wave_shift = side ? side : nc_paged_wave_shift((uint32_t)s.group);
-    p.heads = (uint32_t)(side ? o.num_kv_heads >> p.wave_shift : s.heads);
-    p.rows = (uint32_t)(side ? s.group << p.wave_shift : std::min<uint64_t>(s.group, 64));
-    p.block_keys = nc_paged_step_keys((uint32_t)o.head_dim) * (NC_PAGED_WAVES >> p.wave_shift);
-    const uint64_t units = (o.page_size * o.max_pages + p.block_keys - 1) / p.block_keys + nc_paged_head_units((uint32_t)o.head_dim);
-    p.grid = (uint32_t)std::min<uint64_t>(o.num_seqs * p.heads * units, 1u << p.short_log2);
+    p.wave_shift = nc_paged_wave_shift((uint32_t)s.group);
+    p.side = side;
+    p.rows = (uint32_t)std::min<uint64_t>(s.group, 64);
+    const uint64_t step = nc_paged_step_keys((uint32_t)o.head_dim);
+    // A piece is written and read once more: at most a quarter of what its run reads of the cache. (Neighbouring heads' are at
+    // most 16 rows, and no more than a block's reads.)
+    p.each_least = (uint32_t)std::max<uint64_t>(1, 8 * p.rows / (step * (NC_PAGED_WAVES >> p.wave_shift)));
+    // Units there may be, in both ways of taking the heads.
+    auto units = [&](uint64_t heads, uint32_t shift) {
+        const uint64_t keys = step * (NC_PAGED_WAVES >> shift);
+        return o.num_seqs * heads * ((o.page_size * o.max_pages + keys - 1) / keys + nc_paged_head_units((uint32_t)o.head_dim));
+    };
+    const uint64_t most = std::max(units(s.heads, p.wave_shift), side ? units(s.heads >> side, side) : 0);
+    p.grid = (uint32_t)std::min<uint64_t>(most, 1u << p.short_log2);
+    const uint64_t rows = std::max<uint64_t>(p.rows, side ? s.group << side : 0);
     // More heads than workgroups: where a workgroup has several short ones, its waves take one each (200 requests of 60
     // tokens, 32 heads of 64, pages of 24, 41.8 -> 26.8 us; 256 of 50, 8 heads of 128, 15.9 -> 13.3; 128 of 120 over 8 heads,
     // two a workgroup, 13.9 -> 14.3). That code makes every call 0.1 us longer, so it has kernels of its own.
-    const bool many = !side && s.group <= 16 && o_vec && o.num_seqs * s.heads > 1u << p.short_log2;
-    p.kernel = kDecode + 12 * d + (side ? 8 : many ? 4 : 0) + (uniform ? 0 : 2) + (o.element_type == NC_ELEMENT_BF16 ? 1 : 0);
+    p.many = s.group <= 16 && o_vec && o.num_seqs * s.heads > 1u << p.short_log2;
+    p.kernel = kDecode + 12 * d + (side ? 8 : p.many ? 4 : 0) + (uniform ? 0 : 2) + (o.element_type == NC_ELEMENT_BF16 ? 1 : 0);
     p.piece_ml = NC_PAGED_ROUNDS * 2 * NC_PAGED_MAX_WGS * 4;
-    p.piece_o = p.piece_ml + (uint64_t)p.grid * 2 * p.rows * 2 * 4;
-    p.bytes = p.piece_o + (uint64_t)p.grid * 2 * p.rows * o.head_dim * 4;
+    p.piece_o = p.piece_ml + p.grid * 2 * rows * 2 * 4;
+    p.bytes = p.piece_o + p.grid * 2 * rows * o.head_dim * 4;
     return p;
 }
 
@@ -411,16 +421,15 @@ int nc_paged_decode(nc_module module, const nc_paged_decode_buffers *buffers, co
     a.part_ml = reinterpret_cast<float *>(static_cast<char *>(t.workspace) + plan.piece_ml);
     a.part_o = reinterpret_cast<float *>(static_cast<char *>(t.workspace) + plan.piece_o);
     a.rows = plan.rows;
-    a.fan = nc_paged_fan(plan.rows, (uint32_t)op.head_dim);
+    a.wave_shift = plan.wave_shift;
+    a.side = plan.side;
+    a.many = plan.many;
     a.long_log2 = plan.long_log2;
     a.short_log2 = plan.short_log2;
-    a.heads = nc_paged_make_div(plan.heads);
-    a.wave_shift = plan.wave_shift;
+    a.each_least = plan.each_least;
+    a.heads = nc_paged_make_div((uint32_t)s.heads);
     a.group_inverse = (uint32_t)(65536 / s.group + 1);
     a.head_parts = nc_paged_head_parts((uint32_t)s.group);
-    // A piece is written and read once more: at most a quarter of what its run reads of the cache.
-    const uint64_t kv_rows = plan.block_keys * (plan.rows / std::min<uint64_t>(s.group, 64));
-    a.each_least = (uint32_t)std::max<uint64_t>(1, 8 * plan.rows / kv_rows);
     a.q_vec = address(t.q) % 16 == 0 && (op.q_stride | op.q_head_stride) % 8 == 0;
     a.o_vec = o_vec;
     a.table_stride = op.table_stride;

@@ -249,8 +249,8 @@ NC_APPEND(_d16_unaligned, false, false)
 // prefix sum over the requests' lengths. A run that begins or ends inside a request's keys leaves a piece
 // (max, sum, O), and the workgroups that arrive last add the pieces up, in rounds and in a fixed order. Heads of
 // at most two blocks are not split, and where there are more heads than workgroups a wave takes a short one for itself.
-// Where the heads of a token are next to each other (_next), two or four waves take neighbouring heads of the same keys, so
-// that what shares a line or a row of memory is read at one time; their query heads are one piece.
+// Where the heads of a token are next to each other (_next) and a request is long, two or four waves take neighbouring heads
+// of the same keys, so that what shares a line or a row of memory is read at one time; their query heads are one piece.
 //
 // One wave takes KT x 32 keys of a block at a time. Scores: S = K Q^T with K rows straight from memory as the
 // A operand (lane l: key l%16, dims 8(l/16)..+7 of 32), so lane l holds the scores of query l%16 and keys
@@ -431,10 +431,13 @@ struct Decode {
     floatx4 acc[E];
     float m, l;
 
-    // bk = WK * (NW >> wave_shift)
-    __device__ __forceinline__ uint32_t blocks_of(uint32_t len) const {
-        return (len + bk - 1) >> (__builtin_ctz(WK * NW) - wave_shift);
+    // Blocks of WK * (NW >> shift) keys.
+    static __device__ __forceinline__ uint32_t blocks_by(uint32_t len, uint32_t shift) {
+        return (len + (WK * NW >> shift) - 1u) >> (__builtin_ctz(WK * NW) - shift);
     }
+    __device__ __forceinline__ uint32_t blocks_of(uint32_t len) const { return blocks_by(len, wave_shift); }
+    // Query heads of a piece.
+    __device__ __forceinline__ uint32_t piece_rows(Args a) const { return NEXT ? a->group << wave_shift : a->rows; }
     static __device__ __forceinline__ uint32_t units_of(uint32_t nb) { return nb ? nb + nc_paged_head_units(D) : 0u; }
 
     // Q of a block's query heads as the B operand: lane (c, g) holds query c of the wave's 16, dims KE*g.. of 32.
@@ -718,13 +721,14 @@ struct Decode {
     __device__ __forceinline__ void merge_few(uint32_t lead, uint32_t stride, uint32_t count, uint32_t first, uint32_t rows, float *o) {
         const Args a = again(args);
         const float *part_ml = a->part_ml, *part_o = a->part_o;
+        const uint32_t per_piece = piece_rows(a);
         for (uint32_t it = threadIdx.x; it < rows * (D / 4); it += THREADS) {
             const uint32_t q = it / (D / 4), x = 4 * (it % (D / 4));
             float pm[N], pl[N], top = neg_inf(), sum = 0.f;
             floatx4 po[N], out = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (uint32_t n = 0; n < N; ++n) {
-                const uint64_t at = piece_row(lead + min(n, count - 1u) * stride, first, a->rows, q);
+                const uint64_t at = piece_row(lead + min(n, count - 1u) * stride, first, per_piece, q);
                 get2(part_ml + 2 * at, pm[n], pl[n]);
                 po[n] = get4(part_o + at * D + x);
             }
@@ -748,7 +752,7 @@ struct Decode {
     __device__ __forceinline__ void merge(uint32_t lead, uint32_t stride, uint32_t count, uint32_t first, bool all, uint32_t rows, float *o) {
         constexpr uint32_t PF = 4;
         const Args a = again(args);
-        const uint32_t items = rows * (D / 4), piece_rows = a->rows;
+        const uint32_t items = rows * (D / 4), per_piece = piece_rows(a);
         const uint32_t groups = items > THREADS / 2 ? 1u : min(THREADS / items, (count - 1u) / PF + 1u);
         float *part_ml = a->part_ml, *part_o = a->part_o;
         float *s_f = &s_o[0][0][0], *s_tot = s_f + NC_PAGED_MERGE_ROWS;
@@ -761,7 +765,7 @@ struct Decode {
             const uint32_t q = it / (D / 4), x = 4 * (it % (D / 4));
 #pragma unroll
             for (uint32_t n = 0; n < PF; ++n)
-                po[n] = get4(part_o + piece_row(lead + min(n0 + n * groups, count - 1u) * stride, first, piece_rows, q) * D + x);
+                po[n] = get4(part_o + piece_row(lead + min(n0 + n * groups, count - 1u) * stride, first, per_piece, q) * D + x);
         };
         if (works && it < items) load(grp);
         const uint32_t lanes = count > 16u ? 6u : count > 4u ? 4u : 2u;  // log2 of a row's
@@ -769,7 +773,7 @@ struct Decode {
         for (uint32_t q0 = w * per; q0 < rows; q0 += NW * per) {
             const uint32_t n = lane & ((1u << lanes) - 1u), q = q0 + (lane >> lanes);
             float pm = neg_inf(), pl = 0.f;
-            if (n < count && q < rows) get2(part_ml + 2 * piece_row(lead + n * stride, first, piece_rows, q), pm, pl);
+            if (n < count && q < rows) get2(part_ml + 2 * piece_row(lead + n * stride, first, per_piece, q), pm, pl);
             float top = near<true>(pm, lanes > 2u);
             if (lanes > 4u) top = quad_max(top);
             const float f = __builtin_amdgcn_exp2f(pm - finite_or_0(top));
@@ -803,7 +807,7 @@ struct Decode {
                 if (all) {
                     store_o(o, q, x, out, s_tot[2 * q + 1]);
                 } else {
-                    const uint64_t at = piece_row(lead, first, piece_rows, q);
+                    const uint64_t at = piece_row(lead, first, per_piece, q);
                     put2(part_o + at * D + x, out[0], out[1]);
                     put2(part_o + at * D + x + 2, out[2], out[3]);
                     if (x == 0) put2(part_ml + 2 * at, s_tot[2 * q], s_tot[2 * q + 1]);
@@ -818,7 +822,8 @@ struct Decode {
     // few ten GB/s: one that adds up all 256 of a long request took longer than its keys.
     __device__ __forceinline__ void join(uint32_t i, uint32_t first, uint32_t last, uint32_t rows, float *o) {
         const Args a = again(args);
-        const uint32_t pieces = last - first + 1u, fan = nc_paged_one_round(pieces, a->rows * D) ? pieces : a->fan;
+        const uint32_t pieces = last - first + 1u, per_piece = piece_rows(a);
+        const uint32_t fan = nc_paged_one_round(pieces, per_piece * D) ? pieces : nc_paged_fan(per_piece, D);
         uint32_t *counters = a->counters;
         uint32_t c = i - first;
         for (uint32_t stride = 1;; stride *= fan) {
@@ -928,7 +933,7 @@ struct Decode {
             if (whole) {
                 store_o(o, q, x, out, lsum);
             } else {
-                const uint64_t at = piece_row(i, first, a->rows, q);
+                const uint64_t at = piece_row(i, first, piece_rows(a), q);
                 put2(a->part_o + at * D + x, out[0], out[1]);
                 put2(a->part_o + at * D + x + 2, out[2], out[3]);
                 if (x == 0) put2(a->part_ml + 2 * at, top, lsum);
@@ -938,38 +943,31 @@ struct Decode {
         __syncthreads();  // LDS is free again
     }
 
-    __device__ __forceinline__ void run() {
+    // scale: of the scores, in bits. mine: units of this lane's requests; some: how many of them have keys; len0: the length of
+    // the last; zero_len: the length of request blockIdx.x.
+    __device__ __forceinline__ void run(float scale, uint32_t mine, uint32_t some, uint32_t len0, int32_t zero_len) {
+        sc = scale;
         const Args a = args;
         const int32_t *lens = a->seq_lens;
         const uint32_t max_tokens = a->max_tokens;
-        sc = a->scale * kLog2e;
         const uint32_t R = a->num_seqs, per = (R + 63u) / 64u;  // requests of a lane
         const uint32_t zero_r = blockIdx.x;
-        const int32_t zero_len = zero_r < R ? as_const(lens)[zero_r] : 1;
-        uint32_t mine = 0, some = 0, len0 = 0;  // units, and requests with keys
-        for (uint32_t j = 0; j < per; ++j) {
-            const uint32_t r = lane * per + j;
-            if (r < R) {
-                len0 = nc_paged_cut(lens[r], max_tokens);
-                mine += units_of(blocks_of(len0));
-                some += len0 != 0;
-            }
-        }
         kat = 2u * (c * (uint32_t)a->token_stride + KE * g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) vat[i] = 2u * ((4 * g + i) * (uint32_t)a->token_stride + E * c);
-        const uint32_t incl = wave_scan32(mine), heads = a->heads.d;
+        const uint32_t incl = wave_scan32(mine), heads = NEXT ? a->heads.d >> wave_shift : a->heads.d;
         const uint32_t total = __builtin_amdgcn_readlane(incl, 63), with_keys = __builtin_amdgcn_readlane(wave_scan32(some), 63);
         const uint32_t units = total * heads, i = blockIdx.x;
         // Heads of many blocks: half the workgroups, which leaves half the pieces to join; one with its loads under way
         // a step ahead keeps a CU's share of the memory busy. Heads of few: the others hide each head's beginning and end.
         const uint32_t most_log2 = total >= NC_PAGED_LONG_UNITS * with_keys ? a->long_log2 : a->short_log2;
-        const uint32_t each = nc_paged_each(units, most_log2, a->each_least), u0 = i * each, u1 = min(u0 + each, units);
+        const uint32_t each = nc_paged_each(units, most_log2, NEXT ? 1u : a->each_least), u0 = i * each, u1 = min(u0 + each, units);
         if (u0 < units) {
             // Request r, of length len, whose units begin behind `pre` of the requests before it (times the heads).
             uint32_t r, len, pre;
             {
-                const uint32_t t = nc_paged_quot(u0, {heads, a->heads.magic, a->heads.shift});  // the same request's unit if it had one head
+                // the same request's unit if it had one head
+                const uint32_t t = nc_paged_quot(u0, nc_paged_div_by({a->heads.d, a->heads.magic, a->heads.shift}, NEXT ? wave_shift : 0u));
                 const uint32_t from = __builtin_ctzll(__ballot(incl - mine <= t && t < incl));
                 pre = __builtin_amdgcn_readlane(incl - mine, from);
                 r = from * per;
@@ -1005,7 +1003,7 @@ struct Decode {
                 // there are heads.
                 uint32_t n = 1;
                 if constexpr (MANY) {
-                    if (nb == 1 && seg >= u0) {
+                    if (nb == 1 && seg >= u0 && a->many) {
                         n = min(min(heads - head, NW), (u1 - seg + units_of(1) - 1u) / units_of(1));
                         if (len > n * WK) n = 1;
                     }
@@ -1019,8 +1017,8 @@ struct Decode {
                         kvh = head / a->head_parts;
                         part = head - kvh * a->head_parts;
                     }
-                    const uint32_t rows = NEXT ? a->rows : min(64u, a->group - 64u * part);
-                    const uint32_t head0 = NEXT ? head * a->rows : kvh * a->group + 64u * part;
+                    const uint32_t rows = NEXT ? piece_rows(a) : min(64u, a->group - 64u * part);
+                    const uint32_t head0 = NEXT ? head * rows : kvh * a->group + 64u * part;
                     load_q(r, head0, rows);
                     m = neg_inf();
                     l = 0.f;
@@ -1056,10 +1054,12 @@ struct Decode {
     }
 };
 
+// NEXT: heads each for themselves (MANY: where a->many says so, short ones a wave each) or neighbouring ones together, whichever
+// the lengths call for; else MANY says it all.
 template <int D, bool BF, bool UNI, bool MANY, bool NEXT>
 __device__ __forceinline__ void decode_body() {
     const Args a = (Args)__builtin_amdgcn_kernarg_segment_ptr();
-    using X = Decode<D, BF, UNI, MANY, NEXT>;
+    using X = Decode<D, BF, UNI, MANY, false>;
     // the waves' O, or a merge's factors, sums of rows and partial sums
     constexpr uint32_t kWaves = X::NW * 16 * X::OP, kMerge = NC_PAGED_MERGE_ROWS + 2 * 64 + 4 * X::THREADS;
     __shared__ __attribute__((aligned(16))) float s_mem[kWaves > kMerge ? kWaves : kMerge];
@@ -1067,16 +1067,44 @@ __device__ __forceinline__ void decode_body() {
     __shared__ uint32_t s_word;
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t shift = a->wave_shift;
-    X x{a, lane, w, lane & 15u, lane >> 4, shift, X::WK * (X::NW >> shift), w & ((1u << shift) - 1u), w >> shift,
-        reinterpret_cast<float (*)[16][X::OP]>(s_mem), s_ml, &s_word};
-    x.run();
+    const uint32_t shift = a->wave_shift, side = NEXT ? a->side : 0u;
+    const int32_t *lens = a->seq_lens;
+    const uint32_t max_tokens = a->max_tokens;
+    const float scale = a->scale * kLog2e;
+    const uint32_t R = a->num_seqs, per = (R + 63u) / 64u;  // requests of a lane
+    // All of these arguments before the first load of a length: scalar loads are waited for together.
+    asm volatile("" ::"s"(lens), "s"(max_tokens), "s"(R), "s"(shift), "s"(side));
+    const int32_t zero_len = blockIdx.x < R ? as_const(lens)[blockIdx.x] : 1;
+    uint32_t mine = 0, some = 0, len0 = 0, mine_next = 0, longest = 0;
+    for (uint32_t j = 0; j < per; ++j) {
+        const uint32_t r = lane * per + j;
+        if (r < R) {
+            len0 = nc_paged_cut(lens[r], max_tokens);
+            mine += X::units_of(X::blocks_by(len0, shift));
+            some += len0 != 0;
+            if constexpr (NEXT) {
+                mine_next += X::units_of(X::blocks_by(len0, side));
+                longest = max(longest, len0);
+            }
+        }
+    }
+    auto *o = reinterpret_cast<float (*)[16][X::OP]>(s_mem);
+    if constexpr (NEXT) {
+        if (__ballot(longest > NC_PAGED_NEXT_TOKENS)) {
+            using Y = Decode<D, BF, UNI, false, true>;
+            Y y{a, lane, w, lane & 15u, lane >> 4, side, Y::WK * (Y::NW >> side), w & ((1u << side) - 1u), w >> side, o, s_ml, &s_word};
+            y.run(scale, mine_next, some, len0, zero_len);
+            return;
+        }
+    }
+    X x{a, lane, w, lane & 15u, lane >> 4, shift, X::WK * (X::NW >> shift), w & ((1u << shift) - 1u), w >> shift, o, s_ml, &s_word};
+    x.run(scale, mine, some, len0, zero_len);
 }
 
 }  // namespace
 
 // `_odd`: pages of any size; the others take sizes that are multiples of 16. `_many`: a wave may take a head for itself.
-// `_next`: the waves take neighbouring heads.
+// `_next`: the waves take neighbouring heads of long requests.
 #define NC_DECODE_KERNEL(NAME, D, BF, UNI, MANY, NEXT)                                                    \
     extern "C" __global__ __launch_bounds__(64 * NC_PAGED_WAVES, 2) void NAME(const nc_paged_decode_args) { \
         decode_body<D, BF, UNI, MANY, NEXT>();                                                            \
@@ -1086,8 +1114,8 @@ __device__ __forceinline__ void decode_body() {
     NC_DECODE_KERNEL(nc_paged_decode_d##D##_odd##T, D, BF, false, false, false)    \
     NC_DECODE_KERNEL(nc_paged_decode_d##D##_many##T, D, BF, true, true, false)     \
     NC_DECODE_KERNEL(nc_paged_decode_d##D##_many_odd##T, D, BF, false, true, false) \
-    NC_DECODE_KERNEL(nc_paged_decode_d##D##_next##T, D, BF, true, false, true)     \
-    NC_DECODE_KERNEL(nc_paged_decode_d##D##_next_odd##T, D, BF, false, false, true)
+    NC_DECODE_KERNEL(nc_paged_decode_d##D##_next##T, D, BF, true, true, true)     \
+    NC_DECODE_KERNEL(nc_paged_decode_d##D##_next_odd##T, D, BF, false, true, true)
 NC_DECODE(16, , false)
 NC_DECODE(32, , false)
 NC_DECODE(64, , false)

@@ -56,8 +56,12 @@ struct nc_paged_append_args {
 // take in a step. A wave takes step_keys of them for 16 query heads; where a key head has more than 16, two or
 // four waves take the same keys for 16 heads each (wave_shift 1 or 2), and past 64 the workgroup's heads count
 // as another head. Neighbouring heads (the _next kernels) are shared out in the same way: 1 << wave_shift of them count
-// as one, a wave each.
+// as one, a wave each. Those kernels have the code of both ways and take neighbouring heads where a request is longer than
+// NC_PAGED_NEXT_TOKENS: the lengths decide it, not the table's width. (In a table of 4096 tokens' pages, neighbouring heads
+// and not: 2 requests of 200 over 8 heads of 32 6.4 and 4.7 us, 4 of 300 over 8 of 16 6.8 and 5.6; 8 of 400 over 8 of 128 9.4
+// and 9.5.)
 #define NC_PAGED_WAVES 4u
+#define NC_PAGED_NEXT_TOKENS 512u
 NC_HD uint32_t nc_paged_step_keys(uint32_t head_dim) { return head_dim <= 32 ? 64u : 32u; }
 NC_HD uint32_t nc_paged_wave_shift(uint32_t group) { return group <= 16 ? 0u : group <= 32 ? 1u : 2u; }
 NC_HD uint32_t nc_paged_head_parts(uint32_t group) { return (group + 63u) / 64u; }
@@ -105,16 +109,23 @@ struct nc_paged_decode_args {
     uint64_t table_stride, page_stride, head_stride, token_stride, q_stride, q_head_stride, o_stride, o_head_stride;
     uint32_t num_seqs, num_q_heads, num_kv_heads, group; // group = num_q_heads / num_kv_heads
     uint32_t num_pages, max_tokens;                      // max_tokens = max_pages * page_size
-    uint32_t rows;                                       // query heads of a piece: min(group, 64), or of its neighbouring heads
     uint32_t group_inverse;                              // q * group_inverse >> 16 is q / group for q < 64, group <= 16
+    uint32_t rows;                                       // query heads of a piece: min(group, 64)
     uint32_t wave_shift, head_parts;
-    uint32_t fan; // nc_paged_fan()
     uint32_t long_log2, short_log2, each_least; // workgroups for long heads and for short ones, units of a share
-    nc_paged_div heads;                         // num_kv_heads * head_parts, or of neighbouring heads so many fewer
+    nc_paged_div heads;                         // num_kv_heads * head_parts
+    uint32_t side;                              // _next kernels: wave_shift of neighbouring heads
+    uint32_t many;                              // a wave may take a short head for itself
     uint32_t q_vec, o_vec;                               // Q, O rows are 16-byte aligned
     float scale;
     nc_paged_div ps;
 };
+
+// The divisor d / 2^side where 2^side divides d: the same multiplier, as 2^(31+shift) / d is.
+NC_HD nc_paged_div nc_paged_div_by(nc_paged_div v, uint32_t side) {
+    nc_paged_div r = {v.d >> side, v.magic, v.shift - side};
+    return r;
+}
 
 // A length from device memory, cut to what the table's row can hold.
 NC_HD uint32_t nc_paged_cut(int32_t len, uint32_t most) {
