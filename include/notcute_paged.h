@@ -70,8 +70,8 @@ void nc_paged_options_init(nc_paged_options *opts);
  * head_dim or element_type, a stride that makes two rows overlap, a cache stride that is no multiple of
  * 8 elements (16 bytes). NC_ERROR_OVERFLOW: more than 2^31 - 1 slots in the pool, tokens in a table row,
  * requests or outputs of a request (num_q_heads * head_dim); more than 2^30 blocks of keys to share out
- * (per request and key head, a block for every 32 tokens of the table's row and two more are always within
- * what counts); a tensor past 2^60 elements. */
+ * (for each request, key head and part of up to 64 of the key head's query heads, a block for every 32 tokens
+ * of the table's row and two more are always within what counts); a tensor past 2^60 elements. */
 int nc_paged_validate(const nc_paged_options *opts);
 
 /* Block tables, slot map and row offsets of one step, from the requests' lengths.

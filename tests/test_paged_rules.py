@@ -1,7 +1,12 @@
 """Paged cache, on the CPU: index arithmetic and counts of csrc/paged_args.h beyond those of test_paged.py."""
 
 import os
+import re
 import subprocess
+
+import pytest
+
+import notcute_flash as nc
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "not-cute-zig_amd", "csrc")
@@ -34,3 +39,20 @@ def test_divisor_of_neighbouring_heads(tmp_path):
             }
         }
     }""")
+
+
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("group", [1, 16, 17, 32, 33, 64, 65, 128, 129, 1000])
+@pytest.mark.parametrize("heads", [1, 3])
+def test_blocks_that_the_header_promises_to_accept(d, group, heads):
+    """The header's count of blocks: as many as it names are accepted, and 8 times as many (32-token blocks, of which a wave's
+    step may hold up to 8) are not."""
+    text = " ".join(re.sub(r"\n \*", " ", open(os.path.join(ROOT, "include", "notcute_paged.h")).read()).split())
+    assert "for each request, key head and part of up to 64 of the key head's query heads, a block for every 32 tokens of the table's row and two more" in text
+    parts, tokens = -(-group // 64), 2 ** 20
+    seqs = 2 ** 30 // (heads * parts * (tokens // 32 + 2))
+    o = dict(num_q_heads=heads * group, num_kv_heads=heads, head_dim=d, page_size=16, num_pages=4, max_pages=tokens // 16)
+    nc.paged_validate(nc.paged_options(num_seqs=seqs, **o))
+    with pytest.raises(nc.NcError) as e:
+        nc.paged_validate(nc.paged_options(num_seqs=8 * seqs + 8, **o))
+    assert e.value.name == "Overflow"
