@@ -10,8 +10,8 @@
  * plain device pointers with element counts, f16 (or bf16) bit patterns as uint16_t, O in f32,
  * asynchronous on the given stream. A call's tensors come as one block of pointers and lengths in elements,
  * which it reads before it returns. No call allocates, synchronises or copies; every one may be captured
- * into a HIP graph (nc_paged_build may be two launches, the others are one). The kernels are in the
- * embedded code object: `module` is one from nc_module_load_embedded.
+ * into a HIP graph (nc_paged_build may be two launches, the others are one). `module` is one from
+ * nc_module_load_embedded; the first of these calls through it loads the kernels (about 1.4 ms, once).
  *
  * The cache. K and V are each a pool of `num_pages` pages of `page_size` tokens. The row of token t and
  * key head h in page p starts at element p*page_stride + h*head_stride + t*token_stride and holds
