@@ -1031,11 +1031,22 @@ struct Decode {
                         finish(rows, r, head0, b0 == 0 && b1 == nb, i, b_lo, nb, each);
                 }
                 seg += n * units_of(nb);
+                if (seg >= u1) break;
                 if ((head += n) == heads) {
                     head = 0;
-                    do len = ++r < R ? nc_paged_cut(as_const(lens)[r], max_tokens) : 1u;
-                    while (len == 0);
-                    if (r >= R) break;
+                    // The next request with keys: the next one, or behind empty ones 64 at a time (one by one, and to the end
+                    // where there was none, a batch of 4096 of which only the first had keys took 271 us).
+                    len = ++r < R ? nc_paged_cut(as_const(lens)[r], max_tokens) : 0u;
+                    for (uint32_t r0 = r + 1u; len == 0 && r0 < R; r0 += 64) {
+                        const uint32_t x = r0 + lane < R ? nc_paged_cut(lens[r0 + lane], max_tokens) : 0u;
+                        const uint64_t hit = __ballot(x != 0);
+                        if (hit) {
+                            const uint32_t y = __builtin_ctzll(hit);
+                            r = r0 + y;
+                            len = __builtin_amdgcn_readlane(x, y);
+                        }
+                    }
+                    if (len == 0) break;
                     nb = blocks_of(len);
                 }
             }
