@@ -148,11 +148,11 @@ uint64_t nc_paged_workspace_bytes(const nc_paged_options *opts);
 /* O[r][i] = sum_j p_j V[j] over the seq_lens[r] tokens j of request r, p = softmax_j(scale * Q[r][i] . K[j]),
  * for every query head i. Scores, maxima, exponentials and sums are f32. The weights enter the product with V as the sum of
  * two (f16) or three (bf16) 16-bit numbers, which is the f32 weight to 2^-21 or better for weights down to 2^-29 (f16) or
- * 2^-70 (bf16) of the largest one, and below that off by at most 2^-51 or 2^-93 of the largest one. In bf16, V below 2^-94
- * may count as 0. A request of
- * length 0, one whose pages are all absent and one whose scores are all -infinity get zeros. A NaN among the
- * keys that count gives NaN, and so does an infinite V among them; what lies elsewhere in the pools may be
- * anything. Q at any element alignment, O at any
+ * 2^-70 (bf16) of the largest one, and below that off by at most 2^-51 or 2^-93 of the largest one. In bf16, what is
+ * below 2^-94, of V or of a weight (over the largest one) times V, may count as 0. A request of length 0, one whose pages
+ * are all absent and one whose scores are all -infinity get zeros. A NaN among the keys that count gives NaN, and so does a
+ * score of +infinity or an infinite V among them; what lies elsewhere in the pools may be anything. Q at any element
+ * alignment, O at any
  * float; caches and workspace 16-byte aligned. O and the workspace overlap nothing else
  * (NC_ERROR_INVALID_VALUE). Rows of O behind the last request are not touched. How the keys are split over
  * workgroups follows the lengths of all requests, so a request's rounding may differ with its neighbours;

@@ -179,21 +179,29 @@ DecodePlan decode_plan(const Shape &s, bool o_vec) {
     // A 16-key tile lies in one page, and a page's byte offsets fit 32 bits.
     const bool uniform = o.page_size % 16 == 0 && o.page_stride < (1ull << 31) && o.page_size * o.token_stride < (1ull << 30);
     const uint32_t d = o.head_dim == 16 ? 0 : o.head_dim == 32 ? 1 : o.head_dim == 64 ? 2 : 3;
-    // Workgroups for long heads: one per CU where a step's loads are wide and a step ahead. Two for small heads, and for pages
-    // of any size where waves share their keys and have half as much under way (4 requests of 20000 over 4 heads, 20 query
-    // heads each: heads of 64 38.6 -> 30.4 us, of 128 62.1 -> 54.6; on pages of 16 heads of 64 lose 7 %, of 128 28 %).
+    // Workgroups for long heads: one per CU for heads of 64 and 128, whose loads are wide. Two for small heads, and on pages of
+    // any size where waves share their keys and have half as much under way. 4 requests of 20000 over 4 key heads, 20 query
+    // heads each, one and two per CU:
+    //   pages of 24   heads of 64  39.2  31.1 us    heads of 128  59.6  54.3
+    //   pages of 16   heads of 64  32.9  30.9       heads of 128  54.2  55.9   (96 of 4000 over 8 of 64: 167  175)
     const bool two = o.head_dim <= 32 || (!uniform && s.group > 16);
     p.long_log2 = kCusLog2 + (two ? 1 : 0);
-    // Short heads: as many as are resident (heads of 64 and 128 with twice as many: 512 requests of 100 over 8 heads of 128
-    // 48.9 -> 52.2 us).
+    // Short heads: as many as are resident. (Heads of 64 and 128 with twice as many: 512 requests of 100 over 8 heads of 128
+    // 48.6 -> 50.0 us.)
     p.short_log2 = kCusLog2 + (o.head_dim <= 32 ? 2 : 1);
     // Where a token's heads are next to each other and its neighbour's rows are not, two or four waves take neighbouring heads
-    // of the same keys rather than different keys of one head, if their pieces stay small: heads that share a 128-byte line
-    // (100 requests of 4000 over 4 heads of 16, pages of 1, 67.4 -> 36.0 us; 200 of up to 1000 over 8 18.6 -> 13.5; with 16 query
-    // heads to each of 2 10.8 -> 13.1), and wider ones for their order in memory, unless there are many (one of 120001 over 8
-    // heads of 64 59.0 -> 54.4, 8 of 4000 over 8 of 128 32.7 -> 31.2; 30 of up to 6000 over 2 of 128 13.1 -> 14.5, 210 of up to 122
-    // over 32 of 128 40.1 -> 45.1). Short requests are faster over all waves, so the kernel looks at the lengths
-    // (NC_PAGED_NEXT_TOKENS: 0.2 us where it finds them short); where the table has no room for a long one, it need not.
+    // of the same keys rather than different keys of one head, if their pieces stay small. Small heads share a 128-byte line;
+    // wide ones gain by their order in memory, unless there are many. Each head for itself and neighbouring ones:
+    //   100 requests of 4000 over 4 heads of 16, pages of 1             67.6  36.8 us
+    //   200 of up to 1000 over 8 heads of 16                            18.7  13.3
+    //   16 of 6000 over 2 heads of 16, 16 query heads each              10.8  13.4 (not taken: large pieces)
+    //   one of 120001 over 8 heads of 64                                59.1  54.5
+    //   8 of 4000 over 8 heads of 128                                   31.9  30.5
+    //   30 of up to 6000 over 2 heads of 128                            12.9  14.2 (not taken: two heads)
+    //   160 of 3000 over 8 heads of 128                                331   338   (not taken: many; but 100 of up to 2000
+    //                                               over 32 heads would be 105 and 87, 200 of up to 4000 over 8 of 64 57 and 46)
+    // Short requests are faster over all waves, so the kernel looks at the lengths (NC_PAGED_NEXT_TOKENS; 0.1 to 0.3 us where it
+    // finds them short); where the table has no room for a long one, it need not.
     uint32_t side = 0;
     if ((o.head_stride < o.token_stride || o.page_size == 1) && o.max_pages * o.page_size > NC_PAGED_NEXT_TOKENS) {
         const uint64_t numbers = s.group * o.head_dim;  // of one head's piece
@@ -217,9 +225,11 @@ DecodePlan decode_plan(const Shape &s, bool o_vec) {
     const uint64_t most = std::max(units(s.heads, p.wave_shift), side ? units(s.heads >> side, side) : 0);
     p.grid = (uint32_t)std::min<uint64_t>(most, 1u << p.short_log2);
     const uint64_t rows = std::max<uint64_t>(p.rows, side ? s.group << side : 0);
-    // More heads than workgroups: where a workgroup has several short ones, its waves take one each (200 requests of 60
-    // tokens, 32 heads of 64, pages of 24, 41.8 -> 26.8 us; 256 of 50, 8 heads of 128, 15.9 -> 13.3; 128 of 120 over 8 heads,
-    // two a workgroup, 13.9 -> 14.3). That code makes every call 0.1 us longer, so it has kernels of its own.
+    // More heads than workgroups: where a workgroup has several short ones, its waves take one each. Without and with:
+    //   200 requests of 60, 32 heads of 64, pages of 24   42.7  26.7 us
+    //   256 of 50, 8 heads of 128                         15.8  13.2
+    //   128 of 120, 8 heads of 128, two a workgroup       14.1  14.1
+    // That code makes a call up to 0.1 us longer, so it has kernels of its own.
     p.many = s.group <= 16 && o_vec && o.num_seqs * s.heads > 1u << p.short_log2;
     p.kernel = kDecode + 12 * d + (side ? 8 : p.many ? 4 : 0) + (uniform ? 0 : 2) + (o.element_type == NC_ELEMENT_BF16 ? 1 : 0);
     p.piece_ml = NC_PAGED_ROUNDS * 2 * NC_PAGED_MAX_WGS * 4;
@@ -303,8 +313,10 @@ int nc_paged_build(nc_module module, const nc_paged_build_buffers *buffers, cons
     a.ps = nc_paged_make_div((uint32_t)o.page_size);
     const uint32_t threads = o.num_seqs <= 64 ? 64 : o.num_seqs <= 256 ? 256 : 1024;
     // One workgroup where its threads write a slot each, or a request's thread its few. Else a slot a thread, or two where a
-    // workgroup needs several rounds to scan the requests: 3 requests of 1400 rows 3.9 us (one workgroup 17.1, of 1024 threads
-    // 7.1), 256 of 140000 5.3 (two a thread 5.7, four 7.0), 2000 of 530000 11.4 (one 17.7, four 12.9).
+    // workgroup needs several rounds to scan the requests. This rule, twice as many a thread, and all in one workgroup:
+    //   3 requests of up to 946 rows, 1400 together   4.0   4.5   17 us
+    //   256 of up to 4096, 121000 together            5.3   5.8  337
+    //   2000 of up to 2000, 530000 together          11.4  12.8  454
     const uint64_t chunk = threads * (o.num_seqs > 1024 ? 2 : 1);
     const uint64_t single = std::max<uint64_t>(threads, std::min<uint64_t>(4096, 8 * o.num_seqs));
     const uint64_t wgs = t.slots_len <= single ? 1 : std::min<uint64_t>((t.slots_len + chunk - 1) / chunk, 1024);

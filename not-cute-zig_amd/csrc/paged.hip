@@ -190,8 +190,8 @@ extern "C" __global__ __launch_bounds__(1024) void nc_paged_build(const nc_paged
 // -------------------------------------------------------------------------------------------------
 // Row append: a copy, 16 bytes of K and of V per thread (more in flight per thread, or four times the rows per
 // workgroup, took 2-25 % longer). What bounds it is the copy's rate. Streaming stores: 30000 rows x 8 heads x 64, off
-// alignment, 26.1 -> 20.5 us (6.0 TB/s of rows read and written), 2048 x 8 x 128 4.1 -> 3.6 us; but where a head's
-// row is 32 bytes and stands alone (page size 1) 8.7 -> 10.7 us, so not for head_dim 16. VEC: the rows are
+// alignment, 26.2 -> 20.5 us (6.0 TB/s of rows read and written), 2048 x 8 x 128 4.1 -> 3.5 us; but where a head's
+// row is 32 bytes and stands alone (page size 1) 8.6 -> 10.7 us, so not for head_dim 16. VEC: the rows are
 // 16-byte aligned.
 // -------------------------------------------------------------------------------------------------
 namespace {
@@ -259,13 +259,17 @@ NC_APPEND(_d16_unaligned, false, false)
 // Nothing but the final join of the four waves goes through LDS. K and V are read once and the rest is small, so
 // the read rate bounds it; the matrix cores have time for weights in two (f16) or three (bf16) parts, whose
 // sum is the f32 weight to 2^-21 or better (UNIT says down to which weight): rounding them to one 16-bit number would
-// cost 2^-11 or 2^-8. The f16 parts' own accumulators cost 0 to 2 % (33 requests of up to 2047 over 16 heads of 32 11.1 -> 11.4
-// us with the product with UNIT; 96 of 8192 over 8 of 128 536 on both sides).
+// cost 2^-11 or 2^-8. The product with UNIT and the f16 parts' own accumulators cost 0 to 2 % (33 requests of up to 2047 over 16
+// heads of 32 11.1 -> 11.4 us; 96 of 8192 over 8 of 128 537 on both sides).
 //
-// Measured in replayed graphs (bytes of K and V that count): 96 requests of 8192 over 8 heads of 128, 64 query heads, 532 us
-// (6.0 TB/s; a large copy moves 4.95); one of 120001 over 8 heads of 64, 49 us (5.0), token-major 54 (4.5); 64 ragged ones of up to 16000 over
-// 4 heads of 64, 29 us (4.3); 16 of 1000 over 8 of 128, 16.5 us (4.0); one of 100 4.4 us. The short ones are a chain of waits:
-// launch, lengths, table, K and V, O, and for a piece the stores, the count and the others' pieces.
+// Measured in replayed graphs (bytes of K and V that count):
+//   96 requests of 8192 over 8 heads of 128, 64 query heads    537 us  6.0 TB/s (a large copy moves 4.9)
+//   one of 120001 over 8 heads of 64                            51     4.8      (token-major 54 to 56)
+//   64 ragged ones of up to 16000 over 4 heads of 64            28.7   4.3
+//   16 of 1000 over 8 of 128                                    16.4   4.0
+//   one of 100                                                   4.4
+// The short ones are a chain of waits: launch, lengths, table, K and V, O, and for a piece the stores, the count and the
+// others' pieces. More than 64 requests' lengths are read one after the other by a lane (4096 requests: 26 us).
 // -------------------------------------------------------------------------------------------------
 namespace {
 
@@ -378,10 +382,11 @@ struct Decode {
     static constexpr int E = D / 16;            // dims of a lane in V and O
     static constexpr int KK = D < 32 ? 1 : D / 32;  // products of a score
     static constexpr int KE = D == 16 ? 4 : 8;  // dims of a lane in one product
-    // Whether a step's loads are under way before the one before it is computed. It costs registers, and pays where a
-    // step's loads are wide: 2 requests of 105543 keys over 2 heads of 64 on pages of 1 56.8 -> 48.0 us. Heads of 16 or 32
-    // are better off with more workgroups instead (33 requests of up to 2047, 16 heads of 32, 13.7 -> 11.5 us on pages of
-    // 16, and 14.5 -> 11.2 of 7), and with heads of 128 on odd pages both the addresses and two steps do not fit (2 % slower).
+    // Whether a step's loads are under way before the one before it is computed. It costs registers, and pays where a step's
+    // loads are wide and heads end at different times: 64 ragged requests over 4 heads of 64 31.6 -> 28.7 us, 32 of 2048 over 8
+    // of 64 28.0 -> 27.6 (but one of 120001 over 8 of 64, token-major, 53 -> 56). Heads of 16 or 32 are better off with more
+    // workgroups instead (33 requests of up to 2047, 16 heads of 32, 11.9 -> 11.1 us on pages of 16, and 14.4 -> 11.4 of 7), and
+    // with heads of 128 on odd pages both the addresses and two steps do not fit (1 % slower).
     static constexpr bool AHEAD = D == 64 || (D == 128 && UNI);
     static constexpr int OP = D + 4;            // pitch of a row of partial O in LDS
     static constexpr uint32_t NW = NC_PAGED_WAVES, THREADS = 64 * NW;

@@ -57,9 +57,9 @@ struct nc_paged_append_args {
 // four waves take the same keys for 16 heads each (wave_shift 1 or 2), and past 64 the workgroup's heads count
 // as another head. Neighbouring heads (the _next kernels) are shared out in the same way: 1 << wave_shift of them count
 // as one, a wave each. Those kernels have the code of both ways and take neighbouring heads where a request is longer than
-// NC_PAGED_NEXT_TOKENS: the lengths decide it, not the table's width. (In a table of 4096 tokens' pages, neighbouring heads
-// and not: 2 requests of 200 over 8 heads of 32 6.4 and 4.7 us, 4 of 300 over 8 of 16 6.8 and 5.6; 8 of 400 over 8 of 128 9.4
-// and 9.5.)
+// NC_PAGED_NEXT_TOKENS: the lengths decide it, not the table's width. In a table of 4096 tokens' pages, neighbouring heads and
+// each for itself: 2 requests of 200 over 8 heads of 32 6.4 and 4.7 us, 4 of 300 over 8 of 16 6.8 and 5.5; 8 of 400 over 8 of
+// 128 9.4 and 9.5.
 #define NC_PAGED_WAVES 4u
 #define NC_PAGED_NEXT_TOKENS 512u
 NC_HD uint32_t nc_paged_step_keys(uint32_t head_dim) { return head_dim <= 32 ? 64u : 32u; }
@@ -68,15 +68,17 @@ NC_HD uint32_t nc_paged_head_parts(uint32_t group) { return (group + 63u) / 64u;
 
 // Shares are counted in units: one per block, and before a head's first block so many for what a head costs however
 // short it is. Workgroup i takes units [i * each, (i + 1) * each), where `each` is the least that 2^most_log2
-// workgroups can do with, and no less than `least`. (One unit a head instead of two: 33 requests of up to 2047, 16 heads of
-// 32, 11.3 -> 10.7 us, but 16 of 1000 over 8 heads of 128 16.7 -> 17.1 and 64 ragged ones over 4 of 64 29.6 -> 30.1; two only
-// for heads of two blocks or fewer: the first 15.9, the last 33.)
+// workgroups can do with, and no less than `least`. With one unit a head and with two:
+//   33 requests of up to 2047, 16 heads of 32   11.1  11.8 us
+//   118 of up to 2719, 3 heads of 32            10.8  11.8
+//   16 of 1000, 8 heads of 128                  17.2  16.5
+//   64 of up to 16000, 4 heads of 64            29.6  28.6
 NC_HD uint32_t nc_paged_head_units(uint32_t head_dim) { return head_dim <= 32 ? 1u : 2u; }
 // A head of no more blocks than this is not split: the workgroup that has its first unit takes all of it. (Of 1: 118
-// requests of up to 2719, 3 heads of 32, 11.5 -> 12.0 us; of 4: 12.3, and 4 of 500 over 8 heads of 128 7.6 -> 9.5.)
+// requests of up to 2719, 3 heads of 32, 10.8 -> 11.1 us; of 4: 12.0, and 4 of 500 over 8 heads of 128 7.6 -> 9.4.)
 #define NC_PAGED_WHOLE_BLOCKS 2u
-// Heads of this many units on the average are long ones. (From 14 on: 16 requests of 1000 over 8 heads of 128 16.5 -> 17.3 us,
-// 200 ragged ones of up to 8000 141 -> 148; from 5 on: no change.)
+// Heads of this many units on the average are long ones. (From 14 on: 16 requests of 1000 over 8 heads of 128 16.5 -> 17.2 us,
+// 200 ragged ones of up to 8000 137 -> 145; from 5 on: no change.)
 #define NC_PAGED_LONG_UNITS 8u
 NC_HD uint32_t nc_paged_each(uint32_t units, uint32_t most_log2, uint32_t least) {
     const uint32_t each = (units + (1u << most_log2) - 1u) >> most_log2;
@@ -84,15 +86,15 @@ NC_HD uint32_t nc_paged_each(uint32_t units, uint32_t most_log2, uint32_t least)
 }
 
 // Pieces that one workgroup adds up in a round, by their size: of up to 16 KB reading 16 of them takes about as long as
-// another round (4: 63 pieces of 1 KB 8.7 -> 10.6 us), of more only 4. All in one round, one request of 100000 tokens, 8
-// query heads on one key head of 128, took 36 us, in rounds 20.5; with 64 query heads 194 and 58. At most NC_PAGED_MAX_WGS pieces are one after NC_PAGED_ROUNDS rounds, and
-// NC_PAGED_MERGE_ROWS holds the rows of all that one adds up.
+// another round (4: 63 pieces of 1 KB 8.7 -> 10.6 us), of more only 4. A CU reads pieces at a few ten GB/s, so that many or
+// large ones have to go to several: one request of 100000 tokens takes 20.5 us with 8 query heads on one key head of 128, and
+// 58 with 64. At most NC_PAGED_MAX_WGS pieces are one after NC_PAGED_ROUNDS rounds, and NC_PAGED_MERGE_ROWS holds the rows of
+// all that one adds up.
 #define NC_PAGED_MAX_WGS 1024u
 #define NC_PAGED_ROUNDS 5u
 #define NC_PAGED_MERGE_ROWS 1024u
 // Pieces of few numbers leave threads over, which take every so many-th one: up to 64 at once while all are within 32 KB.
-// A request of 120001 tokens over 8 heads of 64, 32 pieces of 1 KB a head: 59.6 -> 58.9 us; 21 pieces of 512 bytes: 9.4 -> 8.0; but
-// 63 pieces of 1 KB 8.7 -> 9.6.
+// 21 pieces of 512 bytes 9.4 -> 8.1 us, 32 of 1 KB no change; but 63 of 1 KB, which pass that, 8.7 -> 9.6.
 #define NC_PAGED_MERGE_PIECES 64u
 NC_HD bool nc_paged_one_round(uint32_t pieces, uint32_t numbers) {
     return pieces <= NC_PAGED_MERGE_PIECES && pieces * numbers <= 8192u;
