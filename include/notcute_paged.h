@@ -151,7 +151,8 @@ uint64_t nc_paged_workspace_bytes(const nc_paged_options *opts);
  * 2^-70 (bf16) of the largest one, and below that off by at most 2^-51 or 2^-93 of the largest one. In bf16, what is
  * below 2^-94, of V or of a weight (over the largest one) times V, may count as 0. A request of length 0, one whose pages
  * are all absent and one whose scores are all -infinity get zeros. A NaN among the keys that count gives NaN, and so does a
- * score of +infinity or an infinite V among them; what lies elsewhere in the pools may be anything. Q at any element
+ * score of +infinity. An infinite V among them gives that infinity, and NaN together with the other one or where its weight
+ * is below 2^-39 (f16) or 2^-93 (bf16) of the largest one. What lies elsewhere in the pools may be anything. Q at any element
  * alignment, O at any
  * float; caches and workspace 16-byte aligned. O and the workspace overlap nothing else
  * (NC_ERROR_INVALID_VALUE). Rows of O behind the last request are not touched. How the keys are split over

@@ -633,7 +633,7 @@ struct Decode {
         constexpr int G = E < 2 ? E : 2;  // products of so many dims in turn: each waits for its last one
 #pragma unroll
         for (int i0 = 0; i0 < E; i0 += G) {
-            floatx4 low[G];  // the f16 low parts' product, in units of its own
+            floatx4 low[G];  // the lower parts' products
 #pragma unroll
             for (int i = 0; i < G; ++i) low[i] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -651,16 +651,17 @@ struct Decode {
                 for (int n = 0; n < PARTS; ++n)
 #pragma unroll
                     for (int i = 0; i < G; ++i) {
-                        floatx4 &sum = !BF && n ? low[i] : acc[i0 + i];
+                        floatx4 &sum = n ? low[i] : acc[i0 + i];
                         sum = mfma_k32<BF>(x[i], p[u][n], sum);
                     }
             }
-            if constexpr (!BF) {
+            // An infinite V times a lower part, which may be 0 or negative, must not undo what its high part gave: no such
+            // sum of finite V comes near 2^100.
 #pragma unroll
-                for (int i = 0; i < G; ++i)
+            for (int i = 0; i < G; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i0 + i][j] = __builtin_fmaf(low[i][j], 1.f / kLowUnit, acc[i0 + i][j]);
-            }
+                for (int j = 0; j < 4; ++j)
+                    acc[i0 + i][j] = __builtin_fmaf(__builtin_amdgcn_fmed3f(low[i][j], -0x1p100f, 0x1p100f), BF ? 1.f : 1.f / kLowUnit, acc[i0 + i][j]);
         }
     }
 

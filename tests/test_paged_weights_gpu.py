@@ -104,3 +104,21 @@ def test_small_weights_where_the_largest_counts_for_nothing(gpu, d, ps, least, m
     bound = units * 2.0 ** -24 * (w * np.abs(values)).sum(1) + {"f16": 2.0 ** -51, "bf16": 2.0 ** -93}[dtype] * np.abs(values).sum(1)
     off = (np.abs(out - want[:, None]).max(1) / bound).max()
     assert off <= 1.0, f"off by {off:.2f} bounds"
+
+
+@pytest.mark.parametrize("n", [1, 40, 700, 20000])
+@pytest.mark.parametrize("d,ps,dtype", [(16, 16, "f16"), (64, 16, "bf16"), (64, 7, "f16"), (128, 16, "f16")])
+def test_scores_and_values_of_infinity_are_not_hidden(gpu, n, d, ps, dtype):
+    """A score of +infinity among the keys that count gives NaN, and an infinite V that infinity: at the first key, the last
+    and one between, whichever wave and piece has it."""
+    rng = np.random.default_rng(n + d)
+    at = sorted({0, n // 3, n - 1})
+    keys, values = np.zeros((2 * len(at) + 1, n, 3)), np.ones((2 * len(at) + 1, n))
+    keys[:, :, 1] = -rng.integers(0, 256, (2 * len(at) + 1, n))
+    for i, j in enumerate(at):
+        keys[2 * i, j, 0] = np.inf
+        values[2 * i + 1, j] = -np.inf
+    out = attend(gpu, rng, keys, values, d, ps, dtype)
+    assert np.all(np.isnan(out[:-1:2]))
+    assert np.all(out[1:-1:2] == -np.inf)
+    assert np.all(np.abs(out[-1] - 1.0) <= (n + 40) * 2.0 ** -23)
