@@ -153,8 +153,7 @@ uint64_t nc_paged_workspace_bytes(const nc_paged_options *opts);
  * are all absent and one whose scores are all -infinity get zeros. A NaN among the keys that count gives NaN, and so does a
  * score of +infinity. An infinite V among them gives that infinity, and NaN together with the other one or where its weight
  * is below 2^-39 (f16) or 2^-93 (bf16) of the largest one. What lies elsewhere in the pools may be anything. Q at any element
- * alignment, O at any
- * float; caches and workspace 16-byte aligned. O and the workspace overlap nothing else
+ * alignment, O at any float; caches and workspace 16-byte aligned. O and the workspace overlap nothing else
  * (NC_ERROR_INVALID_VALUE). Rows of O behind the last request are not touched. How the keys are split over
  * workgroups follows the lengths of all requests, so a request's rounding may differ with its neighbours;
  * equal calls give equal bits. */
