@@ -28,12 +28,12 @@ struct nc_function_st {
 
 struct nc_module_st {
     hipModule_t mod = nullptr;
-    // The embedded module's second code object (the paged cache's kernels), loaded onto the module's device when the first of
-    // them is asked for: it takes 1.2-1.4 ms, which a program without a cache need not wait for (the module's own 3.1-4.9).
-    // Guarded by `lock`; device is -1 in a module from other data, which has none.
-    hipModule_t paged = nullptr;
+    // The embedded module's second and third code objects (the paged cache's kernels and the smaller cache's), each loaded onto
+    // the module's device when the first of its kernels is asked for: it takes 1.2-1.4 ms, which a program without a cache need
+    // not wait for (the module's own 3.1-4.9). Guarded by `lock`; device is -1 in a module from other data, which has none.
+    hipModule_t paged = nullptr, paged4 = nullptr;
     int device = -1;
-    std::atomic<nc_function> paged_functions[NC_PAGED_KERNELS] = {};  // its functions, once looked up
+    std::atomic<nc_function> paged_functions[NC_PAGED_KERNELS + NC_PAGED4_KERNELS] = {};  // their functions, once looked up
     // Guards `functions`: several host threads may launch through one module (hipModuleGetFunction,
     // the lookup the cache saves, is itself thread-safe). Entries are never removed before unload,
     // so a returned nc_function stays valid without the lock.
@@ -52,6 +52,7 @@ struct nc_module_st {
 extern "C" const unsigned char nc_embedded_code_object[];
 extern "C" const unsigned char nc_embedded_code_object_end[];
 extern "C" const unsigned char nc_embedded_paged_object[];
+extern "C" const unsigned char nc_embedded_paged4_object[];
 
 namespace {
 
@@ -236,7 +237,7 @@ int nc_module_load_embedded(nc_module *out) {
 
 // The paged cache's code object, with the module's lock held. Its first launch may be one that a stream records into a
 // graph: loading belongs to no stream, which the relaxed mode says.
-static int load_paged(nc_module module) {
+static int load_paged(nc_module module, const unsigned char *object, hipModule_t *out) {
     int current = 0;
     int st = check(hipGetDevice(&current), "hipGetDevice");
     if (!st && current != module->device) st = check(hipSetDevice(module->device), "hipSetDevice");
@@ -245,8 +246,8 @@ static int load_paged(nc_module module) {
     st = check(hipThreadExchangeStreamCaptureMode(&mode), "hipThreadExchangeStreamCaptureMode");
     if (!st) {
         hipModule_t m = nullptr;
-        st = check(hipModuleLoadData(&m, nc_embedded_paged_object), "hipModuleLoadData");
-        if (!st) module->paged = m;
+        st = check(hipModuleLoadData(&m, object), "hipModuleLoadData");
+        if (!st) *out = m;
         (void)hipThreadExchangeStreamCaptureMode(&mode);
     }
     if (current != module->device) (void)hipSetDevice(current);
@@ -261,10 +262,11 @@ int nc_module_unload(nc_module module) {
         const int s2 = check(hipFree(p), "hipFree(retired workspace)");
         if (!st) st = s2;
     }
-    if (module->paged) {
-        const int s2 = check(hipModuleUnload(module->paged), "hipModuleUnload");
-        if (!st) st = s2;
-    }
+    for (hipModule_t m : {module->paged, module->paged4})
+        if (m) {
+            const int s2 = check(hipModuleUnload(m), "hipModuleUnload");
+            if (!st) st = s2;
+        }
     int st2 = check(hipModuleUnload(module->mod), "hipModuleUnload");
     delete module;
     return st ? st : st2;
@@ -323,10 +325,13 @@ int nc_module_get_function(nc_function *out, nc_module module, const char *name)
         return NC_SUCCESS;
     }
     const bool paged = module->device >= 0 && std::strncmp(name, "nc_paged_", 9) == 0;
-    int st = paged && !module->paged ? load_paged(module) : NC_SUCCESS;
+    const bool paged4 = module->device >= 0 && std::strncmp(name, "nc_paged4_", 10) == 0;
+    int st = NC_SUCCESS;
+    if (paged && !module->paged) st = load_paged(module, nc_embedded_paged_object, &module->paged);
+    if (paged4 && !module->paged4) st = load_paged(module, nc_embedded_paged4_object, &module->paged4);
     if (st) return st;
     hipFunction_t f = nullptr;
-    st = check(hipModuleGetFunction(&f, paged ? module->paged : module->mod, name), "hipModuleGetFunction");
+    st = check(hipModuleGetFunction(&f, paged ? module->paged : paged4 ? module->paged4 : module->mod, name), "hipModuleGetFunction");
     if (st) return st;
     auto fn = std::make_unique<nc_function_st>();
     fn->fn = f;
@@ -336,9 +341,9 @@ int nc_module_get_function(nc_function *out, nc_module module, const char *name)
     return NC_SUCCESS;
 }
 
-// A function kept under `slot`, so that a launch neither takes the lock nor hashes the name. For paged.cpp.
+// A function kept under `slot`, so that a launch neither takes the lock nor hashes the name. For paged.cpp and paged4.cpp.
 extern "C" int nc_internal_module_kept_function(nc_module module, uint32_t slot, const char *name, nc_function *out) {
-    if (!module || slot >= NC_PAGED_KERNELS) return fail(NC_ERROR_INVALID_VALUE, "function: invalid argument");
+    if (!module || slot >= NC_PAGED_KERNELS + NC_PAGED4_KERNELS) return fail(NC_ERROR_INVALID_VALUE, "function: invalid argument");
     *out = module->paged_functions[slot].load(std::memory_order_acquire);
     if (*out) return NC_SUCCESS;
     int st;

@@ -1,4 +1,4 @@
-// hw_probe.hip — single-wave probes of the gfx950 instruction semantics flash_fwd.hip is built on.
+// hw_probe.hip — single-wave probes of the gfx950 instruction semantics flash_fwd.hip and paged4.hip are built on.
 //
 // Not part of the flash path: the GPU tests load this code object and compare each probe's output
 // with the layout the kernels assume, so a change of hardware or compiler behaviour shows up as a
@@ -8,6 +8,8 @@
 //   nc_probe_mfma32x32x16   v_mfma_f32_32x32x16_{f16,bf16}: operand and accumulator lane layout
 //   nc_probe_ds_read_tr     ds_read_b64_tr_b16: which LDS elements each lane of a 16-lane group gets
 //   nc_probe_permlane32     v_permlane32_swap: the lane-pair exchange used for row max / row sum
+//   nc_probe_mfma_fp4_fp8   v_mfma_scale_f32_16x16x128_f8f6f4, 4-bit rows times 8-bit columns: lane layout and scales
+//   nc_probe_fp4_convert, nc_probe_fp8_convert   rounding of the conversions to and from 4 and 8 bits
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -73,4 +75,61 @@ extern "C" __global__ __launch_bounds__(64) void nc_probe_permlane32(uint32_t *o
     auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
     out[threadIdx.x * 2] = r[0];
     out[threadIdx.x * 2 + 1] = r[1];
+}
+
+namespace {
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+}  // namespace
+
+// v_mfma_scale_f32_16x16x128_f8f6f4 with A in 4 bits (e2m1) and B in 8 (e4m3), as the 4-bit cache's attention uses it.
+// a: 16 rows of 64 bytes (two values a byte, the first in the low half), as_: 16 x 4 scale bytes 2^(byte - 127) of 32
+// values each; b: 16 columns of 128 bytes, bs: 16 x 4. Of g = l / 16, lane l supplies values 32 g..+31 of row l % 16 of A, but
+// values 16 g..+15 and 64 + 16 g..+15 of column l % 16 of B; its scales are those of values 32 g..+31 of both. It stores its 4
+// accumulator registers.
+extern "C" __global__ __launch_bounds__(64) void nc_probe_mfma_fp4_fp8(const uint8_t *a, const uint8_t *as_, const uint8_t *b,
+                                                                        const uint8_t *bs, float *d) {
+    const int l = threadIdx.x, c = l % 16, g = l / 16;
+    const i32x4 x = *reinterpret_cast<const i32x4 *>(a + c * 64 + 16 * g);
+    const i32x4 y0 = *reinterpret_cast<const i32x4 *>(b + c * 128 + 16 * g);
+    const i32x4 y1 = *reinterpret_cast<const i32x4 *>(b + c * 128 + 64 + 16 * g);
+    const i32x8 y = {y0[0], y0[1], y0[2], y0[3], y1[0], y1[1], y1[2], y1[3]};
+    const i32x8 w = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+    floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, y, acc, 4, 0, 0, as_[c * 4 + g], 0, bs[c * 4 + g]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) d[l * 4 + r] = acc[r];
+}
+
+// The conversions of the 4-bit cache, a word a lane of `n`: words of 8 codes times a scale (f32, a power of two) to 8
+// bf16, and of 8 f32 over the scale to a word of codes.
+extern "C" __global__ __launch_bounds__(64) void nc_probe_fp4_convert(const uint32_t *codes, const float *scales, uint32_t *to_bf16,
+                                                                       const float *x, uint32_t *to_codes, uint32_t n) {
+    for (uint32_t i = threadIdx.x; i < n; i += 64) {
+        const uint32_t w = codes[i];
+        const float s = scales[i];
+        to_bf16[4 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
+        to_bf16[4 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
+        to_bf16[4 * i + 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
+        to_bf16[4 * i + 3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
+        const float *y = x + 8 * i;
+        uint32_t q = 0;
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[0], y[1], s, 0);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[2], y[3], s, 1);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[4], y[5], s, 2);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[6], y[7], s, 3);
+        to_codes[i] = q;
+    }
+}
+
+// Pairs of f32 to e4m3 bytes and back: out[3 i] the bytes (in the low half), out[3 i + 1..2] their values.
+extern "C" __global__ __launch_bounds__(64) void nc_probe_fp8_convert(const float *x, uint32_t *out, uint32_t n) {
+    for (uint32_t i = threadIdx.x; i < n; i += 64) {
+        const int q = __builtin_amdgcn_cvt_pk_fp8_f32(x[2 * i], x[2 * i + 1], 0, false);
+        const auto y = __builtin_amdgcn_cvt_pk_f32_fp8(q, false);
+        out[3 * i] = (uint32_t)q;
+        out[3 * i + 1] = __builtin_bit_cast(uint32_t, (float)y[0]);
+        out[3 * i + 2] = __builtin_bit_cast(uint32_t, (float)y[1]);
+    }
 }

@@ -1,0 +1,457 @@
+// paged4.hip — kernels of a smaller paged cache for MI355X (gfx950, wave64): rows into pages of 4 bits and back
+// (nc_paged4_append, nc_paged4_read), single-token attention over them (nc_paged4_decode_*), attention that keeps its scores
+// (nc_paged4_mass_*) and the weights by token out of those (nc_paged4_weights), and eviction by them (nc_paged4_select,
+// nc_paged4_move). The interface is described in include/notcute_paged4.h.
+
+#include "paged_decode.h"
+
+#include "paged4_args.h"
+
+// -------------------------------------------------------------------------------------------------
+// Rows into 4-bit pages: of every 32 values x of a row the scale 2^k, k the least with max |x| <= 7 2^k (then the largest is at
+// most half a step off), and x 2^-k to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign, halves to the even code. Both are
+// exact arithmetic: the sum that finds k is one of integers, the product by a power of two. A thread takes 8 values of K and of V,
+// four neighbouring lanes a group.
+// -------------------------------------------------------------------------------------------------
+namespace {
+
+__device__ __forceinline__ u32x4 load_eight(const uint16_t *p) {
+    u32x4 r;
+    __builtin_memcpy(&r, p, 16);  // one load: global memory takes them at any alignment
+    return r;
+}
+
+// The largest over each 4 neighbouring lanes.
+__device__ __forceinline__ uint32_t near_max(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, x, 0xb1, 0xf, 0xf, false));  // quad_perm 1,0,3,2 and 2,3,0,1
+    return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, x, 0x4e, 0xf, 0xf, false));
+}
+
+// The lane's 8 codes, and its group's scale byte.
+__device__ __forceinline__ uint32_t quantise(u32x4 w, bool bf, uint32_t &byte) {
+    float x[8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t u = w[i];  // a bit cast of a vector's element reads its first one
+        const half2v h = __builtin_bit_cast(half2v, u);
+        x[2 * i] = bf ? __uint_as_float(u << 16) : (float)h[0];
+        x[2 * i + 1] = bf ? __uint_as_float(u & 0xffff0000u) : (float)h[1];
+        top = max(top, max(__float_as_uint(x[2 * i]) & 0x7fffffffu, __float_as_uint(x[2 * i + 1]) & 0x7fffffffu));
+    }
+    top = near_max(top);
+    const bool fine = top < 0x7f800000u;
+    // 7 = 1.75 * 4: one more where the fraction is above 0.75
+    const int e = (int)((top + 0x1fffffu) >> 23) - 2;
+    const int b = min(max(e, bf ? NC_PAGED4_LEAST_BF16 : NC_PAGED4_LEAST_F16), bf ? NC_PAGED4_MOST_BF16 : NC_PAGED4_MOST_F16);
+    byte = fine ? (uint32_t)b : 255u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __builtin_ldexpf(x[i], 127 - b);
+    uint32_t q = 0;
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, x[0], x[1], 1.f, 0);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, x[2], x[3], 1.f, 1);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, x[4], x[5], 1.f, 2);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, x[6], x[7], 1.f, 3);
+    return fine ? q : 0u;
+}
+
+// The value of 8 codes in the rows' type.
+__device__ __forceinline__ u32x4 values(uint32_t q, uint32_t byte, bool bf) {
+    const float s = __uint_as_float(byte << 23);
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t b = pair_of_fours(q, s, i);
+        const half2v h = {(_Float16)__uint_as_float(b << 16), (_Float16)__uint_as_float(b & 0xffff0000u)};
+        r[i] = bf ? b : __builtin_bit_cast(uint32_t, h);
+    }
+    return r;
+}
+
+// Where a unit of 8 values of a row is: of the rows, and of the cache.
+struct Place {
+    uint64_t row, cache;
+    bool in;
+};
+__device__ __forceinline__ Place place_of(const nc_paged4_rows_args &a, uint64_t row0, uint32_t u) {
+    const uint32_t i = nc_paged_quot(u, a.chunks), c = u - i * a.chunks.d;
+    const uint32_t h = c >> a.chunk_shift, x = c & ((1u << a.chunk_shift) - 1u);
+    const uint32_t slot = (uint32_t)a.slots[row0 + i];
+    Place p;
+    p.in = slot < a.num_slots;
+    const uint32_t page = nc_paged_quot(p.in ? slot : 0u, a.ps), t = (p.in ? slot : 0u) - page * a.ps.d;
+    p.row = (row0 + i) * a.row_stride + h * a.row_head_stride + 8 * x;
+    p.cache = page * a.page_stride + h * a.head_stride + t * a.token_stride + 8 * x;
+    return p;
+}
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(256) void nc_paged4_append(const nc_paged4_rows_args a) {
+    const uint64_t row0 = (uint64_t)blockIdx.x * a.wg_rows;
+    const uint32_t rows = (uint32_t)min((uint64_t)a.wg_rows, a.num_rows - row0), total = rows * a.chunks.d;
+    for (uint32_t u = threadIdx.x; u < total; u += blockDim.x) {
+        const Place p = place_of(a, row0, u);
+        if (!p.in) continue;  // all four lanes of a group
+        const u32x4 kw = load_eight(a.k_in + p.row), vw = load_eight(a.v_in + p.row);
+        uint32_t kb, vb;
+        const uint32_t kq = quantise(kw, a.bf, kb), vq = quantise(vw, a.bf, vb);
+        *reinterpret_cast<uint32_t *>(a.k + p.cache / 2) = kq;
+        *reinterpret_cast<uint32_t *>(a.v + p.cache / 2) = vq;
+        if (u % 4 == 0) {
+            a.k_scales[p.cache / 32] = (uint8_t)kb;
+            a.v_scales[p.cache / 32] = (uint8_t)vb;
+        }
+    }
+}
+
+extern "C" __global__ __launch_bounds__(256) void nc_paged4_read(const nc_paged4_rows_args a) {
+    const uint64_t row0 = (uint64_t)blockIdx.x * a.wg_rows;
+    const uint32_t rows = (uint32_t)min((uint64_t)a.wg_rows, a.num_rows - row0), total = rows * a.chunks.d;
+    for (uint32_t u = threadIdx.x; u < total; u += blockDim.x) {
+        const Place p = place_of(a, row0, u);
+        u32x4 k = {0u, 0u, 0u, 0u}, v = k;
+        if (p.in) {
+            const uint32_t kq = *reinterpret_cast<const uint32_t *>(a.k + p.cache / 2), vq = *reinterpret_cast<const uint32_t *>(a.v + p.cache / 2);
+            k = values(kq, a.k_scales[p.cache / 32], a.bf);
+            v = values(vq, a.v_scales[p.cache / 32], a.bf);
+        }
+        __builtin_memcpy(a.k_out + p.row, &k, 16);
+        __builtin_memcpy(a.v_out + p.row, &v, 16);
+    }
+}
+
+// -------------------------------------------------------------------------------------------------
+// Weights by token: mass[r][j] += sum over the query heads of exp2(score - max) / sum, out of the scores that an attention has
+// kept. Four tokens a lane, every fourth head a wave; the waves' sums are added in their order.
+// -------------------------------------------------------------------------------------------------
+extern "C" __global__ __launch_bounds__(256) void nc_paged4_weights(const nc_paged_mass_args a) {
+    __shared__ float s_sum[4][256];
+    const uint32_t lane = threadIdx.x & 63u, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (uint32_t r = blockIdx.y; r < a.num_seqs; r += gridDim.y) {
+        const uint32_t len = nc_paged_cut(as_const(a.seq_lens)[r], a.max_tokens);
+        for (uint32_t t0 = blockIdx.x * 256u; t0 < len; t0 += gridDim.x * 256u) {
+            const uint32_t t = t0 + 4 * lane;
+            floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+            if (t < len) {
+                const uint64_t row0 = (uint64_t)r * a.num_q_heads;
+#pragma unroll 4
+                for (uint32_t h = w; h < a.num_q_heads; h += 4) {
+                    const floatx4 s = *reinterpret_cast<const floatx4 *>(a.scores + (row0 + h) * a.score_pitch + t);
+                    const float top = a.row_ml[2 * (row0 + h)], inv = a.row_ml[2 * (row0 + h) + 1];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(s[i] - top) * inv;
+                }
+            }
+            *reinterpret_cast<floatx4 *>(&s_sum[w][4 * lane]) = sum;
+            __syncthreads();
+            const uint32_t j = t0 + threadIdx.x;
+            if (j < len) a.mass[r * a.mass_stride + j] += s_sum[0][threadIdx.x] + s_sum[1][threadIdx.x] + s_sum[2][threadIdx.x] + s_sum[3][threadIdx.x];
+            __syncthreads();
+        }
+    }
+}
+
+// -------------------------------------------------------------------------------------------------
+// Eviction. A workgroup a request finds the least mass that is kept by its bits, 11 at a time from the top (a histogram of the
+// masses that agree in the bits above, until all of a bin are kept), and then lists the tokens that stay, in their order. A
+// wave of it has a contiguous part of the tokens and keeps the first of them in registers.
+// -------------------------------------------------------------------------------------------------
+namespace {
+
+constexpr uint32_t kSelectWaves = 16, kSelectHeld = 8;  // waves of a selection, tokens that a lane of it keeps
+
+// Masses in ascending order as numbers: both zeros are one, a NaN is the largest.
+__device__ __forceinline__ uint32_t order_of(float x) {
+    const uint32_t u = __float_as_uint(x);
+    if (x != x) return 0xffffffffu;
+    if (x == 0.f) return 0x80000000u;
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ uint32_t pages_of(uint32_t tokens, nc_paged_div ps) {
+    const uint32_t n = nc_paged_quot(tokens, ps);
+    return n + (n * ps.d != tokens);
+}
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(64 * kSelectWaves) void nc_paged4_select(const nc_paged_evict_args a) {
+    __shared__ uint32_t s_bins[2048];
+    __shared__ uint32_t s_a[kSelectWaves], s_b[kSelectWaves], s_c[kSelectWaves], s_d[kSelectWaves];
+    __shared__ uint32_t s_bin, s_above, s_count, s_first;
+    const uint32_t r = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t n = nc_paged_cut(as_const(a.seq_lens)[r], a.max_tokens);
+    const bool cut = n > a.limit;
+    const uint32_t keep = cut ? a.budget : n;
+    if (tid == 0) {
+        a.news[r] = (int32_t)keep;
+        a.olds[r] = (int32_t)n;
+        if (!cut) a.first[r] = (int32_t)n;
+        s_first = n;
+    }
+    if (!cut && r != 0) return;
+
+    // Pages that become free: of all requests, and of those before this one.
+    uint32_t all = 0, before = 0, cuts = 0, dropped = 0;
+    for (uint32_t q = tid; q < a.num_seqs; q += blockDim.x) {
+        const uint32_t m = nc_paged_cut(a.seq_lens[q], a.max_tokens);
+        if (m > a.limit) {
+            const uint32_t f = pages_of(m, a.ps) - pages_of(a.budget, a.ps);
+            all += f;
+            before += q < r ? f : 0u;
+            cuts += 1u;
+            dropped += m - a.budget;
+        }
+    }
+    all = wave_scan32(all);
+    before = wave_scan32(before);
+    cuts = wave_scan32(cuts);
+    dropped = wave_scan32(dropped);
+    if (lane == 63) {
+        s_a[w] = all;
+        s_b[w] = before;
+        s_c[w] = cuts;
+        s_d[w] = dropped;
+    }
+    __syncthreads();
+    all = before = cuts = dropped = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kSelectWaves; ++i) {
+        all += s_a[i];
+        before += s_b[i];
+        cuts += s_c[i];
+        dropped += s_d[i];
+    }
+    const int64_t base = (int64_t)a.cursor[0] - all;
+    if (r == 0 && tid == 0) {
+        a.totals[0] = (int32_t)max(base, (int64_t)0);
+        a.totals[1] = (int32_t)cuts;
+        a.totals[2] = (int32_t)all;
+        a.totals[3] = (int32_t)dropped;
+    }
+    if (!cut) return;
+    const int32_t *row = a.table + r * a.table_stride;
+    const uint32_t held = pages_of(n, a.ps), stay = pages_of(keep, a.ps);
+    for (uint32_t p = stay + tid; p < held; p += blockDim.x) {
+        const int64_t at = base + before + (p - stay);
+        if (at >= 0 && at < (int64_t)a.free_len) a.free_pages[at] = row[p];
+    }
+
+    // The wave's tokens, and their order.
+    const float *mass = a.mass + r * a.mass_stride;
+    const uint32_t lo = a.sinks, hi = n - a.recent, need = a.budget - a.sinks - a.recent;
+    const uint32_t part = (n + 64u * kSelectWaves - 1u) / (64u * kSelectWaves) * 64u, begin = min(w * part, n), end = min(begin + part, n);
+    uint32_t key[kSelectHeld];
+#pragma unroll
+    for (uint32_t i = 0; i < kSelectHeld; ++i) {
+        const uint32_t t = begin + 64u * i + lane;
+        key[i] = t < end ? order_of(mass[t]) : 0u;
+    }
+    // fn(place, order, whether there is one) for all of the wave's tokens, 64 neighbours at a time
+    auto each = [&](auto &&fn) {
+#pragma unroll
+        for (uint32_t i = 0; i < kSelectHeld; ++i)
+            if (begin + 64u * i < end) fn(begin + 64u * i + lane, key[i], begin + 64u * i + lane < end);
+        for (uint32_t t = begin + 64u * kSelectHeld; t < end; t += 64u) {
+            const bool in = t + lane < end;
+            fn(t + lane, in ? order_of(mass[t + lane]) : 0u, in);
+        }
+    };
+    // All orders from `least` on are kept, and the first `ties` tokens of order `least - 1`.
+    uint64_t least = 1ull << 32;
+    uint32_t ties = 0;
+    if (need) {
+        uint32_t prefix = 0, left = need;  // the bits above the present ones, kept tokens that agree in them
+        for (int shift = 21, bits = 11;;) {
+            for (uint32_t i = tid; i < 2048; i += blockDim.x) s_bins[i] = 0;
+            __syncthreads();
+            each([&](uint32_t t, uint32_t k, bool in) {
+                const bool mine = in && t >= lo && t < hi && (uint64_t)k >> (shift + bits) == prefix;
+                const uint32_t bin = k >> shift & ((1u << bits) - 1u);
+                // equal masses are common (zeros): the first lane counts for all that share its bin
+                const uint64_t who = __ballot(mine);
+                if (!who) return;
+                const uint32_t one = __builtin_amdgcn_readlane(bin, __builtin_ctzll(who));
+                const uint64_t same = __ballot(mine && bin == one);
+                if (mine && bin != one) atomicAdd(&s_bins[bin], 1u);
+                if (lane == (uint32_t)__builtin_ctzll(same)) atomicAdd(&s_bins[one], (uint32_t)__builtin_popcountll(same));
+            });
+            __syncthreads();
+            // Bins from the top, two a thread; the one that the last token to be kept is in.
+            const uint32_t x = s_bins[2047u - 2u * tid], y = s_bins[2046u - 2u * tid];
+            const uint32_t incl = wave_scan32(x + y);
+            if (lane == 63) s_a[w] = incl;
+            __syncthreads();
+            uint32_t above = incl - x - y;
+            for (uint32_t i = 0; i < w; ++i) above += s_a[i];
+            if (above < left && left <= above + x + y) {
+                const bool first = left <= above + x;
+                s_bin = first ? 2047u - 2u * tid : 2046u - 2u * tid;
+                s_above = first ? above : above + x;
+                s_count = first ? x : y;
+            }
+            __syncthreads();
+            prefix = prefix << bits | s_bin;
+            left -= s_above;
+            if (s_count == left || shift == 0) {
+                // the whole bin, or all its bits: then the first ones of it
+                least = (uint64_t)prefix << shift;
+                if (s_count != left) {
+                    least += 1;
+                    ties = left;
+                }
+                break;
+            }
+            bits = shift == 21 ? 11 : 10;
+            shift = shift == 21 ? 10 : 0;
+            __syncthreads();
+        }
+    }
+    // How many of the wave's tokens stay for sure, and how many are of the last order.
+    uint32_t sure = 0, last = 0;
+    each([&](uint32_t t, uint32_t k, bool in) {
+        const bool s = in && (t < lo || t >= hi || k >= least), l = in && !s && (uint64_t)k + 1 == least;
+        sure += __builtin_popcountll(__ballot(s));
+        last += __builtin_popcountll(__ballot(l));
+    });
+    __syncthreads();
+    if (lane == 0) {
+        s_a[w] = sure;
+        s_b[w] = last;
+    }
+    __syncthreads();
+    sure = last = 0;
+    for (uint32_t i = 0; i < w; ++i) {
+        sure += s_a[i];
+        last += s_b[i];
+    }
+    int32_t *source = a.source + (uint64_t)r * a.max_tokens;
+    float *kept = a.kept_mass + (uint64_t)r * a.max_tokens;
+    uint32_t gone = n;
+    each([&](uint32_t t, uint32_t k, bool in) {
+        const bool s = in && (t < lo || t >= hi || k >= least), l = in && !s && (uint64_t)k + 1 == least;
+        const uint64_t ws = __ballot(s), wl = __ballot(l), below = (1ull << lane) - 1ull;
+        const uint32_t ns = sure + __builtin_popcountll(ws & below), nl = last + __builtin_popcountll(wl & below);
+        if (s || (l && nl < ties)) {
+            const uint32_t to = ns + min(nl, ties);
+            const uint32_t at = nc_paged_quot(t, a.ps), page = (uint32_t)row[at];
+            source[to] = page < a.num_pages ? (int32_t)(page * a.ps.d + (t - at * a.ps.d)) : -1;
+            kept[to] = mass[t];
+        } else if (in) {
+            gone = min(gone, t);
+        }
+        sure += __builtin_popcountll(ws);
+        last += __builtin_popcountll(wl);
+    });
+    if (gone < n) atomicMin(&s_first, gone);
+    __syncthreads();
+    if (tid == 0) a.first[r] = (int32_t)s_first;
+}
+
+// The rows that stay, to the front. Every wave has a column of them, 16-byte units (four bits: 32 values and their scale) of one
+// head of K or V, and moves it row by row: no row's place is behind its source, the wave loads rows in ascending order, and stores
+// one when it and those before it have arrived. So no wave waits for another, and nothing is overwritten before it is read.
+namespace {
+
+template <bool FOUR>
+__device__ __forceinline__ void move_body(const nc_paged_evict_args &a, uint32_t r, uint32_t column, uint32_t keep, uint32_t first) {
+    constexpr uint32_t AT_ONCE = 8;
+    constexpr uint32_t UE = FOUR ? 32 : 8;  // values of a unit
+    const uint32_t lane = threadIdx.x & 63u, rows = 64u >> a.slice_log2;
+    const uint32_t slices = a.units >> a.slice_log2, slice = column % slices, head = column / slices >> 1, v = column / slices & 1u;
+    const uint64_t base = head * a.head_stride + UE * ((slice << a.slice_log2) + (lane & ((1u << a.slice_log2) - 1u)));
+    uint8_t *codes = v ? a.v : a.k, *scales = v ? a.v_scales : a.k_scales;
+    const int32_t *row = a.table + r * a.table_stride, *source = a.source + (uint64_t)r * a.max_tokens;
+    const uint32_t num_slots = a.num_pages * a.ps.d;
+    struct Batch {
+        u32x4 x[AT_ONCE];
+        uint32_t s[AT_ONCE];
+        uint64_t to[AT_ONCE];
+        bool in[AT_ONCE];
+    };
+    auto load = [&](Batch &b, uint32_t j0) {
+#pragma unroll
+        for (uint32_t i = 0; i < AT_ONCE; ++i) {
+            const uint32_t j = j0 + i * rows + (lane >> (a.slice_log2));
+            const uint32_t jj = min(j, keep - 1u);
+            const uint32_t slot = (uint32_t)source[jj], at = nc_paged_quot(jj, a.ps), page = (uint32_t)row[at];
+            b.in[i] = j < keep && slot < num_slots && page < a.num_pages;
+            const uint32_t from = b.in[i] ? slot : 0u, p = nc_paged_quot(from, a.ps);
+            const uint64_t src = p * a.page_stride + (from - p * a.ps.d) * a.token_stride + base;
+            b.to[i] = page * a.page_stride + (jj - at * a.ps.d) * a.token_stride + base;
+            b.x[i] = *reinterpret_cast<const u32x4 *>(codes + (FOUR ? src / 2 : src * 2));
+            if constexpr (FOUR) b.s[i] = scales[src / 32];
+        }
+    };
+    auto store = [&](const Batch &b) {
+#pragma unroll
+        for (uint32_t i = 0; i < AT_ONCE; ++i)
+            if (b.in[i]) {
+                *reinterpret_cast<u32x4 *>(codes + (FOUR ? b.to[i] / 2 : b.to[i] * 2)) = b.x[i];
+                if constexpr (FOUR) scales[b.to[i] / 32] = (uint8_t)b.s[i];
+            }
+    };
+    const uint32_t step = AT_ONCE * rows;
+    Batch x;
+    for (uint32_t j = first; j < keep; j += step) {
+        load(x, j);
+        // all of the batch's rows have arrived before the first is stored
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        store(x);
+    }
+}
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(256) void nc_paged4_move(const nc_paged_evict_args a) {
+    const uint32_t column = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (uint32_t r = blockIdx.y; r < a.num_seqs; r += gridDim.y) {
+        const uint32_t keep = (uint32_t)a.news[r], old = (uint32_t)a.olds[r], first = (uint32_t)a.first[r];
+        if (blockIdx.x == gridDim.x - 1u) {  // what else the selection left
+            if (threadIdx.x == 0) a.kept_lens[r] = (int32_t)keep;
+            if (r == 0 && threadIdx.x < 4) a.counts[threadIdx.x] = a.totals[threadIdx.x];
+            float *mass = a.mass + r * a.mass_stride;
+            const float *kept = a.kept_mass + (uint64_t)r * a.max_tokens;
+            if (keep < old)
+                for (uint32_t t = first + threadIdx.x; t < old; t += blockDim.x) mass[t] = t < keep ? kept[t] : 0.f;
+        } else if (column < a.waves && keep < old && first < keep) {
+            if (a.four)
+                move_body<true>(a, r, column, keep, first);
+            else
+                move_body<false>(a, r, column, keep, first);
+        }
+    }
+}
+
+// -------------------------------------------------------------------------------------------------
+// Attention: paged_decode.h.
+// -------------------------------------------------------------------------------------------------
+#define NC_DECODE4_KERNEL(NAME, D, BF, UNI, MANY, NEXT, FOUR, MASS)                                     \
+    extern "C" __global__ __launch_bounds__(64 * NC_PAGED_WAVES, 2) void NAME(const nc_paged_more_args) { \
+        decode_body<D, BF, UNI, MANY, NEXT, FOUR, MASS>();                                              \
+    }
+#define NC_DECODE4(D)                                                                        \
+    NC_DECODE4_KERNEL(nc_paged4_decode_d##D, D, true, true, false, false, true, false)            \
+    NC_DECODE4_KERNEL(nc_paged4_decode_d##D##_odd, D, true, false, false, false, true, false)      \
+    NC_DECODE4_KERNEL(nc_paged4_decode_d##D##_many, D, true, true, true, false, true, false)       \
+    NC_DECODE4_KERNEL(nc_paged4_decode_d##D##_many_odd, D, true, false, true, false, true, false)  \
+    NC_DECODE4_KERNEL(nc_paged4_decode_d##D##_next, D, true, true, true, true, true, false)        \
+    NC_DECODE4_KERNEL(nc_paged4_decode_d##D##_next_odd, D, true, false, true, true, true, false)   \
+    NC_DECODE4_KERNEL(nc_paged4_mass4_d##D, D, true, true, false, false, true, true)               \
+    NC_DECODE4_KERNEL(nc_paged4_mass4_d##D##_odd, D, true, false, false, false, true, true)
+NC_DECODE4(32)
+NC_DECODE4(64)
+NC_DECODE4(128)
+// Scores kept over caches in 16 bits.
+#define NC_MASS(D, T, BF)                                                                  \
+    NC_DECODE4_KERNEL(nc_paged4_mass_d##D##T, D, BF, true, false, false, false, true)           \
+    NC_DECODE4_KERNEL(nc_paged4_mass_d##D##_odd##T, D, BF, false, false, false, false, true)
+NC_MASS(16, , false)
+NC_MASS(32, , false)
+NC_MASS(64, , false)
+NC_MASS(128, , false)
+NC_MASS(16, _bf16, true)
+NC_MASS(32, _bf16, true)
+NC_MASS(64, _bf16, true)
+NC_MASS(128, _bf16, true)

@@ -26,7 +26,8 @@ NC_HD uint32_t nc_paged_quot(uint32_t n, nc_paged_div v) {
     return (uint32_t)(((uint64_t)(2u * n) * v.magic) >> 32) >> v.shift;
 }
 
-#define NC_PAGED_KERNELS 53u // kernels of paged.hip
+#define NC_PAGED_KERNELS 53u  // kernels of paged.hip
+#define NC_PAGED4_KERNELS 45u // and of paged4.hip
 
 struct nc_paged_build_args {
     const int32_t *cached, *fresh, *free_pages, *cursor;
@@ -73,7 +74,10 @@ NC_HD uint32_t nc_paged_head_parts(uint32_t group) { return (group + 63u) / 64u;
 //   118 of up to 2719, 3 heads of 32            10.8  11.8
 //   16 of 1000, 8 heads of 128                  17.2  16.5
 //   64 of up to 16000, 4 heads of 64            29.6  28.6
-NC_HD uint32_t nc_paged_head_units(uint32_t head_dim) { return head_dim <= 32 ? 1u : 2u; }
+NC_HD constexpr uint32_t nc_paged_head_units(uint32_t head_dim) { return head_dim <= 32 ? 1u : 2u; }
+// Caches in 4 bits.
+NC_HD constexpr uint32_t nc_paged4_head_units(uint32_t head_dim) { return head_dim <= 64 ? 1u : 2u; }
+#define NC_PAGED4_STEP_KEYS 64u
 // A head of no more blocks than this is not split: the workgroup that has its first unit takes all of it. (Of 1: 118
 // requests of up to 2719, 3 heads of 32, 10.8 -> 11.1 us; of 4: 12.0, and 4 of 500 over 8 heads of 128 7.6 -> 9.4.)
 #define NC_PAGED_WHOLE_BLOCKS 2u
@@ -121,6 +125,17 @@ struct nc_paged_decode_args {
     uint32_t q_vec, o_vec;                               // Q, O rows are 16-byte aligned
     float scale;
     nc_paged_div ps;
+};
+
+// Behind these, for caches in 4 bits (k and v are then bytes of two values, the strides still count values) and for kernels that
+// keep their scores.
+struct nc_paged_more_args {
+    nc_paged_decode_args a;
+    const uint8_t *k_scales, *v_scales; // a byte for every 32 values
+    float *scores;                      // a row of score_pitch per request and query head
+    float *row_ml;                      // and its (max, 1 / sum)
+    uint64_t score_pitch;
+    uint32_t bf;                        // Q is bf16
 };
 
 // The divisor d / 2^side where 2^side divides d: the same multiplier, as 2^(31+shift) / d is.

@@ -1,5 +1,5 @@
 """Python binding of the MI355X flash-attention C ABI (``include/notcute_flash.h``, and the paged
-key-value cache of ``include/notcute_paged.h``).
+key-value cache of ``include/notcute_paged.h`` and ``include/notcute_paged4.h``).
 
 This is a ctypes mirror of the reference's public ``flash`` / ``cuda`` / ``benchmark`` modules
 (src/flash.zig, src/cuda.zig, src/benchmark.zig) over ``libnotcute_flash.so``. It holds no compute:
@@ -196,6 +196,12 @@ class PagedOptions(ctypes.Structure):
         "o_stride", "o_head_stride")] + [("scale", ctypes.c_float), ("element_type", ctypes.c_uint32)]
 
 
+class EvictRules(ctypes.Structure):
+    """nc_paged_evict_rules (include/notcute_paged4.h)."""
+
+    _fields_ = [(name, ctypes.c_uint64) for name in ("limit", "budget", "sinks", "recent")]
+
+
 _P = ctypes.c_void_p
 _U64 = ctypes.c_uint64
 _SIGS = {
@@ -268,6 +274,16 @@ _SIGS = {
     "nc_paged_build": (ctypes.c_int, [_P, _P, _P, _P]),
     "nc_paged_append": (ctypes.c_int, [_P, _P, _P, _P]),
     "nc_paged_decode": (ctypes.c_int, [_P, _P, _P, _P]),
+    "nc_paged4_validate": (ctypes.c_int, [ctypes.POINTER(PagedOptions)]),
+    "nc_paged4_append": (ctypes.c_int, [_P, _P, _P, _P]),
+    "nc_paged4_read": (ctypes.c_int, [_P, _P, _P, _P]),
+    "nc_paged4_workspace_bytes": (_U64, [ctypes.POINTER(PagedOptions), ctypes.c_int]),
+    "nc_paged4_decode": (ctypes.c_int, [_P, _P, _P, _P, _P]),
+    "nc_paged_mass_workspace_bytes": (_U64, [ctypes.POINTER(PagedOptions)]),
+    "nc_paged_decode_mass": (ctypes.c_int, [_P, _P, _P, _P, _P]),
+    "nc_paged_evict_workspace_bytes": (_U64, [ctypes.POINTER(PagedOptions)]),
+    "nc_paged_evict": (ctypes.c_int, [_P, _P, _P, _P, _P]),
+    "nc_paged4_evict": (ctypes.c_int, [_P, _P, _P, _P, _P]),
     "nc_benchmark_options_init": (None, [ctypes.POINTER(BenchmarkOptions)]),
     "nc_benchmark_run_kernel": (
         ctypes.c_int,
@@ -770,6 +786,141 @@ def paged_decode(module: Module, q: DeviceBuffer, k_cache: DeviceBuffer, v_cache
         workspace.nbytes), ctypes.byref(opts), stream)
     if st:
         check(st, "paged.decode")
+
+
+# ---------------------------------------------------------------------------------------------
+# smaller paged cache (include/notcute_paged4.h): fewer bits a value, fewer tokens a request
+# ---------------------------------------------------------------------------------------------
+
+_ROWS4_BUFFERS = struct.Struct("=15Q")
+_DECODE4_BUFFERS = struct.Struct("=18Q")
+_MASS = struct.Struct("=3Q")
+_EVICT_BUFFERS = struct.Struct("=21Q")
+_EVICT4_BUFFERS = struct.Struct("=25Q")
+
+
+def paged4_validate(opts: PagedOptions) -> None:
+    check(lib().nc_paged4_validate(ctypes.byref(opts)), "paged4.validate")
+
+
+def paged4_workspace_bytes(opts: PagedOptions, mass: bool = False) -> int:
+    """Bytes of device memory that paged4_decode needs for these options, with a mass or without one, to be zeroed once; 0 for
+    invalid ones."""
+    return int(lib().nc_paged4_workspace_bytes(ctypes.byref(opts), int(mass)))
+
+
+def paged_mass_workspace_bytes(opts: PagedOptions) -> int:
+    """The same for paged_decode_mass."""
+    return int(lib().nc_paged_mass_workspace_bytes(ctypes.byref(opts)))
+
+
+def paged_evict_workspace_bytes(opts: PagedOptions) -> int:
+    """Bytes of device memory that paged_evict and paged4_evict need for these options; 0 for invalid ones."""
+    return int(lib().nc_paged_evict_workspace_bytes(ctypes.byref(opts)))
+
+
+def evict_rules(*, limit: int, budget: int, sinks: int = 0, recent: int = 0) -> EvictRules:
+    """Requests of more than `limit` tokens keep `budget`: the first `sinks`, the last `recent` and the heaviest others."""
+    return EvictRules(limit, budget, sinks, recent)
+
+
+def _cache4(k: DeviceBuffer, v: DeviceBuffer, k_scales: DeviceBuffer, v_scales: DeviceBuffer) -> tuple:
+    return (k.ptr, k.nbytes, v.ptr, v.nbytes, k_scales.ptr, k_scales.nbytes, v_scales.ptr, v_scales.nbytes)
+
+
+def _mass(mass: Optional[DeviceBuffer], stride: int) -> Optional[bytes]:
+    return None if mass is None else _MASS.pack(mass.ptr, mass.nbytes >> 2, stride)
+
+
+def _num_rows(name: str, slots: DeviceBuffer, num_rows: Optional[int]) -> int:
+    n = slots.nbytes >> 2 if num_rows is None else num_rows
+    if n < 0:
+        raise ValueError(f"{name}: num_rows {n}")
+    return n
+
+
+def paged4_append(module: Module, k_rows: DeviceBuffer, v_rows: DeviceBuffer, slots: DeviceBuffer, k: DeviceBuffer,
+                  v: DeviceBuffer, k_scales: DeviceBuffer, v_scales: DeviceBuffer, opts: PagedOptions,
+                  stream: Optional[int] = None, *, num_rows: Optional[int] = None) -> None:
+    """New K and V rows into 4-bit pages (nc_paged4_append): row i to slots[i], for the first num_rows rows (by default as
+    many as there are slots). k and v are the codes, two a byte."""
+    n = _num_rows("paged4_append", slots, num_rows)
+    st = (_lib or lib()).nc_paged4_append(module.handle, _ROWS4_BUFFERS.pack(
+        k_rows.ptr, k_rows.nbytes >> 1, v_rows.ptr, v_rows.nbytes >> 1, slots.ptr, slots.nbytes >> 2,
+        *_cache4(k, v, k_scales, v_scales), n), ctypes.byref(opts), stream)
+    if st:
+        check(st, "paged4.append")
+
+
+def paged4_read(module: Module, k: DeviceBuffer, v: DeviceBuffer, k_scales: DeviceBuffer, v_scales: DeviceBuffer,
+                slots: DeviceBuffer, k_rows: DeviceBuffer, v_rows: DeviceBuffer, opts: PagedOptions,
+                stream: Optional[int] = None, *, num_rows: Optional[int] = None) -> None:
+    """K and V rows out of 4-bit pages (nc_paged4_read): the row at slots[i] to row i; zeros for a slot outside the pool."""
+    n = _num_rows("paged4_read", slots, num_rows)
+    st = (_lib or lib()).nc_paged4_read(module.handle, _ROWS4_BUFFERS.pack(
+        *_cache4(k, v, k_scales, v_scales), slots.ptr, slots.nbytes >> 2, k_rows.ptr, k_rows.nbytes >> 1, v_rows.ptr,
+        v_rows.nbytes >> 1, n), ctypes.byref(opts), stream)
+    if st:
+        check(st, "paged4.read")
+
+
+def paged4_decode(module: Module, q: DeviceBuffer, k: DeviceBuffer, v: DeviceBuffer, k_scales: DeviceBuffer,
+                  v_scales: DeviceBuffer, block_table: DeviceBuffer, seq_lens: DeviceBuffer, o: DeviceBuffer,
+                  workspace: DeviceBuffer, opts: PagedOptions, stream: Optional[int] = None, *,
+                  mass: Optional[DeviceBuffer] = None, mass_stride: int = 0) -> None:
+    """Attention of one new token per request over its 4-bit pages (nc_paged4_decode); with a mass every token's share of
+    the weights is added to it. `workspace` is a zeroed buffer of paged4_workspace_bytes(opts, mass) and more."""
+    st = (_lib or lib()).nc_paged4_decode(module.handle, _DECODE4_BUFFERS.pack(
+        q.ptr, q.nbytes >> 1, *_cache4(k, v, k_scales, v_scales), block_table.ptr, block_table.nbytes >> 2, seq_lens.ptr,
+        seq_lens.nbytes >> 2, o.ptr, o.nbytes >> 2, workspace.ptr, workspace.nbytes), _mass(mass, mass_stride),
+        ctypes.byref(opts), stream)
+    if st:
+        check(st, "paged4.decode")
+
+
+def paged_decode_mass(module: Module, q: DeviceBuffer, k_cache: DeviceBuffer, v_cache: DeviceBuffer,
+                      block_table: DeviceBuffer, seq_lens: DeviceBuffer, o: DeviceBuffer, mass: DeviceBuffer,
+                      workspace: DeviceBuffer, opts: PagedOptions, stream: Optional[int] = None, *,
+                      mass_stride: int = 0) -> None:
+    """paged_decode, and every token's share of the weights added to its mass (nc_paged_decode_mass). `workspace` is a
+    zeroed buffer of paged_mass_workspace_bytes(opts) and more."""
+    st = (_lib or lib()).nc_paged_decode_mass(module.handle, _DECODE_BUFFERS.pack(
+        q.ptr, q.nbytes >> 1, k_cache.ptr, k_cache.nbytes >> 1, v_cache.ptr, v_cache.nbytes >> 1, block_table.ptr,
+        block_table.nbytes >> 2, seq_lens.ptr, seq_lens.nbytes >> 2, o.ptr, o.nbytes >> 2, workspace.ptr,
+        workspace.nbytes), _mass(mass, mass_stride), ctypes.byref(opts), stream)
+    if st:
+        check(st, "paged.decode_mass")
+
+
+def _evict_lists(table, lens, mass, mass_stride, free_pages, cursor, kept_lens, counts, workspace) -> tuple:
+    return (table.ptr, table.nbytes >> 2, lens.ptr, lens.nbytes >> 2, mass.ptr, mass.nbytes >> 2, mass_stride, free_pages.ptr,
+            free_pages.nbytes >> 2, cursor.ptr, cursor.nbytes >> 2, kept_lens.ptr, kept_lens.nbytes >> 2, counts.ptr,
+            counts.nbytes >> 2, workspace.ptr, workspace.nbytes)
+
+
+def paged_evict(module: Module, block_table: DeviceBuffer, seq_lens: DeviceBuffer, mass: DeviceBuffer,
+                k_cache: DeviceBuffer, v_cache: DeviceBuffer, free_pages: DeviceBuffer, cursor: DeviceBuffer,
+                kept_lens: DeviceBuffer, counts: DeviceBuffer, workspace: DeviceBuffer, rules: EvictRules,
+                opts: PagedOptions, stream: Optional[int] = None, *, mass_stride: int = 0) -> None:
+    """Cuts requests that are too long to their first, last and heaviest tokens (nc_paged_evict). kept_lens may be seq_lens,
+    and counts may be cursor; `workspace` is a buffer of paged_evict_workspace_bytes(opts) and more."""
+    st = (_lib or lib()).nc_paged_evict(module.handle, _EVICT_BUFFERS.pack(
+        *_evict_lists(block_table, seq_lens, mass, mass_stride, free_pages, cursor, kept_lens, counts, workspace),
+        k_cache.ptr, k_cache.nbytes >> 1, v_cache.ptr, v_cache.nbytes >> 1), ctypes.byref(rules), ctypes.byref(opts), stream)
+    if st:
+        check(st, "paged.evict")
+
+
+def paged4_evict(module: Module, block_table: DeviceBuffer, seq_lens: DeviceBuffer, mass: DeviceBuffer, k: DeviceBuffer,
+                 v: DeviceBuffer, k_scales: DeviceBuffer, v_scales: DeviceBuffer, free_pages: DeviceBuffer,
+                 cursor: DeviceBuffer, kept_lens: DeviceBuffer, counts: DeviceBuffer, workspace: DeviceBuffer,
+                 rules: EvictRules, opts: PagedOptions, stream: Optional[int] = None, *, mass_stride: int = 0) -> None:
+    """paged_evict over 4-bit pages (nc_paged4_evict)."""
+    st = (_lib or lib()).nc_paged4_evict(module.handle, _EVICT4_BUFFERS.pack(
+        *_evict_lists(block_table, seq_lens, mass, mass_stride, free_pages, cursor, kept_lens, counts, workspace),
+        *_cache4(k, v, k_scales, v_scales)), ctypes.byref(rules), ctypes.byref(opts), stream)
+    if st:
+        check(st, "paged4.evict")
 
 
 # ---------------------------------------------------------------------------------------------
