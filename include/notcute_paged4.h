@@ -42,7 +42,7 @@ typedef struct nc_paged4_cache {
 } nc_paged4_cache;
 
 /* What nc_paged_validate refuses, another head_dim and a cache stride that is no multiple of 32
- * (NC_ERROR_INVALID_VALUE). */
+ * (NC_ERROR_INVALID_VALUE), a pool of more than 2^37 values (NC_ERROR_OVERFLOW). */
 int nc_paged4_validate(const nc_paged_options *opts);
 
 /* K and V rows into the cache, as nc_paged_append: row i to slot slots[i], for the num_rows first rows; a slot outside the pool is

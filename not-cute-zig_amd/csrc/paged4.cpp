@@ -10,27 +10,30 @@ using namespace nc_paged;
 namespace {
 
 // Every kernel of paged4.hip by its place here, under which the module keeps its function.
-#define NC_DECODE4_NAMES(D)                                                                                                   \
-    "nc_paged4_decode_d" #D, "nc_paged4_decode_d" #D "_odd", "nc_paged4_decode_d" #D "_many", "nc_paged4_decode_d" #D "_many_odd", \
-        "nc_paged4_decode_d" #D "_next", "nc_paged4_decode_d" #D "_next_odd", "nc_paged4_mass4_d" #D, "nc_paged4_mass4_d" #D "_odd"
+#define NC_DECODE4_NAMES(D, T) \
+    "nc_paged4_decode_d" #D T, "nc_paged4_decode_d" #D T "_odd", "nc_paged4_mass4_d" #D T, "nc_paged4_mass4_d" #D T "_odd"
+#define NC_DECODE4_ALL(D) NC_DECODE4_NAMES(D, ""), NC_DECODE4_NAMES(D, "_by2"), NC_DECODE4_NAMES(D, "_by4")
 #define NC_MASS_NAMES(D) \
     "nc_paged4_mass_d" #D, "nc_paged4_mass_d" #D "_bf16", "nc_paged4_mass_d" #D "_odd", "nc_paged4_mass_d" #D "_odd_bf16"
 const char *const kKernels[] = {
-    "nc_paged4_append", "nc_paged4_read",     "nc_paged4_weights",  "nc_paged4_select",    "nc_paged4_move",
-    NC_DECODE4_NAMES(32), NC_DECODE4_NAMES(64), NC_DECODE4_NAMES(128), NC_MASS_NAMES(16), NC_MASS_NAMES(32),
+    "nc_paged4_append", "nc_paged4_read", "nc_paged4_weights", "nc_paged4_select", "nc_paged4_select_short", "nc_paged4_move",
+    NC_DECODE4_ALL(32), NC_DECODE4_ALL(64), NC_DECODE4_ALL(128), NC_MASS_NAMES(16), NC_MASS_NAMES(32),
     NC_MASS_NAMES(64),  NC_MASS_NAMES(128),
 };
-enum : uint32_t { kAppend, kRead, kWeights, kSelect, kMove, kDecode4, kMass = kDecode4 + 3 * 8 };
+enum : uint32_t { kAppend, kRead, kWeights, kSelect, kSelectShort, kMove, kDecode4, kMass = kDecode4 + 3 * 12 };
 static_assert(sizeof kKernels / sizeof kKernels[0] == NC_PAGED4_KERNELS, "one place per kernel");
 
 int launch(nc_module module, uint32_t kernel, uint32_t grid, uint32_t grid_y, uint32_t threads, void *args, nc_stream stream) {
     return launch_kernel(module, NC_PAGED_KERNELS + kernel, kKernels[kernel], grid, grid_y, threads, args, stream);
 }
 
+constexpr uint64_t kMostValues = 1ull << 37;  // of a pool in 4 bits: the kernels count 32 at a time, in 32 bits
+
 int resolve4(const nc_paged_options *opts, Shape *s) {
     int st = resolve(opts, s);
     if (st) return st;
-    return s->o.head_dim < 32 || (s->o.page_stride | s->o.head_stride | s->o.token_stride) % 32 ? NC_ERROR_INVALID_VALUE : NC_SUCCESS;
+    if (s->o.head_dim < 32 || (s->o.page_stride | s->o.head_stride | s->o.token_stride) % 32) return NC_ERROR_INVALID_VALUE;
+    return s->cache_len > kMostValues ? NC_ERROR_OVERFLOW : NC_SUCCESS;
 }
 
 int check_cache(const Shape &s, const nc_paged4_cache &c) {
@@ -224,11 +227,15 @@ int evict(nc_module module, const nc_paged_evict_lists &t, const nc_paged_evict_
     a.recent = (uint32_t)std::min<uint64_t>(rules->recent, kMost31);
     a.ps = nc_paged_make_div((uint32_t)o.page_size);
     a.units = (uint32_t)o.head_dim / (a.four ? 32 : 8);
+    // Of a row 128 bytes a wave, or less where that leaves most CUs idle.
     a.slice_log2 = std::min(3u, (uint32_t)__builtin_ctz(a.units));
+    while (a.slice_log2 && (o.num_seqs * 2 * o.num_kv_heads * a.units >> a.slice_log2) < 512) --a.slice_log2;
     const uint64_t waves = 2 * o.num_kv_heads * (a.units >> a.slice_log2);
     if (waves > kMost31 / 256) return NC_ERROR_OVERFLOW;
     a.waves = (uint32_t)waves;
-    st = launch(module, kSelect, (uint32_t)o.num_seqs, 1, 1024, &a, stream);
+    // a short table's requests are a few waves' work
+    const bool small = a.max_tokens <= 2048;
+    st = launch(module, small ? kSelectShort : kSelect, (uint32_t)o.num_seqs, 1, small ? 256 : 1024, &a, stream);
     if (st) return st;
     return launch(module, kMove, (uint32_t)((waves + 3) / 4 + 1), (uint32_t)std::min<uint64_t>(o.num_seqs, 65535), 256, &a, stream);
 }
@@ -373,8 +380,9 @@ int nc_paged4_decode(nc_module module, const nc_paged4_decode_buffers *buffers, 
     a.v_scales = t.cache.v_scales;
     a.bf = s.o.element_type == NC_ELEMENT_BF16;
     if (mass) more_args(plan, x, &a);
-    const uint32_t way = mass ? 6 : plan.side ? 4 : plan.many ? 2 : 0;
-    st = launch(module, kDecode4 + 8 * (plan.size - 1) + way + plan.odd, plan.grid, 1, 64 * NC_PAGED_WAVES, &a, stream);
+    a.values = s.cache_len;
+    const uint32_t pack = s.group <= 4 ? 2 : s.group <= 8 ? 1 : 0;
+    st = launch(module, kDecode4 + 12 * (plan.size - 1) + 4 * pack + (mass ? 2 : 0) + plan.odd, plan.grid, 1, 64 * NC_PAGED_WAVES, &a, stream);
     return st || !mass ? st : launch_weights(module, s, plan, x, mass->mass, stride, stream);
 }
 

@@ -92,8 +92,8 @@ extern "C" __global__ __launch_bounds__(256) void nc_paged4_append(const nc_page
     const uint32_t rows = (uint32_t)min((uint64_t)a.wg_rows, a.num_rows - row0), total = rows * a.chunks.d;
     for (uint32_t u = threadIdx.x; u < total; u += blockDim.x) {
         const Place p = place_of(a, row0, u);
+        const u32x4 kw = load_eight(a.k_in + p.row), vw = load_eight(a.v_in + p.row);  // on their way beside the slot
         if (!p.in) continue;  // all four lanes of a group
-        const u32x4 kw = load_eight(a.k_in + p.row), vw = load_eight(a.v_in + p.row);
         uint32_t kb, vb;
         const uint32_t kq = quantise(kw, a.bf, kb), vq = quantise(vw, a.bf, vb);
         *reinterpret_cast<uint32_t *>(a.k + p.cache / 2) = kq;
@@ -131,11 +131,12 @@ extern "C" __global__ __launch_bounds__(256) void nc_paged4_weights(const nc_pag
     for (uint32_t r = blockIdx.y; r < a.num_seqs; r += gridDim.y) {
         const uint32_t len = nc_paged_cut(as_const(a.seq_lens)[r], a.max_tokens);
         for (uint32_t t0 = blockIdx.x * 256u; t0 < len; t0 += gridDim.x * 256u) {
-            const uint32_t t = t0 + 4 * lane;
+            const uint32_t t = t0 + 4 * lane, j = t0 + threadIdx.x;
+            const float old = j < len ? a.mass[r * a.mass_stride + j] : 0.f;  // on its way beside the scores
             floatx4 sum = {0.f, 0.f, 0.f, 0.f};
             if (t < len) {
                 const uint64_t row0 = (uint64_t)r * a.num_q_heads;
-#pragma unroll 4
+#pragma unroll 8
                 for (uint32_t h = w; h < a.num_q_heads; h += 4) {
                     const floatx4 s = *reinterpret_cast<const floatx4 *>(a.scores + (row0 + h) * a.score_pitch + t);
                     const float top = a.row_ml[2 * (row0 + h)], inv = a.row_ml[2 * (row0 + h) + 1];
@@ -145,8 +146,7 @@ extern "C" __global__ __launch_bounds__(256) void nc_paged4_weights(const nc_pag
             }
             *reinterpret_cast<floatx4 *>(&s_sum[w][4 * lane]) = sum;
             __syncthreads();
-            const uint32_t j = t0 + threadIdx.x;
-            if (j < len) a.mass[r * a.mass_stride + j] += s_sum[0][threadIdx.x] + s_sum[1][threadIdx.x] + s_sum[2][threadIdx.x] + s_sum[3][threadIdx.x];
+            if (j < len) a.mass[r * a.mass_stride + j] = old + (s_sum[0][threadIdx.x] + s_sum[1][threadIdx.x] + s_sum[2][threadIdx.x] + s_sum[3][threadIdx.x]);
             __syncthreads();
         }
     }
@@ -155,11 +155,13 @@ extern "C" __global__ __launch_bounds__(256) void nc_paged4_weights(const nc_pag
 // -------------------------------------------------------------------------------------------------
 // Eviction. A workgroup a request finds the least mass that is kept by its bits, 11 at a time from the top (a histogram of the
 // masses that agree in the bits above, until all of a bin are kept), and then lists the tokens that stay, in their order. A
-// wave of it has a contiguous part of the tokens and keeps the first of them in registers.
+// wave of it has a contiguous part of the tokens and keeps the first of them in registers; of a longer part it reads as many at once
+// again in every pass (one by one, 60001 tokens took 69 us). It is a chain of barriers, loads and LDS additions: a short table's
+// requests have 4 waves, whose barriers cost less than those of 16.
 // -------------------------------------------------------------------------------------------------
 namespace {
 
-constexpr uint32_t kSelectWaves = 16, kSelectHeld = 8;  // waves of a selection, tokens that a lane of it keeps
+constexpr uint32_t kSelectHeld = 8;  // tokens that a lane of a selection keeps, and reads at once
 
 // Masses in ascending order as numbers: both zeros are one, a NaN is the largest.
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -174,11 +176,14 @@ __device__ __forceinline__ uint32_t pages_of(uint32_t tokens, nc_paged_div ps) {
     return n + (n * ps.d != tokens);
 }
 
-}  // namespace
-
-extern "C" __global__ __launch_bounds__(64 * kSelectWaves) void nc_paged4_select(const nc_paged_evict_args a) {
-    __shared__ uint32_t s_bins[2048];
-    __shared__ uint32_t s_a[kSelectWaves], s_b[kSelectWaves], s_c[kSelectWaves], s_d[kSelectWaves];
+template <uint32_t WAVES>
+__device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
+    constexpr uint32_t EACH = 2048 / (64 * WAVES);  // bins of a thread
+    // Equal masses are LDS additions to one address, one after the other: every bin COPIES times, a lane to its own. (60001 tokens of
+    // few different masses 59 us with one.)
+    constexpr uint32_t COPIES = WAVES == 16 ? 8 : 2;
+    __shared__ uint32_t s_bins[2048 * COPIES];
+    __shared__ uint32_t s_a[WAVES], s_b[WAVES], s_c[WAVES], s_d[WAVES];
     __shared__ uint32_t s_bin, s_above, s_count, s_first;
     const uint32_t r = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t n = nc_paged_cut(as_const(a.seq_lens)[r], a.max_tokens);
@@ -191,6 +196,14 @@ extern "C" __global__ __launch_bounds__(64 * kSelectWaves) void nc_paged4_select
         s_first = n;
     }
     if (!cut && r != 0) return;
+
+    // The wave's tokens.
+    const float *mass = a.mass + r * a.mass_stride;
+    const uint32_t lo = a.sinks, hi = n - a.recent, need = a.budget - a.sinks - a.recent;
+    const uint32_t part = (n + 64u * WAVES - 1u) / (64u * WAVES) * 64u, begin = min(w * part, n), end = min(begin + part, n);
+    float held_mass[kSelectHeld];
+#pragma unroll
+    for (uint32_t i = 0; i < kSelectHeld; ++i) held_mass[i] = cut && begin + 64u * i + lane < end ? mass[begin + 64u * i + lane] : 0.f;
 
     // Pages that become free: of all requests, and of those before this one.
     uint32_t all = 0, before = 0, cuts = 0, dropped = 0;
@@ -215,14 +228,15 @@ extern "C" __global__ __launch_bounds__(64 * kSelectWaves) void nc_paged4_select
         s_d[w] = dropped;
     }
     __syncthreads();
-    all = before = cuts = dropped = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kSelectWaves; ++i) {
-        all += s_a[i];
-        before += s_b[i];
-        cuts += s_c[i];
-        dropped += s_d[i];
-    }
+    // Sums over the waves, in a lane of each: of all of them, or of those before this one.
+    auto sum_of = [&](const uint32_t *sums, uint32_t waves) {
+        const uint32_t scan = wave_scan32(lane < waves ? sums[lane] : 0u);
+        return (uint32_t)__builtin_amdgcn_readlane(scan, 63);
+    };
+    all = sum_of(s_a, WAVES);
+    before = sum_of(s_b, WAVES);
+    cuts = sum_of(s_c, WAVES);
+    dropped = sum_of(s_d, WAVES);
     const int64_t base = (int64_t)a.cursor[0] - all;
     if (r == 0 && tid == 0) {
         a.totals[0] = (int32_t)max(base, (int64_t)0);
@@ -238,24 +252,21 @@ extern "C" __global__ __launch_bounds__(64 * kSelectWaves) void nc_paged4_select
         if (at >= 0 && at < (int64_t)a.free_len) a.free_pages[at] = row[p];
     }
 
-    // The wave's tokens, and their order.
-    const float *mass = a.mass + r * a.mass_stride;
-    const uint32_t lo = a.sinks, hi = n - a.recent, need = a.budget - a.sinks - a.recent;
-    const uint32_t part = (n + 64u * kSelectWaves - 1u) / (64u * kSelectWaves) * 64u, begin = min(w * part, n), end = min(begin + part, n);
-    uint32_t key[kSelectHeld];
+    uint32_t key[kSelectHeld];  // the orders of the first of them
 #pragma unroll
-    for (uint32_t i = 0; i < kSelectHeld; ++i) {
-        const uint32_t t = begin + 64u * i + lane;
-        key[i] = t < end ? order_of(mass[t]) : 0u;
-    }
+    for (uint32_t i = 0; i < kSelectHeld; ++i) key[i] = order_of(held_mass[i]);
     // fn(place, order, whether there is one) for all of the wave's tokens, 64 neighbours at a time
     auto each = [&](auto &&fn) {
 #pragma unroll
         for (uint32_t i = 0; i < kSelectHeld; ++i)
             if (begin + 64u * i < end) fn(begin + 64u * i + lane, key[i], begin + 64u * i + lane < end);
-        for (uint32_t t = begin + 64u * kSelectHeld; t < end; t += 64u) {
-            const bool in = t + lane < end;
-            fn(t + lane, in ? order_of(mass[t + lane]) : 0u, in);
+        for (uint32_t t0 = begin + 64u * kSelectHeld; t0 < end; t0 += 64u * kSelectHeld) {
+            float x[kSelectHeld];
+#pragma unroll
+            for (uint32_t i = 0; i < kSelectHeld; ++i) x[i] = t0 + 64u * i + lane < end ? mass[t0 + 64u * i + lane] : 0.f;
+#pragma unroll
+            for (uint32_t i = 0; i < kSelectHeld; ++i)
+                if (t0 + 64u * i < end) fn(t0 + 64u * i + lane, order_of(x[i]), t0 + 64u * i + lane < end);
         }
     };
     // All orders from `least` on are kept, and the first `ties` tokens of order `least - 1`.
@@ -264,7 +275,7 @@ extern "C" __global__ __launch_bounds__(64 * kSelectWaves) void nc_paged4_select
     if (need) {
         uint32_t prefix = 0, left = need;  // the bits above the present ones, kept tokens that agree in them
         for (int shift = 21, bits = 11;;) {
-            for (uint32_t i = tid; i < 2048; i += blockDim.x) s_bins[i] = 0;
+            for (uint32_t i = tid; i < 2048 * COPIES; i += 64 * WAVES) s_bins[i] = 0;
             __syncthreads();
             each([&](uint32_t t, uint32_t k, bool in) {
                 const bool mine = in && t >= lo && t < hi && (uint64_t)k >> (shift + bits) == prefix;
@@ -274,22 +285,33 @@ extern "C" __global__ __launch_bounds__(64 * kSelectWaves) void nc_paged4_select
                 if (!who) return;
                 const uint32_t one = __builtin_amdgcn_readlane(bin, __builtin_ctzll(who));
                 const uint64_t same = __ballot(mine && bin == one);
-                if (mine && bin != one) atomicAdd(&s_bins[bin], 1u);
-                if (lane == (uint32_t)__builtin_ctzll(same)) atomicAdd(&s_bins[one], (uint32_t)__builtin_popcountll(same));
+                if (mine && bin != one) atomicAdd(&s_bins[bin * COPIES + lane % COPIES], 1u);
+                if (lane == (uint32_t)__builtin_ctzll(same)) atomicAdd(&s_bins[one * COPIES], (uint32_t)__builtin_popcountll(same));
             });
             __syncthreads();
-            // Bins from the top, two a thread; the one that the last token to be kept is in.
-            const uint32_t x = s_bins[2047u - 2u * tid], y = s_bins[2046u - 2u * tid];
-            const uint32_t incl = wave_scan32(x + y);
+            // Bins from the top, EACH a thread; the one that the last token to be kept is in.
+            uint32_t bin[EACH], mine = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < EACH; ++i) {
+                bin[i] = 0;
+#pragma unroll
+                for (uint32_t x = 0; x < COPIES; ++x) bin[i] += s_bins[(2047u - EACH * tid - i) * COPIES + x];
+                mine += bin[i];
+            }
+            const uint32_t incl = wave_scan32(mine);
             if (lane == 63) s_a[w] = incl;
             __syncthreads();
-            uint32_t above = incl - x - y;
-            for (uint32_t i = 0; i < w; ++i) above += s_a[i];
-            if (above < left && left <= above + x + y) {
-                const bool first = left <= above + x;
-                s_bin = first ? 2047u - 2u * tid : 2046u - 2u * tid;
-                s_above = first ? above : above + x;
-                s_count = first ? x : y;
+            uint32_t above = incl - mine + sum_of(s_a, w);
+            if (above < left && left <= above + mine) {
+#pragma unroll
+                for (uint32_t i = 0; i < EACH; ++i) {
+                    if (above < left && left <= above + bin[i]) {
+                        s_bin = 2047u - EACH * tid - i;
+                        s_above = above;
+                        s_count = bin[i];
+                    }
+                    above += bin[i];
+                }
             }
             __syncthreads();
             prefix = prefix << bits | s_bin;
@@ -321,11 +343,8 @@ extern "C" __global__ __launch_bounds__(64 * kSelectWaves) void nc_paged4_select
         s_b[w] = last;
     }
     __syncthreads();
-    sure = last = 0;
-    for (uint32_t i = 0; i < w; ++i) {
-        sure += s_a[i];
-        last += s_b[i];
-    }
+    sure = sum_of(s_a, w);
+    last = sum_of(s_b, w);
     int32_t *source = a.source + (uint64_t)r * a.max_tokens;
     float *kept = a.kept_mass + (uint64_t)r * a.max_tokens;
     uint32_t gone = n;
@@ -349,6 +368,11 @@ extern "C" __global__ __launch_bounds__(64 * kSelectWaves) void nc_paged4_select
     if (tid == 0) a.first[r] = (int32_t)s_first;
 }
 
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(1024) void nc_paged4_select(const nc_paged_evict_args a) { select_body<16>(a); }
+extern "C" __global__ __launch_bounds__(256) void nc_paged4_select_short(const nc_paged_evict_args a) { select_body<4>(a); }
+
 // The rows that stay, to the front. Every wave has a column of them, 16-byte units (four bits: 32 values and their scale) of one
 // head of K or V, and moves it row by row: no row's place is behind its source, the wave loads rows in ascending order, and stores
 // one when it and those before it have arrived. So no wave waits for another, and nothing is overwritten before it is read.
@@ -364,41 +388,41 @@ __device__ __forceinline__ void move_body(const nc_paged_evict_args &a, uint32_t
     uint8_t *codes = v ? a.v : a.k, *scales = v ? a.v_scales : a.k_scales;
     const int32_t *row = a.table + r * a.table_stride, *source = a.source + (uint64_t)r * a.max_tokens;
     const uint32_t num_slots = a.num_pages * a.ps.d;
-    struct Batch {
+    // Source slots and the places' pages of a batch's rows; of the next one they are on their way while this one's rows are.
+    uint32_t slot[AT_ONCE], page[AT_ONCE];
+    auto look = [&](uint32_t j0) {
+#pragma unroll
+        for (uint32_t i = 0; i < AT_ONCE; ++i) {
+            const uint32_t j = j0 + i * rows + (lane >> a.slice_log2), jj = min(j, keep - 1u);
+            slot[i] = j < keep ? (uint32_t)source[jj] : ~0u;
+            page[i] = (uint32_t)row[nc_paged_quot(jj, a.ps)];
+        }
+    };
+    look(first);
+    for (uint32_t j0 = first; j0 < keep; j0 += AT_ONCE * rows) {
         u32x4 x[AT_ONCE];
         uint32_t s[AT_ONCE];
         uint64_t to[AT_ONCE];
         bool in[AT_ONCE];
-    };
-    auto load = [&](Batch &b, uint32_t j0) {
 #pragma unroll
         for (uint32_t i = 0; i < AT_ONCE; ++i) {
-            const uint32_t j = j0 + i * rows + (lane >> (a.slice_log2));
-            const uint32_t jj = min(j, keep - 1u);
-            const uint32_t slot = (uint32_t)source[jj], at = nc_paged_quot(jj, a.ps), page = (uint32_t)row[at];
-            b.in[i] = j < keep && slot < num_slots && page < a.num_pages;
-            const uint32_t from = b.in[i] ? slot : 0u, p = nc_paged_quot(from, a.ps);
+            const uint32_t j = min(j0 + i * rows + (lane >> a.slice_log2), keep - 1u), tok = j - nc_paged_quot(j, a.ps) * a.ps.d;
+            in[i] = slot[i] < num_slots && page[i] < a.num_pages;
+            const uint32_t from = in[i] ? slot[i] : 0u, p = nc_paged_quot(from, a.ps);
             const uint64_t src = p * a.page_stride + (from - p * a.ps.d) * a.token_stride + base;
-            b.to[i] = page * a.page_stride + (jj - at * a.ps.d) * a.token_stride + base;
-            b.x[i] = *reinterpret_cast<const u32x4 *>(codes + (FOUR ? src / 2 : src * 2));
-            if constexpr (FOUR) b.s[i] = scales[src / 32];
+            to[i] = page[i] * a.page_stride + tok * a.token_stride + base;
+            x[i] = *reinterpret_cast<const u32x4 *>(codes + (FOUR ? src / 2 : src * 2));
+            if constexpr (FOUR) s[i] = scales[src / 32];
         }
-    };
-    auto store = [&](const Batch &b) {
-#pragma unroll
-        for (uint32_t i = 0; i < AT_ONCE; ++i)
-            if (b.in[i]) {
-                *reinterpret_cast<u32x4 *>(codes + (FOUR ? b.to[i] / 2 : b.to[i] * 2)) = b.x[i];
-                if constexpr (FOUR) scales[b.to[i] / 32] = (uint8_t)b.s[i];
-            }
-    };
-    const uint32_t step = AT_ONCE * rows;
-    Batch x;
-    for (uint32_t j = first; j < keep; j += step) {
-        load(x, j);
+        look(j0 + AT_ONCE * rows);
         // all of the batch's rows have arrived before the first is stored
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        store(x);
+#pragma unroll
+        for (uint32_t i = 0; i < AT_ONCE; ++i)
+            if (in[i]) {
+                *reinterpret_cast<u32x4 *>(codes + (FOUR ? to[i] / 2 : to[i] * 2)) = x[i];
+                if constexpr (FOUR) scales[to[i] / 32] = (uint8_t)s[i];
+            }
     }
 }
 
@@ -427,26 +451,26 @@ extern "C" __global__ __launch_bounds__(256) void nc_paged4_move(const nc_paged_
 // -------------------------------------------------------------------------------------------------
 // Attention: paged_decode.h.
 // -------------------------------------------------------------------------------------------------
-#define NC_DECODE4_KERNEL(NAME, D, BF, UNI, MANY, NEXT, FOUR, MASS)                                     \
+#define NC_DECODE4_KERNEL(NAME, D, BF, UNI, MANY, NEXT, FOUR, MASS, PACK)                               \
     extern "C" __global__ __launch_bounds__(64 * NC_PAGED_WAVES, 2) void NAME(const nc_paged_more_args) { \
-        decode_body<D, BF, UNI, MANY, NEXT, FOUR, MASS>();                                              \
+        decode_body<D, BF, UNI, MANY, NEXT, FOUR, MASS, PACK>();                                        \
     }
-#define NC_DECODE4(D)                                                                        \
-    NC_DECODE4_KERNEL(nc_paged4_decode_d##D, D, true, true, false, false, true, false)            \
-    NC_DECODE4_KERNEL(nc_paged4_decode_d##D##_odd, D, true, false, false, false, true, false)      \
-    NC_DECODE4_KERNEL(nc_paged4_decode_d##D##_many, D, true, true, true, false, true, false)       \
-    NC_DECODE4_KERNEL(nc_paged4_decode_d##D##_many_odd, D, true, false, true, false, true, false)  \
-    NC_DECODE4_KERNEL(nc_paged4_decode_d##D##_next, D, true, true, true, true, true, false)        \
-    NC_DECODE4_KERNEL(nc_paged4_decode_d##D##_next_odd, D, true, false, true, true, true, false)   \
-    NC_DECODE4_KERNEL(nc_paged4_mass4_d##D, D, true, true, false, false, true, true)               \
-    NC_DECODE4_KERNEL(nc_paged4_mass4_d##D##_odd, D, true, false, false, false, true, true)
+#define NC_DECODE4_PACK(D, T, PACK, NEXT)                                                        \
+    NC_DECODE4_KERNEL(nc_paged4_decode_d##D##T, D, true, true, true, NEXT, true, false, PACK)        \
+    NC_DECODE4_KERNEL(nc_paged4_decode_d##D##T##_odd, D, true, false, true, NEXT, true, false, PACK) \
+    NC_DECODE4_KERNEL(nc_paged4_mass4_d##D##T, D, true, true, true, NEXT, true, true, PACK)          \
+    NC_DECODE4_KERNEL(nc_paged4_mass4_d##D##T##_odd, D, true, false, true, NEXT, true, true, PACK)
+#define NC_DECODE4(D)                 \
+    NC_DECODE4_PACK(D, , 1, false)    \
+    NC_DECODE4_PACK(D, _by2, 2, true) \
+    NC_DECODE4_PACK(D, _by4, 4, true)
 NC_DECODE4(32)
 NC_DECODE4(64)
 NC_DECODE4(128)
 // Scores kept over caches in 16 bits.
 #define NC_MASS(D, T, BF)                                                                  \
-    NC_DECODE4_KERNEL(nc_paged4_mass_d##D##T, D, BF, true, false, false, false, true)           \
-    NC_DECODE4_KERNEL(nc_paged4_mass_d##D##_odd##T, D, BF, false, false, false, false, true)
+    NC_DECODE4_KERNEL(nc_paged4_mass_d##D##T, D, BF, true, false, false, false, true, 1)           \
+    NC_DECODE4_KERNEL(nc_paged4_mass_d##D##_odd##T, D, BF, false, false, false, false, true, 1)
 NC_MASS(16, , false)
 NC_MASS(32, , false)
 NC_MASS(64, , false)

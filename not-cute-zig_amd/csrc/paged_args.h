@@ -27,7 +27,7 @@ NC_HD uint32_t nc_paged_quot(uint32_t n, nc_paged_div v) {
 }
 
 #define NC_PAGED_KERNELS 53u  // kernels of paged.hip
-#define NC_PAGED4_KERNELS 45u // and of paged4.hip
+#define NC_PAGED4_KERNELS 58u // and of paged4.hip
 
 struct nc_paged_build_args {
     const int32_t *cached, *fresh, *free_pages, *cursor;
@@ -77,7 +77,7 @@ NC_HD uint32_t nc_paged_head_parts(uint32_t group) { return (group + 63u) / 64u;
 NC_HD constexpr uint32_t nc_paged_head_units(uint32_t head_dim) { return head_dim <= 32 ? 1u : 2u; }
 // Caches in 4 bits.
 NC_HD constexpr uint32_t nc_paged4_head_units(uint32_t head_dim) { return head_dim <= 64 ? 1u : 2u; }
-#define NC_PAGED4_STEP_KEYS 64u
+NC_HD constexpr uint32_t nc_paged4_step_keys(uint32_t head_dim) { return head_dim <= 128 ? 64u : 32u; }
 // A head of no more blocks than this is not split: the workgroup that has its first unit takes all of it. (Of 1: 118
 // requests of up to 2719, 3 heads of 32, 10.8 -> 11.1 us; of 4: 12.0, and 4 of 500 over 8 heads of 128 7.6 -> 9.4.)
 #define NC_PAGED_WHOLE_BLOCKS 2u
@@ -135,6 +135,7 @@ struct nc_paged_more_args {
     float *scores;                      // a row of score_pitch per request and query head
     float *row_ml;                      // and its (max, 1 / sum)
     uint64_t score_pitch;
+    uint64_t values;                    // of a 4-bit pool
     uint32_t bf;                        // Q is bf16
 };
 

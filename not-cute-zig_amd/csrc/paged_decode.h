@@ -218,11 +218,12 @@ __device__ __forceinline__ uint32_t take_eights(float (&x)[4]) {
 // neighbours in fixed point, which keeps 13 bits below the largest (with parts of up to 16 the scores were off by 2^-13). V is
 // turned into bf16, which holds every value of a 4-bit cache, and BF is true.
 // MASS: every query head's scores are kept, and its maximum and sum, for the weights' kernel.
-template <int D, bool BF, bool UNI, bool MANY, bool NEXT, bool FOUR = false, bool MASS = false>
+// PACK: where a key head has at most 8 or 4 query heads, the 16 columns are 2 or 4 groups of them, each with a maximum, a sum and an
+// O of its own, that take every second or fourth tile: a step's scores then are half or a quarter of the registers.
+template <int D, bool BF, bool UNI, bool MANY, bool NEXT, bool FOUR = false, bool MASS = false, int PACK = 1>
 struct Decode {
     static_assert((BF && D >= 32) || !FOUR, "a 4-bit cache's V is bf16, and a group of 32 is a row's or part of it");
-    static_assert(!(MASS && (MANY || NEXT)), "scores are kept by one kind of kernel");
-    static constexpr int KT = FOUR || D <= 32 ? 2 : 1;  // 32-key tiles of a wave's step
+    static constexpr int KT = FOUR ? nc_paged4_step_keys(D) / 32 : D <= 32 ? 2 : 1;  // 32-key tiles of a wave's step
     static constexpr int NT = 2 * KT;           // 16-key tiles
     static constexpr uint32_t WK = 32 * KT;     // keys of a wave's step: nc_paged_step_keys(D)
     static constexpr int E = D / 16;            // dims of a lane in V and O
@@ -235,7 +236,9 @@ struct Decode {
     // of 64 28.0 -> 27.6 (but one of 120001 over 8 of 64, token-major, 53 -> 56). Heads of 16 or 32 are better off with more
     // workgroups instead (33 requests of up to 2047, 16 heads of 32, 11.9 -> 11.1 us on pages of 16, and 14.4 -> 11.4 of 7), and
     // with heads of 128 on odd pages both the addresses and two steps do not fit (1 % slower).
-    static constexpr bool AHEAD = FOUR ? UNI : D == 64 || (D == 128 && UNI);
+    static constexpr uint32_t COLS = 16 / PACK;  // query heads of a column group
+    static constexpr int SETS = NT / PACK;       // tiles of a column group
+    static constexpr bool AHEAD = FOUR ? false : D == 64 || (D == 128 && UNI);
     static constexpr int OP = D + 4;            // pitch of a row of partial O in LDS
     static constexpr uint32_t NW = NC_PAGED_WAVES, THREADS = 64 * NW;
     // Weights are 2^(score - max) times UNIT, in 16-bit parts. f16: the largest fits, the high part is normal down to 2^-29 of
@@ -271,6 +274,7 @@ struct Decode {
         const int32_t *table;
         const Elem *k, *v;
         const uint8_t *ks, *vs;
+        uint64_t values;  // FOUR: of the pool, from there on
         Off page_stride, token_stride;
         uint32_t num_pages;
         nc_paged_div ps;
@@ -291,6 +295,7 @@ struct Decode {
     i32x8 q8[FOUR ? KK : 1];  // FOUR: Q's parts and the bytes of their scales
     uint32_t qs[FOUR ? KK : 1];
     uint32_t ksat, vsat[4];   // and byte offsets of the scales
+    const uint16_t *q_row;    // the lane's query
     float *score;             // MASS: the lane's row of scores, at its keys of a tile; null for a column without a query
     float *row_ml;            // and the head's (max, 1 / sum)
     floatx4 acc[E];
@@ -308,16 +313,17 @@ struct Decode {
     // Q of a block's query heads as the B operand: lane (c, g) holds query c of the wave's 16, dims KE*g.. of 32.
     __device__ __forceinline__ void load_q(uint32_t r, uint32_t head0, uint32_t rows) {
         const Args a = again(args);
-        const uint32_t row = NEXT ? qt * a->group + min(c, a->group - 1u) : min(16u * qt + c, rows - 1u);
+        const uint32_t col = c & (COLS - 1u);
+        const uint32_t row = NEXT ? qt * a->group + min(col, a->group - 1u) : min(16u * qt + col, rows - 1u);
         const uint16_t *p = a->q + r * a->q_stride + (head0 + row) * a->q_head_stride;
         if constexpr (MASS) {
             const auto more = more_of(a);
             float *s = more->scores + ((uint64_t)r * a->num_q_heads + head0 + row) * more->score_pitch + 4 * g;
-            score = 16u * qt + c < rows ? s : nullptr;
+            score = (NEXT ? col < a->group : 16u * qt + col < rows) ? s : nullptr;
             row_ml = more->row_ml + 2 * ((uint64_t)r * a->num_q_heads + head0);
         }
-        if constexpr (FOUR) {
-            load_q8(a, p);
+        if constexpr (FOUR) {  // loaded in sweep(), behind what it has to wait for longer
+            q_row = p;
             return;
         }
 #pragma unroll
@@ -344,33 +350,42 @@ struct Decode {
     // and 1, then of part 2 and nothing; 32: the dims of parts 0, 1, 2 and nothing. K's are its dims as often. Lane (c, g) holds
     // columns 16g..+15 and 64+16g..+15, and the scale of columns 32g..+31 (hw_probe.hip has the layout). The parts' scale is
     // the query's largest value's power of two, so what three parts leave is 2^-20 of that at most.
-    __device__ __forceinline__ void load_q8(Args a, const uint16_t *p) {
-        constexpr int RUNS = D == 128 ? 2 : 1;  // of 16 dims
-        const bool bf = more_of(a)->bf;
-        uint32_t w[RUNS][8], top = 0;
+    static constexpr int RUNS = D == 128 ? 2 : 1;  // of 16 dims of a lane
+    struct RawQ {
+        uint32_t w[RUNS][8];
+        bool bf;
+    };
+    __device__ __forceinline__ RawQ load_q8() const {
+        const Args a = again(args);
+        RawQ q;
+        q.bf = more_of(a)->bf;
 #pragma unroll
         for (int u = 0; u < RUNS; ++u) {
-            const uint16_t *x = p + 64 * u + 16 * (D == 32 ? g & 1u : g);
+            const uint16_t *x = q_row + 64 * u + 16 * (D == 32 ? g & 1u : g);
             if (a->q_vec) {
                 const u32x4 y = *reinterpret_cast<const u32x4 *>(x), z = *reinterpret_cast<const u32x4 *>(x + 8);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    w[u][i] = y[i];
-                    w[u][4 + i] = z[i];
+                    q.w[u][i] = y[i];
+                    q.w[u][4 + i] = z[i];
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[u][i] = uint32_t(x[2 * i]) | uint32_t(x[2 * i + 1]) << 16;
+                for (int i = 0; i < 8; ++i) q.w[u][i] = uint32_t(x[2 * i]) | uint32_t(x[2 * i + 1]) << 16;
             }
         }
+        return q;
+    }
+    __device__ __forceinline__ void split_q8(const RawQ &q) {
+        uint32_t top = 0;
         float f[RUNS][16];
 #pragma unroll
         for (int u = 0; u < RUNS; ++u)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const half2v h = __builtin_bit_cast(half2v, w[u][i]);
-                f[u][2 * i] = bf ? __uint_as_float(w[u][i] << 16) : (float)h[0];
-                f[u][2 * i + 1] = bf ? __uint_as_float(w[u][i] & 0xffff0000u) : (float)h[1];
+                const half2v h = __builtin_bit_cast(half2v, q.w[u][i]);
+                f[u][2 * i] = q.bf ? __uint_as_float(q.w[u][i] << 16) : (float)h[0];
+                f[u][2 * i + 1] = q.bf ? __uint_as_float(q.w[u][i] & 0xffff0000u) : (float)h[1];
                 top = max(top, max(__float_as_uint(f[u][2 * i]) & 0x7fffffffu, __float_as_uint(f[u][2 * i + 1]) & 0x7fffffffu));
             }
         const uint32_t e = max(quad_max(top) >> 23, 30u);  // 255 where Q is not finite: so are all its scores' scales
@@ -434,36 +449,7 @@ struct Decode {
     // UNI: a tile is a buffer of its own whose length ends with its last key that counts, so that what lies
     // behind is neither read nor waited for, and is 0. Else rows that do not count read the pool's first row.
     __device__ __forceinline__ void issue(Step &st, const Cache &a, const Pages &pages, uint32_t k0, uint32_t end) const {
-        if constexpr (UNI && FOUR) {
-            const uint32_t ts = a.token_stride / 2u, ss = a.token_stride / 32u;  // bytes of codes and of scales
-            __amdgpu_buffer_rsrc_t vb[NT], sb[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const uint32_t k1 = k0 + 16 * t;
-                const bool in = k1 < end && pages.e[t] < a.num_pages;
-                const uint32_t n = in ? min(end - k1, 16u) : 0u;
-                st.seen[t] = n;
-                const uint32_t tok = k1 - nc_paged_quot(k1, a.ps) * a.ps.d;
-                const uint64_t at = in ? (uint64_t)pages.e[t] * a.page_stride + tok * a.token_stride : 0u;
-                const __amdgpu_buffer_rsrc_t kb = tile(a.k + at / 2, n * ts), ks = tile(a.ks + at / 32, n * ss);
-                vb[t] = tile(a.v + at / 2, n * ts);
-                sb[t] = tile(a.vs + at / 32, n * ss);
-                st.k[t][0] = __builtin_amdgcn_raw_buffer_load_b128(kb, kat, 0, 0);
-                st.scale.k[t] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(ks, ksat, 0, 0);
-            }
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (E == 8)
-                        st.v[t][i] = __builtin_amdgcn_raw_buffer_load_b32(vb[t], vat[i], 0, 0);
-                    else if constexpr (E == 4)
-                        st.v[t][i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vb[t], vat[i], 0, 0);
-                    else
-                        st.v[t][i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(vb[t], vat[i], 0, 0);
-                    st.scale.v[t][i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(sb[t], vsat[i], 0, 0);
-                }
-        } else if constexpr (UNI) {
+        if constexpr (UNI) {
             const uint32_t ts = 2u * a.token_stride;
             __amdgpu_buffer_rsrc_t vb[NT];
 #pragma unroll
@@ -497,36 +483,6 @@ struct Decode {
                     else
                         st.v[t][i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vb[t], vat[i], 0, 0);
                 }
-        } else if constexpr (FOUR) {
-            uint64_t vb[NT][4];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const uint32_t key = k0 + 16 * t + c;
-                const bool in = key < end && pages.e[t] < a.num_pages;
-                st.seen[t] = (uint32_t)__ballot(in) & 0xffffu;
-                const uint64_t at = in ? pages.e[t] * a.page_stride + (key - nc_paged_quot(key, a.ps) * a.ps.d) * a.token_stride : 0u;
-                st.k[t][0] = *reinterpret_cast<const u32x4 *>(a.k + at / 2 + 16 * k_group());
-                st.scale.k[t] = a.ks[at / 32 + k_group()];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int from = 4 * (int)g + i;
-                    const uint32_t lo = __shfl((uint32_t)at, from, 64), hi = __shfl((uint32_t)(at >> 32), from, 64);
-                    vb[t][i] = ((uint64_t)hi << 32 | lo) + E * c;
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint8_t *x = a.v + vb[t][i] / 2;
-                    if constexpr (E == 8)
-                        st.v[t][i] = *reinterpret_cast<const uint32_t *>(x);
-                    else if constexpr (E == 4)
-                        st.v[t][i] = *reinterpret_cast<const uint16_t *>(x);
-                    else
-                        st.v[t][i] = *x;
-                    st.scale.v[t][i] = a.vs[vb[t][i] / 32];
-                }
         } else {
             const uint16_t *vb[NT][4];
 #pragma unroll
@@ -557,6 +513,141 @@ struct Decode {
         }
     }
 
+    // The same of a 4-bit cache where a tile lies in one page: `at` has, by lane, the places of NT tiles of as many steps as there are
+    // lanes for, in units of 32 values (all ones: on no page, or past the end); these are the tiles of step `n`. A pool is one
+    // buffer, whose bytes 32 bits can count; rows that do not count are read too.
+    __device__ __forceinline__ void issue_tiles(Step &st, const Cache &a, uint32_t places, uint32_t n, uint32_t k0, uint32_t end) const {
+        const uint32_t codes = (uint32_t)(a.values / 2u), scales = (uint32_t)(a.values / 32u);
+        const __amdgpu_buffer_rsrc_t kb = tile(a.k, codes), vb = tile(a.v, codes), ks = tile(a.ks, scales), vs = tile(a.vs, scales);
+        uint32_t at[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            at[t] = __builtin_amdgcn_readlane(places, NT * n + t);
+            const bool in = at[t] != ~0u;
+            st.seen[t] = in ? min(end - (k0 + 16 * t), 16u) : 0u;
+            at[t] = in ? at[t] : 0u;
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            st.k[t][0] = __builtin_amdgcn_raw_buffer_load_b128(kb, kat, 16u * at[t], 0);
+            st.scale.k[t] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(ks, ksat, at[t], 0);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (E == 8)
+                    st.v[t][i] = __builtin_amdgcn_raw_buffer_load_b32(vb, vat[i], 16u * at[t], 0);
+                else if constexpr (E == 4)
+                    st.v[t][i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vb, vat[i], 16u * at[t], 0);
+                else
+                    st.v[t][i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(vb, vat[i], 16u * at[t], 0);
+                st.scale.v[t][i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(vs, vsat[i], at[t], 0);
+            }
+    }
+
+    // On pages of any size: lane j has the place of key j of the step, as above.
+    __device__ __forceinline__ void issue_keys(Step &st, const Cache &a, uint32_t places, uint32_t k0) const {
+        const uint64_t here = __ballot(places != ~0u);
+        places = places != ~0u ? places : 0u;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            st.seen[t] = (uint32_t)(here >> (16 * t)) & 0xffffu;
+            const uint64_t at = (uint32_t)__shfl((int)places, 16 * t + (int)c, 64);
+            st.k[t][0] = *reinterpret_cast<const u32x4 *>(a.k + 16u * at + 16u * k_group());
+            st.scale.k[t] = a.ks[at + k_group()];
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint64_t at = (uint32_t)__shfl((int)places, 16 * t + 4 * (int)g + i, 64);
+                const uint8_t *x = a.v + 16u * at + E / 2 * c;
+                if constexpr (E == 8)
+                    st.v[t][i] = *reinterpret_cast<const uint32_t *>(x);
+                else if constexpr (E == 4)
+                    st.v[t][i] = *reinterpret_cast<const uint16_t *>(x);
+                else
+                    st.v[t][i] = *x;
+                st.scale.v[t][i] = a.vs[at + E * c / 32u];
+            }
+    }
+
+    // The steps of sweep() over such a cache; the table's entries a step ahead.
+    __device__ __forceinline__ void sweep_keys(const Cache &a, uint32_t k0, uint32_t end, uint32_t by) {
+        static_assert(WK == 64 || !FOUR, "a key a lane");
+        auto entry_of = [&](uint32_t from) {
+            const uint32_t key = from + lane;
+            return key < end ? (uint32_t)a.table[nc_paged_quot(key, a.ps)] : ~0u;
+        };
+        auto place_of = [&](uint32_t from, uint32_t entry) {
+            const uint32_t key = from + lane;
+            return entry < a.num_pages ? (uint32_t)((entry * a.page_stride + (key - nc_paged_quot(key, a.ps) * a.ps.d) * a.token_stride) / 32u) : ~0u;
+        };
+        uint32_t entry = entry_of(k0);
+        const RawQ q = load_q8();
+        Step x;
+        issue_keys(x, a, place_of(k0, entry), k0);
+        entry = entry_of(k0 + by);
+        split_q8(q);
+        while (true) {
+            compute(x, k0, end);
+            if ((k0 += by) >= end) return;
+            issue_keys(x, a, place_of(k0, entry), k0);
+            entry = entry_of(k0 + by);
+        }
+    }
+
+    // The steps of sweep() over a 4-bit cache whose tiles lie in one page each. The table's entries are read 64 / NT steps at a time, that many steps ahead: as
+    // scalar loads, one after the other, they took a third of a step.
+    __device__ __forceinline__ void sweep_tiles(const Cache &a, uint32_t k0, uint32_t end, uint32_t by) {
+        constexpr uint32_t STEPS = 64 / NT;
+        const uint32_t mine = lane / NT * by + 16u * (lane % NT);  // the lane's tile, behind the batch's first key
+        auto entry_of = [&](uint32_t from) {
+            const uint32_t key = from + mine;
+            return key < end ? (uint32_t)a.table[nc_paged_quot(key, a.ps)] : ~0u;
+        };
+        auto place_of = [&](uint32_t from, uint32_t entry) {
+            const uint32_t key = from + mine;
+            return entry < a.num_pages ? (entry * a.page_stride + (key - nc_paged_quot(key, a.ps) * a.ps.d) * a.token_stride) / 32u : ~0u;
+        };
+        uint32_t batch = k0, n = 0, entry = entry_of(k0);
+        const RawQ q = load_q8();
+        uint32_t places = place_of(k0, entry);
+        auto next = [&](Step &st, uint32_t key) {
+            if (n == STEPS) {
+                batch += STEPS * by;
+                places = place_of(batch, entry);
+                entry = entry_of(batch + STEPS * by);
+                n = 0;
+            }
+            issue_tiles(st, a, places, n++, key, end);
+        };
+        Step x;
+        next(x, k0);
+        entry = entry_of(k0 + STEPS * by);
+        if constexpr (!AHEAD) {
+            split_q8(q);
+            while (true) {
+                compute(x, k0, end);
+                if ((k0 += by) >= end) return;
+                next(x, k0);
+            }
+        } else {
+            Step y;
+            next(y, k0 + by);
+            split_q8(q);
+            while (true) {
+                compute(x, k0, end);
+                if ((k0 += by) >= end) return;
+                next(x, k0 + by);
+                compute(y, k0, end);
+                if ((k0 += by) >= end) return;
+                next(y, k0 + by);
+            }
+        }
+    }
+
     // A raw buffer of `bytes` bytes.
     static __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile(const Elem *p, uint32_t bytes) {
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<Elem *>(p), 0, (int)bytes, 0x00020000);
@@ -582,7 +673,7 @@ struct Decode {
         bool full = true;
 #pragma unroll
         for (int t = 0; t < NT; ++t) full = full && st.seen[t] == (UNI ? 16u : 0xffffu);
-        float s[NT][4];
+        float s[SETS][4];
         float top = neg_inf();
         floatx4 dot[NT];
 #pragma unroll
@@ -599,18 +690,24 @@ struct Decode {
                 else
                     dot[t] = mfma_k32<BF>(st.k[t][kk], qv[kk], x);
             }
+        const uint32_t part = c / COLS;  // the column group
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < SETS; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[t][i] = dot[t][i] * sc;
+            for (int i = 0; i < 4; ++i) {
+                float x = dot[PACK * t][i];
+#pragma unroll
+                for (int n = 1; n < PACK; ++n) x = part == (uint32_t)n ? dot[PACK * t + n][i] : x;
+                s[t][i] = x * sc;
+            }
         if (!full) {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const bool in = UNI ? 4 * g + i < st.seen[t] : st.seen[t] >> (4 * g + i) & 1u;
-                    s[t][i] = in ? s[t][i] : neg_inf();
-                    if constexpr (!UNI) {  // 0 * NaN would be NaN
+                    if (PACK == 1 || part == (uint32_t)(t % PACK)) s[t / PACK][i] = in ? s[t / PACK][i] : neg_inf();
+                    if constexpr (FOUR || !UNI) {  // 0 * NaN would be NaN
                         if constexpr (FOUR) {
                             st.scale.v[t][i] = in ? st.scale.v[t][i] : 0u;
                         } else if constexpr (E > 2) {
@@ -625,12 +722,14 @@ struct Decode {
         if constexpr (MASS) {  // a row holds whole tiles; keys that do not count have -infinity
             if (score) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
-                    if (k0 + 16 * t < end) *reinterpret_cast<floatx4 *>(score + k0 + 16 * t) = floatx4{s[t][0], s[t][1], s[t][2], s[t][3]};
+                for (int t = 0; t < SETS; ++t) {
+                    const uint32_t at = k0 + 16 * (PACK * t + part);
+                    if (at < end) *reinterpret_cast<floatx4 *>(score + at) = floatx4{s[t][0], s[t][1], s[t][2], s[t][3]};
+                }
             }
         }
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < SETS; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][i]);
         top = fmaxf(m, quad_max(top));
@@ -643,20 +742,36 @@ struct Decode {
             m = top;
         }
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < SETS; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - ref) * UNIT;
                 l += s[t][i];
             }
         u32x4 p[KT][PARTS];
+        if constexpr (PACK == 1) {
 #pragma unroll
-        for (int u = 0; u < KT; ++u)
+            for (int u = 0; u < KT; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int n = 0; n < PARTS; ++n)
-                    p[u][n][j] = take_pair<BF>(s[2 * u + j / 2][2 * (j % 2)], s[2 * u + j / 2][2 * (j % 2) + 1]);
+                    for (int n = 0; n < PARTS; ++n)
+                        p[u][n][j] = take_pair<BF>(s[2 * u + j / 2][2 * (j % 2)], s[2 * u + j / 2][2 * (j % 2) + 1]);
+        } else {  // a column group's weights stand at its own tile's keys, the others' are 0
+#pragma unroll
+            for (int t = 0; t < SETS; ++t)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int n = 0; n < PARTS; ++n) {
+                        const uint32_t w = take_pair<BF>(s[t][2 * j], s[t][2 * j + 1]);
+#pragma unroll
+                        for (int x = 0; x < PACK; ++x) {
+                            const int at = PACK * t + x;  // the tile
+                            p[at / 2][n][2 * (at % 2) + j] = part == (uint32_t)x ? w : 0u;
+                        }
+                    }
+        }
         constexpr int G = E < 2 ? E : 2;  // products of so many dims in turn: each waits for its last one
 #pragma unroll
         for (int i0 = 0; i0 < E; i0 += G) {
@@ -708,6 +823,7 @@ struct Decode {
             cache.v = reinterpret_cast<const uint8_t *>(a->v) + at / 2;
             cache.ks = more->k_scales + at / 32;
             cache.vs = more->v_scales + at / 32;
+            cache.values = more->values - at;
         } else {
             cache.k = a->k + kvh * a->head_stride;
             cache.v = a->v + kvh * a->head_stride;
@@ -718,6 +834,15 @@ struct Decode {
         cache.ps.d = a->ps.d;
         cache.ps.magic = a->ps.magic;
         cache.ps.shift = a->ps.shift;
+        if constexpr (FOUR && UNI)
+            sweep_tiles(cache, k0, end, by);
+        else if constexpr (FOUR)
+            sweep_keys(cache, k0, end, by);
+        else
+            sweep_steps(cache, k0, end, len, by);
+    }
+
+    __device__ __forceinline__ void sweep_steps(const Cache &cache, uint32_t k0, uint32_t end, uint32_t len, uint32_t by) {
         Step x, y;
         Pages pages = load_pages(cache, k0, len);
         issue(x, cache, pages, k0, end);
@@ -896,13 +1021,16 @@ struct Decode {
         }
     }
 
+    // What the weights' kernel needs of row q's sum.
+    __device__ __forceinline__ void put_ml(uint32_t q, float top, float sum) const {
+        row_ml[2 * q] = finite_or_0(top);
+        row_ml[2 * q + 1] = sum == 0.f ? 0.f : __builtin_amdgcn_rcpf(sum) * UNIT;
+    }
+
     __device__ __forceinline__ void store_o(float *o, uint32_t q, uint32_t x, floatx4 v, float sum, float top) {
         const float inv = __builtin_amdgcn_rcpf(sum);  // to an ulp
         if constexpr (MASS) {
-            if (x == 0) {
-                row_ml[2 * q] = finite_or_0(top);
-                row_ml[2 * q + 1] = sum == 0.f ? 0.f : inv * UNIT;
-            }
+            if (x == 0) put_ml(q, top, sum);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = sum == 0.f ? 0.f : v[i] * inv;
@@ -916,11 +1044,34 @@ struct Decode {
         }
     }
 
+    // The column groups' (m, l, O) as one, which all of them get.
+    __device__ __forceinline__ void join_columns() {
+        if constexpr (PACK > 1) {
+            auto add = [](float u, float v) { return u + v; };
+            auto over = [](float x, auto &&f) {
+                if constexpr (PACK == 4) x = f(x, dpp<0x124>(x));  // row_ror:4 and 8
+                return f(x, dpp<0x128>(x));
+            };
+            const float top = over(m, [](float u, float v) { return fmaxf(u, v); });
+            const float f = __builtin_amdgcn_exp2f(m - finite_or_0(top));
+            m = top;
+            l = over(f * l, add);
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = over(f * acc[i][j], add);
+        }
+    }
+
     // O of a head that the wave had to itself: lane (c, g) has dims 4gE..4gE+4E-1 of query c.
     __device__ __forceinline__ void finish_wave(uint32_t r, uint32_t head0, uint32_t rows) {
         const Args a = again(args);
+        join_columns();
         const float sum = quad_sum(l);
         if (c >= rows) return;
+        if constexpr (MASS) {
+            if (g == 0) put_ml(c, m, sum);
+        }
         float *o = a->o + r * a->o_stride + head0 * a->o_head_stride;
         const float inv = __builtin_amdgcn_rcpf(sum);  // to an ulp
         o += c * a->o_head_stride + 4 * E * g;
@@ -944,6 +1095,7 @@ struct Decode {
             last = (b_lo + nb - 1u) / each;
         }
         float *o = a->o + r * a->o_stride + head0 * a->o_head_stride;
+        join_columns();
         const float sum = quad_sum(l);
         if (g == 0) {
             s_ml[w][c][0] = m;
@@ -1063,7 +1215,7 @@ struct Decode {
                 // there are heads.
                 uint32_t n = 1;
                 if constexpr (MANY) {
-                    if (nb == 1 && seg >= u0 && a->many) {
+                    if (nb == 1 && seg >= u0 && a->many && (!NEXT || wave_shift == 0)) {
                         n = min(min(heads - head, NW), (u1 - seg + units_of(1) - 1u) / units_of(1));
                         if (len > n * WK) n = 1;
                     }
@@ -1072,13 +1224,13 @@ struct Decode {
                 if (alone ? w < n : b0 < b1) {
                     uint32_t kvh = alone ? head + w : head, part = 0;
                     if constexpr (NEXT) {
-                        kvh = (head << wave_shift) + qt;
+                        if (!alone) kvh = (head << wave_shift) + qt;
                     } else if (a->head_parts > 1) {
                         kvh = head / a->head_parts;
                         part = head - kvh * a->head_parts;
                     }
                     const uint32_t rows = NEXT ? piece_rows(a) : min(64u, a->group - 64u * part);
-                    const uint32_t head0 = NEXT ? head * rows : kvh * a->group + 64u * part;
+                    const uint32_t head0 = NEXT ? (alone ? kvh : head) * rows : kvh * a->group + 64u * part;
                     load_q(r, head0, rows);
                     m = neg_inf();
                     l = 0.f;
@@ -1127,10 +1279,10 @@ struct Decode {
 
 // NEXT: heads each for themselves (MANY: where a->many says so, short ones a wave each) or neighbouring ones together, whichever
 // the lengths call for; else MANY says it all.
-template <int D, bool BF, bool UNI, bool MANY, bool NEXT, bool FOUR = false, bool MASS = false>
+template <int D, bool BF, bool UNI, bool MANY, bool NEXT, bool FOUR = false, bool MASS = false, int PACK = 1>
 __device__ __forceinline__ void decode_body() {
     const Args a = (Args)__builtin_amdgcn_kernarg_segment_ptr();
-    using X = Decode<D, BF, UNI, MANY, false, FOUR, MASS>;
+    using X = Decode<D, BF, UNI, MANY, false, FOUR, MASS, PACK>;
     // the waves' O, or a merge's factors, sums of rows and partial sums
     constexpr uint32_t kWaves = X::NW * 16 * X::OP, kMerge = NC_PAGED_MERGE_ROWS + 2 * 64 + 4 * X::THREADS;
     __shared__ __attribute__((aligned(16))) float s_mem[kWaves > kMerge ? kWaves : kMerge];
@@ -1160,9 +1312,16 @@ __device__ __forceinline__ void decode_body() {
         }
     }
     auto *o = reinterpret_cast<float (*)[16][X::OP]>(s_mem);
-    if constexpr (NEXT) {
+    if constexpr (FOUR && NEXT) {  // heads each for themselves are neighbouring ones of one
+        using Y = Decode<D, BF, UNI, MANY, true, FOUR, MASS, PACK>;
+        const bool next = __ballot(longest > NC_PAGED_NEXT_TOKENS) != 0;
+        const uint32_t by = next ? side : 0u;
+        Y y{a, lane, w, lane & 15u, lane >> 4, by, Y::WK * (Y::NW >> by), w & ((1u << by) - 1u), w >> by, o, s_ml, &s_word};
+        y.run(scale, next ? mine_next : mine, some, len0, zero_len);
+        return;
+    } else if constexpr (NEXT) {
         if (__ballot(longest > NC_PAGED_NEXT_TOKENS)) {
-            using Y = Decode<D, BF, UNI, false, true, FOUR>;
+            using Y = Decode<D, BF, UNI, false, true>;
             Y y{a, lane, w, lane & 15u, lane >> 4, side, Y::WK * (Y::NW >> side), w & ((1u << side) - 1u), w >> side, o, s_ml, &s_word};
             y.run(scale, mine_next, some, len0, zero_len);
             return;

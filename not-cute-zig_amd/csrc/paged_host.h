@@ -147,7 +147,8 @@ inline DecodePlan decode_plan(const Shape &s, bool o_vec, bool four = false, boo
     const nc_paged_options &o = s.o;
     DecodePlan p;
     // A 16-key tile lies in one page, and a page's byte offsets fit 32 bits.
-    const bool uniform = o.page_size % 16 == 0 && o.page_stride < (1ull << 31) && o.page_size * o.token_stride < (1ull << 30);
+    // (4 bits: so do the whole pool's values.)
+    const bool uniform = o.page_size % 16 == 0 && (four ? s.cache_len <= 0xffffffffull : o.page_stride < (1ull << 31) && o.page_size * o.token_stride < (1ull << 30));
     const uint32_t d = o.head_dim == 16 ? 0 : o.head_dim == 32 ? 1 : o.head_dim == 64 ? 2 : 3;
     // Workgroups for long heads: one per CU for heads of 64 and 128, whose loads are wide. Two for small heads, and on pages of
     // any size where waves share their keys and have half as much under way. 4 requests of 20000 over 4 key heads, 20 query
@@ -156,7 +157,10 @@ inline DecodePlan decode_plan(const Shape &s, bool o_vec, bool four = false, boo
     //   pages of 16   heads of 64  32.9  30.9       heads of 128  54.2  55.9   (96 of 4000 over 8 of 64: 167  175)
     const bool two = o.head_dim <= 32 || (!uniform && s.group > 16);
     const uint32_t head_units = four ? nc_paged4_head_units((uint32_t)o.head_dim) : nc_paged_head_units((uint32_t)o.head_dim);
-    p.long_log2 = kCusLog2 + (two ? 1 : 0);
+    // 4 bits: two as well, whose loads hide each other's steps, but for a few heads, whose pieces they double. One and two per CU:
+    //   96 requests of 4000 over 8 heads of 64, 8 query heads each   82.6  66.6 us     16 of 4000 over 8 of 128   22.1  21.7
+    //   2 of 20000 over 8 of 64, 8 query heads each                  15.6  18.2        one of 30000 over 8 of 128  17.9  18.7
+    p.long_log2 = kCusLog2 + ((four ? o.num_seqs * s.heads > 16 : two) ? 1 : 0);
     // Short heads: as many as are resident. (Heads of 64 and 128 with twice as many: 512 requests of 100 over 8 heads of 128
     // 48.6 -> 50.0 us.)
     p.short_log2 = kCusLog2 + (o.head_dim <= 32 ? 2 : 1);
@@ -174,9 +178,11 @@ inline DecodePlan decode_plan(const Shape &s, bool o_vec, bool four = false, boo
     // Short requests are faster over all waves, so the kernel looks at the lengths (NC_PAGED_NEXT_TOKENS; 0.1 to 0.3 us where it
     // finds them short); where the table has no room for a long one, it need not.
     uint32_t side = 0;
-    if (!mass && (o.head_stride < o.token_stride || o.page_size == 1) && o.max_pages * o.page_size > NC_PAGED_NEXT_TOKENS) {
+    if ((!mass || four) && (o.head_stride < o.token_stride || o.page_size == 1) && o.max_pages * o.page_size > NC_PAGED_NEXT_TOKENS) {
         const uint64_t numbers = s.group * o.head_dim;  // of one head's piece
-        if (o.head_dim <= 32)
+        if (four)
+            side = s.group > 4 ? 0 : o.num_kv_heads % 4 == 0 && o.head_dim <= 64 ? 2 : o.num_kv_heads % 2 == 0 && (o.head_dim <= 64 || uniform) ? 1 : 0;
+        else if (o.head_dim <= 32)
             side = o.num_kv_heads % 4 == 0 && numbers <= 64 ? 2 : o.num_kv_heads % 2 == 0 && numbers <= 128 ? 1 : 0;
         else
             side = o.num_kv_heads % 4 == 0 && s.group <= 4 && o.num_seqs * s.heads <= 2u << p.short_log2;
@@ -184,7 +190,7 @@ inline DecodePlan decode_plan(const Shape &s, bool o_vec, bool four = false, boo
     p.wave_shift = nc_paged_wave_shift((uint32_t)s.group);
     p.side = side;
     p.rows = (uint32_t)std::min<uint64_t>(s.group, 64);
-    const uint64_t step = four ? NC_PAGED4_STEP_KEYS : nc_paged_step_keys((uint32_t)o.head_dim);
+    const uint64_t step = four ? nc_paged4_step_keys((uint32_t)o.head_dim) : nc_paged_step_keys((uint32_t)o.head_dim);
     // A piece is written and read once more: at most a quarter of what its run reads of the cache. (Neighbouring heads' are at
     // most 16 rows, and no more than a block's reads.)
     p.each_least = (uint32_t)std::max<uint64_t>(1, 8 * p.rows / (step * (NC_PAGED_WAVES >> p.wave_shift)));
@@ -201,7 +207,7 @@ inline DecodePlan decode_plan(const Shape &s, bool o_vec, bool four = false, boo
     //   256 of 50, 8 heads of 128                         15.8  13.2
     //   128 of 120, 8 heads of 128, two a workgroup       14.1  14.1
     // That code makes a call up to 0.1 us longer, so it has kernels of its own.
-    p.many = !mass && s.group <= 16 && o_vec && o.num_seqs * s.heads > 1u << p.short_log2;
+    p.many = (!mass || four) && s.group <= 16 && o_vec && o.num_seqs * s.heads > 1u << p.short_log2;
     p.size = d;
     p.odd = uniform ? 0 : 1;
     p.piece_ml = NC_PAGED_ROUNDS * 2 * NC_PAGED_MAX_WGS * 4;

@@ -76,7 +76,7 @@ def test_blocks_match_binding(tmp_path):
 @pytest.mark.parametrize("kw,want", [
     (dict(head_dim=16), INVALID), (dict(head_dim=48), INVALID), (dict(token_stride=72), INVALID), (dict(token_stride=80), INVALID),
     (dict(token_stride=96, head_stride=64), INVALID), (dict(page_stride=2 * 16 * 64 + 16), INVALID), (dict(num_q_heads=7), INVALID),
-    (dict(max_pages=2 ** 27), OVERFLOW),
+    (dict(max_pages=2 ** 27), OVERFLOW), (dict(num_pages=2 ** 26 + 1, page_stride=2048), OVERFLOW),
 ])
 def test_validate_refuses(kw, want):
     with pytest.raises(nc.NcError) as e:
