@@ -235,7 +235,7 @@ int evict(nc_module module, const nc_paged_evict_lists &t, const nc_paged_evict_
     a.waves = (uint32_t)waves;
     // a short table's requests are a few waves' work
     const bool small = a.max_tokens <= 2048;
-    st = launch(module, small ? kSelectShort : kSelect, (uint32_t)o.num_seqs, 1, small ? 256 : 1024, &a, stream);
+    st = launch(module, small ? kSelectShort : kSelect, (uint32_t)o.num_seqs, 1, small ? 512 : 1024, &a, stream);
     if (st) return st;
     return launch(module, kMove, (uint32_t)((waves + 3) / 4 + 1), (uint32_t)std::min<uint64_t>(o.num_seqs, 65535), 256, &a, stream);
 }

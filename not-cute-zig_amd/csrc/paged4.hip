@@ -156,12 +156,11 @@ extern "C" __global__ __launch_bounds__(256) void nc_paged4_weights(const nc_pag
 // Eviction. A workgroup a request finds the least mass that is kept by its bits, 11 at a time from the top (a histogram of the
 // masses that agree in the bits above, until all of a bin are kept), and then lists the tokens that stay, in their order. A
 // wave of it has a contiguous part of the tokens and keeps the first of them in registers; of a longer part it reads as many at once
-// again in every pass (one by one, 60001 tokens took 69 us). It is a chain of barriers, loads and LDS additions: a short table's
-// requests have 4 waves, whose barriers cost less than those of 16.
+// again in every pass (one by one, 60001 tokens took 69 us). It is a chain of barriers, loads and LDS additions, and of code that
+// runs once: a short table's requests have 8 waves of 2 tokens a lane (one of 300 tokens, with its move: 9.7 us; 4 waves of 8 11.5,
+// 16 of 8 10.8).
 // -------------------------------------------------------------------------------------------------
 namespace {
-
-constexpr uint32_t kSelectHeld = 8;  // tokens that a lane of a selection keeps, and reads at once
 
 // Masses in ascending order as numbers: both zeros are one, a NaN is the largest.
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -176,7 +175,18 @@ __device__ __forceinline__ uint32_t pages_of(uint32_t tokens, nc_paged_div ps) {
     return n + (n * ps.d != tokens);
 }
 
-template <uint32_t WAVES>
+// A barrier of waves that only exchange what is in LDS: their stores to memory need not have arrived.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t lanes_below(uint64_t who) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
+}
+
+// The mass of an order.
+__device__ __forceinline__ float mass_of(uint32_t order) { return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order); }
+
+// HELD: tokens that a lane keeps, and of others reads at once.
+template <uint32_t WAVES, uint32_t HELD>
 __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
     constexpr uint32_t EACH = 2048 / (64 * WAVES);  // bins of a thread
     // Equal masses are LDS additions to one address, one after the other: every bin COPIES times, a lane to its own. (60001 tokens of
@@ -201,9 +211,15 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
     const float *mass = a.mass + r * a.mass_stride;
     const uint32_t lo = a.sinks, hi = n - a.recent, need = a.budget - a.sinks - a.recent;
     const uint32_t part = (n + 64u * WAVES - 1u) / (64u * WAVES) * 64u, begin = min(w * part, n), end = min(begin + part, n);
-    float held_mass[kSelectHeld];
+    const int32_t *row = a.table + r * a.table_stride;
+    float held_mass[HELD];
+    uint32_t held_page[HELD];
 #pragma unroll
-    for (uint32_t i = 0; i < kSelectHeld; ++i) held_mass[i] = cut && begin + 64u * i + lane < end ? mass[begin + 64u * i + lane] : 0.f;
+    for (uint32_t i = 0; i < HELD; ++i) {
+        const uint32_t t = begin + 64u * i + lane;
+        held_mass[i] = cut && t < end ? mass[t] : 0.f;
+        held_page[i] = cut && t < end ? (uint32_t)row[nc_paged_quot(t, a.ps)] : 0u;
+    }
 
     // Pages that become free: of all requests, and of those before this one.
     uint32_t all = 0, before = 0, cuts = 0, dropped = 0;
@@ -227,7 +243,7 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
         s_c[w] = cuts;
         s_d[w] = dropped;
     }
-    __syncthreads();
+    lds_barrier();
     // Sums over the waves, in a lane of each: of all of them, or of those before this one.
     auto sum_of = [&](const uint32_t *sums, uint32_t waves) {
         const uint32_t scan = wave_scan32(lane < waves ? sums[lane] : 0u);
@@ -245,40 +261,41 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
         a.totals[3] = (int32_t)dropped;
     }
     if (!cut) return;
-    const int32_t *row = a.table + r * a.table_stride;
     const uint32_t held = pages_of(n, a.ps), stay = pages_of(keep, a.ps);
     for (uint32_t p = stay + tid; p < held; p += blockDim.x) {
         const int64_t at = base + before + (p - stay);
         if (at >= 0 && at < (int64_t)a.free_len) a.free_pages[at] = row[p];
     }
 
-    uint32_t key[kSelectHeld];  // the orders of the first of them
+    // fn(64 neighbours' first place, the lane's mass) for all of the wave's tokens that are not in registers, so many read at once
+    auto rest = [&](auto &&fn) {
+        for (uint32_t t0 = begin + 64u * HELD; t0 < end; t0 += 64u * HELD) {
+            float x[HELD];
 #pragma unroll
-    for (uint32_t i = 0; i < kSelectHeld; ++i) key[i] = order_of(held_mass[i]);
-    // fn(place, order, whether there is one) for all of the wave's tokens, 64 neighbours at a time
-    auto each = [&](auto &&fn) {
+            for (uint32_t i = 0; i < HELD; ++i) x[i] = t0 + 64u * i + lane < end ? mass[t0 + 64u * i + lane] : 0.f;
 #pragma unroll
-        for (uint32_t i = 0; i < kSelectHeld; ++i)
-            if (begin + 64u * i < end) fn(begin + 64u * i + lane, key[i], begin + 64u * i + lane < end);
-        for (uint32_t t0 = begin + 64u * kSelectHeld; t0 < end; t0 += 64u * kSelectHeld) {
-            float x[kSelectHeld];
-#pragma unroll
-            for (uint32_t i = 0; i < kSelectHeld; ++i) x[i] = t0 + 64u * i + lane < end ? mass[t0 + 64u * i + lane] : 0.f;
-#pragma unroll
-            for (uint32_t i = 0; i < kSelectHeld; ++i)
-                if (t0 + 64u * i < end) fn(t0 + 64u * i + lane, order_of(x[i]), t0 + 64u * i + lane < end);
+            for (uint32_t i = 0; i < HELD; ++i)
+                if (t0 + 64u * i < end) fn(t0 + 64u * i, x[i]);
         }
     };
-    // All orders from `least` on are kept, and the first `ties` tokens of order `least - 1`.
-    uint64_t least = 1ull << 32;
+    auto each = [&](auto &&fn) {
+#pragma unroll
+        for (uint32_t i = 0; i < HELD; ++i)
+            if (begin + 64u * i < end) fn(begin + 64u * i, held_mass[i]);
+        rest(fn);
+    };
+    // All masses above `edge` are kept (all_nan: no such), and the first `ties` tokens of that mass.
+    float edge = __builtin_inff();
     uint32_t ties = 0;
+    bool all_nan = true;
     if (need) {
         uint32_t prefix = 0, left = need;  // the bits above the present ones, kept tokens that agree in them
         for (int shift = 21, bits = 11;;) {
             for (uint32_t i = tid; i < 2048 * COPIES; i += 64 * WAVES) s_bins[i] = 0;
-            __syncthreads();
-            each([&](uint32_t t, uint32_t k, bool in) {
-                const bool mine = in && t >= lo && t < hi && (uint64_t)k >> (shift + bits) == prefix;
+            lds_barrier();
+            each([&](uint32_t t0, float x) {
+                const uint32_t t = t0 + lane, k = order_of(x);
+                const bool mine = t >= lo && t < hi && t < end && (shift == 21 || k >> (shift + bits) == prefix);
                 const uint32_t bin = k >> shift & ((1u << bits) - 1u);
                 // equal masses are common (zeros): the first lane counts for all that share its bin
                 const uint64_t who = __ballot(mine);
@@ -288,7 +305,7 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
                 if (mine && bin != one) atomicAdd(&s_bins[bin * COPIES + lane % COPIES], 1u);
                 if (lane == (uint32_t)__builtin_ctzll(same)) atomicAdd(&s_bins[one * COPIES], (uint32_t)__builtin_popcountll(same));
             });
-            __syncthreads();
+            lds_barrier();
             // Bins from the top, EACH a thread; the one that the last token to be kept is in.
             uint32_t bin[EACH], mine = 0;
 #pragma unroll
@@ -300,7 +317,7 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
             }
             const uint32_t incl = wave_scan32(mine);
             if (lane == 63) s_a[w] = incl;
-            __syncthreads();
+            lds_barrier();
             uint32_t above = incl - mine + sum_of(s_a, w);
             if (above < left && left <= above + mine) {
 #pragma unroll
@@ -313,65 +330,96 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
                     above += bin[i];
                 }
             }
-            __syncthreads();
+            lds_barrier();
             prefix = prefix << bits | s_bin;
             left -= s_above;
             if (s_count == left || shift == 0) {
-                // the whole bin, or all its bits: then the first ones of it
-                least = (uint64_t)prefix << shift;
-                if (s_count != left) {
-                    least += 1;
-                    ties = left;
+                // The whole bin, so that the edge is the order below its least one; or all the bits of an order, and its first ones.
+                // Orders that no mass has: below 0's, whose mass would be -0, and between infinity's and NaN's. (Below -infinity's the
+                // mass is a NaN, above which is everything.)
+                uint32_t order = prefix;
+                if (s_count == left) {
+                    order = prefix << shift;
+                    order -= order != 0u;
+                    order = order == 0x7fffffffu ? 0x7ffffffeu : min(order, 0xff800000u);
                 }
+                ties = s_count == left ? 0u : left;
+                all_nan = order == 0xffffffffu;
+                edge = mass_of(order);
                 break;
             }
             bits = shift == 21 ? 11 : 10;
             shift = shift == 21 ? 10 : 0;
-            __syncthreads();
+            lds_barrier();
         }
     }
-    // How many of the wave's tokens stay for sure, and how many are of the last order.
+    // Which of 64 neighbours stay for sure, and which have the edge's mass. (A NaN is above every number.)
+    auto sure_of = [&](uint32_t t0, float x) {
+        const bool above = !all_nan && !(x <= edge);
+        if (t0 >= lo && t0 + 64u <= hi) return __ballot(above);
+        const uint32_t t = t0 + lane;
+        return __ballot(t < end && (t < lo || t >= hi || above));
+    };
+    auto last_of = [&](uint32_t t0, float x) {
+        const bool equal = all_nan ? x != x : x == edge;
+        const uint32_t t = t0 + lane;
+        return t0 >= lo && t0 + 64u <= hi ? __ballot(equal) : __ballot(equal && t >= lo && t < hi && t < end);
+    };
     uint32_t sure = 0, last = 0;
-    each([&](uint32_t t, uint32_t k, bool in) {
-        const bool s = in && (t < lo || t >= hi || k >= least), l = in && !s && (uint64_t)k + 1 == least;
-        sure += __builtin_popcountll(__ballot(s));
-        last += __builtin_popcountll(__ballot(l));
+    each([&](uint32_t t0, float x) {
+        sure += __builtin_popcountll(sure_of(t0, x));
+        if (ties) last += __builtin_popcountll(last_of(t0, x));
     });
-    __syncthreads();
+    lds_barrier();
     if (lane == 0) {
         s_a[w] = sure;
         s_b[w] = last;
     }
-    __syncthreads();
+    lds_barrier();
     sure = sum_of(s_a, w);
     last = sum_of(s_b, w);
     int32_t *source = a.source + (uint64_t)r * a.max_tokens;
     float *kept = a.kept_mass + (uint64_t)r * a.max_tokens;
     uint32_t gone = n;
-    each([&](uint32_t t, uint32_t k, bool in) {
-        const bool s = in && (t < lo || t >= hi || k >= least), l = in && !s && (uint64_t)k + 1 == least;
-        const uint64_t ws = __ballot(s), wl = __ballot(l), below = (1ull << lane) - 1ull;
-        const uint32_t ns = sure + __builtin_popcountll(ws & below), nl = last + __builtin_popcountll(wl & below);
-        if (s || (l && nl < ties)) {
-            const uint32_t to = ns + min(nl, ties);
-            const uint32_t at = nc_paged_quot(t, a.ps), page = (uint32_t)row[at];
-            source[to] = page < a.num_pages ? (int32_t)(page * a.ps.d + (t - at * a.ps.d)) : -1;
-            kept[to] = mass[t];
-        } else if (in) {
+    auto list = [&](uint32_t t0, float x, uint32_t page) {
+        const uint32_t t = t0 + lane;
+        const uint64_t ws = sure_of(t0, x), wl = ties ? last_of(t0, x) : 0ull;
+        const uint32_t nl = last + lanes_below(wl), to = sure + lanes_below(ws) + min(nl, ties);
+        const bool stays = ws >> lane & 1ull || (wl >> lane & 1ull && nl < ties);
+        if (stays) {
+            source[to] = page < a.num_pages ? (int32_t)(page * a.ps.d + (t - nc_paged_quot(t, a.ps) * a.ps.d)) : -1;
+            kept[to] = x;
+        } else if (t < end) {
             gone = min(gone, t);
         }
         sure += __builtin_popcountll(ws);
         last += __builtin_popcountll(wl);
-    });
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < HELD; ++i)
+        if (begin + 64u * i < end) list(begin + 64u * i, held_mass[i], held_page[i]);
+    for (uint32_t t0 = begin + 64u * HELD; t0 < end; t0 += 64u * HELD) {
+        float x[HELD];
+        uint32_t page[HELD];
+#pragma unroll
+        for (uint32_t i = 0; i < HELD; ++i) {
+            const uint32_t t = min(t0 + 64u * i + lane, n - 1u);
+            x[i] = mass[t];
+            page[i] = (uint32_t)row[nc_paged_quot(t, a.ps)];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < HELD; ++i)
+            if (t0 + 64u * i < end) list(t0 + 64u * i, x[i], page[i]);
+    }
     if (gone < n) atomicMin(&s_first, gone);
-    __syncthreads();
+    lds_barrier();
     if (tid == 0) a.first[r] = (int32_t)s_first;
 }
 
 }  // namespace
 
-extern "C" __global__ __launch_bounds__(1024) void nc_paged4_select(const nc_paged_evict_args a) { select_body<16>(a); }
-extern "C" __global__ __launch_bounds__(256) void nc_paged4_select_short(const nc_paged_evict_args a) { select_body<4>(a); }
+extern "C" __global__ __launch_bounds__(1024) void nc_paged4_select(const nc_paged_evict_args a) { select_body<16, 8>(a); }
+extern "C" __global__ __launch_bounds__(512) void nc_paged4_select_short(const nc_paged_evict_args a) { select_body<8, 2>(a); }
 
 // The rows that stay, to the front. Every wave has a column of them, 16-byte units (four bits: 32 values and their scale) of one
 // head of K or V, and moves it row by row: no row's place is behind its source, the wave loads rows in ascending order, and stores
