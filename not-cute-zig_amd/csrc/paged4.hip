@@ -164,10 +164,8 @@ namespace {
 
 // Masses in ascending order as numbers: both zeros are one, a NaN is the largest.
 __device__ __forceinline__ uint32_t order_of(float x) {
-    const uint32_t u = __float_as_uint(x);
-    if (x != x) return 0xffffffffu;
-    if (x == 0.f) return 0x80000000u;
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    const uint32_t u = __float_as_uint(x + 0.f);  // -0 + 0 is 0
+    return x != x ? 0xffffffffu : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
 __device__ __forceinline__ uint32_t pages_of(uint32_t tokens, nc_paged_div ps) {
@@ -297,13 +295,7 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
                 const uint32_t t = t0 + lane, k = order_of(x);
                 const bool mine = t >= lo && t < hi && t < end && (shift == 21 || k >> (shift + bits) == prefix);
                 const uint32_t bin = k >> shift & ((1u << bits) - 1u);
-                // equal masses are common (zeros): the first lane counts for all that share its bin
-                const uint64_t who = __ballot(mine);
-                if (!who) return;
-                const uint32_t one = __builtin_amdgcn_readlane(bin, __builtin_ctzll(who));
-                const uint64_t same = __ballot(mine && bin == one);
-                if (mine && bin != one) atomicAdd(&s_bins[bin * COPIES + lane % COPIES], 1u);
-                if (lane == (uint32_t)__builtin_ctzll(same)) atomicAdd(&s_bins[one * COPIES], (uint32_t)__builtin_popcountll(same));
+                if (mine) atomicAdd(&s_bins[bin * COPIES + lane % COPIES], 1u);
             });
             lds_barrier();
             // Bins from the top, EACH a thread; the one that the last token to be kept is in.
@@ -381,17 +373,22 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
     int32_t *source = a.source + (uint64_t)r * a.max_tokens;
     float *kept = a.kept_mass + (uint64_t)r * a.max_tokens;
     uint32_t gone = n;
+    // The place in its page of the lane's token of 64 neighbours, who are listed one after the other.
+    const uint32_t at64 = nc_paged_quot(64u, a.ps), tok64 = 64u - at64 * a.ps.d;
+    uint32_t tok = begin + lane - nc_paged_quot(begin + lane, a.ps) * a.ps.d;
     auto list = [&](uint32_t t0, float x, uint32_t page) {
         const uint32_t t = t0 + lane;
         const uint64_t ws = sure_of(t0, x), wl = ties ? last_of(t0, x) : 0ull;
         const uint32_t nl = last + lanes_below(wl), to = sure + lanes_below(ws) + min(nl, ties);
         const bool stays = ws >> lane & 1ull || (wl >> lane & 1ull && nl < ties);
         if (stays) {
-            source[to] = page < a.num_pages ? (int32_t)(page * a.ps.d + (t - nc_paged_quot(t, a.ps) * a.ps.d)) : -1;
+            source[to] = page < a.num_pages ? (int32_t)(page * a.ps.d + tok) : -1;
             kept[to] = x;
         } else if (t < end) {
             gone = min(gone, t);
         }
+        tok += tok64;
+        tok -= tok >= a.ps.d ? a.ps.d : 0u;
         sure += __builtin_popcountll(ws);
         last += __builtin_popcountll(wl);
     };

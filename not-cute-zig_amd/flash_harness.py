@@ -12,6 +12,7 @@ runner (modal_run.py:34-69), on one MI355X through the C ABI.
                                                   # (the Nsight Compute run of modal_run.py:108-146)
     python flash_harness.py benchmark-flash       # runFlashBenchmark (src/main.zig:760-766)
     python flash_harness.py paged                 # decoding steps over a paged cache (an extension), JSONL
+    python flash_harness.py paged4                # the same over one in 4 bits whose long requests are cut, JSONL
     python flash_harness.py timeline --workload c3    # per-wave timeline of the selected kernel
     python flash_harness.py compare-table FILE... # the baseline-vs-not-cute table (modal_run.py:34-69)
 
@@ -845,6 +846,104 @@ def cmd_paged(module: nc.Module, args) -> int:
     return status
 
 
+# ---------------------------------------------------------------------------------------------
+# paged4: the same over a cache in 4 bits, whose requests keep their heaviest tokens
+# ---------------------------------------------------------------------------------------------
+
+# (requests, query heads, key heads, head_dim, page_size, longest prompt, element type, limit, budget)
+PAGED4_CASES = [(1, 8, 8, 64, 16, 100, "f16", 90, 60), (8, 32, 8, 64, 16, 1000, "f16", 600, 400),
+                (33, 16, 4, 32, 7, 500, "bf16", 300, 200), (16, 32, 4, 128, 64, 777, "bf16", 512, 256)]
+
+
+class Paged4Batch(PagedBatch):
+    """A batch over a 4-bit cache; `rows` holds the values that were read back from it."""
+
+    def __init__(self, seqs, q_heads, kv_heads, head_dim, page_size, longest, dtype, limit, budget, seed=0):
+        super().__init__(seqs, q_heads, kv_heads, head_dim, page_size, longest, dtype, seed)
+        values = self.k.nbytes // 2
+        self.cache = [nc.DeviceBuffer(n) for n in (values // 2, values // 2, values // 32, values // 32)]
+        self.work = nc.DeviceBuffer(nc.paged4_workspace_bytes(self.opts, mass=True))
+        self.work.memset(0)
+        self.evict_work = nc.DeviceBuffer(nc.paged_evict_workspace_bytes(self.opts))
+        self.room = self.opts.max_pages * page_size
+        self.mass = nc.DeviceBuffer.from_array(np.zeros((seqs, self.room), np.float32))
+        self.rules = nc.evict_rules(limit=limit, budget=budget, sinks=4, recent=budget // 4)
+
+    def step(self, module, new, stream=None):
+        """One step's launches: tables and slots, rows into the cache, attention that adds the weights up."""
+        total = int(sum(new))
+        bufs = [nc.DeviceBuffer.from_array(x) for x in (
+            np.asarray(new, np.int32), self._random(total, self.kv_heads, self.d), self._random(total, self.kv_heads, self.d))]
+        q = self._random(*self.shape_q)
+        dq, slots, o = nc.DeviceBuffer.from_array(q), nc.DeviceBuffer(4 * total), nc.DeviceBuffer(4 * q.size)
+        nc.paged_build(module, self.lens, bufs[0], self.free, _Part(self.counts, 4), self.table, self.lens, self.offsets,
+                       slots, self.counts, self.opts, stream)
+        nc.paged4_append(module, bufs[1], bufs[2], slots, *self.cache, self.opts, stream)
+        nc.paged4_decode(module, dq, *self.cache, self.table, self.lens, o, self.work, self.opts, stream, mass=self.mass)
+        back = [nc.DeviceBuffer(x.nbytes) for x in bufs[1:]]
+        nc.paged4_read(module, *self.cache, slots, *back, self.opts, stream)
+        nc.synchronize()
+        k, v = (b.download(np.uint16, total * self.kv_heads * self.d).reshape(total, self.kv_heads, self.d) for b in back)
+        at = np.concatenate([[0], np.cumsum(new)])
+        for r, rows in enumerate(self.rows):
+            rows += [(k[i], v[i]) for i in range(at[r], at[r + 1])]
+        self.last = (dq, o)
+        return o, q
+
+    def evict(self, module, stream=None):
+        """Cuts the requests that are too long, and keeps `rows` in step by the masses that they had."""
+        mass = self.mass.download(np.float32, self.mass.nbytes // 4).reshape(-1, self.room)
+        nc.paged4_evict(module, self.table, self.lens, self.mass, *self.cache, self.free, _Part(self.counts, 4), self.lens,
+                        self.counts, self.evict_work, self.rules, self.opts, stream)
+        nc.synchronize()
+        p = self.rules
+        for r, rows in enumerate(self.rows):
+            n = len(rows)
+            if n > p.limit:
+                others = sorted(range(p.sinks, n - p.recent), key=lambda j: (-mass[r, j], j))
+                heavy = sorted(others[:p.budget - p.sinks - p.recent])
+                self.rows[r] = [rows[j] for j in [*range(p.sinks), *heavy, *range(n - p.recent, n)]]
+
+
+def cmd_paged4(module: nc.Module, args) -> int:
+    """Prompts of ragged lengths, then single tokens with evictions between, for each case; every step's attention
+    against float64 over the rows that are left, and the last step's attention timed by an event pair per launch."""
+    status = 0
+    for case in PAGED4_CASES:
+        seqs, q_heads, kv_heads, d, page_size, longest, dtype, limit, budget = case
+        batch = Paged4Batch(*case)
+        shape = (f"seqs={seqs},q_heads={q_heads},kv_heads={kv_heads},head={d},page={page_size},longest={longest},{dtype},"
+                 f"limit={limit},budget={budget}")
+        prompts = batch.rng.integers(0, longest + 1, seqs)
+        prompts[0] = longest
+        err, wrong = 0.0, 0
+        for new in (prompts, np.ones(seqs, int), batch.rng.integers(0, 2, seqs)):
+            if new.sum() == 0:
+                continue
+            o, q = batch.step(module, new)
+            wrong += int(batch.counts.download(np.int32, 4)[3])
+            err = max(err, float(np.max(np.abs(o.download(np.float32, q.size).reshape(q.shape) - batch.reference(q)))))
+            batch.evict(module)
+            wrong += batch.lens.download(np.int32, seqs).tolist() != [len(r) for r in batch.rows]
+        (dq, ob), start, stop, samples = batch.last, nc.Event(), nc.Event(), []
+        for i in range(args.warmup + args.iters):
+            start.record()
+            nc.paged4_decode(module, dq, *batch.cache, batch.table, batch.lens, ob, batch.work, batch.opts)
+            stop.record()
+            stop.synchronize()
+            if i >= args.warmup:
+                samples.append(nc.Event.elapsed(start, stop))
+        start.destroy()
+        stop.destroy()
+        tokens = sum(len(r) for r in batch.rows)
+        flops, bytes_ = 4 * tokens * q_heads * d, tokens * kv_heads * (d + d // 16) + seqs * q_heads * d * 6
+        ok = err <= PAGED_TOL and wrong == 0
+        status |= 0 if ok else 1
+        rec = make_record("not_cute", shape, ok, sum(samples) / len(samples), min(samples), max(samples), bytes_, flops, err)
+        emit({**rec, "kernel": "paged4_attention"})
+    return status
+
+
 def cmd_table(args) -> int:
     recs = []
     for path in args.files:
@@ -868,7 +967,8 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
     m.add_argument("--limit", type=int, default=0, help="only the first N shapes")
     for q in (p, b, m, sub.add_parser("profile-flash", help="attributes and occupancy of the c3 kernel"),
               sub.add_parser("benchmark-flash", help="runFlashBenchmark's five cases"),
-              sub.add_parser("paged", help="decoding steps over a paged cache, checked and timed (JSONL on stdout)")):
+              sub.add_parser("paged", help="decoding steps over a paged cache, checked and timed (JSONL on stdout)"),
+              sub.add_parser("paged4", help="the same over a cache in 4 bits whose long requests are cut")):
         q.add_argument("--warmup", type=int, default=5)
         q.add_argument("--iters", type=int, default=20)
     pf = sub.choices["profile-flash"]
@@ -897,7 +997,7 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
     nc.init()
     module = nc.Module.load_embedded()
     return {"flash": cmd_flash, "compare": cmd_compare, "profile-flash": cmd_profile,
-            "benchmark-flash": cmd_benchmark, "materialized": cmd_materialized, "paged": cmd_paged}[args.cmd](module, args)
+            "benchmark-flash": cmd_benchmark, "materialized": cmd_materialized, "paged": cmd_paged, "paged4": cmd_paged4}[args.cmd](module, args)
 
 
 if __name__ == "__main__":
