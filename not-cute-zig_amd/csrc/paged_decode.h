@@ -109,11 +109,12 @@ __device__ __forceinline__ floatx4 mfma_k16(u32x2 x, u32x2 y, floatx4 c) {
 // Two f32 rounded to nearest as a pair of 16-bit numbers; x and y become what that leaves, in f16 times kLowUnit: at most
 // half a step of a number below 2^16, times 2^12 below 2^16 too, and exact.
 constexpr float kLowUnit = 0x1p12f;
-template <bool BF>
+template <bool BF, bool ONCE = false>
 __device__ __forceinline__ uint32_t take_pair(float &x, float &y) {
     if constexpr (BF) {
         const bf16x2 h = {(__bf16)x, (__bf16)y};
-        const uint32_t u = __builtin_bit_cast(uint32_t, h);
+        uint32_t u = __builtin_bit_cast(uint32_t, h);
+        if constexpr (ONCE) asm("" : "+v"(u));  // else it is converted again, by halves
         x -= __uint_as_float(u << 16);
         y -= __uint_as_float(u & 0xffff0000u);
         return u;
@@ -235,10 +236,11 @@ struct Decode {
     // loads are wide and heads end at different times: 64 ragged requests over 4 heads of 64 31.6 -> 28.7 us, 32 of 2048 over 8
     // of 64 28.0 -> 27.6 (but one of 120001 over 8 of 64, token-major, 53 -> 56). Heads of 16 or 32 are better off with more
     // workgroups instead (33 requests of up to 2047, 16 heads of 32, 11.9 -> 11.1 us on pages of 16, and 14.4 -> 11.4 of 7), and
-    // with heads of 128 on odd pages both the addresses and two steps do not fit (1 % slower).
+    // with heads of 128 on odd pages both the addresses and two steps do not fit (1 % slower). 4-bit caches' steps are shorter and
+    // two workgroups of a CU hide each other's (16 of 1000 over 8 heads of 128 16.6 -> 14.4 us without, 96 of 8192 191 -> 170).
+    static constexpr bool AHEAD = !FOUR && (D == 64 || (D == 128 && UNI));
     static constexpr uint32_t COLS = 16 / PACK;  // query heads of a column group
     static constexpr int SETS = NT / PACK;       // tiles of a column group
-    static constexpr bool AHEAD = FOUR ? false : D == 64 || (D == 128 && UNI);
     static constexpr int OP = D + 4;            // pitch of a row of partial O in LDS
     static constexpr uint32_t NW = NC_PAGED_WAVES, THREADS = 64 * NW;
     // Weights are 2^(score - max) times UNIT, in 16-bit parts. f16: the largest fits, the high part is normal down to 2^-29 of
@@ -253,8 +255,10 @@ struct Decode {
     using VReg = typename std::conditional<FOUR || E <= 2, uint32_t, typename std::conditional<E == 4, u32x2, u32x4>::type>::type;
     using Elem = typename std::conditional<FOUR, uint8_t, uint16_t>::type;
     struct NoScales {};
+    // Of V a lane loads one scale of a tile, that of key 4g + c % 4 and its own dims; the lane's four keys' are those of the four
+    // lanes next to each other.
     struct Scales {
-        uint32_t k[NT], v[NT][4];
+        uint32_t k[NT], v[NT];
     };
 
     // K and V of a wave's step, on their way or there, and which keys count: the first seen[t] of a tile, or
@@ -294,7 +298,7 @@ struct Decode {
     u32x4 qv[FOUR ? 1 : KK];
     i32x8 q8[FOUR ? KK : 1];  // FOUR: Q's parts and the bytes of their scales
     uint32_t qs[FOUR ? KK : 1];
-    uint32_t ksat, vsat[4];   // and byte offsets of the scales
+    uint32_t ksat, vsat;      // and byte offsets of the scales
     const uint16_t *q_row;    // the lane's query
     float *score;             // MASS: the lane's row of scores, at its keys of a tile; null for a column without a query
     float *row_ml;            // and the head's (max, 1 / sum)
@@ -531,6 +535,7 @@ struct Decode {
         for (int t = 0; t < NT; ++t) {
             st.k[t][0] = __builtin_amdgcn_raw_buffer_load_b128(kb, kat, 16u * at[t], 0);
             st.scale.k[t] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(ks, ksat, at[t], 0);
+            st.scale.v[t] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(vs, vsat, at[t], 0);
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -542,7 +547,6 @@ struct Decode {
                     st.v[t][i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vb, vat[i], 16u * at[t], 0);
                 else
                     st.v[t][i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(vb, vat[i], 16u * at[t], 0);
-                st.scale.v[t][i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(vs, vsat[i], at[t], 0);
             }
     }
 
@@ -556,6 +560,8 @@ struct Decode {
             const uint64_t at = (uint32_t)__shfl((int)places, 16 * t + (int)c, 64);
             st.k[t][0] = *reinterpret_cast<const u32x4 *>(a.k + 16u * at + 16u * k_group());
             st.scale.k[t] = a.ks[at + k_group()];
+            const uint64_t vat = (uint32_t)__shfl((int)places, 16 * t + 4 * (int)g + (int)(c % 4u), 64);
+            st.scale.v[t] = a.vs[vat + E * c / 32u];
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -569,7 +575,6 @@ struct Decode {
                     st.v[t][i] = *reinterpret_cast<const uint16_t *>(x);
                 else
                     st.v[t][i] = *x;
-                st.scale.v[t][i] = a.vs[at + E * c / 32u];
             }
     }
 
@@ -598,8 +603,10 @@ struct Decode {
         }
     }
 
-    // The steps of sweep() over a 4-bit cache whose tiles lie in one page each. The table's entries are read 64 / NT steps at a time, that many steps ahead: as
-    // scalar loads, one after the other, they took a third of a step.
+    // The steps of sweep() over a 4-bit cache whose tiles lie in one page each. The table's entries are read 64 / NT steps at a time,
+    // that many steps ahead: as scalar loads, one after the other, they took a third of a step. Q's loads are under way beside the
+    // first entries', and it is split while the first step's are. (With one place in the code for a step's loads, and that split
+    // behind a branch, long requests took 8 % longer and short ones 2 % less.)
     __device__ __forceinline__ void sweep_tiles(const Cache &a, uint32_t k0, uint32_t end, uint32_t by) {
         constexpr uint32_t STEPS = 64 / NT;
         const uint32_t mine = lane / NT * by + 16u * (lane % NT);  // the lane's tile, behind the batch's first key
@@ -626,25 +633,11 @@ struct Decode {
         Step x;
         next(x, k0);
         entry = entry_of(k0 + STEPS * by);
-        if constexpr (!AHEAD) {
-            split_q8(q);
-            while (true) {
-                compute(x, k0, end);
-                if ((k0 += by) >= end) return;
-                next(x, k0);
-            }
-        } else {
-            Step y;
-            next(y, k0 + by);
-            split_q8(q);
-            while (true) {
-                compute(x, k0, end);
-                if ((k0 += by) >= end) return;
-                next(x, k0 + by);
-                compute(y, k0, end);
-                if ((k0 += by) >= end) return;
-                next(y, k0 + by);
-            }
+        split_q8(q);
+        while (true) {
+            compute(x, k0, end);
+            if ((k0 += by) >= end) return;
+            next(x, k0);
         }
     }
 
@@ -660,10 +653,20 @@ struct Decode {
             return v;
     }
 
+    // What lane j of each 4 has.
+    static __device__ __forceinline__ float v_scale(uint32_t x, int j) {
+        switch (j) {
+            case 0: return __uint_as_float(__builtin_amdgcn_update_dpp(0, x, 0x00, 0xf, 0xf, true));  // quad_perm j,j,j,j
+            case 1: return __uint_as_float(__builtin_amdgcn_update_dpp(0, x, 0x55, 0xf, 0xf, true));
+            case 2: return __uint_as_float(__builtin_amdgcn_update_dpp(0, x, 0xaa, 0xf, 0xf, true));
+            default: return __uint_as_float(__builtin_amdgcn_update_dpp(0, x, 0xff, 0xf, 0xf, true));
+        }
+    }
+
     // V's dims 2i, 2i+1 of key j of tile t.
     static __device__ __forceinline__ uint32_t v_pair(const Step &st, int t, int j, int i) {
         if constexpr (FOUR)
-            return pair_of_fours(st.v[t][j], __uint_as_float(st.scale.v[t][j] << 23), i);
+            return pair_of_fours(st.v[t][j], v_scale(st.scale.v[t] << 23, j), i);
         else
             return word(st.v[t][j], i);
     }
@@ -702,15 +705,13 @@ struct Decode {
             }
         if (!full) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const bool in = UNI ? 4 * g + i < st.seen[t] : st.seen[t] >> (4 * g + i) & 1u;
                     if (PACK == 1 || part == (uint32_t)(t % PACK)) s[t / PACK][i] = in ? s[t / PACK][i] : neg_inf();
-                    if constexpr (FOUR || !UNI) {  // 0 * NaN would be NaN
-                        if constexpr (FOUR) {
-                            st.scale.v[t][i] = in ? st.scale.v[t][i] : 0u;
-                        } else if constexpr (E > 2) {
+                    if constexpr (!FOUR && !UNI) {  // 0 * NaN would be NaN
+                        if constexpr (E > 2) {
 #pragma unroll
                             for (int j = 0; j < E / 2; ++j) st.v[t][i][j] = in ? st.v[t][i][j] : 0u;
                         } else {
@@ -718,6 +719,11 @@ struct Decode {
                         }
                     }
                 }
+                if constexpr (FOUR) {
+                    const uint32_t key = 4 * g + c % 4u;
+                    if (UNI ? key >= st.seen[t] : !(st.seen[t] >> key & 1u)) st.scale.v[t] = 0u;
+                }
+            }
         }
         if constexpr (MASS) {  // a row holds whole tiles; keys that do not count have -infinity
             if (score) {
@@ -756,7 +762,7 @@ struct Decode {
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int n = 0; n < PARTS; ++n)
-                        p[u][n][j] = take_pair<BF>(s[2 * u + j / 2][2 * (j % 2)], s[2 * u + j / 2][2 * (j % 2) + 1]);
+                        p[u][n][j] = take_pair<BF, FOUR>(s[2 * u + j / 2][2 * (j % 2)], s[2 * u + j / 2][2 * (j % 2) + 1]);
         } else {  // a column group's weights stand at its own tile's keys, the others' are 0
 #pragma unroll
             for (int t = 0; t < SETS; ++t)
@@ -764,7 +770,7 @@ struct Decode {
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int n = 0; n < PARTS; ++n) {
-                        const uint32_t w = take_pair<BF>(s[t][2 * j], s[t][2 * j + 1]);
+                        const uint32_t w = take_pair<BF, FOUR>(s[t][2 * j], s[t][2 * j + 1]);
 #pragma unroll
                         for (int x = 0; x < PACK; ++x) {
                             const int at = PACK * t + x;  // the tile
@@ -1157,11 +1163,9 @@ struct Decode {
             const uint32_t ts = (uint32_t)a->token_stride / 2u, ss = (uint32_t)a->token_stride / 32u;
             kat = c * ts + 16u * k_group();
             ksat = c * ss + k_group();
+            vsat = (4 * g + c % 4u) * ss + E * c / 32u;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                vat[i] = (4 * g + i) * ts + E / 2 * c;
-                vsat[i] = (4 * g + i) * ss + E * c / 32u;
-            }
+            for (int i = 0; i < 4; ++i) vat[i] = (4 * g + i) * ts + E / 2 * c;
         } else {
             kat = 2u * (c * (uint32_t)a->token_stride + KE * g);
 #pragma unroll

@@ -160,7 +160,7 @@ inline DecodePlan decode_plan(const Shape &s, bool o_vec, bool four = false, boo
     // 4 bits: two as well, whose loads hide each other's steps, but for a few heads, whose pieces they double. One and two per CU:
     //   96 requests of 4000 over 8 heads of 64, 8 query heads each   82.6  66.6 us     16 of 4000 over 8 of 128   22.1  21.7
     //   2 of 20000 over 8 of 64, 8 query heads each                  15.6  18.2        one of 30000 over 8 of 128  17.9  18.7
-    p.long_log2 = kCusLog2 + ((four ? o.num_seqs * s.heads > 16 : two) ? 1 : 0);
+    p.long_log2 = kCusLog2 + (two || (four && o.num_seqs * s.heads > 16) ? 1 : 0);
     // Short heads: as many as are resident. (Heads of 64 and 128 with twice as many: 512 requests of 100 over 8 heads of 128
     // 48.6 -> 50.0 us.)
     p.short_log2 = kCusLog2 + (o.head_dim <= 32 ? 2 : 1);
@@ -181,7 +181,7 @@ inline DecodePlan decode_plan(const Shape &s, bool o_vec, bool four = false, boo
     if ((!mass || four) && (o.head_stride < o.token_stride || o.page_size == 1) && o.max_pages * o.page_size > NC_PAGED_NEXT_TOKENS) {
         const uint64_t numbers = s.group * o.head_dim;  // of one head's piece
         if (four)
-            side = s.group > 4 ? 0 : o.num_kv_heads % 4 == 0 && o.head_dim <= 64 ? 2 : o.num_kv_heads % 2 == 0 && (o.head_dim <= 64 || uniform) ? 1 : 0;
+            side = s.group > (o.page_size == 1 ? 8 : 4) ? 0 : o.num_kv_heads % 4 == 0 && o.head_dim <= 64 ? 2 : o.num_kv_heads % 2 == 0 && (o.head_dim <= 64 || uniform) ? 1 : 0;
         else if (o.head_dim <= 32)
             side = o.num_kv_heads % 4 == 0 && numbers <= 64 ? 2 : o.num_kv_heads % 2 == 0 && numbers <= 128 ? 1 : 0;
         else
