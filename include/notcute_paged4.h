@@ -42,7 +42,7 @@ typedef struct nc_paged4_cache {
 } nc_paged4_cache;
 
 /* What nc_paged_validate refuses, another head_dim and a cache stride that is no multiple of 32
- * (NC_ERROR_INVALID_VALUE), a pool of more than 2^37 values (NC_ERROR_OVERFLOW). */
+ * (NC_ERROR_INVALID_VALUE), a pool of 2^37 values or more (NC_ERROR_OVERFLOW). */
 int nc_paged4_validate(const nc_paged_options *opts);
 
 /* K and V rows into the cache, as nc_paged_append: row i to slot slots[i], for the num_rows first rows; a slot outside the pool is
@@ -132,7 +132,7 @@ typedef struct nc_paged_evict_rules {
 /* The tokens that stay are moved together at the front, in their order, within the request's own pages: K, V and masses (those
  * behind the last one become 0). kept_lens[r] is the new length, the old one (cut to the table's row, negative: 0) where nothing
  * was evicted. The pages behind the new length go back to the list that nc_paged_build takes pages from: free_pages[cursor - n..cursor - 1]
- * are the n pages that became free, in the requests' order and the tables'. Those that find no place on the list (a cursor below n, or
+ * are the n pages that became free, in the requests' order and the tables', entries outside the pool among them. Those that find no place on the list (a cursor below n, or
  * beyond free_len) are lost. The tables are not changed: what they list behind the new length is the list's.
  *
  * counts[0] = cursor - n (at least 0), counts[1] = requests cut, counts[2] = n, counts[3] = tokens evicted.

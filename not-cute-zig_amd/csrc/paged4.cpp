@@ -27,7 +27,8 @@ int launch(nc_module module, uint32_t kernel, uint32_t grid, uint32_t grid_y, ui
     return launch_kernel(module, NC_PAGED_KERNELS + kernel, kKernels[kernel], grid, grid_y, threads, args, stream);
 }
 
-constexpr uint64_t kMostValues = 1ull << 37;  // of a pool in 4 bits: the kernels count 32 at a time, in 32 bits
+// Values of a pool in 4 bits: the kernels count 32 at a time, in 32 bits, of which all ones stand for no place.
+constexpr uint64_t kMostValues = (1ull << 37) - 32;
 
 int resolve4(const nc_paged_options *opts, Shape *s) {
     int st = resolve(opts, s);

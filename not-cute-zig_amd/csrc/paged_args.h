@@ -1,5 +1,5 @@
-// paged_args.h — what paged.cpp and paged.hip share: the kernels' argument blocks and the index
-// arithmetic that both sides (and the CPU tests) have to agree on.
+// paged_args.h — what the host side (paged.cpp, paged4.cpp) and the kernels (paged.hip, paged4.hip) share: argument blocks and
+// the index arithmetic that both sides (and the CPU tests) have to agree on.
 #ifndef NOTCUTE_PAGED_ARGS_H
 #define NOTCUTE_PAGED_ARGS_H
 
@@ -63,6 +63,7 @@ struct nc_paged_append_args {
 // 128 9.4 and 9.5.
 #define NC_PAGED_WAVES 4u
 #define NC_PAGED_NEXT_TOKENS 512u
+#define NC_PAGED4_STEP_KEYS 64u // a wave's step over a cache in 4 bits, of any head_dim
 NC_HD uint32_t nc_paged_step_keys(uint32_t head_dim) { return head_dim <= 32 ? 64u : 32u; }
 NC_HD uint32_t nc_paged_wave_shift(uint32_t group) { return group <= 16 ? 0u : group <= 32 ? 1u : 2u; }
 NC_HD uint32_t nc_paged_head_parts(uint32_t group) { return (group + 63u) / 64u; }
@@ -77,7 +78,6 @@ NC_HD uint32_t nc_paged_head_parts(uint32_t group) { return (group + 63u) / 64u;
 NC_HD constexpr uint32_t nc_paged_head_units(uint32_t head_dim) { return head_dim <= 32 ? 1u : 2u; }
 // Caches in 4 bits.
 NC_HD constexpr uint32_t nc_paged4_head_units(uint32_t head_dim) { return head_dim <= 64 ? 1u : 2u; }
-NC_HD constexpr uint32_t nc_paged4_step_keys(uint32_t head_dim) { return head_dim <= 128 ? 64u : 32u; }
 // A head of no more blocks than this is not split: the workgroup that has its first unit takes all of it. (Of 1: 118
 // requests of up to 2719, 3 heads of 32, 10.8 -> 11.1 us; of 4: 12.0, and 4 of 500 over 8 heads of 128 7.6 -> 9.4.)
 #define NC_PAGED_WHOLE_BLOCKS 2u

@@ -224,9 +224,9 @@ __device__ __forceinline__ uint32_t take_eights(float (&x)[4]) {
 template <int D, bool BF, bool UNI, bool MANY, bool NEXT, bool FOUR = false, bool MASS = false, int PACK = 1>
 struct Decode {
     static_assert((BF && D >= 32) || !FOUR, "a 4-bit cache's V is bf16, and a group of 32 is a row's or part of it");
-    static constexpr int KT = FOUR ? nc_paged4_step_keys(D) / 32 : D <= 32 ? 2 : 1;  // 32-key tiles of a wave's step
+    static constexpr int KT = FOUR ? NC_PAGED4_STEP_KEYS / 32 : D <= 32 ? 2 : 1;  // 32-key tiles of a wave's step
     static constexpr int NT = 2 * KT;           // 16-key tiles
-    static constexpr uint32_t WK = 32 * KT;     // keys of a wave's step: nc_paged_step_keys(D)
+    static constexpr uint32_t WK = 32 * KT;     // keys of a wave's step
     static constexpr int E = D / 16;            // dims of a lane in V and O
     static constexpr int KK = FOUR ? (D == 128 ? 3 : D / 32) : D < 32 ? 1 : D / 32;  // products of a score
     static constexpr int KL = FOUR ? 1 : KK;    // loads of a row of K

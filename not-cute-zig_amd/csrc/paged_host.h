@@ -190,7 +190,7 @@ inline DecodePlan decode_plan(const Shape &s, bool o_vec, bool four = false, boo
     p.wave_shift = nc_paged_wave_shift((uint32_t)s.group);
     p.side = side;
     p.rows = (uint32_t)std::min<uint64_t>(s.group, 64);
-    const uint64_t step = four ? nc_paged4_step_keys((uint32_t)o.head_dim) : nc_paged_step_keys((uint32_t)o.head_dim);
+    const uint64_t step = four ? NC_PAGED4_STEP_KEYS : nc_paged_step_keys((uint32_t)o.head_dim);
     // A piece is written and read once more: at most a quarter of what its run reads of the cache. (Neighbouring heads' are at
     // most 16 rows, and no more than a block's reads.)
     p.each_least = (uint32_t)std::max<uint64_t>(1, 8 * p.rows / (step * (NC_PAGED_WAVES >> p.wave_shift)));

@@ -821,6 +821,8 @@ def paged_evict_workspace_bytes(opts: PagedOptions) -> int:
 
 def evict_rules(*, limit: int, budget: int, sinks: int = 0, recent: int = 0) -> EvictRules:
     """Requests of more than `limit` tokens keep `budget`: the first `sinks`, the last `recent` and the heaviest others."""
+    if min(limit, budget, sinks, recent) < 0:
+        raise ValueError(f"evict_rules: {limit}, {budget}, {sinks}, {recent}")
     return EvictRules(limit, budget, sinks, recent)
 
 

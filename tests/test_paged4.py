@@ -77,6 +77,7 @@ def test_blocks_match_binding(tmp_path):
     (dict(head_dim=16), INVALID), (dict(head_dim=48), INVALID), (dict(token_stride=72), INVALID), (dict(token_stride=80), INVALID),
     (dict(token_stride=96, head_stride=64), INVALID), (dict(page_stride=2 * 16 * 64 + 16), INVALID), (dict(num_q_heads=7), INVALID),
     (dict(max_pages=2 ** 27), OVERFLOW), (dict(num_pages=2 ** 26 + 1, page_stride=2048), OVERFLOW),
+    (dict(num_pages=2 ** 26), OVERFLOW),
 ])
 def test_validate_refuses(kw, want):
     with pytest.raises(nc.NcError) as e:
@@ -86,7 +87,7 @@ def test_validate_refuses(kw, want):
 
 
 @pytest.mark.parametrize("kw", [dict(), dict(head_dim=32), dict(head_dim=128), dict(token_stride=96), dict(page_size=7),
-                                dict(token_stride=128, head_stride=64), dict(num_q_heads=200), dict(dtype="bf16")])
+                                dict(token_stride=128, head_stride=64), dict(num_q_heads=200), dict(dtype="bf16"), dict(num_pages=2 ** 26 - 1)])
 def test_validate_accepts_and_workspaces_grow(kw):
     nc.paged4_validate(good(**kw))
     o = good(**kw)
@@ -240,6 +241,12 @@ def test_evictions_refuse_too_many_requests():
     with pytest.raises(nc.NcError) as e:
         evict_call(o, False, table=big, lens=big, mass=big, kept=big, work=big)
     assert e.value.name == OVERFLOW
+
+
+def test_negative_rules_are_refused():
+    for kw in (dict(limit=-1, budget=1), dict(limit=2, budget=-1), dict(limit=2, budget=1, sinks=-1), dict(limit=2, budget=1, recent=-1)):
+        with pytest.raises(ValueError):
+            nc.evict_rules(**kw)
 
 
 def test_null_blocks_are_refused():
