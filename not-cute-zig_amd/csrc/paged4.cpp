@@ -148,7 +148,7 @@ void more_args(const DecodePlan &plan, const DecodeTensors &t, nc_paged_more_arg
 
 // Offsets of the eviction's workspace.
 struct EvictSpace {
-    uint64_t news, olds, first, source, kept_mass, bytes;
+    uint64_t news, olds, first, cuts, taken, read, source, kept_mass, bytes;
 };
 EvictSpace evict_space(const Shape &s) {
     const uint64_t seqs = 4 * ((s.o.num_seqs + 3) / 4 * 4), tokens = 4 * s.o.num_seqs * s.o.max_pages * s.o.page_size;
@@ -156,7 +156,12 @@ EvictSpace evict_space(const Shape &s) {
     e.news = 16;
     e.olds = e.news + seqs;
     e.first = e.olds + seqs;
-    e.source = e.first + seqs;
+    e.cuts = e.first + seqs;
+    // chains and chunks there may be, in 16 bits, which has more of them
+    const uint64_t chains = 2 * s.o.num_kv_heads, chunks = s.o.max_pages * s.o.page_size * (s.o.head_dim / 8) / (NC_PAGED4_MOVE_ROWS * NC_PAGED4_MOVE_THREADS) + 1;
+    e.taken = e.cuts + seqs;
+    e.read = e.taken + (4 * s.o.num_seqs * chains + 15) / 16 * 16;
+    e.source = e.read + (4 * s.o.num_seqs * chains * chunks + 15) / 16 * 16;
     e.kept_mass = e.source + (tokens + 15) / 16 * 16;
     e.bytes = e.kept_mass + tokens;
     return e;
@@ -210,6 +215,9 @@ int evict(nc_module module, const nc_paged_evict_lists &t, const nc_paged_evict_
     a.news = reinterpret_cast<int32_t *>(work + space.news);
     a.olds = reinterpret_cast<int32_t *>(work + space.olds);
     a.first = reinterpret_cast<int32_t *>(work + space.first);
+    a.cuts = reinterpret_cast<int32_t *>(work + space.cuts);
+    a.taken = reinterpret_cast<uint32_t *>(work + space.taken);
+    a.read = reinterpret_cast<uint32_t *>(work + space.read);
     a.source = reinterpret_cast<int32_t *>(work + space.source);
     a.kept_mass = reinterpret_cast<float *>(work + space.kept_mass);
     a.table_stride = o.table_stride;
@@ -227,18 +235,28 @@ int evict(nc_module module, const nc_paged_evict_lists &t, const nc_paged_evict_
     a.sinks = (uint32_t)std::min<uint64_t>(rules->sinks, kMost31);
     a.recent = (uint32_t)std::min<uint64_t>(rules->recent, kMost31);
     a.ps = nc_paged_make_div((uint32_t)o.page_size);
-    a.units = (uint32_t)o.head_dim / (a.four ? 32 : 8);
-    // Of a row 128 bytes a wave, or less where that leaves most CUs idle.
-    a.slice_log2 = std::min(3u, (uint32_t)__builtin_ctz(a.units));
-    while (a.slice_log2 && (o.num_seqs * 2 * o.num_kv_heads * a.units >> a.slice_log2) < 512) --a.slice_log2;
-    const uint64_t waves = 2 * o.num_kv_heads * (a.units >> a.slice_log2);
-    if (waves > kMost31 / 256) return NC_ERROR_OVERFLOW;
-    a.waves = (uint32_t)waves;
+    a.unit_log2 = (uint32_t)__builtin_ctz((uint32_t)o.head_dim / (a.four ? 32 : 8));
+    // Heads that are next to each other share a chain up to 128 bytes.
+    a.row_log2 = a.unit_log2;
+    if (o.head_stride == o.head_dim)
+        while (a.row_log2 < 3 && o.num_kv_heads % (2ull << (a.row_log2 - a.unit_log2)) == 0) ++a.row_log2;
+    const uint64_t chains = 2 * (o.num_kv_heads >> (a.row_log2 - a.unit_log2)), size = nc_paged4_chunk(a.row_log2);
+    const uint64_t most = std::min<uint64_t>(a.budget, a.max_tokens) - std::min<uint64_t>(a.sinks, a.max_tokens);  // rows of a chain
+    const uint64_t chunks = (most + size - 1) / size;
+    if (chains * std::max<uint64_t>(chunks, 1) > kMost31 || o.num_seqs * chains > kMost31) return NC_ERROR_OVERFLOW;
+    a.chains = (uint32_t)chains;
+    a.chunks = (uint32_t)chunks;
+    // A workgroup a chunk, but no more than a few thousand, which then take turns: most requests of a batch may not be cut.
+    constexpr uint64_t kMoveWgs = 4096;
+    a.side_chunks = (uint32_t)std::min(std::max<uint64_t>(chunks, 1), std::max<uint64_t>(1, kMoveWgs / chains));
+    a.side_chains = (uint32_t)std::min(o.num_seqs * chains, std::max<uint64_t>(1, kMoveWgs / a.side_chunks));
+    a.mass_parts = (a.max_tokens + NC_PAGED4_MASS_PART - 1) / NC_PAGED4_MASS_PART;
+    a.mass_wgs = (uint32_t)std::min<uint64_t>(o.num_seqs * a.mass_parts, 512);
     // a short table's requests are a few waves' work
     const bool small = a.max_tokens <= 2048;
     st = launch(module, small ? kSelectShort : kSelect, (uint32_t)o.num_seqs, 1, small ? 512 : 1024, &a, stream);
     if (st) return st;
-    return launch(module, kMove, (uint32_t)((waves + 3) / 4 + 1), (uint32_t)std::min<uint64_t>(o.num_seqs, 65535), 256, &a, stream);
+    return launch(module, kMove, a.mass_wgs + (chunks ? a.side_chunks * a.side_chains : 0), 1, NC_PAGED4_MOVE_THREADS, &a, stream);
 }
 
 }  // namespace

@@ -191,7 +191,7 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
     // few different masses 59 us with one.)
     constexpr uint32_t COPIES = WAVES == 16 ? 8 : 2;
     __shared__ uint32_t s_bins[2048 * COPIES];
-    __shared__ uint32_t s_a[WAVES], s_b[WAVES], s_c[WAVES], s_d[WAVES];
+    __shared__ uint32_t s_a[WAVES], s_b[WAVES], s_c[WAVES], s_d[WAVES], s_e[WAVES];
     __shared__ uint32_t s_bin, s_above, s_count, s_first;
     const uint32_t r = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t n = nc_paged_cut(as_const(a.seq_lens)[r], a.max_tokens);
@@ -200,10 +200,13 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
     if (tid == 0) {
         a.news[r] = (int32_t)keep;
         a.olds[r] = (int32_t)n;
-        if (!cut) a.first[r] = (int32_t)n;
         s_first = n;
     }
     if (!cut && r != 0) return;
+    if (cut && a.chunks > 1) {
+        for (uint32_t i = tid; i < a.chains; i += 64 * WAVES) a.taken[(uint64_t)r * a.chains + i] = 0;
+        for (uint32_t i = tid; i < a.chains * a.chunks; i += 64 * WAVES) a.read[(uint64_t)r * a.chains * a.chunks + i] = 0;
+    }
 
     // The wave's tokens.
     const float *mass = a.mass + r * a.mass_stride;
@@ -220,7 +223,7 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
     }
 
     // Pages that become free: of all requests, and of those before this one.
-    uint32_t all = 0, before = 0, cuts = 0, dropped = 0;
+    uint32_t all = 0, before = 0, cuts = 0, cuts_before = 0, dropped = 0;
     for (uint32_t q = tid; q < a.num_seqs; q += blockDim.x) {
         const uint32_t m = nc_paged_cut(a.seq_lens[q], a.max_tokens);
         if (m > a.limit) {
@@ -228,18 +231,21 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
             all += f;
             before += q < r ? f : 0u;
             cuts += 1u;
+            cuts_before += q < r ? 1u : 0u;
             dropped += m - a.budget;
         }
     }
     all = wave_scan32(all);
     before = wave_scan32(before);
     cuts = wave_scan32(cuts);
+    cuts_before = wave_scan32(cuts_before);
     dropped = wave_scan32(dropped);
     if (lane == 63) {
         s_a[w] = all;
         s_b[w] = before;
         s_c[w] = cuts;
         s_d[w] = dropped;
+        s_e[w] = cuts_before;
     }
     lds_barrier();
     // Sums over the waves, in a lane of each: of all of them, or of those before this one.
@@ -259,6 +265,8 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
         a.totals[3] = (int32_t)dropped;
     }
     if (!cut) return;
+    cuts_before = sum_of(s_e, WAVES);
+    if (tid == 0) a.cuts[cuts_before] = (int32_t)r;
     const uint32_t held = pages_of(n, a.ps), stay = pages_of(keep, a.ps);
     for (uint32_t p = stay + tid; p < held; p += blockDim.x) {
         const int64_t at = base + before + (p - stay);
@@ -418,77 +426,113 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
 extern "C" __global__ __launch_bounds__(1024) void nc_paged4_select(const nc_paged_evict_args a) { select_body<16, 8>(a); }
 extern "C" __global__ __launch_bounds__(512) void nc_paged4_select_short(const nc_paged_evict_args a) { select_body<8, 2>(a); }
 
-// The rows that stay, to the front. Every wave has a column of them, 16-byte units (four bits: 32 values and their scale) of one
-// head of K or V, and moves it row by row: no row's place is behind its source, the wave loads rows in ascending order, and stores
-// one when it and those before it have arrived. So no wave waits for another, and nothing is overwritten before it is read.
+// The rows that stay, to the front, in place and all at once. A chunk's workgroup reads its rows, says so, and stores them when the
+// chunks before it in the chain have been read: a place holds a row that goes to itself or to a place before it. Chunks are
+// taken by a count, in their order, and reading waits for nothing, so whoever waits does so for workgroups that run; that needs no
+// order among workgroups, and not all of them at once.
 namespace {
 
+// A store that is asked for has been seen by whoever reads the flag: waits as in Decode::join().
+__device__ __forceinline__ void wait_for_chunks(const uint32_t *read, uint32_t chunk) {
+    const uint32_t lane = threadIdx.x & 63u;
+    for (uint32_t c0 = 0; c0 < chunk; c0 += 64) {
+        // The count ends the wait where the workspace was not this call's alone.
+        for (uint32_t tries = 0; tries < 1u << 20; ++tries) {
+            const bool there = c0 + lane >= chunk || __hip_atomic_load(read + c0 + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0u;
+            if (__all(there)) break;
+            __builtin_amdgcn_s_sleep(2);
+        }
+    }
+}
+
 template <bool FOUR>
-__device__ __forceinline__ void move_body(const nc_paged_evict_args &a, uint32_t r, uint32_t column, uint32_t keep, uint32_t first) {
-    constexpr uint32_t AT_ONCE = 8;
+__device__ __forceinline__ void move_chunk(const nc_paged_evict_args &a, uint32_t r, uint32_t chain, uint32_t chunk, uint32_t keep, uint32_t first,
+                                           uint32_t *read) {
+    constexpr uint32_t ROWS = NC_PAGED4_MOVE_ROWS;
     constexpr uint32_t UE = FOUR ? 32 : 8;  // values of a unit
-    const uint32_t lane = threadIdx.x & 63u, rows = 64u >> a.slice_log2;
-    const uint32_t slices = a.units >> a.slice_log2, slice = column % slices, head = column / slices >> 1, v = column / slices & 1u;
-    const uint64_t base = head * a.head_stride + UE * ((slice << a.slice_log2) + (lane & ((1u << a.slice_log2) - 1u)));
+    const uint32_t tid = threadIdx.x, at_once = NC_PAGED4_MOVE_THREADS >> a.row_log2;
+    const uint32_t v = chain & 1u, unit = tid & ((1u << a.row_log2) - 1u);
+    const uint32_t head = ((chain >> 1) << (a.row_log2 - a.unit_log2)) + (unit >> a.unit_log2);
+    const uint64_t base = head * a.head_stride + UE * (unit & ((1u << a.unit_log2) - 1u));
     uint8_t *codes = v ? a.v : a.k, *scales = v ? a.v_scales : a.k_scales;
     const int32_t *row = a.table + r * a.table_stride, *source = a.source + (uint64_t)r * a.max_tokens;
-    const uint32_t num_slots = a.num_pages * a.ps.d;
-    // Source slots and the places' pages of a batch's rows; of the next one they are on their way while this one's rows are.
-    uint32_t slot[AT_ONCE], page[AT_ONCE];
-    auto look = [&](uint32_t j0) {
+    const uint32_t num_slots = a.num_pages * a.ps.d, j0 = first + chunk * (ROWS * at_once) + (tid >> a.row_log2);
+    uint32_t slot[ROWS], page[ROWS];
 #pragma unroll
-        for (uint32_t i = 0; i < AT_ONCE; ++i) {
-            const uint32_t j = j0 + i * rows + (lane >> a.slice_log2), jj = min(j, keep - 1u);
-            slot[i] = j < keep ? (uint32_t)source[jj] : ~0u;
-            page[i] = (uint32_t)row[nc_paged_quot(jj, a.ps)];
-        }
-    };
-    look(first);
-    for (uint32_t j0 = first; j0 < keep; j0 += AT_ONCE * rows) {
-        u32x4 x[AT_ONCE];
-        uint32_t s[AT_ONCE];
-        uint64_t to[AT_ONCE];
-        bool in[AT_ONCE];
-#pragma unroll
-        for (uint32_t i = 0; i < AT_ONCE; ++i) {
-            const uint32_t j = min(j0 + i * rows + (lane >> a.slice_log2), keep - 1u), tok = j - nc_paged_quot(j, a.ps) * a.ps.d;
-            in[i] = slot[i] < num_slots && page[i] < a.num_pages;
-            const uint32_t from = in[i] ? slot[i] : 0u, p = nc_paged_quot(from, a.ps);
-            const uint64_t src = p * a.page_stride + (from - p * a.ps.d) * a.token_stride + base;
-            to[i] = page[i] * a.page_stride + tok * a.token_stride + base;
-            x[i] = *reinterpret_cast<const u32x4 *>(codes + (FOUR ? src / 2 : src * 2));
-            if constexpr (FOUR) s[i] = scales[src / 32];
-        }
-        look(j0 + AT_ONCE * rows);
-        // all of the batch's rows have arrived before the first is stored
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-#pragma unroll
-        for (uint32_t i = 0; i < AT_ONCE; ++i)
-            if (in[i]) {
-                *reinterpret_cast<u32x4 *>(codes + (FOUR ? to[i] / 2 : to[i] * 2)) = x[i];
-                if constexpr (FOUR) scales[to[i] / 32] = (uint8_t)s[i];
-            }
+    for (uint32_t i = 0; i < ROWS; ++i) {
+        const uint32_t j = j0 + i * at_once, jj = min(j, keep - 1u);
+        slot[i] = j < keep ? (uint32_t)source[jj] : ~0u;
+        page[i] = (uint32_t)row[nc_paged_quot(jj, a.ps)];
     }
+    u32x4 x[ROWS];
+    uint32_t s[ROWS];
+    bool in[ROWS];
+#pragma unroll
+    for (uint32_t i = 0; i < ROWS; ++i) {
+        in[i] = slot[i] < num_slots && page[i] < a.num_pages;
+        const uint32_t from = in[i] ? slot[i] : 0u, p = nc_paged_quot(from, a.ps);
+        const uint64_t src = p * a.page_stride + (from - p * a.ps.d) * a.token_stride + base;
+        x[i] = *reinterpret_cast<const u32x4 *>(codes + (FOUR ? src / 2 : src * 2));
+        if constexpr (FOUR) s[i] = scales[src / 32];
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (a.chunks > 1) {
+        if (tid == 0) __hip_atomic_store(read + chunk, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (chunk) {
+            if (tid < 64) wait_for_chunks(read, chunk);
+            __syncthreads();
+        }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < ROWS; ++i)
+        if (in[i]) {
+            const uint32_t j = j0 + i * at_once, tok = j - nc_paged_quot(j, a.ps) * a.ps.d;
+            const uint64_t to = page[i] * a.page_stride + tok * a.token_stride + base;
+            *reinterpret_cast<u32x4 *>(codes + (FOUR ? to / 2 : to * 2)) = x[i];
+            if constexpr (FOUR) scales[to / 32] = (uint8_t)s[i];
+        }
 }
 
 }  // namespace
 
-extern "C" __global__ __launch_bounds__(256) void nc_paged4_move(const nc_paged_evict_args a) {
-    const uint32_t column = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (uint32_t r = blockIdx.y; r < a.num_seqs; r += gridDim.y) {
-        const uint32_t keep = (uint32_t)a.news[r], old = (uint32_t)a.olds[r], first = (uint32_t)a.first[r];
-        if (blockIdx.x == gridDim.x - 1u) {  // what else the selection left
-            if (threadIdx.x == 0) a.kept_lens[r] = (int32_t)keep;
-            if (r == 0 && threadIdx.x < 4) a.counts[threadIdx.x] = a.totals[threadIdx.x];
+extern "C" __global__ __launch_bounds__(NC_PAGED4_MOVE_THREADS) void nc_paged4_move(const nc_paged_evict_args a) {
+    __shared__ uint32_t s_chunk;
+    const uint32_t cuts = (uint32_t)as_const(a.totals)[1];
+    if (blockIdx.x < a.mass_wgs) {  // what else the selection left
+        if (blockIdx.x == 0 && threadIdx.x < 4) a.counts[threadIdx.x] = a.totals[threadIdx.x];
+        for (uint32_t r = blockIdx.x * NC_PAGED4_MOVE_THREADS + threadIdx.x; r < a.num_seqs; r += a.mass_wgs * NC_PAGED4_MOVE_THREADS) a.kept_lens[r] = a.news[r];
+        for (uint64_t p = blockIdx.x; p < (uint64_t)cuts * a.mass_parts; p += a.mass_wgs) {
+            const uint32_t k = (uint32_t)(p / a.mass_parts), r = (uint32_t)as_const(a.cuts)[k];
+            const uint32_t keep = (uint32_t)as_const(a.news)[r], old = (uint32_t)as_const(a.olds)[r], first = (uint32_t)as_const(a.first)[r];
+            const uint32_t lo = (uint32_t)(p - (uint64_t)k * a.mass_parts) * NC_PAGED4_MASS_PART, end = min(lo + NC_PAGED4_MASS_PART, old);
             float *mass = a.mass + r * a.mass_stride;
             const float *kept = a.kept_mass + (uint64_t)r * a.max_tokens;
-            if (keep < old)
-                for (uint32_t t = first + threadIdx.x; t < old; t += blockDim.x) mass[t] = t < keep ? kept[t] : 0.f;
-        } else if (column < a.waves && keep < old && first < keep) {
+            for (uint32_t t = lo + threadIdx.x; t < end; t += NC_PAGED4_MOVE_THREADS)
+                if (t >= first) mass[t] = t < keep ? kept[t] : 0.f;
+        }
+        return;
+    }
+    const uint32_t b = blockIdx.x - a.mass_wgs, all = cuts * a.chains;
+    for (uint32_t q = b % a.side_chains; q < all; q += a.side_chains) {
+        const uint32_t k = q / a.chains, chain = q - k * a.chains, r = (uint32_t)as_const(a.cuts)[k];
+        const uint32_t keep = (uint32_t)as_const(a.news)[r], first = (uint32_t)as_const(a.first)[r], size = nc_paged4_chunk(a.row_log2);
+        const uint32_t chunks = (keep - first + size - 1u) / size;
+        const uint64_t at = (uint64_t)r * a.chains + chain;
+        while (true) {
+            uint32_t chunk = 0;
+            if (a.chunks > 1) {
+                if (threadIdx.x == 0) s_chunk = __hip_atomic_fetch_add(a.taken + at, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __syncthreads();
+                chunk = __builtin_amdgcn_readfirstlane(s_chunk);
+                __syncthreads();
+            }
+            if (chunk >= chunks) break;
             if (a.four)
-                move_body<true>(a, r, column, keep, first);
+                move_chunk<true>(a, r, chain, chunk, keep, first, a.read + at * a.chunks);
             else
-                move_body<false>(a, r, column, keep, first);
+                move_chunk<false>(a, r, chain, chunk, keep, first, a.read + at * a.chunks);
+            if (a.side_chunks >= a.chunks) break;  // every chunk has a workgroup
         }
     }
 }

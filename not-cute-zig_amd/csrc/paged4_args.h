@@ -38,21 +38,34 @@ struct nc_paged_mass_args {
 };
 
 // Eviction. The selection leaves, by request, its new length, the first place that another token's row moves to, the source slot
-// of every place of the new length and that token's mass.
+// of every place of the new length and that token's mass; which requests are cut; and the move's counts and flags at 0.
+//
+// The move's work is counted in chunks: NC_PAGED4_MOVE_ROWS rows a thread of 1 << row_log2 16-byte units each, of one chain: K or V of
+// one request's head (or of a few that are next to each other).
 struct nc_paged_evict_args {
     const int32_t *table, *seq_lens, *cursor;
     float *mass;
     int32_t *free_pages, *kept_lens, *counts;
     uint8_t *k, *v, *k_scales, *v_scales;
     int32_t *news, *olds, *first, *totals; // workspace: by request; totals: cursor, requests cut, pages, tokens
+    int32_t *cuts;                         // the requests that are cut
+    uint32_t *taken, *read;                // by chain: chunks taken, and by chunk whether its rows have been read
     int32_t *source;                       // num_seqs rows of max_tokens
     float *kept_mass;                      // the same
     uint64_t table_stride, mass_stride, page_stride, head_stride, token_stride;
     uint32_t num_seqs, num_pages, max_tokens, free_len;
     uint32_t limit, budget, sinks, recent;
-    uint32_t units, slice_log2, waves; // 16-byte units of a row, log2 of those of a wave, waves that move a request's rows
+    uint32_t unit_log2, row_log2;          // log2 of a head's 16-byte units (4 bits: of 32 values, and their scale), and of a chain's
+    uint32_t chains, chunks;               // chains of a request, most chunks of one
+    uint32_t mass_wgs, mass_parts;         // workgroups that move masses, their parts of a request
+    uint32_t side_chains, side_chunks;     // workgroups that move rows: side_chunks for each of side_chains chains at a time
     uint32_t four;
     nc_paged_div ps;
 };
+#define NC_PAGED4_MOVE_THREADS 256u
+#define NC_PAGED4_MOVE_ROWS 8u
+#define NC_PAGED4_MASS_PART 2048u // masses that a workgroup moves at a time
+// Rows of a chunk.
+NC_HD uint32_t nc_paged4_chunk(uint32_t row_log2) { return NC_PAGED4_MOVE_ROWS * (NC_PAGED4_MOVE_THREADS >> row_log2); }
 
 #endif

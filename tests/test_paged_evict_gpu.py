@@ -79,6 +79,11 @@ CASES = [  # lens, limit, budget, sinks, recent, masses, four, heads, d, page si
     ([20000, 30, 12345], 5000, 5000, 4, 1000, "ties", True, 1, 32, 16, "nhd"), ([17000], 16384, 16000, 0, 0, "close", False, 1, 16, 64, "hnd"),
     ([40] * 1100, 39, 20, 2, 5, "exp", False, 1, 16, 16, "hnd"), ([0, 0, 0], 5, 5, 0, 0, "exp", False, 1, 16, 16, "hnd"),
     ([12000], 2, 1, 0, 0, "odd", False, 1, 16, 16, "hnd"), ([700, 650, 3], 600, 599, 0, 0, "exp", True, 5, 128, 16, "nhd"),
+    # rows moved by several workgroups each: by one place, most of them, with others' heads, chains in turn, chunks in turn
+    ([3000, 5, 2999], 2998, 2998, 0, 0, "zeros", False, 2, 128, 16, "hnd"), ([6000, 5999], 5999, 5998, 1, 0, "exp", True, 3, 128, 7, "nhd"),
+    ([3000, 1700], 1699, 1000, 0, 900, "exp", False, 4, 32, 16, "nhd"), ([5000], 4000, 3000, 8, 8, "ties", True, 8, 32, 16, "nhd"),
+    ([5000, 4100], 4000, 3900, 8, 8, "exp", True, 6, 64, 16, "nhd"), ([4000], 3999, 3998, 0, 0, "exp", False, 12, 16, 5, "nhd"),
+    ([1300] * 150, 1299, 1200, 0, 10, "exp", False, 8, 16, 16, "hnd"), ([1000], 990, 950, 3, 10, "exp", False, 300, 128, 16, "nhd"),
 ]
 
 
