@@ -16,11 +16,12 @@ namespace {
 #define NC_MASS_NAMES(D) \
     "nc_paged4_mass_d" #D, "nc_paged4_mass_d" #D "_bf16", "nc_paged4_mass_d" #D "_odd", "nc_paged4_mass_d" #D "_odd_bf16"
 const char *const kKernels[] = {
-    "nc_paged4_append", "nc_paged4_read", "nc_paged4_weights", "nc_paged4_select", "nc_paged4_select_short", "nc_paged4_move",
+    "nc_paged4_append", "nc_paged4_read", "nc_paged4_weights", "nc_paged4_select", "nc_paged4_select_short", "nc_paged4_part_first",
+    "nc_paged4_part_second", "nc_paged4_part_third", "nc_paged4_part_list", "nc_paged4_move",
     NC_DECODE4_ALL(32), NC_DECODE4_ALL(64), NC_DECODE4_ALL(128), NC_MASS_NAMES(16), NC_MASS_NAMES(32),
     NC_MASS_NAMES(64),  NC_MASS_NAMES(128),
 };
-enum : uint32_t { kAppend, kRead, kWeights, kSelect, kSelectShort, kMove, kDecode4, kMass = kDecode4 + 3 * 12 };
+enum : uint32_t { kAppend, kRead, kWeights, kSelect, kSelectShort, kPartFirst, kMove = kPartFirst + 4, kDecode4, kMass = kDecode4 + 3 * 12 };
 static_assert(sizeof kKernels / sizeof kKernels[0] == NC_PAGED4_KERNELS, "one place per kernel");
 
 int launch(nc_module module, uint32_t kernel, uint32_t grid, uint32_t grid_y, uint32_t threads, void *args, nc_stream stream) {
@@ -148,8 +149,12 @@ void more_args(const DecodePlan &plan, const DecodeTensors &t, nc_paged_more_arg
 
 // Offsets of the eviction's workspace.
 struct EvictSpace {
-    uint64_t news, olds, first, cuts, taken, read, source, kept_mass, bytes;
+    uint64_t news, olds, first, cuts, taken, read, states, lows, counts, source, kept_mass, bytes;
+    uint64_t parts, part;  // 0: one workgroup a request
 };
+// A table of so many tokens is selected from by parts, unless the requests are so many that this is too many workgroups.
+constexpr uint64_t kLongTable = 12288, kMostPartWgs = 1u << 16;
+
 EvictSpace evict_space(const Shape &s) {
     const uint64_t seqs = 4 * ((s.o.num_seqs + 3) / 4 * 4), tokens = 4 * s.o.num_seqs * s.o.max_pages * s.o.page_size;
     EvictSpace e;
@@ -161,9 +166,17 @@ EvictSpace evict_space(const Shape &s) {
     const uint64_t chains = 2 * s.o.num_kv_heads, chunks = s.o.max_pages * s.o.page_size * (s.o.head_dim / 8) / (NC_PAGED4_MOVE_ROWS * NC_PAGED4_MOVE_THREADS) + 1;
     e.taken = e.cuts + seqs;
     e.read = e.taken + (4 * s.o.num_seqs * chains + 15) / 16 * 16;
-    e.source = e.read + (4 * s.o.num_seqs * chains * chunks + 15) / 16 * 16;
+    e.states = e.read + (4 * s.o.num_seqs * chains * chunks + 15) / 16 * 16;
+    const uint64_t width = s.o.max_pages * s.o.page_size;
+    e.part = std::max<uint64_t>(2048, (width + 2048 * NC_PAGED4_MOST_PARTS - 1) / (2048 * NC_PAGED4_MOST_PARTS) * 2048);
+    e.parts = (width + e.part - 1) / e.part;
+    if (width < kLongTable || s.o.num_seqs * (e.parts + 1) > kMostPartWgs) e.parts = 0;
+    e.lows = e.states + (e.parts ? 32 * s.o.num_seqs : 0);
+    e.counts = e.lows + (8 * s.o.num_seqs * e.parts + 15) / 16 * 16;
+    e.source = e.counts + 4 * s.o.num_seqs * e.parts * NC_PAGED4_BINS;
+    // the second pass's counts have the place of what is listed later
     e.kept_mass = e.source + (tokens + 15) / 16 * 16;
-    e.bytes = e.kept_mass + tokens;
+    e.bytes = e.kept_mass + std::max(tokens, 4 * s.o.num_seqs * e.parts * NC_PAGED4_BINS);
     return e;
 }
 
@@ -218,6 +231,12 @@ int evict(nc_module module, const nc_paged_evict_lists &t, const nc_paged_evict_
     a.cuts = reinterpret_cast<int32_t *>(work + space.cuts);
     a.taken = reinterpret_cast<uint32_t *>(work + space.taken);
     a.read = reinterpret_cast<uint32_t *>(work + space.read);
+    a.states = reinterpret_cast<uint32_t *>(work + space.states);
+    a.lows = reinterpret_cast<uint32_t *>(work + space.lows);
+    a.counts1 = reinterpret_cast<uint32_t *>(work + space.counts);
+    a.counts2 = reinterpret_cast<uint32_t *>(work + space.kept_mass);
+    a.parts = (uint32_t)space.parts;
+    a.part = (uint32_t)space.part;
     a.source = reinterpret_cast<int32_t *>(work + space.source);
     a.kept_mass = reinterpret_cast<float *>(work + space.kept_mass);
     a.table_stride = o.table_stride;
@@ -254,7 +273,12 @@ int evict(nc_module module, const nc_paged_evict_lists &t, const nc_paged_evict_
     a.mass_wgs = (uint32_t)std::min<uint64_t>(o.num_seqs * a.mass_parts, 512);
     // a short table's requests are a few waves' work
     const bool small = a.max_tokens <= 2048;
-    st = launch(module, small ? kSelectShort : kSelect, (uint32_t)o.num_seqs, 1, small ? 512 : 1024, &a, stream);
+    if (a.parts) {
+        for (uint32_t pass = 0; pass < 4 && !st; ++pass)
+            st = launch(module, kPartFirst + pass, (uint32_t)o.num_seqs * (a.parts + (pass == 0 ? 1 : 0)), 1, 512, &a, stream);
+    } else {
+        st = launch(module, small ? kSelectShort : kSelect, (uint32_t)o.num_seqs, 1, small ? 512 : 1024, &a, stream);
+    }
     if (st) return st;
     return launch(module, kMove, a.mass_wgs + (chunks ? a.side_chunks * a.side_chains : 0), 1, NC_PAGED4_MOVE_THREADS, &a, stream);
 }

@@ -183,17 +183,223 @@ __device__ __forceinline__ uint32_t lanes_below(uint64_t who) {
 // The mass of an order.
 __device__ __forceinline__ float mass_of(uint32_t order) { return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order); }
 
-// HELD: tokens that a lane keeps, and of others reads at once.
+// What is kept of the tokens that are neither first nor last: all masses above `edge` (all_nan: no such), and the first `ties` tokens
+// of that mass.
+struct Edge {
+    float edge;
+    uint32_t ties;
+    bool all_nan;
+};
+// From the bits of orders down to `shift`: `whole`, all of those with these bits are kept, so that the edge is the order below
+// the least of them; else all bits are known, and `left` of those are kept. Orders that no mass has: below 0's, whose mass would be -0, and
+// between infinity's and NaN's. (Below -infinity's the mass is a NaN, above which is everything.)
+__device__ __forceinline__ Edge edge_of(uint32_t prefix, int shift, bool whole, uint32_t left) {
+    uint32_t order = prefix;
+    if (whole) {
+        order = prefix << shift;
+        order -= order != 0u;
+        order = order == 0x7fffffffu ? 0x7ffffffeu : min(order, 0xff800000u);
+    }
+    return {mass_of(order), whole ? 0u : left, order == 0xffffffffu};
+}
+
+constexpr uint32_t kBins = NC_PAGED4_BINS;
+
+// A workgroup's tokens of a request, begin..end-1 of them a wave's. HELD: tokens that a lane keeps, and of others reads at once.
+template <uint32_t WAVES, uint32_t HELD>
+struct Tokens {
+    static constexpr uint32_t THREADS = 64 * WAVES;
+    static constexpr uint32_t EACH = kBins / THREADS;  // bins of a thread
+    // Equal masses are LDS additions to one address, one after the other: every bin COPIES times, a lane to its own. (60001 tokens of
+    // few different masses, by one workgroup: 59 us with one.)
+    static constexpr uint32_t COPIES = WAVES == 16 ? 8 : 2;
+
+    const nc_paged_evict_args &a;
+    const uint32_t r, n, tid, lane, w, lo, hi, need;
+    const float *mass;
+    const int32_t *row;
+    uint32_t begin, end;
+    float held_mass[HELD];
+    uint32_t held_page[HELD];
+
+    __device__ __forceinline__ Tokens(const nc_paged_evict_args &args, uint32_t request, uint32_t len, uint32_t wave)
+        : a(args), r(request), n(len), tid(threadIdx.x), lane(threadIdx.x & 63u), w(wave), lo(args.sinks), hi(len - args.recent),
+          need(args.budget - args.sinks - args.recent), mass(args.mass + request * args.mass_stride), row(args.table + request * args.table_stride) {}
+
+    // Those of `from`..`from + 64 * WAVES * x - 1` that there are, shared out among the waves.
+    __device__ __forceinline__ void take(uint32_t from, uint32_t tokens, bool there, bool pages) {
+        const uint32_t part = (tokens + 64u * WAVES - 1u) / (64u * WAVES) * 64u, stop = min(from + tokens, n);
+        begin = min(from + w * part, stop);
+        end = min(begin + part, stop);
+#pragma unroll
+        for (uint32_t i = 0; i < HELD; ++i) {
+            const uint32_t t = begin + 64u * i + lane;
+            held_mass[i] = there && t < end ? mass[t] : 0.f;
+            held_page[i] = there && pages && t < end ? (uint32_t)row[nc_paged_quot(t, a.ps)] : 0u;
+        }
+    }
+
+    // fn(64 neighbours' first place, the lane's mass) for all of the wave's tokens; those that are not in registers so many read at once.
+    template <class F>
+    __device__ __forceinline__ void each(F &&fn) const {
+#pragma unroll
+        for (uint32_t i = 0; i < HELD; ++i)
+            if (begin + 64u * i < end) fn(begin + 64u * i, held_mass[i]);
+        for (uint32_t t0 = begin + 64u * HELD; t0 < end; t0 += 64u * HELD) {
+            float x[HELD];
+#pragma unroll
+            for (uint32_t i = 0; i < HELD; ++i) x[i] = t0 + 64u * i + lane < end ? mass[t0 + 64u * i + lane] : 0.f;
+#pragma unroll
+            for (uint32_t i = 0; i < HELD; ++i)
+                if (t0 + 64u * i < end) fn(t0 + 64u * i, x[i]);
+        }
+    }
+
+    // Sums over the waves' numbers: of all of them, or of those before this one.
+    __device__ __forceinline__ uint32_t sum_of(const uint32_t *sums, uint32_t waves) const {
+        const uint32_t scan = wave_scan32(lane < waves ? sums[lane] : 0u);
+        return (uint32_t)__builtin_amdgcn_readlane(scan, 63);
+    }
+
+    // Counts, by `bits` bits from `shift` on, of the orders that have `prefix` above those.
+    __device__ __forceinline__ void count(uint32_t *bins, uint32_t prefix, int shift, int bits) const {
+        for (uint32_t i = tid; i < kBins * COPIES; i += THREADS) bins[i] = 0;
+        lds_barrier();
+        each([&](uint32_t t0, float x) {
+            const uint32_t t = t0 + lane, k = order_of(x);
+            const bool mine = t >= lo && t < hi && t < end && (shift == 21 || k >> (shift + bits) == prefix);
+            const uint32_t bin = k >> shift & ((1u << bits) - 1u);
+            if (mine) atomicAdd(&bins[bin * COPIES + lane % COPIES], 1u);
+        });
+        lds_barrier();
+    }
+    // Bin 2047 - EACH * tid - i.
+    __device__ __forceinline__ uint32_t bin_of(const uint32_t *bins, uint32_t i) const {
+        uint32_t sum = 0;
+#pragma unroll
+        for (uint32_t x = 0; x < COPIES; ++x) sum += bins[(kBins - 1u - EACH * tid - i) * COPIES + x];
+        return sum;
+    }
+
+    // Pages that become free: to the list, behind those of the requests before this one; which requests are cut, and the totals.
+    __device__ __forceinline__ void sums(bool cut, uint32_t keep, uint32_t (*s_sums)[WAVES]) const {
+        if (cut && a.chunks > 1) {
+            for (uint32_t i = tid; i < a.chains; i += THREADS) a.taken[(uint64_t)r * a.chains + i] = 0;
+            for (uint32_t i = tid; i < a.chains * a.chunks; i += THREADS) a.read[(uint64_t)r * a.chains * a.chunks + i] = 0;
+        }
+        uint32_t x[5] = {0, 0, 0, 0, 0};  // pages of all, and of those before this one; requests cut, and before; tokens
+        for (uint32_t q = tid; q < a.num_seqs; q += THREADS) {
+            const uint32_t m = nc_paged_cut(a.seq_lens[q], a.max_tokens);
+            if (m > a.limit) {
+                const uint32_t f = pages_of(m, a.ps) - pages_of(a.budget, a.ps);
+                x[0] += f;
+                x[1] += q < r ? f : 0u;
+                x[2] += 1u;
+                x[3] += q < r ? 1u : 0u;
+                x[4] += m - a.budget;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+            x[i] = wave_scan32(x[i]);
+            if (lane == 63) s_sums[i][w] = x[i];
+        }
+        lds_barrier();
+#pragma unroll
+        for (int i = 0; i < 5; ++i) x[i] = sum_of(s_sums[i], WAVES);
+        const int64_t base = (int64_t)a.cursor[0] - x[0];
+        if (r == 0 && tid == 0) {
+            a.totals[0] = (int32_t)max(base, (int64_t)0);
+            a.totals[1] = (int32_t)x[2];
+            a.totals[2] = (int32_t)x[0];
+            a.totals[3] = (int32_t)x[4];
+        }
+        if (!cut) return;
+        if (tid == 0) a.cuts[x[3]] = (int32_t)r;
+        const uint32_t held = pages_of(n, a.ps), stay = pages_of(keep, a.ps);
+        for (uint32_t p = stay + tid; p < held; p += THREADS) {
+            const int64_t at = base + x[1] + (p - stay);
+            if (at >= 0 && at < (int64_t)a.free_len) a.free_pages[at] = row[p];
+        }
+    }
+
+    // Lists the tokens that stay, behind `sure` that stay for sure and `last` of the edge's mass. The least that goes.
+    __device__ __forceinline__ uint32_t list(const Edge &e, uint32_t sure, uint32_t last, uint32_t *s_a, uint32_t *s_b) const {
+        // Which of 64 neighbours stay for sure, and which have the edge's mass. (A NaN is above every number.)
+        auto sure_of = [&](uint32_t t0, float x) {
+            const bool above = !e.all_nan && !(x <= e.edge);
+            if (t0 >= lo && t0 + 64u <= hi) return __ballot(above);
+            const uint32_t t = t0 + lane;
+            return __ballot(t < end && (t < lo || t >= hi || above));
+        };
+        auto last_of = [&](uint32_t t0, float x) {
+            const bool equal = e.all_nan ? x != x : x == e.edge;
+            const uint32_t t = t0 + lane;
+            return t0 >= lo && t0 + 64u <= hi ? __ballot(equal) : __ballot(equal && t >= lo && t < hi && t < end);
+        };
+        uint32_t ws = 0, wl = 0;
+        each([&](uint32_t t0, float x) {
+            ws += __builtin_popcountll(sure_of(t0, x));
+            if (e.ties) wl += __builtin_popcountll(last_of(t0, x));
+        });
+        lds_barrier();
+        if (lane == 0) {
+            s_a[w] = ws;
+            s_b[w] = wl;
+        }
+        lds_barrier();
+        sure += sum_of(s_a, w);
+        last += sum_of(s_b, w);
+        int32_t *source = a.source + (uint64_t)r * a.max_tokens;
+        float *kept = a.kept_mass + (uint64_t)r * a.max_tokens;
+        uint32_t gone = n;
+        // The place in its page of the lane's token of 64 neighbours, who are listed one after the other.
+        const uint32_t at64 = nc_paged_quot(64u, a.ps), tok64 = 64u - at64 * a.ps.d;
+        uint32_t tok = begin + lane - nc_paged_quot(begin + lane, a.ps) * a.ps.d;
+        auto put = [&](uint32_t t0, float x, uint32_t page) {
+            const uint32_t t = t0 + lane;
+            const uint64_t who = sure_of(t0, x), tie = e.ties ? last_of(t0, x) : 0ull;
+            const uint32_t nl = last + lanes_below(tie), to = sure + lanes_below(who) + min(nl, e.ties);
+            const bool stays = who >> lane & 1ull || (tie >> lane & 1ull && nl < e.ties);
+            if (stays) {
+                source[to] = page < a.num_pages ? (int32_t)(page * a.ps.d + tok) : -1;
+                kept[to] = x;
+            } else if (t < end) {
+                gone = min(gone, t);
+            }
+            tok += tok64;
+            tok -= tok >= a.ps.d ? a.ps.d : 0u;
+            sure += __builtin_popcountll(who);
+            last += __builtin_popcountll(tie);
+        };
+#pragma unroll
+        for (uint32_t i = 0; i < HELD; ++i)
+            if (begin + 64u * i < end) put(begin + 64u * i, held_mass[i], held_page[i]);
+        for (uint32_t t0 = begin + 64u * HELD; t0 < end; t0 += 64u * HELD) {
+            float x[HELD];
+            uint32_t page[HELD];
+#pragma unroll
+            for (uint32_t i = 0; i < HELD; ++i) {
+                const uint32_t t = min(t0 + 64u * i + lane, n - 1u);
+                x[i] = mass[t];
+                page[i] = (uint32_t)row[nc_paged_quot(t, a.ps)];
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < HELD; ++i)
+                if (t0 + 64u * i < end) put(t0 + 64u * i, x[i], page[i]);
+        }
+        return gone;
+    }
+};
+
+// All of a request by one workgroup.
 template <uint32_t WAVES, uint32_t HELD>
 __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
-    constexpr uint32_t EACH = 2048 / (64 * WAVES);  // bins of a thread
-    // Equal masses are LDS additions to one address, one after the other: every bin COPIES times, a lane to its own. (60001 tokens of
-    // few different masses 59 us with one.)
-    constexpr uint32_t COPIES = WAVES == 16 ? 8 : 2;
-    __shared__ uint32_t s_bins[2048 * COPIES];
-    __shared__ uint32_t s_a[WAVES], s_b[WAVES], s_c[WAVES], s_d[WAVES], s_e[WAVES];
+    using T = Tokens<WAVES, HELD>;
+    __shared__ uint32_t s_bins[kBins * T::COPIES];
+    __shared__ uint32_t s_sums[5][WAVES];
     __shared__ uint32_t s_bin, s_above, s_count, s_first;
-    const uint32_t r = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t r = blockIdx.x, tid = threadIdx.x;
     const uint32_t n = nc_paged_cut(as_const(a.seq_lens)[r], a.max_tokens);
     const bool cut = n > a.limit;
     const uint32_t keep = cut ? a.budget : n;
@@ -203,127 +409,28 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
         s_first = n;
     }
     if (!cut && r != 0) return;
-    if (cut && a.chunks > 1) {
-        for (uint32_t i = tid; i < a.chains; i += 64 * WAVES) a.taken[(uint64_t)r * a.chains + i] = 0;
-        for (uint32_t i = tid; i < a.chains * a.chunks; i += 64 * WAVES) a.read[(uint64_t)r * a.chains * a.chunks + i] = 0;
-    }
-
-    // The wave's tokens.
-    const float *mass = a.mass + r * a.mass_stride;
-    const uint32_t lo = a.sinks, hi = n - a.recent, need = a.budget - a.sinks - a.recent;
-    const uint32_t part = (n + 64u * WAVES - 1u) / (64u * WAVES) * 64u, begin = min(w * part, n), end = min(begin + part, n);
-    const int32_t *row = a.table + r * a.table_stride;
-    float held_mass[HELD];
-    uint32_t held_page[HELD];
-#pragma unroll
-    for (uint32_t i = 0; i < HELD; ++i) {
-        const uint32_t t = begin + 64u * i + lane;
-        held_mass[i] = cut && t < end ? mass[t] : 0.f;
-        held_page[i] = cut && t < end ? (uint32_t)row[nc_paged_quot(t, a.ps)] : 0u;
-    }
-
-    // Pages that become free: of all requests, and of those before this one.
-    uint32_t all = 0, before = 0, cuts = 0, cuts_before = 0, dropped = 0;
-    for (uint32_t q = tid; q < a.num_seqs; q += blockDim.x) {
-        const uint32_t m = nc_paged_cut(a.seq_lens[q], a.max_tokens);
-        if (m > a.limit) {
-            const uint32_t f = pages_of(m, a.ps) - pages_of(a.budget, a.ps);
-            all += f;
-            before += q < r ? f : 0u;
-            cuts += 1u;
-            cuts_before += q < r ? 1u : 0u;
-            dropped += m - a.budget;
-        }
-    }
-    all = wave_scan32(all);
-    before = wave_scan32(before);
-    cuts = wave_scan32(cuts);
-    cuts_before = wave_scan32(cuts_before);
-    dropped = wave_scan32(dropped);
-    if (lane == 63) {
-        s_a[w] = all;
-        s_b[w] = before;
-        s_c[w] = cuts;
-        s_d[w] = dropped;
-        s_e[w] = cuts_before;
-    }
-    lds_barrier();
-    // Sums over the waves, in a lane of each: of all of them, or of those before this one.
-    auto sum_of = [&](const uint32_t *sums, uint32_t waves) {
-        const uint32_t scan = wave_scan32(lane < waves ? sums[lane] : 0u);
-        return (uint32_t)__builtin_amdgcn_readlane(scan, 63);
-    };
-    all = sum_of(s_a, WAVES);
-    before = sum_of(s_b, WAVES);
-    cuts = sum_of(s_c, WAVES);
-    dropped = sum_of(s_d, WAVES);
-    const int64_t base = (int64_t)a.cursor[0] - all;
-    if (r == 0 && tid == 0) {
-        a.totals[0] = (int32_t)max(base, (int64_t)0);
-        a.totals[1] = (int32_t)cuts;
-        a.totals[2] = (int32_t)all;
-        a.totals[3] = (int32_t)dropped;
-    }
+    T x(a, r, n, __builtin_amdgcn_readfirstlane(tid >> 6));
+    x.take(0, n, cut, true);
+    x.sums(cut, keep, s_sums);
     if (!cut) return;
-    cuts_before = sum_of(s_e, WAVES);
-    if (tid == 0) a.cuts[cuts_before] = (int32_t)r;
-    const uint32_t held = pages_of(n, a.ps), stay = pages_of(keep, a.ps);
-    for (uint32_t p = stay + tid; p < held; p += blockDim.x) {
-        const int64_t at = base + before + (p - stay);
-        if (at >= 0 && at < (int64_t)a.free_len) a.free_pages[at] = row[p];
-    }
-
-    // fn(64 neighbours' first place, the lane's mass) for all of the wave's tokens that are not in registers, so many read at once
-    auto rest = [&](auto &&fn) {
-        for (uint32_t t0 = begin + 64u * HELD; t0 < end; t0 += 64u * HELD) {
-            float x[HELD];
-#pragma unroll
-            for (uint32_t i = 0; i < HELD; ++i) x[i] = t0 + 64u * i + lane < end ? mass[t0 + 64u * i + lane] : 0.f;
-#pragma unroll
-            for (uint32_t i = 0; i < HELD; ++i)
-                if (t0 + 64u * i < end) fn(t0 + 64u * i, x[i]);
-        }
-    };
-    auto each = [&](auto &&fn) {
-#pragma unroll
-        for (uint32_t i = 0; i < HELD; ++i)
-            if (begin + 64u * i < end) fn(begin + 64u * i, held_mass[i]);
-        rest(fn);
-    };
-    // All masses above `edge` are kept (all_nan: no such), and the first `ties` tokens of that mass.
-    float edge = __builtin_inff();
-    uint32_t ties = 0;
-    bool all_nan = true;
-    if (need) {
-        uint32_t prefix = 0, left = need;  // the bits above the present ones, kept tokens that agree in them
+    Edge e = {__builtin_inff(), 0u, true};
+    if (x.need) {
+        uint32_t prefix = 0, left = x.need;  // the bits above the present ones, kept tokens that agree in them
         for (int shift = 21, bits = 11;;) {
-            for (uint32_t i = tid; i < 2048 * COPIES; i += 64 * WAVES) s_bins[i] = 0;
-            lds_barrier();
-            each([&](uint32_t t0, float x) {
-                const uint32_t t = t0 + lane, k = order_of(x);
-                const bool mine = t >= lo && t < hi && t < end && (shift == 21 || k >> (shift + bits) == prefix);
-                const uint32_t bin = k >> shift & ((1u << bits) - 1u);
-                if (mine) atomicAdd(&s_bins[bin * COPIES + lane % COPIES], 1u);
-            });
-            lds_barrier();
+            x.count(s_bins, prefix, shift, bits);
             // Bins from the top, EACH a thread; the one that the last token to be kept is in.
-            uint32_t bin[EACH], mine = 0;
+            uint32_t bin[T::EACH], mine = 0;
 #pragma unroll
-            for (uint32_t i = 0; i < EACH; ++i) {
-                bin[i] = 0;
-#pragma unroll
-                for (uint32_t x = 0; x < COPIES; ++x) bin[i] += s_bins[(2047u - EACH * tid - i) * COPIES + x];
-                mine += bin[i];
-            }
+            for (uint32_t i = 0; i < T::EACH; ++i) mine += bin[i] = x.bin_of(s_bins, i);
             const uint32_t incl = wave_scan32(mine);
-            if (lane == 63) s_a[w] = incl;
+            if (x.lane == 63) s_sums[0][x.w] = incl;
             lds_barrier();
-            uint32_t above = incl - mine + sum_of(s_a, w);
+            uint32_t above = incl - mine + x.sum_of(s_sums[0], x.w);
             if (above < left && left <= above + mine) {
 #pragma unroll
-                for (uint32_t i = 0; i < EACH; ++i) {
+                for (uint32_t i = 0; i < T::EACH; ++i) {
                     if (above < left && left <= above + bin[i]) {
-                        s_bin = 2047u - EACH * tid - i;
+                        s_bin = kBins - 1u - T::EACH * tid - i;
                         s_above = above;
                         s_count = bin[i];
                     }
@@ -334,18 +441,7 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
             prefix = prefix << bits | s_bin;
             left -= s_above;
             if (s_count == left || shift == 0) {
-                // The whole bin, so that the edge is the order below its least one; or all the bits of an order, and its first ones.
-                // Orders that no mass has: below 0's, whose mass would be -0, and between infinity's and NaN's. (Below -infinity's the
-                // mass is a NaN, above which is everything.)
-                uint32_t order = prefix;
-                if (s_count == left) {
-                    order = prefix << shift;
-                    order -= order != 0u;
-                    order = order == 0x7fffffffu ? 0x7ffffffeu : min(order, 0xff800000u);
-                }
-                ties = s_count == left ? 0u : left;
-                all_nan = order == 0xffffffffu;
-                edge = mass_of(order);
+                e = edge_of(prefix, shift, s_count == left, left);
                 break;
             }
             bits = shift == 21 ? 11 : 10;
@@ -353,78 +449,130 @@ __device__ __forceinline__ void select_body(const nc_paged_evict_args &a) {
             lds_barrier();
         }
     }
-    // Which of 64 neighbours stay for sure, and which have the edge's mass. (A NaN is above every number.)
-    auto sure_of = [&](uint32_t t0, float x) {
-        const bool above = !all_nan && !(x <= edge);
-        if (t0 >= lo && t0 + 64u <= hi) return __ballot(above);
-        const uint32_t t = t0 + lane;
-        return __ballot(t < end && (t < lo || t >= hi || above));
-    };
-    auto last_of = [&](uint32_t t0, float x) {
-        const bool equal = all_nan ? x != x : x == edge;
-        const uint32_t t = t0 + lane;
-        return t0 >= lo && t0 + 64u <= hi ? __ballot(equal) : __ballot(equal && t >= lo && t < hi && t < end);
-    };
-    uint32_t sure = 0, last = 0;
-    each([&](uint32_t t0, float x) {
-        sure += __builtin_popcountll(sure_of(t0, x));
-        if (ties) last += __builtin_popcountll(last_of(t0, x));
-    });
-    lds_barrier();
-    if (lane == 0) {
-        s_a[w] = sure;
-        s_b[w] = last;
-    }
-    lds_barrier();
-    sure = sum_of(s_a, w);
-    last = sum_of(s_b, w);
-    int32_t *source = a.source + (uint64_t)r * a.max_tokens;
-    float *kept = a.kept_mass + (uint64_t)r * a.max_tokens;
-    uint32_t gone = n;
-    // The place in its page of the lane's token of 64 neighbours, who are listed one after the other.
-    const uint32_t at64 = nc_paged_quot(64u, a.ps), tok64 = 64u - at64 * a.ps.d;
-    uint32_t tok = begin + lane - nc_paged_quot(begin + lane, a.ps) * a.ps.d;
-    auto list = [&](uint32_t t0, float x, uint32_t page) {
-        const uint32_t t = t0 + lane;
-        const uint64_t ws = sure_of(t0, x), wl = ties ? last_of(t0, x) : 0ull;
-        const uint32_t nl = last + lanes_below(wl), to = sure + lanes_below(ws) + min(nl, ties);
-        const bool stays = ws >> lane & 1ull || (wl >> lane & 1ull && nl < ties);
-        if (stays) {
-            source[to] = page < a.num_pages ? (int32_t)(page * a.ps.d + tok) : -1;
-            kept[to] = x;
-        } else if (t < end) {
-            gone = min(gone, t);
-        }
-        tok += tok64;
-        tok -= tok >= a.ps.d ? a.ps.d : 0u;
-        sure += __builtin_popcountll(ws);
-        last += __builtin_popcountll(wl);
-    };
-#pragma unroll
-    for (uint32_t i = 0; i < HELD; ++i)
-        if (begin + 64u * i < end) list(begin + 64u * i, held_mass[i], held_page[i]);
-    for (uint32_t t0 = begin + 64u * HELD; t0 < end; t0 += 64u * HELD) {
-        float x[HELD];
-        uint32_t page[HELD];
-#pragma unroll
-        for (uint32_t i = 0; i < HELD; ++i) {
-            const uint32_t t = min(t0 + 64u * i + lane, n - 1u);
-            x[i] = mass[t];
-            page[i] = (uint32_t)row[nc_paged_quot(t, a.ps)];
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < HELD; ++i)
-            if (t0 + 64u * i < end) list(t0 + 64u * i, x[i], page[i]);
-    }
+    const uint32_t gone = x.list(e, 0, 0, s_sums[0], s_sums[1]);
     if (gone < n) atomicMin(&s_first, gone);
     lds_barrier();
     if (tid == 0) a.first[r] = (int32_t)s_first;
+}
+
+// A long request by several workgroups, `part` tokens each, in four launches: three that count, and one that lists. Each part leaves its
+// counts, and every workgroup of the next launch adds up all of the request's (64 parts at most), and those before its own, which says
+// where what it lists begins.
+constexpr uint32_t PART_WAVES = 8, PART_HELD = 4;
+
+// What a launch has found: the bits so far, kept tokens among those that agree in them, and whether that is all of them (`whole`, at
+// `shift`).
+struct PartState {
+    uint32_t prefix, left, whole, shift;
+};
+
+template <int PASS>
+__device__ __forceinline__ void part_body(const nc_paged_evict_args &a) {
+    using T = Tokens<PART_WAVES, PART_HELD>;
+    static_assert(T::EACH == 4, "a thread's bins are one load");
+    __shared__ uint32_t s_bins[PASS < 4 ? kBins * T::COPIES : 1];
+    __shared__ uint32_t s_sums[5][PART_WAVES];
+    __shared__ uint32_t s_bin, s_above, s_count, s_low, s_low_at, s_first;
+    const uint32_t wgs = a.parts + (PASS == 1), r = blockIdx.x / wgs, p = blockIdx.x - r * wgs, tid = threadIdx.x;
+    const uint32_t n = nc_paged_cut(as_const(a.seq_lens)[r], a.max_tokens);
+    const bool cut = n > a.limit;
+    T x(a, r, n, __builtin_amdgcn_readfirstlane(tid >> 6));
+    if (PASS == 1 && p == a.parts) {  // beside the parts'
+        const uint32_t keep = cut ? a.budget : n;
+        if (tid == 0) {
+            a.news[r] = (int32_t)keep;
+            a.olds[r] = (int32_t)n;
+            a.first[r] = (int32_t)n;
+        }
+        if (cut || r == 0) x.sums(cut, keep, s_sums);
+        return;
+    }
+    const uint32_t from = p * a.part;
+    if (!cut || from >= n || (PASS < 4 && !x.need)) return;
+    x.take(from, a.part, true, PASS == 4);
+    const uint32_t parts = (n - 1u) / a.part + 1u;
+    PartState *states = reinterpret_cast<PartState *>(a.states) + 2 * (uint64_t)r;  // of passes 2 and 3
+    uint32_t *lows = a.lows + 2 * ((uint64_t)r * a.parts + p);                       // kept ones in the parts before this one
+    // Passes 1 and 3 leave their counts in one place, pass 2 in another.
+    auto counts_of = [&](int pass) { return (pass == 2 ? a.counts2 : a.counts1) + (uint64_t)r * a.parts * kBins; };
+
+    PartState state = {0u, x.need, 0u, 21u};
+    uint32_t low = 0, low_at = 0;
+    if (PASS > 2 && x.need) {
+        state = states[PASS > 2 ? PASS - 3 : 0];
+        low = lows[PASS > 2 ? PASS - 3 : 0];
+    }
+    if (PASS > 1 && x.need && !state.whole) {
+        const uint32_t *counts = counts_of(PASS - 1);
+        u32x4 all = {0u, 0u, 0u, 0u}, before = all;  // bins 2044 - 4 tid.., of all parts and of those before this one
+        const uint32_t at = kBins - 4u - 4u * tid;
+#pragma unroll 8
+        for (uint32_t q = 0; q < parts; ++q) {
+            const u32x4 y = *reinterpret_cast<const u32x4 *>(counts + (uint64_t)q * kBins + at);
+            all += y;
+            if (q < p) before += y;
+        }
+        const uint32_t mine = all[0] + all[1] + all[2] + all[3], mine_low = before[0] + before[1] + before[2] + before[3];
+        const uint32_t incl = wave_scan32(mine), incl_low = wave_scan32(mine_low);
+        if (x.lane == 63) {
+            s_sums[0][x.w] = incl;
+            s_sums[1][x.w] = incl_low;
+        }
+        lds_barrier();
+        uint32_t above = incl - mine + x.sum_of(s_sums[0], x.w), lower = incl_low - mine_low + x.sum_of(s_sums[1], x.w);
+        if (above < state.left && state.left <= above + mine) {
+#pragma unroll
+            for (int i = 3; i >= 0; --i) {
+                if (above < state.left && state.left <= above + all[i]) {
+                    s_bin = at + i;
+                    s_above = above;
+                    s_count = all[i];
+                    s_low = lower;
+                    s_low_at = before[i];
+                }
+                above += all[i];
+                lower += before[i];
+            }
+        }
+        lds_barrier();
+        state.shift = PASS == 2 ? 21u : PASS == 3 ? 10u : 0u;
+        state.prefix = state.prefix << (PASS == 4 ? 10 : 11) | s_bin;
+        state.left -= s_above;
+        state.whole = s_count == state.left;
+        low += s_low + (state.whole ? s_low_at : 0u);
+        low_at = state.whole ? 0u : s_low_at;
+    }
+    if constexpr (PASS < 4) {
+        if constexpr (PASS > 1) {
+            if (tid == 0) {
+                if (p == 0) states[PASS - 2] = state;
+                lows[PASS - 2] = low;
+            }
+            if (state.whole) return;
+        }
+        x.count(s_bins, state.prefix, PASS == 1 ? 21 : PASS == 2 ? 10 : 0, PASS == 3 ? 10 : 11);
+        u32x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = x.bin_of(s_bins, 3 - i);
+        *reinterpret_cast<u32x4 *>(counts_of(PASS) + (uint64_t)p * kBins + kBins - 4u - 4u * tid) = y;
+    } else {
+        const Edge e = x.need ? edge_of(state.prefix, (int)state.shift, state.whole, state.left) : Edge{__builtin_inff(), 0u, true};
+        if (tid == 0) s_first = n;
+        const uint32_t gone = x.list(e, low + min(from, x.lo) + (from > x.hi ? from - x.hi : 0u), low_at, s_sums[2], s_sums[3]);
+        if (gone < n) atomicMin(&s_first, gone);
+        lds_barrier();
+        if (tid == 0 && s_first < n) atomicMin(reinterpret_cast<uint32_t *>(a.first) + r, s_first);
+    }
 }
 
 }  // namespace
 
 extern "C" __global__ __launch_bounds__(1024) void nc_paged4_select(const nc_paged_evict_args a) { select_body<16, 8>(a); }
 extern "C" __global__ __launch_bounds__(512) void nc_paged4_select_short(const nc_paged_evict_args a) { select_body<8, 2>(a); }
+extern "C" __global__ __launch_bounds__(64 * PART_WAVES) void nc_paged4_part_first(const nc_paged_evict_args a) { part_body<1>(a); }
+extern "C" __global__ __launch_bounds__(64 * PART_WAVES) void nc_paged4_part_second(const nc_paged_evict_args a) { part_body<2>(a); }
+extern "C" __global__ __launch_bounds__(64 * PART_WAVES) void nc_paged4_part_third(const nc_paged_evict_args a) { part_body<3>(a); }
+extern "C" __global__ __launch_bounds__(64 * PART_WAVES) void nc_paged4_part_list(const nc_paged_evict_args a) { part_body<4>(a); }
 
 // The rows that stay, to the front, in place and all at once. A chunk's workgroup reads its rows, says so, and stores them when the
 // chunks before it in the chain have been read: a place holds a row that goes to itself or to a place before it. Chunks are

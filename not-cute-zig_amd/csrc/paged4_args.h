@@ -50,6 +50,8 @@ struct nc_paged_evict_args {
     int32_t *news, *olds, *first, *totals; // workspace: by request; totals: cursor, requests cut, pages, tokens
     int32_t *cuts;                         // the requests that are cut
     uint32_t *taken, *read;                // by chain: chunks taken, and by chunk whether its rows have been read
+    uint32_t *states, *lows;               // of a selection by parts: by request and pass, and by part
+    uint32_t *counts1, *counts2;           // by part, NC_PAGED4_BINS each
     int32_t *source;                       // num_seqs rows of max_tokens
     float *kept_mass;                      // the same
     uint64_t table_stride, mass_stride, page_stride, head_stride, token_stride;
@@ -57,11 +59,14 @@ struct nc_paged_evict_args {
     uint32_t limit, budget, sinks, recent;
     uint32_t unit_log2, row_log2;          // log2 of a head's 16-byte units (4 bits: of 32 values, and their scale), and of a chain's
     uint32_t chains, chunks;               // chains of a request, most chunks of one
+    uint32_t parts, part;                  // parts of a request at most, and their tokens
     uint32_t mass_wgs, mass_parts;         // workgroups that move masses, their parts of a request
     uint32_t side_chains, side_chunks;     // workgroups that move rows: side_chunks for each of side_chains chains at a time
     uint32_t four;
     nc_paged_div ps;
 };
+#define NC_PAGED4_BINS 2048u
+#define NC_PAGED4_MOST_PARTS 64u
 #define NC_PAGED4_MOVE_THREADS 256u
 #define NC_PAGED4_MOVE_ROWS 8u
 #define NC_PAGED4_MASS_PART 2048u // masses that a workgroup moves at a time

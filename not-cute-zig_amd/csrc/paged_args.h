@@ -27,7 +27,7 @@ NC_HD uint32_t nc_paged_quot(uint32_t n, nc_paged_div v) {
 }
 
 #define NC_PAGED_KERNELS 53u  // kernels of paged.hip
-#define NC_PAGED4_KERNELS 58u // and of paged4.hip
+#define NC_PAGED4_KERNELS 62u // and of paged4.hip
 
 struct nc_paged_build_args {
     const int32_t *cached, *fresh, *free_pages, *cursor;

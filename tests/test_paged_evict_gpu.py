@@ -84,6 +84,10 @@ CASES = [  # lens, limit, budget, sinks, recent, masses, four, heads, d, page si
     ([3000, 1700], 1699, 1000, 0, 900, "exp", False, 4, 32, 16, "nhd"), ([5000], 4000, 3000, 8, 8, "ties", True, 8, 32, 16, "nhd"),
     ([5000, 4100], 4000, 3900, 8, 8, "exp", True, 6, 64, 16, "nhd"), ([4000], 3999, 3998, 0, 0, "exp", False, 12, 16, 5, "nhd"),
     ([1300] * 150, 1299, 1200, 0, 10, "exp", False, 8, 16, 16, "hnd"), ([1000], 990, 950, 3, 10, "exp", False, 300, 128, 16, "nhd"),
+    # selected from by several workgroups: nothing to choose, parts of more than a sweep, the edge in each of the passes, empty parts
+    ([13000, 12300, 10], 8000, 5000, 2000, 3000, "exp", False, 1, 16, 64, "hnd"), ([140001, 70000], 60000, 50000, 7, 100, "close", False, 1, 16, 64, "hnd"),
+    ([140001], 60000, 59999, 0, 0, "zeros", False, 1, 16, 64, "hnd"), ([30000, 9000, 2049], 2048, 2047, 2047, 0, "odd", False, 1, 16, 24, "nhd"),
+    ([16384, 8193, 100], 4000, 2100, 2050, 1, "odd", True, 1, 32, 16, "hnd"), ([12288, 4096, 4097], 4095, 2000, 0, 1999, "ties", False, 1, 16, 16, "hnd"),
 ]
 
 
