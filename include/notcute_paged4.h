@@ -141,7 +141,7 @@ typedef struct nc_paged_evict_rules {
  * (NC_ERROR_INVALID_VALUE). A page of a request that is cut belongs to it alone: rows of pages that two requests share, or that one lists
  * twice, may be moved in any order. A row on a page outside the pool is not moved, nor is one moved there. Lengths in elements as for the
  * other calls; counts_len >= 4, cursor_len >= 1; workspace 16-byte aligned, nc_paged_evict_workspace_bytes, which need not be
- * cleared. At most 2^20 requests (NC_ERROR_OVERFLOW). */
+ * cleared; calls that overlap in time need workspaces of their own. At most 2^20 requests (NC_ERROR_OVERFLOW). */
 typedef struct nc_paged_evict_lists {
     const int32_t *block_table;
     uint64_t table_len;

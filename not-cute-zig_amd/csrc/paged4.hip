@@ -361,10 +361,10 @@ struct Tokens {
             const uint64_t who = sure_of(t0, x), tie = e.ties ? last_of(t0, x) : 0ull;
             const uint32_t nl = last + lanes_below(tie), to = sure + lanes_below(who) + min(nl, e.ties);
             const bool stays = who >> lane & 1ull || (tie >> lane & 1ull && nl < e.ties);
-            if (stays) {
+            if (stays && to < a.budget) {  // as it is, unless something changes the masses meanwhile
                 source[to] = page < a.num_pages ? (int32_t)(page * a.ps.d + tok) : -1;
                 kept[to] = x;
-            } else if (t < end) {
+            } else if (!stays && t < end) {
                 gone = min(gone, t);
             }
             tok += tok64;
@@ -584,8 +584,8 @@ namespace {
 __device__ __forceinline__ void wait_for_chunks(const uint32_t *read, uint32_t chunk) {
     const uint32_t lane = threadIdx.x & 63u;
     for (uint32_t c0 = 0; c0 < chunk; c0 += 64) {
-        // The count ends the wait where the workspace was not this call's alone.
-        for (uint32_t tries = 0; tries < 1u << 20; ++tries) {
+        // The count, some tenth of a second, ends the wait where the workspace was not this call's alone.
+        for (uint32_t tries = 0; tries < 1u << 16; ++tries) {
             const bool there = c0 + lane >= chunk || __hip_atomic_load(read + c0 + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0u;
             if (__all(there)) break;
             __builtin_amdgcn_s_sleep(2);
@@ -644,29 +644,43 @@ __device__ __forceinline__ void move_chunk(const nc_paged_evict_args &a, uint32_
 
 }  // namespace
 
+// What the selection left of the k-th request that is cut. It is held to what there is, so that a workspace that another call
+// changes meanwhile costs a wrong result and nothing else.
+struct Cut {
+    uint32_t r, old, keep, first;
+};
+__device__ __forceinline__ Cut cut_of(const nc_paged_evict_args &a, uint32_t k) {
+    Cut c;
+    c.r = min((uint32_t)as_const(a.cuts)[k], a.num_seqs - 1u);
+    c.old = min((uint32_t)as_const(a.olds)[c.r], a.max_tokens);
+    c.keep = min((uint32_t)as_const(a.news)[c.r], c.old);
+    c.first = min((uint32_t)as_const(a.first)[c.r], c.keep);
+    return c;
+}
+
 extern "C" __global__ __launch_bounds__(NC_PAGED4_MOVE_THREADS) void nc_paged4_move(const nc_paged_evict_args a) {
     __shared__ uint32_t s_chunk;
-    const uint32_t cuts = (uint32_t)as_const(a.totals)[1];
+    const uint32_t cuts = min((uint32_t)as_const(a.totals)[1], a.num_seqs);
     if (blockIdx.x < a.mass_wgs) {  // what else the selection left
         if (blockIdx.x == 0 && threadIdx.x < 4) a.counts[threadIdx.x] = a.totals[threadIdx.x];
         for (uint32_t r = blockIdx.x * NC_PAGED4_MOVE_THREADS + threadIdx.x; r < a.num_seqs; r += a.mass_wgs * NC_PAGED4_MOVE_THREADS) a.kept_lens[r] = a.news[r];
         for (uint64_t p = blockIdx.x; p < (uint64_t)cuts * a.mass_parts; p += a.mass_wgs) {
-            const uint32_t k = (uint32_t)(p / a.mass_parts), r = (uint32_t)as_const(a.cuts)[k];
-            const uint32_t keep = (uint32_t)as_const(a.news)[r], old = (uint32_t)as_const(a.olds)[r], first = (uint32_t)as_const(a.first)[r];
-            const uint32_t lo = (uint32_t)(p - (uint64_t)k * a.mass_parts) * NC_PAGED4_MASS_PART, end = min(lo + NC_PAGED4_MASS_PART, old);
-            float *mass = a.mass + r * a.mass_stride;
-            const float *kept = a.kept_mass + (uint64_t)r * a.max_tokens;
+            const uint32_t k = (uint32_t)(p / a.mass_parts);
+            const Cut c = cut_of(a, k);
+            const uint32_t lo = (uint32_t)(p - (uint64_t)k * a.mass_parts) * NC_PAGED4_MASS_PART, end = min(lo + NC_PAGED4_MASS_PART, c.old);
+            float *mass = a.mass + c.r * a.mass_stride;
+            const float *kept = a.kept_mass + (uint64_t)c.r * a.max_tokens;
             for (uint32_t t = lo + threadIdx.x; t < end; t += NC_PAGED4_MOVE_THREADS)
-                if (t >= first) mass[t] = t < keep ? kept[t] : 0.f;
+                if (t >= c.first) mass[t] = t < c.keep ? kept[t] : 0.f;
         }
         return;
     }
     const uint32_t b = blockIdx.x - a.mass_wgs, all = cuts * a.chains;
     for (uint32_t q = b % a.side_chains; q < all; q += a.side_chains) {
-        const uint32_t k = q / a.chains, chain = q - k * a.chains, r = (uint32_t)as_const(a.cuts)[k];
-        const uint32_t keep = (uint32_t)as_const(a.news)[r], first = (uint32_t)as_const(a.first)[r], size = nc_paged4_chunk(a.row_log2);
-        const uint32_t chunks = (keep - first + size - 1u) / size;
-        const uint64_t at = (uint64_t)r * a.chains + chain;
+        const uint32_t k = q / a.chains, chain = q - k * a.chains, size = nc_paged4_chunk(a.row_log2);
+        const Cut c = cut_of(a, k);
+        const uint32_t chunks = min((c.keep - c.first + size - 1u) / size, a.chunks);
+        const uint64_t at = (uint64_t)c.r * a.chains + chain;
         while (true) {
             uint32_t chunk = 0;
             if (a.chunks > 1) {
@@ -677,9 +691,9 @@ extern "C" __global__ __launch_bounds__(NC_PAGED4_MOVE_THREADS) void nc_paged4_m
             }
             if (chunk >= chunks) break;
             if (a.four)
-                move_chunk<true>(a, r, chain, chunk, keep, first, a.read + at * a.chunks);
+                move_chunk<true>(a, c.r, chain, chunk, c.keep, c.first, a.read + at * a.chunks);
             else
-                move_chunk<false>(a, r, chain, chunk, keep, first, a.read + at * a.chunks);
+                move_chunk<false>(a, c.r, chain, chunk, c.keep, c.first, a.read + at * a.chunks);
             if (a.side_chunks >= a.chunks) break;  // every chunk has a workgroup
         }
     }
