@@ -11,7 +11,7 @@
  * An extension: the reference has no cache. Conventions and options are those of notcute_paged.h, whose block tables
  * (nc_paged_build) serve both kinds of cache. Every call may be captured into a HIP graph; nc_paged_decode_mass,
  * nc_paged4_decode with a mass and the evictions are two launches (of tables for 12288 tokens and more five), the others one. The first of these calls through a module
- * loads their kernels (about 1.4 ms, once).
+ * loads their kernels (about 2.5 ms, once).
  *
  * A cache in 4 bits. K and V are each a pool of codes, two values a byte (the value of the even place in the low half), and a
  * pool of scales, a byte for every 32 values of a row (the microscaling format MXFP4: e2m1 values, e8m0 scales). A code is a

@@ -29,8 +29,8 @@ struct nc_function_st {
 struct nc_module_st {
     hipModule_t mod = nullptr;
     // The embedded module's second and third code objects (the paged cache's kernels and the smaller cache's), each loaded onto
-    // the module's device when the first of its kernels is asked for: it takes 1.2-1.4 ms, which a program without a cache need
-    // not wait for (the module's own 3.1-4.9). Guarded by `lock`; device is -1 in a module from other data, which has none.
+    // the module's device when the first of its kernels is asked for: it takes 1.2-1.4 ms and 2.5, which a program without a
+    // cache need not wait for (the module's own 3.1-4.9). Guarded by `lock`; device is -1 in a module from other data, which has none.
     hipModule_t paged = nullptr, paged4 = nullptr;
     int device = -1;
     std::atomic<nc_function> paged_functions[NC_PAGED_KERNELS + NC_PAGED4_KERNELS] = {};  // their functions, once looked up

@@ -152,7 +152,8 @@ struct EvictSpace {
     uint64_t news, olds, first, cuts, taken, read, states, lows, counts, source, kept_mass, bytes;
     uint64_t parts, part;  // 0: one workgroup a request
 };
-// A table of so many tokens is selected from by parts, unless the requests are so many that this is too many workgroups.
+// A table of so many tokens is selected from by parts, unless the requests are so many that this is too many workgroups, most of them for
+// requests that are not cut.
 constexpr uint64_t kLongTable = 12288, kMostPartWgs = 1u << 16;
 
 EvictSpace evict_space(const Shape &s) {
@@ -271,7 +272,7 @@ int evict(nc_module module, const nc_paged_evict_lists &t, const nc_paged_evict_
     a.side_chains = (uint32_t)std::min(o.num_seqs * chains, std::max<uint64_t>(1, kMoveWgs / a.side_chunks));
     a.mass_parts = (a.max_tokens + NC_PAGED4_MASS_PART - 1) / NC_PAGED4_MASS_PART;
     a.mass_wgs = (uint32_t)std::min<uint64_t>(o.num_seqs * a.mass_parts, 512);
-    // a short table's requests are a few waves' work
+    // Figures of the three ways are at the kernels. A short table's requests are a few waves' work.
     const bool small = a.max_tokens <= 2048;
     if (a.parts) {
         for (uint32_t pass = 0; pass < 4 && !st; ++pass)
@@ -424,6 +425,8 @@ int nc_paged4_decode(nc_module module, const nc_paged4_decode_buffers *buffers, 
     a.bf = s.o.element_type == NC_ELEMENT_BF16;
     if (mass) more_args(plan, x, &a);
     a.values = s.cache_len;
+    // Column groups: 4, 2 or one. 64 requests of 8000 over 8 heads of 64 with 4 query heads each take 65.7, 70.6 and 75.6 us, with 8 each 69.3
+    // and 76.0 (two groups, one); 16 of 1000 over 8 of 128 14.3, 14.5 and 14.4.
     const uint32_t pack = s.group <= 4 ? 2 : s.group <= 8 ? 1 : 0;
     st = launch(module, kDecode4 + 12 * (plan.size - 1) + 4 * pack + (mass ? 2 : 0) + plan.odd, plan.grid, 1, 64 * NC_PAGED_WAVES, &a, stream);
     return st || !mass ? st : launch_weights(module, s, plan, x, mass->mass, stride, stream);

@@ -1,7 +1,7 @@
 // paged4.hip — kernels of a smaller paged cache for MI355X (gfx950, wave64): rows into pages of 4 bits and back
 // (nc_paged4_append, nc_paged4_read), single-token attention over them (nc_paged4_decode_*), attention that keeps its scores
 // (nc_paged4_mass_*) and the weights by token out of those (nc_paged4_weights), and eviction by them (nc_paged4_select,
-// nc_paged4_move). The interface is described in include/notcute_paged4.h.
+// nc_paged4_part_*, nc_paged4_move). The interface is described in include/notcute_paged4.h.
 
 #include "paged_decode.h"
 
@@ -11,7 +11,10 @@
 // Rows into 4-bit pages: of every 32 values x of a row the scale 2^k, k the least with max |x| <= 7 2^k (then the largest is at
 // most half a step off), and x 2^-k to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign, halves to the even code. Both are
 // exact arithmetic: the sum that finds k is one of integers, the product by a power of two. A thread takes 8 values of K and of V,
-// four neighbouring lanes a group.
+// four neighbouring lanes a group. Rows come in and go out at 16 bytes a lane, codes at 4, and the slots' loads stand beside the rows':
+// what there is to move bounds both. 30000 rows of 8 heads of 64, at odd addresses: append 21 us, 3.7 TB/s, read 14.6 us, 5.3 TB/s (a large
+// copy moves 4.8). One step of 16 requests is two launches' latency, 4.8 us for both. (2 or 4 rows a thread, a head's rows a workgroup,
+// and stores that bypass the caches were slower.)
 // -------------------------------------------------------------------------------------------------
 namespace {
 
@@ -123,7 +126,8 @@ extern "C" __global__ __launch_bounds__(256) void nc_paged4_read(const nc_paged4
 
 // -------------------------------------------------------------------------------------------------
 // Weights by token: mass[r][j] += sum over the query heads of exp2(score - max) / sum, out of the scores that an attention has
-// kept. Four tokens a lane, every fourth head a wave; the waves' sums are added in their order.
+// kept. Four tokens a lane, every fourth head a wave; the waves' sums are added in their order. The scores are in the caches
+// or were on their way out: 5 us for 16 requests of 4096 tokens and 32 heads (8.4 MB), 4.7 for 64 ragged ones.
 // -------------------------------------------------------------------------------------------------
 extern "C" __global__ __launch_bounds__(256) void nc_paged4_weights(const nc_paged_mass_args a) {
     __shared__ float s_sum[4][256];
@@ -153,12 +157,24 @@ extern "C" __global__ __launch_bounds__(256) void nc_paged4_weights(const nc_pag
 }
 
 // -------------------------------------------------------------------------------------------------
-// Eviction. A workgroup a request finds the least mass that is kept by its bits, 11 at a time from the top (a histogram of the
-// masses that agree in the bits above, until all of a bin are kept), and then lists the tokens that stay, in their order. A
-// wave of it has a contiguous part of the tokens and keeps the first of them in registers; of a longer part it reads as many at once
-// again in every pass (one by one, 60001 tokens took 69 us). It is a chain of barriers, loads and LDS additions, and of code that
-// runs once: a short table's requests have 8 waves of 2 tokens a lane (one of 300 tokens, with its move: 9.7 us; 4 waves of 8 11.5,
-// 16 of 8 10.8).
+// Eviction: select, then move. The least mass that is kept is found by its bits, 11 at a time from the top (a histogram of the
+// masses that agree in the bits above, until all of a bin are kept); then the tokens that stay are listed, in their order. Masses are read
+// once into registers as far as they fit, and what is left is a chain of barriers, loads and LDS additions in code that runs once:
+//   by one workgroup a request, of 8 waves with 2 tokens a lane (tables of up to 2048 tokens) or of 16 with 8;
+//   by parts in four launches, for tables of 12288 tokens and more.
+// With the rows' move, in replayed graphs and with fresh masses, over 2 heads of 64, half the tokens kept:
+//   requests x tokens    8 waves   16 waves   parts
+//   1 x 300                 9.6      12.3      15.9 us
+//   1 x 1000               12.4      15.3      18.2
+//   200 x 2000             61.0      63.8      69.5
+//   16 x 4097              26.8      25.6      30.9
+//   1 x 8000               25.4      21.0      21.3
+//   16 x 8000              39.7      34.9      38.0
+//   4 x 16000              52.5      39.3      34.5
+//   100 x 16000             221       207       224 (by parts all the same: more often a few of them are cut)
+//   1 x 60000               143      84.8      45.2
+// What bounds short ones is that chain (6.8 us of selection for 300 tokens, 9 for 200 requests of 1001), long ones the four launches of
+// 5 to 12 us, and large moves the rate of a copy.
 // -------------------------------------------------------------------------------------------------
 namespace {
 
@@ -578,6 +594,8 @@ extern "C" __global__ __launch_bounds__(64 * PART_WAVES) void nc_paged4_part_lis
 // chunks before it in the chain have been read: a place holds a row that goes to itself or to a place before it. Chunks are
 // taken by a count, in their order, and reading waits for nothing, so whoever waits does so for workgroups that run; that needs no
 // order among workgroups, and not all of them at once.
+// 16 requests of 4097 tokens cut to 2048, 8 heads of 128: 60 us, 4.5 TB/s read and written; 200 of 1001 cut to 500 173 us, 4.7 (a large
+// copy: 4.8). (A wave a column that walks down the rows, which needs no flags: 16 requests 85 us, one of 60000 280 instead of 82.)
 namespace {
 
 // A store that is asked for has been seen by whoever reads the flag: waits as in Decode::join().

@@ -76,7 +76,13 @@ NC_HD uint32_t nc_paged_head_parts(uint32_t group) { return (group + 63u) / 64u;
 //   16 of 1000, 8 heads of 128                  17.2  16.5
 //   64 of up to 16000, 4 heads of 64            29.6  28.6
 NC_HD constexpr uint32_t nc_paged_head_units(uint32_t head_dim) { return head_dim <= 32 ? 1u : 2u; }
-// Caches in 4 bits.
+// Caches in 4 bits, with one unit a head and with two:
+//   2 requests of 20000, 8 heads of 64 with 8 query heads each    15.3  16.9 us
+//   118 of up to 2719, 3 heads of 32                              11.4  11.9
+//   96 of 4000, 8 heads of 64 with 8 query heads each             64.9  60.3 (but 64 ragged ones 19.0  18.5)
+//   16 of 4000, 8 heads of 128                                    23.4  21.4
+//   one of 30000, 8 heads of 128                                  19.8  18.0
+//   40 of up to 1500, 8 heads of 128                              12.8  14.9 (200 of up to 500: 26.9  28.1)
 NC_HD constexpr uint32_t nc_paged4_head_units(uint32_t head_dim) { return head_dim <= 64 ? 1u : 2u; }
 // A head of no more blocks than this is not split: the workgroup that has its first unit takes all of it. (Of 1: 118
 // requests of up to 2719, 3 heads of 32, 10.8 -> 11.1 us; of 4: 12.0, and 4 of 500 over 8 heads of 128 7.6 -> 9.4.)

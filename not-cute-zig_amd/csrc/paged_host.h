@@ -180,6 +180,13 @@ inline DecodePlan decode_plan(const Shape &s, bool o_vec, bool four = false, boo
     uint32_t side = 0;
     if ((!mass || four) && (o.head_stride < o.token_stride || o.page_size == 1) && o.max_pages * o.page_size > NC_PAGED_NEXT_TOKENS) {
         const uint64_t numbers = s.group * o.head_dim;  // of one head's piece
+        // 4 bits: rows are a quarter as long, and neighbouring heads' share lines up to heads of 128. Each head for itself, two, four:
+        //   one request of 120001 over 8 heads of 64                 46.0  31.2  32.0 us
+        //   16 of 2000 over 8 heads of 128                           21.9  18.9
+        //   100 of 600 over 32 heads of 64                           121   70    62.6
+        //   64 of up to 16000 over 4 of 64, 8 query heads each       20.0  20.3  25.8 (not taken: wide pieces)
+        //   32 of 4000 over 4 of 64, 8 query heads each, pages of 1  32.9        26.4
+        //   4 of 5000 over 8 of 128, pages of 24                     17.9  20.8       (not taken: addresses by key)
         if (four)
             side = s.group > (o.page_size == 1 ? 8 : 4) ? 0 : o.num_kv_heads % 4 == 0 && o.head_dim <= 64 ? 2 : o.num_kv_heads % 2 == 0 && (o.head_dim <= 64 || uniform) ? 1 : 0;
         else if (o.head_dim <= 32)
