@@ -18,6 +18,8 @@
 // -------------------------------------------------------------------------------------------------
 namespace {
 
+typedef u32x4 __attribute__((aligned(2))) u32x4_loose;  // global memory takes 16 bytes at any alignment
+
 __device__ __forceinline__ u32x4 load_eight(const uint16_t *p) {
     u32x4 r;
     __builtin_memcpy(&r, p, 16);  // one load: global memory takes them at any alignment
@@ -119,8 +121,8 @@ extern "C" __global__ __launch_bounds__(256) void nc_paged4_read(const nc_paged4
             k = values(kq, a.k_scales[p.cache / 32], a.bf);
             v = values(vq, a.v_scales[p.cache / 32], a.bf);
         }
-        __builtin_memcpy(a.k_out + p.row, &k, 16);
-        __builtin_memcpy(a.v_out + p.row, &v, 16);
+        __builtin_nontemporal_store(k, reinterpret_cast<u32x4_loose *>(a.k_out + p.row));
+        __builtin_nontemporal_store(v, reinterpret_cast<u32x4_loose *>(a.v_out + p.row));
     }
 }
 
@@ -655,7 +657,7 @@ __device__ __forceinline__ void move_chunk(const nc_paged_evict_args &a, uint32_
         if (in[i]) {
             const uint32_t j = j0 + i * at_once, tok = j - nc_paged_quot(j, a.ps) * a.ps.d;
             const uint64_t to = page[i] * a.page_stride + tok * a.token_stride + base;
-            *reinterpret_cast<u32x4 *>(codes + (FOUR ? to / 2 : to * 2)) = x[i];
+            __builtin_nontemporal_store(x[i], reinterpret_cast<u32x4 *>(codes + (FOUR ? to / 2 : to * 2)));
             if constexpr (FOUR) scales[to / 32] = (uint8_t)s[i];
         }
 }
