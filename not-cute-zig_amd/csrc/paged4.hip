@@ -12,9 +12,10 @@
 // most half a step off), and x 2^-k to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign, halves to the even code. Both are
 // exact arithmetic: the sum that finds k is one of integers, the product by a power of two. A thread takes 8 values of K and of V,
 // four neighbouring lanes a group. Rows come in and go out at 16 bytes a lane, codes at 4, and the slots' loads stand beside the rows':
-// what there is to move bounds both. 30000 rows of 8 heads of 64, at odd addresses: append 21 us, 3.7 TB/s, read 14.6 us, 5.3 TB/s (a large
-// copy moves 4.8). One step of 16 requests is two launches' latency, 4.8 us for both. (2 or 4 rows a thread, a head's rows a workgroup,
-// and stores that bypass the caches were slower.)
+// what there is to move bounds both. 30000 rows of 8 heads of 64, at odd addresses: append 15.4 us, 5.0 TB/s, read 13.2 us, 5.9 TB/s (a
+// large copy moves 4.8). Rows are stored past the caches, which need the room (14.6 us else, and the append behind it 21); codes, 4
+// bytes a lane, are not (29.2 us for both, 34 with). One step of 16 requests is two launches' latency, 4.8 us for both. (2 or 4 rows a
+// thread, a head's rows a workgroup, and blocks dealt to the XCDs in runs were no faster.)
 // -------------------------------------------------------------------------------------------------
 namespace {
 
@@ -596,8 +597,8 @@ extern "C" __global__ __launch_bounds__(64 * PART_WAVES) void nc_paged4_part_lis
 // chunks before it in the chain have been read: a place holds a row that goes to itself or to a place before it. Chunks are
 // taken by a count, in their order, and reading waits for nothing, so whoever waits does so for workgroups that run; that needs no
 // order among workgroups, and not all of them at once.
-// 16 requests of 4097 tokens cut to 2048, 8 heads of 128: 60 us, 4.5 TB/s read and written; 200 of 1001 cut to 500 173 us, 4.7 (a large
-// copy: 4.8). (A wave a column that walks down the rows, which needs no flags: 16 requests 85 us, one of 60000 280 instead of 82.)
+// Stores go past the caches. 16 requests of 4097 tokens cut to 2048, 8 heads of 128: 52 us, 5.2 TB/s read and written (through the caches
+// 60); with the selection 67.5 us, one of 60000 104. (A wave a column that walks down the rows, which needs no flags: 100 and 346 us.)
 namespace {
 
 // A store that is asked for has been seen by whoever reads the flag: waits as in Decode::join().
