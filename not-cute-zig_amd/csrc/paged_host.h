@@ -186,12 +186,14 @@ inline DecodePlan decode_plan(const Shape &s, bool o_vec, bool four = false, boo
         //   100 of 600 over 32 heads of 64                           121   70    62.6
         //   64 of up to 16000 over 4 of 64, 8 query heads each       20.0  20.3  25.8 (not taken: wide pieces)
         //   32 of 4000 over 4 of 64, 8 query heads each, pages of 1  32.9        26.4
-        //   4 of 5000 over 8 of 128, pages of 24                     17.9  20.8       (not taken: addresses by key)
+        //   4 of 5000 over 8 of 128, pages of 24                     19.1  21.3       (not taken: addresses by key, and few heads)
+        //   16 of 4000 over 8 of 128, pages of 7                     36.2  26.7
+        //   64 of 4000 over 8 of 128, pages of 24                   102.3  80.8       (8 of 2000: 16.0  15.7)
         //   16 of 4000 over 8 of 128, pages of 1                     40.2  29.8  33.5
         //   the same, 8 query heads each                             18.5  22.8  33.0 (not taken)
         if (four) {
-            const bool one = o.page_size == 1, narrow = o.head_dim <= 64;
-            side = s.group > (one && narrow ? 8 : 4) ? 0 : o.num_kv_heads % 4 == 0 && narrow ? 2 : o.num_kv_heads % 2 == 0 && (narrow || uniform || one) ? 1 : 0;
+            const bool narrow = o.head_dim <= 64, pair = narrow || uniform || o.num_seqs * s.heads > 32;
+            side = s.group > (narrow && o.page_size == 1 ? 8 : 4) ? 0 : o.num_kv_heads % 4 == 0 && narrow ? 2 : o.num_kv_heads % 2 == 0 && pair ? 1 : 0;
         }
         else if (o.head_dim <= 32)
             side = o.num_kv_heads % 4 == 0 && numbers <= 64 ? 2 : o.num_kv_heads % 2 == 0 && numbers <= 128 ? 1 : 0;

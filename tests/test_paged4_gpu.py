@@ -137,7 +137,8 @@ SHAPES = [  # lens, kv heads, group, d, page size, layout, type
     ([3000], 4, 4, 64, 16, "nhd", "bf16"), ([3000, 2000], 8, 2, 32, 5, "nhd", "f16"), ([513, 514], 4, 2, 128, 16, "nhd", "f16"),
     ([60] * 90, 8, 2, 64, 16, "hnd", "f16"), ([20] * 300, 8, 1, 32, 7, "hnd", "bf16"), ([30, 0] * 100, 8, 4, 128, 16, "nhd", "bf16"),
     ([12000], 1, 4, 128, 64, "hnd", "f16"), ([700, 3, 1200], 4, 3, 128, 1, "hnd", "f16"), ([900], 6, 4, 128, 1, "nhd", "bf16"),
-    ([800, 100], 4, 8, 64, 1, "nhd", "f16"),
+    ([800, 100], 4, 8, 64, 1, "nhd", "f16"), ([600, 530, 1, 0, 700] * 2, 4, 3, 128, 24, "nhd", "f16"), ([515] * 40, 2, 1, 128, 7, "nhd", "bf16"),
+    ([700, 3, 1200] * 3, 6, 4, 128, 1, "hnd", "f16"),
 ]
 
 
