@@ -425,6 +425,7 @@ int nc_paged4_decode(nc_module module, const nc_paged4_decode_buffers *buffers, 
     a.bf = s.o.element_type == NC_ELEMENT_BF16;
     if (mass) more_args(plan, x, &a);
     a.values = s.cache_len;
+    a.next_least = plan.next_least;
     // Column groups: 4, 2 or one. 64 requests of 8000 over 8 heads of 64 with 4 query heads each take 65.7, 70.6 and 75.6 us, with 8 each 69.3
     // and 76.0 (two groups, one); 16 of 1000 over 8 of 128 14.3, 14.5 and 14.4.
     const uint32_t pack = s.group <= 4 ? 2 : s.group <= 8 ? 1 : 0;

@@ -63,6 +63,14 @@ struct nc_paged_append_args {
 // 128 9.4 and 9.5.
 #define NC_PAGED_WAVES 4u
 #define NC_PAGED_NEXT_TOKENS 512u
+// With 5 to 8 query heads a key head, two neighbouring heads' pieces are as large as 16 query heads': a call over a cache in 4 bits takes
+// neighbouring heads only from so many units on. Each head for itself, and pairs; requests of tokens over 8 heads, 64 query heads:
+//   32 of up to 4000, 64   12.8  14.9 us (fewer units)    64 of 4000, 64      90.4  59.9     one of 120001, 64   49.4  34.0
+//   64 of up to 4000, 64   21.5  17.8                     64 of 4000, 128    99.5  80.9     100 of 600, 64      29.7  22.5
+//   32 of up to 4000, 128  19.6  21.6 (fewer)             16 of 4000, 64      29.1  21.7     4 of 30000, 32      41.5  30.1
+//   4 of 20000, 64         21.2  26.5 and 8 of 16000, 64, 26.4  32.8 (taken all the same: the shares happen to put the heads of the same
+//                          keys on one XCD, which so many tokens to a request and a few more do not)
+#define NC_PAGED4_WIDE_UNITS 1800u
 #define NC_PAGED4_STEP_KEYS 64u // a wave's step over a cache in 4 bits, of any head_dim
 NC_HD uint32_t nc_paged_step_keys(uint32_t head_dim) { return head_dim <= 32 ? 64u : 32u; }
 NC_HD uint32_t nc_paged_wave_shift(uint32_t group) { return group <= 16 ? 0u : group <= 32 ? 1u : 2u; }
@@ -143,6 +151,7 @@ struct nc_paged_more_args {
     uint64_t score_pitch;
     uint64_t values;                    // of a 4-bit pool
     uint32_t bf;                        // Q is bf16
+    uint32_t next_least;                // units that neighbouring heads are for, 4 bits
 };
 
 // The divisor d / 2^side where 2^side divides d: the same multiplier, as 2^(31+shift) / d is.

@@ -1318,7 +1318,8 @@ __device__ __forceinline__ void decode_body() {
     auto *o = reinterpret_cast<float (*)[16][X::OP]>(s_mem);
     if constexpr (FOUR && NEXT) {  // heads each for themselves are neighbouring ones of one
         using Y = Decode<D, BF, UNI, MANY, true, FOUR, MASS, PACK>;
-        const bool next = __ballot(longest > NC_PAGED_NEXT_TOKENS) != 0;
+        const uint32_t units = (uint32_t)__builtin_amdgcn_readlane(wave_scan32(mine), 63) * a->heads.d;
+        const bool next = __ballot(longest > NC_PAGED_NEXT_TOKENS) != 0 && units >= more_of(a)->next_least;
         const uint32_t by = next ? side : 0u;
         Y y{a, lane, w, lane & 15u, lane >> 4, by, Y::WK * (Y::NW >> by), w & ((1u << by) - 1u), w >> by, o, s_ml, &s_word};
         y.run(scale, next ? mine_next : mine, some, len0, zero_len);

@@ -135,7 +135,7 @@ inline uintptr_t address(const void *p) { return reinterpret_cast<uintptr_t>(p);
 // The attention's kernel, grid and workspace for a set of options.
 struct DecodePlan {
     uint32_t size, odd;  // which of the kernels: by head_dim (0 for 16), and for pages that a 16-key tile may pass the end of
-    uint32_t grid, rows, wave_shift, side, many, each_least, long_log2, short_log2;
+    uint32_t grid, rows, wave_shift, side, many, each_least, long_log2, short_log2, next_least;
     uint64_t piece_ml, piece_o, bytes;  // offsets of the partials, and all of the workspace
     uint64_t score_pitch, row_ml, scores;  // of the scores, where they are kept
 };
@@ -178,22 +178,25 @@ inline DecodePlan decode_plan(const Shape &s, bool o_vec, bool four = false, boo
     // Short requests are faster over all waves, so the kernel looks at the lengths (NC_PAGED_NEXT_TOKENS; 0.1 to 0.3 us where it
     // finds them short); where the table has no room for a long one, it need not.
     uint32_t side = 0;
+    p.next_least = 0;
     if ((!mass || four) && (o.head_stride < o.token_stride || o.page_size == 1) && o.max_pages * o.page_size > NC_PAGED_NEXT_TOKENS) {
         const uint64_t numbers = s.group * o.head_dim;  // of one head's piece
         // 4 bits: rows are a quarter as long, and neighbouring heads' share lines up to heads of 128. Each head for itself, two, four:
         //   one request of 120001 over 8 heads of 64                 46.0  31.2  32.0 us
         //   16 of 2000 over 8 heads of 128                           21.9  18.9
         //   100 of 600 over 32 heads of 64                           121   70    62.6
-        //   64 of up to 16000 over 4 of 64, 8 query heads each       20.0  20.3  25.8 (not taken: wide pieces)
         //   32 of 4000 over 4 of 64, 8 query heads each, pages of 1  32.9        26.4
         //   4 of 5000 over 8 of 128, pages of 24                     19.1  21.3       (not taken: addresses by key, and few heads)
         //   16 of 4000 over 8 of 128, pages of 7                     36.2  26.7
         //   64 of 4000 over 8 of 128, pages of 24                   102.3  80.8       (8 of 2000: 16.0  15.7)
         //   16 of 4000 over 8 of 128, pages of 1                     40.2  29.8  33.5
-        //   the same, 8 query heads each                             18.5  22.8  33.0 (not taken)
+        //   the same, 8 query heads each, ragged                     18.5  22.8  33.0
         if (four) {
             const bool narrow = o.head_dim <= 64, pair = narrow || uniform || o.num_seqs * s.heads > 32;
-            side = s.group > (narrow && o.page_size == 1 ? 8 : 4) ? 0 : o.num_kv_heads % 4 == 0 && narrow ? 2 : o.num_kv_heads % 2 == 0 && pair ? 1 : 0;
+            // (wide: only where the lengths say that there is much to read, NC_PAGED4_WIDE_UNITS)
+            const bool wide = s.group > 4 && !(narrow && o.page_size == 1);  // pieces
+            side = s.group > 8 ? 0 : o.num_kv_heads % 4 == 0 && narrow && !wide ? 2 : o.num_kv_heads % 2 == 0 && pair ? 1 : 0;
+            if (wide) p.next_least = NC_PAGED4_WIDE_UNITS;
         }
         else if (o.head_dim <= 32)
             side = o.num_kv_heads % 4 == 0 && numbers <= 64 ? 2 : o.num_kv_heads % 2 == 0 && numbers <= 128 ? 1 : 0;

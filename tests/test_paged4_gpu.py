@@ -138,7 +138,8 @@ SHAPES = [  # lens, kv heads, group, d, page size, layout, type
     ([60] * 90, 8, 2, 64, 16, "hnd", "f16"), ([20] * 300, 8, 1, 32, 7, "hnd", "bf16"), ([30, 0] * 100, 8, 4, 128, 16, "nhd", "bf16"),
     ([12000], 1, 4, 128, 64, "hnd", "f16"), ([700, 3, 1200], 4, 3, 128, 1, "hnd", "f16"), ([900], 6, 4, 128, 1, "nhd", "bf16"),
     ([800, 100], 4, 8, 64, 1, "nhd", "f16"), ([600, 530, 1, 0, 700] * 2, 4, 3, 128, 24, "nhd", "f16"), ([515] * 40, 2, 1, 128, 7, "nhd", "bf16"),
-    ([700, 3, 1200] * 3, 6, 4, 128, 1, "hnd", "f16"),
+    ([700, 3, 1200] * 3, 6, 4, 128, 1, "hnd", "f16"), ([7300, 7600, 600] * 8, 8, 7, 32, 16, "nhd", "f16"),
+    ([15000, 0, 14000, 9] * 2, 8, 8, 64, 16, "nhd", "bf16"), ([14900] * 8, 4, 5, 128, 40, "nhd", "f16"),
 ]
 
 
