@@ -71,6 +71,12 @@ __device__ __forceinline__ uint32_t last_not_above(const uint32_t *s, uint32_t n
 //   64 ragged ones of up to 16000 over 4 heads of 64            28.7   4.3
 //   16 of 1000 over 8 of 128                                    16.4   4.0
 //   one of 100                                                   4.4
+// and in 4 bits (bytes of codes and scales; FOUR below):
+//   96 requests of 8192 over 8 heads of 128, 64 query heads    165 us  5.2 TB/s (VALU 46 % busy)
+//   one of 120001 over 8 heads of 64, token-major               32     2.0      (waits: 7 steps a wave)
+//   16 of 1000 over 8 of 128                                    14.2   1.3
+//   one of 100                                                   5.8
+// Scores kept for the weights by token: 16 of 4096 over 8 of 128, 32 query heads, in 16 bits 59 us (53 without).
 // The short ones are a chain of waits: launch, lengths, table, K and V, O, and for a piece the stores, the count and the
 // others' pieces. More than 64 requests' lengths are read one after the other by a lane (4096 requests: 26 us).
 // -------------------------------------------------------------------------------------------------
