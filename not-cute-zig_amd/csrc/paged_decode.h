@@ -156,11 +156,10 @@ __device__ __forceinline__ float quad_max(float x) {
     auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ __forceinline__ uint32_t quad_max(uint32_t x) {
+// Over the two lanes l, l^16.
+__device__ __forceinline__ uint32_t pair_max(uint32_t x) {
     auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    x = max((uint32_t)a[0], (uint32_t)a[1]);
-    auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    return max((uint32_t)b[0], (uint32_t)b[1]);
+    return max((uint32_t)a[0], (uint32_t)a[1]);
 }
 __device__ __forceinline__ float quad_sum(float x) {
     auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -208,6 +207,8 @@ __device__ __forceinline__ uint32_t pair_of_fours(uint32_t w, float scale, int b
 }
 
 // Four f32 of at most 2 as e4m3 bytes; x becomes 32 times what that leaves, at most 2 again, and exact.
+// Taken kQueryParts times, it leaves what x has below 2^-24, the last part's least step.
+constexpr int kQueryParts = 4;
 __device__ __forceinline__ uint32_t take_eights(float (&x)[4]) {
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
     w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
@@ -220,7 +221,7 @@ __device__ __forceinline__ uint32_t take_eights(float (&x)[4]) {
 }
 
 // FOUR: the cache holds 4-bit values (e2m1) with a scale byte 2^(b - 127) for every 32 of a row. K rows are then the A operand
-// of v_mfma_scale_f32_16x16x128_f8f6f4 as they lie in memory, codes and scales, and Q its B operand as the sum of three
+// of v_mfma_scale_f32_16x16x128_f8f6f4 as they lie in memory, codes and scales, and Q its B operand as the sum of four
 // e4m3 numbers. The product is exact but for f32's rounding as long as those are at most 2: the instruction adds the products of 8
 // neighbours in fixed point, which keeps 13 bits below the largest (with parts of up to 16 the scores were off by 2^-13). V is
 // turned into bf16, which holds every value of a 4-bit cache, and BF is true.
@@ -234,7 +235,7 @@ struct Decode {
     static constexpr int NT = 2 * KT;           // 16-key tiles
     static constexpr uint32_t WK = 32 * KT;     // keys of a wave's step
     static constexpr int E = D / 16;            // dims of a lane in V and O
-    static constexpr int KK = FOUR ? (D == 128 ? 3 : D / 32) : D < 32 ? 1 : D / 32;  // products of a score
+    static constexpr int KK = FOUR ? kQueryParts * D / 128 : D < 32 ? 1 : D / 32;  // products of a score
     static constexpr int KL = FOUR ? 1 : KK;    // loads of a row of K
     static constexpr uint32_t HEAD_UNITS = FOUR ? nc_paged4_head_units(D) : nc_paged_head_units(D);
     static constexpr int KE = D == 16 ? 4 : 8;  // dims of a lane in one product
@@ -357,9 +358,12 @@ struct Decode {
     }
 
     // FOUR: the query's 128 columns are, by 32 that share a scale, D = 128: its dims, once for each part; 64: the dims of parts 0
-    // and 1, then of part 2 and nothing; 32: the dims of parts 0, 1, 2 and nothing. K's are its dims as often. Lane (c, g) holds
+    // and 1, then of parts 2 and 3; 32: the dims of parts 0 to 3. K's are its dims as often. Lane (c, g) holds
     // columns 16g..+15 and 64+16g..+15, and the scale of columns 32g..+31 (hw_probe.hip has the layout). The parts' scale is
-    // the query's largest value's power of two, so what three parts leave is 2^-20 of that at most.
+    // the power of two of the largest value of its 32 dims, so that a large channel takes no bits from the others' dims, and what four
+    // parts leave is 2^-25 of that at most: nothing of an f16 value above 2^-14 of it, or a bf16 value above 2^-17. (Three parts under one
+    // scale for the row left 2^-20 of its largest value: with a channel at 256 times the others, scores were off by 1e-4.) Of heads of
+    // 128 the fourth part is a product more.
     static constexpr int RUNS = D == 128 ? 2 : 1;  // of 16 dims of a lane
     struct RawQ {
         uint32_t w[RUNS][8];
@@ -387,10 +391,11 @@ struct Decode {
         return q;
     }
     __device__ __forceinline__ void split_q8(const RawQ &q) {
-        uint32_t top = 0;
         float f[RUNS][16];
+        uint32_t e[2];  // the exponent of the 32 dims that a run is a half of; 255 where one is not finite: so is the scale then
 #pragma unroll
-        for (int u = 0; u < RUNS; ++u)
+        for (int u = 0; u < RUNS; ++u) {
+            uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const half2v h = __builtin_bit_cast(half2v, q.w[u][i]);
@@ -398,43 +403,50 @@ struct Decode {
                 f[u][2 * i + 1] = q.bf ? __uint_as_float(q.w[u][i] & 0xffff0000u) : (float)h[1];
                 top = max(top, max(__float_as_uint(f[u][2 * i]) & 0x7fffffffu, __float_as_uint(f[u][2 * i + 1]) & 0x7fffffffu));
             }
-        const uint32_t e = max(quad_max(top) >> 23, 30u);  // 255 where Q is not finite: so are all its scores' scales
-        uint32_t part[3][4 * RUNS];
+            // The last part's scale byte is 1 or more; what is smaller than that allows for still has all of bf16's bits.
+            e[u] = max(pair_max(top) >> 23, 1u + 5u * (kQueryParts - 1));
+        }
+        if constexpr (RUNS == 1) e[1] = e[0];
+        // Of a run g = 0, 1 have one 32's exponent and g = 2, 3 the next one's; as scales the four stand one after the other (of fewer dims
+        // the first ones again).
+        const auto half = __builtin_amdgcn_permlane32_swap(e[0], e[1], false, false);
+        const uint32_t base = __builtin_amdgcn_permlane16_swap(half[0], half[1], false, false)[0];
+        uint32_t part[kQueryParts][4 * RUNS];
 #pragma unroll
         for (int u = 0; u < RUNS; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float x[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = __builtin_ldexpf(f[u][4 * i + j], 127 - (int)e);
+                for (int j = 0; j < 4; ++j) x[j] = __builtin_ldexpf(f[u][4 * i + j], 127 - (int)e[u]);
 #pragma unroll
-                for (int n = 0; n < 3; ++n) part[n][4 * u + i] = take_eights(x);
+                for (int n = 0; n < kQueryParts; ++n) part[n][4 * u + i] = take_eights(x);
             }
-        const uint32_t s[3] = {e, e == 255u ? e : e - 5u, e == 255u ? e : e - 10u};
+        auto scale_of = [&](uint32_t n) { return base == 255u ? base : base - 5u * n; };
         if constexpr (D == 128) {
 #pragma unroll
-            for (int n = 0; n < 3; ++n) {
+            for (int n = 0; n < kQueryParts; ++n) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) q8[n][i] = (int)part[n][i];
-                qs[n] = s[n];
+                qs[n] = scale_of(n);
             }
         } else if constexpr (D == 64) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                q8[0][i] = (int)part[0][i];
-                q8[0][4 + i] = (int)part[1][i];
-                q8[1][i] = (int)part[2][i];
-                q8[1][4 + i] = 0;
+            for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    q8[n][i] = (int)part[2 * n][i];
+                    q8[n][4 + i] = (int)part[2 * n + 1][i];
+                }
+                qs[n] = scale_of(2 * n + (g >> 1));
             }
-            qs[0] = g < 2 ? s[0] : s[1];
-            qs[1] = s[2];
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 q8[0][i] = (int)(g < 2 ? part[0][i] : part[1][i]);
-                q8[0][4 + i] = g < 2 ? (int)part[2][i] : 0;
+                q8[0][4 + i] = (int)(g < 2 ? part[2][i] : part[3][i]);
             }
-            qs[0] = g == 0 ? s[0] : g == 1 ? s[1] : s[2];
+            qs[0] = scale_of(g);
         }
     }
 
