@@ -99,8 +99,8 @@ int nc_paged_decode_mass(nc_module module, const nc_paged_decode_buffers *buffer
                          const nc_paged_options *opts, nc_stream stream);
 
 /* nc_paged_decode over a cache in 4 bits. Scores are f32 sums of exact products but for Q: every value of it enters as the sum of
- * four 8-bit numbers, off by at most 2^-25 of the largest of its 32 (dims 0..31, 32..63, ...), and not at all where it is above 2^-14 of
- * that in f16, 2^-17 in bf16. The weights
+ * four 8-bit or five 6-bit numbers, off by at most 2^-25 of the largest of its 32 (dims 0..31, 32..63, ...) or 2^-130, and not at all where it
+ * is above 2^-14 of that in f16, 2^-17 in bf16. The weights
  * enter the product with V as three bf16 parts, as nc_paged_decode's for bf16. A query that is not finite gives NaN, and so do keys
  * that count whose scale byte is 255, in K or in V. A `mass` that is not NULL adds the weights up as nc_paged_decode_mass
  * does. Workspace: nc_paged4_workspace_bytes, with_mass 1 for calls with a mass. */

@@ -9,7 +9,9 @@
 //   nc_probe_ds_read_tr     ds_read_b64_tr_b16: which LDS elements each lane of a 16-lane group gets
 //   nc_probe_permlane32     v_permlane32_swap: the lane-pair exchange used for row max / row sum
 //   nc_probe_mfma_fp4_fp8   v_mfma_scale_f32_16x16x128_f8f6f4, 4-bit rows times 8-bit columns: lane layout and scales
-//   nc_probe_fp4_convert, nc_probe_fp8_convert   rounding of the conversions to and from 4 and 8 bits
+//   nc_probe_mfma_fp4_fp6   the same with 6-bit columns
+//   nc_probe_fp4_convert, nc_probe_fp8_convert, nc_probe_fp8_scaled, nc_probe_fp6_convert   rounding and order of the conversions to
+//                           and from 4, 8 and 6 bits
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -131,5 +133,57 @@ extern "C" __global__ __launch_bounds__(64) void nc_probe_fp8_convert(const floa
         out[3 * i] = (uint32_t)q;
         out[3 * i + 1] = __builtin_bit_cast(uint32_t, (float)y[0]);
         out[3 * i + 2] = __builtin_bit_cast(uint32_t, (float)y[1]);
+    }
+}
+
+// The same product with B in 6 bits (e2m3): lane l supplies values 32 g..+31 of column l % 16, 6 words of codes one after the other from the
+// lowest bit up. b: 16 columns of 4 x 6 words.
+extern "C" __global__ __launch_bounds__(64) void nc_probe_mfma_fp4_fp6(const uint8_t *a, const uint8_t *as_, const uint32_t *b,
+                                                                        const uint8_t *bs, float *d) {
+    const int l = threadIdx.x, c = l % 16, g = l / 16;
+    const i32x4 x = *reinterpret_cast<const i32x4 *>(a + c * 64 + 16 * g);
+    const uint32_t *y = b + (c * 4 + g) * 6;
+    const i32x8 v = {(int)y[0], (int)y[1], (int)y[2], (int)y[3], (int)y[4], (int)y[5], 0, 0};
+    const i32x8 w = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+    floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, v, acc, 4, 2, 0, as_[c * 4 + g], 0, bs[c * 4 + g]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) d[l * 4 + r] = acc[r];
+}
+
+// 32 f32 over a scale to 6 words of e2m3 codes, and those times the scale back: `n` such, one a thread. The first operand's 16 values are the
+// even ones, the second's the odd ones.
+extern "C" __global__ __launch_bounds__(64) void nc_probe_fp6_convert(const float *x, const float *scales, uint32_t *codes, float *back, uint32_t n) {
+    typedef float floatx16 __attribute__((ext_vector_type(16)));
+    for (uint32_t i = threadIdx.x; i < n; i += 64) {
+        floatx16 even, odd;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            even[j] = x[32 * i + 2 * j];
+            odd[j] = x[32 * i + 2 * j + 1];
+        }
+        const auto q = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, scales[i]);
+        const auto y = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(q, scales[i]);
+#pragma unroll
+        for (int j = 0; j < 6; ++j) codes[6 * i + j] = q[j];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) back[32 * i + j] = y[j];
+    }
+}
+
+// Four f32 over a scale to a word of e4m3 bytes, and those times the scale back.
+extern "C" __global__ __launch_bounds__(64) void nc_probe_fp8_scaled(const float *x, const float *scales, uint32_t *codes, float *back, uint32_t n) {
+    typedef short shortx2 __attribute__((ext_vector_type(2)));
+    for (uint32_t i = threadIdx.x; i < n; i += 64) {
+        const float s = scales[i];
+        shortx2 q = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(shortx2{0, 0}, x[4 * i], x[4 * i + 1], s, false);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(q, x[4 * i + 2], x[4 * i + 3], s, true);
+        const uint32_t w = __builtin_bit_cast(uint32_t, q);
+        const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, true);
+        codes[i] = w;
+        back[4 * i] = lo[0];
+        back[4 * i + 1] = lo[1];
+        back[4 * i + 2] = hi[0];
+        back[4 * i + 3] = hi[1];
     }
 }

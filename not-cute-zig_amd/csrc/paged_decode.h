@@ -91,6 +91,11 @@ typedef short short4v __attribute__((ext_vector_type(4)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
+typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
+typedef short shortx2 __attribute__((ext_vector_type(2)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx32 __attribute__((ext_vector_type(32)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 // Memory that no kernel in flight writes, read by scalar loads.
 typedef const __attribute__((address_space(4))) int32_t *const_ints;
@@ -161,6 +166,10 @@ __device__ __forceinline__ uint32_t pair_max(uint32_t x) {
     auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
     return max((uint32_t)a[0], (uint32_t)a[1]);
 }
+__device__ __forceinline__ uint32_t quad_max(uint32_t x) {
+    auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return pair_max(max((uint32_t)b[0], (uint32_t)b[1]));
+}
 __device__ __forceinline__ float quad_sum(float x) {
     auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
@@ -206,24 +215,42 @@ __device__ __forceinline__ uint32_t pair_of_fours(uint32_t w, float scale, int b
     }
 }
 
-// Four f32 of at most 2 as e4m3 bytes; x becomes 32 times what that leaves, at most 2 again, and exact.
-// Taken kQueryParts times, it leaves what x has below 2^-24, the last part's least step.
-constexpr int kQueryParts = 4;
-__device__ __forceinline__ uint32_t take_eights(float (&x)[4]) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
-    x[0] = (x[0] - lo[0]) * 32.f;
-    x[1] = (x[1] - lo[1]) * 32.f;
-    x[2] = (x[2] - hi[0]) * 32.f;
-    x[3] = (x[3] - hi[1]) * 32.f;
-    return (uint32_t)w;
+// Parts of f32 values as small numbers times a power of two. x becomes what that leaves, exactly, which the next part takes with a scale 2^-5
+// of this one (LAST: nothing asks for it). Four values of at most 2 scales as e4m3 bytes:
+template <bool LAST>
+__device__ __forceinline__ uint32_t take_eights(float (&x)[4], float scale) {
+    shortx2 w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(shortx2{0, 0}, x[0], x[1], scale, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x[2], x[3], scale, true);
+    const uint32_t u = __builtin_bit_cast(uint32_t, w);
+    if constexpr (!LAST) {
+        const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(u, scale, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(u, scale, true);
+        x[0] -= lo[0];
+        x[1] -= lo[1];
+        x[2] -= hi[0];
+        x[3] -= hi[1];
+    }
+    return u;
+}
+// 32 values of at most 4 scales, x[i] and y[i] in turn, as e2m3 (eighths below 2, quarters below 4):
+template <bool LAST>
+__device__ __forceinline__ u32x6 take_sixes(floatx16 &x, floatx16 &y, float scale) {
+    const u32x6 w = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(x, y, scale);
+    if constexpr (!LAST) {
+        const floatx32 z = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(w, scale);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            x[i] -= z[2 * i];
+            y[i] -= z[2 * i + 1];
+        }
+    }
+    return w;
 }
 
 // FOUR: the cache holds 4-bit values (e2m1) with a scale byte 2^(b - 127) for every 32 of a row. K rows are then the A operand
-// of v_mfma_scale_f32_16x16x128_f8f6f4 as they lie in memory, codes and scales, and Q its B operand as the sum of four
-// e4m3 numbers. The product is exact but for f32's rounding as long as those are at most 2: the instruction adds the products of 8
-// neighbours in fixed point, which keeps 13 bits below the largest (with parts of up to 16 the scores were off by 2^-13). V is
+// of v_mfma_scale_f32_16x16x128_f8f6f4 as they lie in memory, codes and scales, and Q its B operand as the sum of
+// small numbers, QPARTS each. Products are exact but for f32's rounding: the instruction adds those of 8
+// neighbours in fixed point, which keeps 13 bits below the largest, all that products of e2m3 have, and of e4m3 of at most 2 (of up to 16
+// the scores were off by 2^-13). V is
 // turned into bf16, which holds every value of a 4-bit cache, and BF is true.
 // MASS: every query head's scores are kept, and its maximum and sum, for the weights' kernel.
 // PACK: where a key head has at most 8 or 4 query heads, the 16 columns are 2 or 4 groups of them, each with a maximum, a sum and an
@@ -233,9 +260,16 @@ struct Decode {
     static_assert((BF && D >= 32) || !FOUR, "a 4-bit cache's V is bf16, and a group of 32 is a row's or part of it");
     static constexpr int KT = FOUR ? NC_PAGED4_STEP_KEYS / 32 : D <= 32 ? 2 : 1;  // 32-key tiles of a wave's step
     static constexpr int NT = 2 * KT;           // 16-key tiles
+    // FOUR: parts of Q. Heads of 128 have 6-bit ones, whose products take half the time of 8-bit ones', and whose 32 dims that share a scale
+    // are a lane's. With five of those and with four 8-bit ones: 96 requests of 8192 over 8 heads of 128 169.7 and 173.3 us, 16 of 1000
+    // 14.0 and 14.4. Smaller heads' 8-bit products have columns to spare, and a lane half as much to split: one of 100 over 8 heads of 64 6.04 and
+    // 5.77, 227 of up to 3464 over 8 of 32, whose split leaves room for fewer waves, 37.9 and 29.7.
+    static constexpr bool SIXES = D == 128;
+    static constexpr int QPARTS = SIXES ? 5 : 4;
+    static constexpr int QDIMS = SIXES ? 32 : 16;  // dims of a lane
     static constexpr uint32_t WK = 32 * KT;     // keys of a wave's step
     static constexpr int E = D / 16;            // dims of a lane in V and O
-    static constexpr int KK = FOUR ? kQueryParts * D / 128 : D < 32 ? 1 : D / 32;  // products of a score
+    static constexpr int KK = FOUR ? QPARTS * D / 128 : D < 32 ? 1 : D / 32;  // products of a score
     static constexpr int KL = FOUR ? 1 : KK;    // loads of a row of K
     static constexpr uint32_t HEAD_UNITS = FOUR ? nc_paged4_head_units(D) : nc_paged_head_units(D);
     static constexpr int KE = D == 16 ? 4 : 8;  // dims of a lane in one product
@@ -260,6 +294,7 @@ struct Decode {
     static constexpr int PARTS = BF ? 3 : 2;
     using KReg = typename std::conditional<D == 16, u32x2, u32x4>::type;
     using VReg = typename std::conditional<FOUR || E <= 2, uint32_t, typename std::conditional<E == 4, u32x2, u32x4>::type>::type;
+    using QPart = typename std::conditional<SIXES, u32x6, u32x8>::type;
     using Elem = typename std::conditional<FOUR, uint8_t, uint16_t>::type;
     struct NoScales {};
     // Of V a lane loads one scale of a tile, that of key 4g + c % 4 and its own dims; the lane's four keys' are those of the four
@@ -303,8 +338,9 @@ struct Decode {
     uint32_t kat, vat[4];    // byte offsets of the lane's K and V in a tile
     float sc;                // scale * log2(e)
     u32x4 qv[FOUR ? 1 : KK];
-    i32x8 q8[FOUR ? KK : 1];  // FOUR: Q's parts and the bytes of their scales
+    QPart qp[FOUR ? KK : 1];  // FOUR: Q's parts and the bytes of their scales
     uint32_t qs[FOUR ? KK : 1];
+    float by;                 // SIXES: sc over what the lane's query was multiplied by
     uint32_t ksat, vsat;      // and byte offsets of the scales
     const uint16_t *q_row;    // the lane's query
     float *score;             // MASS: the lane's row of scores, at its keys of a tile; null for a column without a query
@@ -357,101 +393,109 @@ struct Decode {
         }
     }
 
+    // The group of 32 dims that the lane holds of a K row.
+    __device__ __forceinline__ uint32_t k_group() const { return D == 128 ? g : D == 64 ? g & 1u : 0u; }
+
     // FOUR: the query's 128 columns are, by 32 that share a scale, D = 128: its dims, once for each part; 64: the dims of parts 0
-    // and 1, then of parts 2 and 3; 32: the dims of parts 0 to 3. K's are its dims as often. Lane (c, g) holds
-    // columns 16g..+15 and 64+16g..+15, and the scale of columns 32g..+31 (hw_probe.hip has the layout). The parts' scale is
-    // the power of two of the largest value of its 32 dims, so that a large channel takes no bits from the others' dims, and what four
-    // parts leave is 2^-25 of that at most: nothing of an f16 value above 2^-14 of it, or a bf16 value above 2^-17. (Three parts under one
-    // scale for the row left 2^-20 of its largest value: with a channel at 256 times the others, scores were off by 1e-4.) Of heads of
-    // 128 the fourth part is a product more.
-    static constexpr int RUNS = D == 128 ? 2 : 1;  // of 16 dims of a lane
+    // and 1, then of parts 2 and 3; 32: the dims of parts 0 to 3. K's are its dims as often. Lane (c, g) holds the scale of columns 32g..+31,
+    // and those columns in 6 bits, in 8 columns 16g..+15 and 64+16g..+15 (hw_probe.hip has the layouts). The parts' scale is
+    // the power of two of the largest value of its 32 dims, so that a large channel takes no bits from the others' dims, and what the
+    // parts leave is 2^-25 of that at most: nothing of an f16 value above 2^-14 of it, or a bf16 value above 2^-17. (Three e4m3 parts under
+    // one scale for the row left 2^-20 of its largest value: with a channel at 256 times the others, scores were off by 1e-4.)
     struct RawQ {
-        uint32_t w[RUNS][8];
+        uint32_t w[QDIMS / 2];
         bool bf;
     };
-    __device__ __forceinline__ RawQ load_q8() const {
+    __device__ __forceinline__ RawQ load_raw_q() const {
         const Args a = again(args);
         RawQ q;
         q.bf = more_of(a)->bf;
+        const uint16_t *x = q_row + QDIMS * (D == 32 ? g & 1u : g);
+        if (a->q_vec) {
 #pragma unroll
-        for (int u = 0; u < RUNS; ++u) {
-            const uint16_t *x = q_row + 64 * u + 16 * (D == 32 ? g & 1u : g);
-            if (a->q_vec) {
-                const u32x4 y = *reinterpret_cast<const u32x4 *>(x), z = *reinterpret_cast<const u32x4 *>(x + 8);
+            for (int u = 0; u < QDIMS / 8; ++u) {
+                const u32x4 y = *reinterpret_cast<const u32x4 *>(x + 8 * u);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    q.w[u][i] = y[i];
-                    q.w[u][4 + i] = z[i];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) q.w[u][i] = uint32_t(x[2 * i]) | uint32_t(x[2 * i + 1]) << 16;
-            }
-        }
-        return q;
-    }
-    __device__ __forceinline__ void split_q8(const RawQ &q) {
-        float f[RUNS][16];
-        uint32_t e[2];  // the exponent of the 32 dims that a run is a half of; 255 where one is not finite: so is the scale then
-#pragma unroll
-        for (int u = 0; u < RUNS; ++u) {
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const half2v h = __builtin_bit_cast(half2v, q.w[u][i]);
-                f[u][2 * i] = q.bf ? __uint_as_float(q.w[u][i] << 16) : (float)h[0];
-                f[u][2 * i + 1] = q.bf ? __uint_as_float(q.w[u][i] & 0xffff0000u) : (float)h[1];
-                top = max(top, max(__float_as_uint(f[u][2 * i]) & 0x7fffffffu, __float_as_uint(f[u][2 * i + 1]) & 0x7fffffffu));
-            }
-            // The last part's scale byte is 1 or more; what is smaller than that allows for still has all of bf16's bits.
-            e[u] = max(pair_max(top) >> 23, 1u + 5u * (kQueryParts - 1));
-        }
-        if constexpr (RUNS == 1) e[1] = e[0];
-        // Of a run g = 0, 1 have one 32's exponent and g = 2, 3 the next one's; as scales the four stand one after the other (of fewer dims
-        // the first ones again).
-        const auto half = __builtin_amdgcn_permlane32_swap(e[0], e[1], false, false);
-        const uint32_t base = __builtin_amdgcn_permlane16_swap(half[0], half[1], false, false)[0];
-        uint32_t part[kQueryParts][4 * RUNS];
-#pragma unroll
-        for (int u = 0; u < RUNS; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float x[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = __builtin_ldexpf(f[u][4 * i + j], 127 - (int)e[u]);
-#pragma unroll
-                for (int n = 0; n < kQueryParts; ++n) part[n][4 * u + i] = take_eights(x);
-            }
-        auto scale_of = [&](uint32_t n) { return base == 255u ? base : base - 5u * n; };
-        if constexpr (D == 128) {
-#pragma unroll
-            for (int n = 0; n < kQueryParts; ++n) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) q8[n][i] = (int)part[n][i];
-                qs[n] = scale_of(n);
-            }
-        } else if constexpr (D == 64) {
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    q8[n][i] = (int)part[2 * n][i];
-                    q8[n][4 + i] = (int)part[2 * n + 1][i];
-                }
-                qs[n] = scale_of(2 * n + (g >> 1));
+                for (int i = 0; i < 4; ++i) q.w[4 * u + i] = y[i];
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                q8[0][i] = (int)(g < 2 ? part[0][i] : part[1][i]);
-                q8[0][4 + i] = (int)(g < 2 ? part[2][i] : part[3][i]);
+            for (int i = 0; i < QDIMS / 2; ++i) q.w[i] = uint32_t(x[2 * i]) | uint32_t(x[2 * i + 1]) << 16;
+        }
+        return q;
+    }
+    __device__ __forceinline__ void split_q(const RawQ &q) {
+        float f[QDIMS];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < QDIMS / 2; ++i) {
+            const half2v h = __builtin_bit_cast(half2v, q.w[i]);
+            f[2 * i] = q.bf ? __uint_as_float(q.w[i] << 16) : (float)h[0];
+            f[2 * i + 1] = q.bf ? __uint_as_float(q.w[i] & 0xffff0000u) : (float)h[1];
+            top = max(top, max(__float_as_uint(f[2 * i]) & 0x7fffffffu, __float_as_uint(f[2 * i + 1]) & 0x7fffffffu));
+        }
+        if constexpr (SIXES)
+            split_sixes(f, top >> 23);
+        else
+            split_eights(f, pair_max(top) >> 23);
+    }
+    // e: the exponent of the largest of the 32 dims; 255 where one is not finite: so is the scale then.
+    __device__ __forceinline__ void split_eights(const float (&f)[QDIMS], uint32_t e) {
+        // The last part's scale byte is 1 or more; what is smaller than that allows for still has all of bf16's bits.
+        e = max(e, 1u + 5u * (QPARTS - 1));
+        u32x4 part[QPARTS];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float x[4] = {f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]};
+#pragma unroll
+            for (int n = 0; n < QPARTS; ++n) {
+                const float scale = __uint_as_float((e - 5u * n) << 23);
+                part[n][i] = n + 1 < QPARTS ? take_eights<false>(x, scale) : take_eights<true>(x, scale);
             }
-            qs[0] = scale_of(g);
+        }
+        uint32_t n = g;  // the part whose scale is the lane's, in the first product
+        if constexpr (D == 64) {
+            // g = 0, 1 have one 32's exponent and g = 2, 3 the other's; as scales they take turns
+            const auto half = __builtin_amdgcn_permlane32_swap(e, e, false, false);
+            e = __builtin_amdgcn_permlane16_swap(half[0], half[1], false, false)[0];
+            n = g >> 1;
+        }
+#pragma unroll
+        for (int k = 0; k < KK; ++k) {
+            const u32x4 x = D == 64 ? part[2 * k] : g < 2 ? part[0] : part[1], y = D == 64 ? part[2 * k + 1] : g < 2 ? part[2] : part[3];
+            if constexpr (!SIXES) qp[k] = u32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            qs[k] = e == 255u ? e : e - 5u * (n + 2 * k);
         }
     }
-
-    // The group of 32 dims that the lane holds of a K row.
-    __device__ __forceinline__ uint32_t k_group() const { return D == 128 ? g : D == 64 ? g & 1u : 0u; }
+    __device__ __forceinline__ void split_sixes(const float (&f)[QDIMS], uint32_t e) {
+        floatx16 x, y;
+#pragma unroll
+        for (int i = 0; i < QDIMS / 2; ++i) {
+            x[i] = f[2 * i];
+            y[i] = f[2 * i + 1];
+        }
+        // The last part's scale byte is 1 or more here too, which leaves up to 2^-130. A query of less than 2^-47 all over (in bf16) is
+        // taken 2^32 times as large, at which no product overflows.
+        by = sc;
+        if (__any(e < 80u)) {
+            const bool all = quad_max(e) < 80u;
+#pragma unroll
+            for (int i = 0; i < QDIMS / 2; ++i) {
+                x[i] *= all ? 0x1p32f : 1.f;
+                y[i] *= all ? 0x1p32f : 1.f;
+            }
+            e += all ? 32u : 0u;
+            by = all ? sc * 0x1p-32f : sc;
+        }
+        e = max(e, 2u + 5u * (QPARTS - 1));
+#pragma unroll
+        for (int n = 0; n < QPARTS; ++n) {
+            const float scale = __uint_as_float((e - 1u - 5u * n) << 23);  // of n = 0, the largest is 2 to 4 times that
+            const u32x6 w = n + 1 < QPARTS ? take_sixes<false>(x, y, scale) : take_sixes<true>(x, y, scale);
+            if constexpr (SIXES) qp[n] = w;
+            qs[n] = e == 255u ? e : e - 1u - 5u * n;
+        }
+    }
 
     // Table entries of a step's 16-key tiles: uniform where a tile lies in one page, else one per lane (key c
     // of the tile). Past the request's end the last key's entry.
@@ -608,11 +652,11 @@ struct Decode {
             return entry < a.num_pages ? (uint32_t)((entry * a.page_stride + (key - nc_paged_quot(key, a.ps) * a.ps.d) * a.token_stride) / 32u) : ~0u;
         };
         uint32_t entry = entry_of(k0);
-        const RawQ q = load_q8();
+        const RawQ q = load_raw_q();
         Step x;
         issue_keys(x, a, place_of(k0, entry), k0);
         entry = entry_of(k0 + by);
-        split_q8(q);
+        split_q(q);
         while (true) {
             compute(x, k0, end);
             if ((k0 += by) >= end) return;
@@ -637,7 +681,7 @@ struct Decode {
             return entry < a.num_pages ? (entry * a.page_stride + (key - nc_paged_quot(key, a.ps) * a.ps.d) * a.token_stride) / 32u : ~0u;
         };
         uint32_t batch = k0, n = 0, entry = entry_of(k0);
-        const RawQ q = load_q8();
+        const RawQ q = load_raw_q();
         uint32_t places = place_of(k0, entry);
         auto next = [&](Step &st, uint32_t key) {
             if (n == STEPS) {
@@ -651,7 +695,7 @@ struct Decode {
         Step x;
         next(x, k0);
         entry = entry_of(k0 + STEPS * by);
-        split_q8(q);
+        split_q(q);
         while (true) {
             compute(x, k0, end);
             if ((k0 += by) >= end) return;
@@ -704,7 +748,10 @@ struct Decode {
                 const floatx4 x = kk ? dot[t] : floatx4{0.f, 0.f, 0.f, 0.f};
                 if constexpr (FOUR) {
                     const i32x4 y = __builtin_bit_cast(i32x4, st.k[t][0]);
-                    dot[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(i32x8{y[0], y[1], y[2], y[3], 0, 0, 0, 0}, q8[kk], x, 4, 0, 0,
+                    i32x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                    for (int i = 0; i < (SIXES ? 6 : 8); ++i) z[i] = (int)qp[kk][i];
+                    dot[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(i32x8{y[0], y[1], y[2], y[3], 0, 0, 0, 0}, z, x, 4, SIXES ? 2 : 0, 0,
                                                                              (int)st.scale.k[t], 0, (int)qs[kk]);
                 } else if constexpr (D == 16)
                     dot[t] = mfma_k16<BF>(st.k[t][kk], u32x2{qv[kk][0], qv[kk][1]}, x);
@@ -719,7 +766,7 @@ struct Decode {
                 float x = dot[PACK * t][i];
 #pragma unroll
                 for (int n = 1; n < PACK; ++n) x = part == (uint32_t)n ? dot[PACK * t + n][i] : x;
-                s[t][i] = x * sc;
+                s[t][i] = x * (FOUR && SIXES ? by : sc);
             }
         if (!full) {
 #pragma unroll
