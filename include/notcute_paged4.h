@@ -136,13 +136,15 @@ typedef struct nc_paged_evict_rules {
  * are the n pages that became free, in the requests' order and the tables', entries outside the pool among them. Those that find no place on the list (a cursor below n, or
  * beyond free_len) are lost. The tables are not changed: what they list behind the new length is the list's.
  *
- * counts[0] = cursor - n (at least 0), counts[1] = requests cut, counts[2] = n, counts[3] = tokens evicted.
+ * counts[0] = cursor - n (at least 0), counts[1] = requests cut, counts[2] = n, counts[3] = tokens evicted. counts[1] is -1 where rows were
+ * not moved because another call has changed the workspace meanwhile: the cut requests' rows are lost then.
  *
  * kept_lens may be seq_lens itself and counts may be cursor itself; apart from that no output overlaps another buffer
  * (NC_ERROR_INVALID_VALUE). A page of a request that is cut belongs to it alone: rows of pages that two requests share, or that one lists
  * twice, may be moved in any order. A row on a page outside the pool is not moved, nor is one moved there. Lengths in elements as for the
  * other calls; counts_len >= 4, cursor_len >= 1; workspace 16-byte aligned, nc_paged_evict_workspace_bytes, which need not be
- * cleared; calls that overlap in time need workspaces of their own. At most 2^20 requests (NC_ERROR_OVERFLOW). */
+ * cleared; calls that overlap in time need workspaces of their own (what two that share one leave is undefined, and not always told). At
+ * most 2^20 requests (NC_ERROR_OVERFLOW). */
 typedef struct nc_paged_evict_lists {
     const int32_t *block_table;
     uint64_t table_len;

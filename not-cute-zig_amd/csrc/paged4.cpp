@@ -7,6 +7,11 @@
 
 using namespace nc_paged;
 
+// Looks at other chunks' flags before an eviction's move gives up waiting: some tenth of a second's. Tests lower it.
+extern "C" {
+uint32_t nc_internal_evict_tries = 1u << 16;
+}
+
 namespace {
 
 // Every kernel of paged4.hip by its place here, under which the module keeps its function.
@@ -272,6 +277,7 @@ int evict(nc_module module, const nc_paged_evict_lists &t, const nc_paged_evict_
     a.side_chains = (uint32_t)std::min(o.num_seqs * chains, std::max<uint64_t>(1, kMoveWgs / a.side_chunks));
     a.mass_parts = (a.max_tokens + NC_PAGED4_MASS_PART - 1) / NC_PAGED4_MASS_PART;
     a.mass_wgs = (uint32_t)std::min<uint64_t>(o.num_seqs * a.mass_parts, 512);
+    a.tries = nc_internal_evict_tries;
     // Figures of the three ways are at the kernels. A short table's requests are a few waves' work.
     const bool small = a.max_tokens <= 2048;
     if (a.parts) {

@@ -328,10 +328,11 @@ struct Tokens {
         for (int i = 0; i < 5; ++i) x[i] = sum_of(s_sums[i], WAVES);
         const int64_t base = (int64_t)a.cursor[0] - x[0];
         if (r == 0 && tid == 0) {
-            a.totals[0] = (int32_t)max(base, (int64_t)0);
+            a.totals[0] = (int32_t)max(base, (int64_t)0);  // for counts[0], which may be the cursor that others read
             a.totals[1] = (int32_t)x[2];
-            a.totals[2] = (int32_t)x[0];
-            a.totals[3] = (int32_t)x[4];
+            a.counts[1] = (int32_t)x[2];
+            a.counts[2] = (int32_t)x[0];
+            a.counts[3] = (int32_t)x[4];
         }
         if (!cut) return;
         if (tid == 0) a.cuts[x[3]] = (int32_t)r;
@@ -601,22 +602,24 @@ extern "C" __global__ __launch_bounds__(64 * PART_WAVES) void nc_paged4_part_lis
 // 60); with the selection 67.5 us, one of 60000 104. (A wave a column that walks down the rows, which needs no flags: 100 and 346 us.)
 namespace {
 
-// A store that is asked for has been seen by whoever reads the flag: waits as in Decode::join().
-__device__ __forceinline__ void wait_for_chunks(const uint32_t *read, uint32_t chunk) {
+// A store that is asked for has been seen by whoever reads the flag: waits as in Decode::join(). False where the tries, some tenth of
+// a second's, ended the wait: the workspace was not this call's alone.
+__device__ __forceinline__ bool wait_for_chunks(const uint32_t *read, uint32_t chunk, uint32_t most_tries) {
     const uint32_t lane = threadIdx.x & 63u;
     for (uint32_t c0 = 0; c0 < chunk; c0 += 64) {
-        // The count, some tenth of a second, ends the wait where the workspace was not this call's alone.
-        for (uint32_t tries = 0; tries < 1u << 16; ++tries) {
-            const bool there = c0 + lane >= chunk || __hip_atomic_load(read + c0 + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0u;
-            if (__all(there)) break;
-            __builtin_amdgcn_s_sleep(2);
+        bool all = false;
+        for (uint32_t tries = 0; tries < most_tries && !all; ++tries) {
+            if (tries) __builtin_amdgcn_s_sleep(2);
+            all = __all(c0 + lane >= chunk || __hip_atomic_load(read + c0 + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0u);
         }
+        if (!all) return false;
     }
+    return true;
 }
 
 template <bool FOUR>
 __device__ __forceinline__ void move_chunk(const nc_paged_evict_args &a, uint32_t r, uint32_t chain, uint32_t chunk, uint32_t keep, uint32_t first,
-                                           uint32_t *read) {
+                                           uint32_t *read, uint32_t *s_late) {
     constexpr uint32_t ROWS = NC_PAGED4_MOVE_ROWS;
     constexpr uint32_t UE = FOUR ? 32 : 8;  // values of a unit
     const uint32_t tid = threadIdx.x, at_once = NC_PAGED4_MOVE_THREADS >> a.row_log2;
@@ -649,8 +652,15 @@ __device__ __forceinline__ void move_chunk(const nc_paged_evict_args &a, uint32_
     if (a.chunks > 1) {
         if (tid == 0) __hip_atomic_store(read + chunk, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (chunk) {
-            if (tid < 64) wait_for_chunks(read, chunk);
+            if (tid < 64) {
+                const bool there = wait_for_chunks(read, chunk, a.tries);
+                if (tid == 0) *s_late = !there;
+            }
             __syncthreads();
+            if (*s_late) {  // stored, these rows might be where others have still to be read
+                if (tid == 0) __hip_atomic_store(a.counts + 1, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                return;
+            }
         }
     }
 #pragma unroll
@@ -680,10 +690,10 @@ __device__ __forceinline__ Cut cut_of(const nc_paged_evict_args &a, uint32_t k) 
 }
 
 extern "C" __global__ __launch_bounds__(NC_PAGED4_MOVE_THREADS) void nc_paged4_move(const nc_paged_evict_args a) {
-    __shared__ uint32_t s_chunk;
+    __shared__ uint32_t s_chunk, s_late;
     const uint32_t cuts = min((uint32_t)as_const(a.totals)[1], a.num_seqs);
     if (blockIdx.x < a.mass_wgs) {  // what else the selection left
-        if (blockIdx.x == 0 && threadIdx.x < 4) a.counts[threadIdx.x] = a.totals[threadIdx.x];
+        if (blockIdx.x == 0 && threadIdx.x == 0) a.counts[0] = a.totals[0];
         for (uint32_t r = blockIdx.x * NC_PAGED4_MOVE_THREADS + threadIdx.x; r < a.num_seqs; r += a.mass_wgs * NC_PAGED4_MOVE_THREADS) a.kept_lens[r] = a.news[r];
         for (uint64_t p = blockIdx.x; p < (uint64_t)cuts * a.mass_parts; p += a.mass_wgs) {
             const uint32_t k = (uint32_t)(p / a.mass_parts);
@@ -712,9 +722,9 @@ extern "C" __global__ __launch_bounds__(NC_PAGED4_MOVE_THREADS) void nc_paged4_m
             }
             if (chunk >= chunks) break;
             if (a.four)
-                move_chunk<true>(a, c.r, chain, chunk, c.keep, c.first, a.read + at * a.chunks);
+                move_chunk<true>(a, c.r, chain, chunk, c.keep, c.first, a.read + at * a.chunks, &s_late);
             else
-                move_chunk<false>(a, c.r, chain, chunk, c.keep, c.first, a.read + at * a.chunks);
+                move_chunk<false>(a, c.r, chain, chunk, c.keep, c.first, a.read + at * a.chunks, &s_late);
             if (a.side_chunks >= a.chunks) break;  // every chunk has a workgroup
         }
     }

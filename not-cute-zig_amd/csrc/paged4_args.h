@@ -47,7 +47,7 @@ struct nc_paged_evict_args {
     float *mass;
     int32_t *free_pages, *kept_lens, *counts;
     uint8_t *k, *v, *k_scales, *v_scales;
-    int32_t *news, *olds, *first, *totals; // workspace: by request; totals: cursor, requests cut, pages, tokens
+    int32_t *news, *olds, *first, *totals; // workspace: by request; totals: cursor, requests cut
     int32_t *cuts;                         // the requests that are cut
     uint32_t *taken, *read;                // by chain: chunks taken, and by chunk whether its rows have been read
     uint32_t *states, *lows;               // of a selection by parts: by request and pass, and by part
@@ -62,6 +62,7 @@ struct nc_paged_evict_args {
     uint32_t parts, part;                  // parts of a request at most, and their tokens
     uint32_t mass_wgs, mass_parts;         // workgroups that move masses, their parts of a request
     uint32_t side_chains, side_chunks;     // workgroups that move rows: side_chunks for each of side_chains chains at a time
+    uint32_t tries;                        // looks at 64 chunks' flags before a wait gives up
     uint32_t four;
     nc_paged_div ps;
 };
