@@ -34,7 +34,7 @@ struct nc_paged_mass_args {
     const int32_t *seq_lens;
     float *mass;
     uint64_t score_pitch, mass_stride;
-    uint32_t num_seqs, num_q_heads, max_tokens, chunks;
+    uint32_t num_seqs, num_q_heads, max_tokens;
 };
 
 // Eviction. The selection leaves, by request, its new length, the first place that another token's row moves to, the source slot
