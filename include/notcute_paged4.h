@@ -10,12 +10,14 @@
  *
  * An extension: the reference has no cache. Conventions and options are those of notcute_paged.h, whose block tables
  * (nc_paged_build) serve both kinds of cache. Every call may be captured into a HIP graph; nc_paged_decode_mass,
- * nc_paged4_decode with a mass and the evictions are two launches (of tables for 12288 tokens and more five), the others one. The first of these calls through a module
- * loads their kernels (about 2.5 ms, once).
+ * nc_paged4_decode with a mass and the evictions are two launches, or an eviction five where the table is for 12288 tokens and more and the
+ * requests are not tens of thousands; the others are one. The first of these calls through a module loads their kernels (about
+ * 2.5 ms, once).
  *
  * A cache in 4 bits. K and V are each a pool of codes, two values a byte (the value of the even place in the low half), and a
  * pool of scales, a byte for every 32 values of a row (the microscaling format MXFP4: e2m1 values, e8m0 scales). A code is a
- * sign (bit 3) and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6; a scale byte b stands for 2^(b - 127), and 255 for a group of NaN. The
+ * sign (bit 3) and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6; a scale byte b stands for 2^(b - 127), and 255 for a group of NaN. (Values
+ * of 2^128 and more, of bytes 253 and 254, count as infinite in V: O is infinite or NaN then. The append writes none.) The
  * strides of the options count values: the value at element e of the pool (notcute_paged.h) is in byte e / 2 of the codes and has the
  * scale at e / 32. They are multiples of 32, and head_dim is 32, 64 or 128. element_type is the type of Q and of the rows.
  */
@@ -65,7 +67,8 @@ typedef struct nc_paged4_append_buffers {
 int nc_paged4_append(nc_module module, const nc_paged4_append_buffers *buffers, const nc_paged_options *opts, nc_stream stream);
 
 /* The rows at slots[0..num_rows-1] as dense rows of element_type (options' row_stride and row_head_stride, at any element
- * alignment), e.g. for the flash forward of a prompt that goes on behind a cached one. Values are exact where the type holds them,
+ * alignment). nc_flash_launch takes such rows of a prompt that goes on behind a cached one where head_dim is 32 or 64 and every query head
+ * has a key head of its own; it is a square forward, so Q has the cached positions too, and their outputs are computed again. Values are exact where the type holds them,
  * as it does for rows that nc_paged4_append wrote from the same type; the row of a slot outside the pool is zeros. A slot
  * may be listed more than once. The rows overlap neither the cache, nor the slots, nor each other (NC_ERROR_INVALID_VALUE; K's and
  * V's may be interleaved as long as no row of one is part of a row of the other). */
@@ -90,8 +93,11 @@ typedef struct nc_paged_mass {
 } nc_paged_mass;
 
 /* nc_paged_decode, and mass[r][j] += sum over all query heads of p_j for every token j of request r (those behind its last token
- * stay as they are; a request that gets zeros for O adds nothing, one with a NaN or a score of +infinity adds NaN). The sum over the
- * heads is f32, in a fixed order. Clear a request's row when it begins, and nc_paged_evict keeps it in step. The workspace is as
+ * stay as they are; a request that gets zeros for O adds nothing, one with a score that is NaN or +infinity adds NaN). The sum over the
+ * heads is f32, in a fixed order. Clear a request's row when it begins, and nc_paged_evict keeps it in step. Only these calls add
+ * weights: those of a prompt's own queries are not in it, so that right behind a prompt all masses are 0 and an eviction keeps the earlier
+ * tokens. Over 16 bits heads are taken each for itself: where nc_paged_decode takes neighbouring heads, or a wave a short head, this
+ * is slower by more than the scores. The workspace is as
  * nc_paged_decode's, but larger by the scores, 4 bytes for every request, query head and token of the table's row
  * (nc_paged_mass_workspace_bytes). The mass overlaps nothing else (NC_ERROR_INVALID_VALUE). */
 uint64_t nc_paged_mass_workspace_bytes(const nc_paged_options *opts);
@@ -100,9 +106,8 @@ int nc_paged_decode_mass(nc_module module, const nc_paged_decode_buffers *buffer
 
 /* nc_paged_decode over a cache in 4 bits. Scores are f32 sums of exact products but for Q: every value of it enters as the sum of
  * four 8-bit or five 6-bit numbers, off by at most 2^-25 of the largest of its 32 (dims 0..31, 32..63, ...) or 2^-130, and not at all where it
- * is above 2^-14 of that in f16, 2^-17 in bf16. The weights
- * enter the product with V as three bf16 parts, as nc_paged_decode's for bf16. A query that is not finite gives NaN, and so do keys
- * that count whose scale byte is 255, in K or in V. A `mass` that is not NULL adds the weights up as nc_paged_decode_mass
+ * is above 2^-14 of that in f16, 2^-17 in bf16. The weights enter the product with V as three bf16 parts, as nc_paged_decode's for bf16. A
+ * query that is not finite gives NaN, and so do keys that count whose scale byte is 255, in K or in V. A `mass` that is not NULL adds the weights up as nc_paged_decode_mass
  * does. Workspace: nc_paged4_workspace_bytes, with_mass 1 for calls with a mass. */
 typedef struct nc_paged4_decode_buffers {
     const uint16_t *q;
@@ -121,7 +126,8 @@ uint64_t nc_paged4_workspace_bytes(const nc_paged_options *opts, int with_mass);
 int nc_paged4_decode(nc_module module, const nc_paged4_decode_buffers *buffers, const nc_paged_mass *mass,
                      const nc_paged_options *opts, nc_stream stream);
 
-/* Eviction by accumulated weight. A request of more than `limit` tokens keeps `budget` of them: its first `sinks`, its last
+/* Eviction by accumulated weight (whose time grows with the square of the requests that are cut where they are thousands: 4096 of 20 tokens
+ * 54 us, 16384 0.28 ms, 65536 2.7 ms). A request of more than `limit` tokens keeps `budget` of them: its first `sinks`, its last
  * `recent`, and of the others those with the largest mass (of equal ones the earlier; a NaN counts as the largest). */
 typedef struct nc_paged_evict_rules {
     uint64_t limit;  /* at least budget */

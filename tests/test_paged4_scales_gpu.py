@@ -90,3 +90,17 @@ def test_attention_over_the_largest_scales(gpu, d):
     o, mass = attend(gpu, pool, q)
     assert (np.abs(o - want) <= bound).all(), np.max(np.abs(o - want) / bound)
     assert (np.abs(mass - madd[0]) <= mbound[0] + 2.0 ** -23 * mass).all()
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_values_that_f32_does_not_hold(gpu, d):
+    """V of 2^128 and more counts as infinite: its dim of O is infinite or NaN, and no other."""
+    rng = np.random.default_rng(d)
+    pool = p4.Pool4(rng, 4, 1, 16, d, "bf16")
+    codes = rng.integers(0, 3, d).astype(np.uint8)
+    codes[5] = 7  # 6 2^126
+    pool.put(1, 1, 0, 3, codes, np.full(d // 32, 253, np.uint8))
+    q = encode(rng.standard_normal((1, 4, d)), "bf16")
+    o, mass = attend(gpu, pool, q)
+    assert not np.isfinite(o[0, :, 5]).any() and np.isfinite(np.delete(o[0], 5, axis=1)).all()
+    assert np.isfinite(mass).all() and abs(mass.sum() - 4) < 1e-5
