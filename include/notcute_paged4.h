@@ -11,7 +11,7 @@
  * An extension: the reference has no cache. Conventions and options are those of notcute_paged.h, whose block tables
  * (nc_paged_build) serve both kinds of cache. Every call may be captured into a HIP graph; nc_paged_decode_mass,
  * nc_paged4_decode with a mass and the evictions are two launches, or an eviction five where the table is for 12288 tokens and more and the
- * requests are not tens of thousands; the others are one. The first of these calls through a module loads their kernels (about
+ * requests are not thousands (num_seqs * (parts + 1) of at most 65536, parts of 2048 tokens or a 64th); the others are one. The first of these calls through a module loads their kernels (about
  * 2.5 ms, once).
  *
  * A cache in 4 bits. K and V are each a pool of codes, two values a byte (the value of the even place in the low half), and a
